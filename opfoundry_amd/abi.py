@@ -40,7 +40,7 @@ ERRORS = {
 }
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
-# Every symbol include/*.h declares (dsa_mla.h, then dsa_topk.h), in declaration order.
+# Every symbol include/*.h declares (dsa_mla.h, dsa_topk.h, dsa_indexer.h, dsa_chunk.h).
 EXPORTED_SYMBOLS = (
     "dsa_mla_decode_workspace_size",
     "dsa_mla_decode_num_splits",
@@ -63,6 +63,11 @@ EXPORTED_SYMBOLS = (
     "dsa_indexer_scores",
     "dsa_mla_strerror",
     "dsa_mla_abi_version",
+    "dsa_qk_norm_rope",
+    "dsa_kv_append",
+    "dsa_mla_chunk_workspace_size",
+    "dsa_mla_chunk_num_splits",
+    "dsa_mla_chunk",
 )
 
 ABI_VERSION = 8
@@ -183,6 +188,67 @@ class IndexerArgs(ctypes.Structure):
     ]
 
 
+NORMS = {"none": 0, "rms": 1, "layer": 2}                    # dsa_norm
+ROPES = {None: 0, "interleaved": 1, "halves": 2}             # dsa_rope
+
+
+class NormRopeRows(ctypes.Structure):
+    """dsa_norm_rope_rows (include/dsa_chunk.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("stride_t", _i64), ("stride_h", _i64),
+        ("out", _vp), ("out_stride_t", _i64), ("out_stride_h", _i64),
+        ("weight", _vp), ("bias", _vp),
+        ("H", _i32), ("norm", _i32),
+    ]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    """dsa_qk_norm_rope_args (include/dsa_chunk.h)."""
+
+    _fields_ = [
+        ("q", NormRopeRows), ("k", NormRopeRows),
+        ("cos_sin", _vp), ("n_pos", _i64),
+        ("positions", _vp), ("q_indptr", _vp), ("seq_lens", _vp),
+        ("T", _i32), ("B", _i32), ("D", _i32), ("norm_dim", _i32), ("rot_off", _i32),
+        ("rope", _i32), ("inverse", _i32), ("eps", ctypes.c_float),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """dsa_kv_append_args (include/dsa_chunk.h)."""
+
+    _fields_ = [
+        ("kv", _vp), ("kv_stride_t", _i64), ("weight", _vp),
+        ("cache", _vp), ("cache_scale", _vp), ("cache_rope", _vp), ("cache_rows", _i64),
+        ("stride_row", _i64), ("scale_stride_row", _i64), ("rope_stride_row", _i64),
+        ("kv_format", _i32), ("norm", _i32), ("rope", _i32),
+        ("index_norm", _i32), ("index_rope", _i32),
+        ("index_k", _vp), ("index_stride_t", _i64), ("index_weight", _vp), ("index_bias", _vp),
+        ("index_cache", _vp), ("index_rows", _i64), ("index_stride_row", _i64),
+        ("cos_sin", _vp), ("n_pos", _i64),
+        ("q_indptr", _vp), ("seq_lens", _vp),
+        ("block_table", _vp), ("block_table_stride", _i64), ("table_blocks", _i32), ("block_size", _i32),
+        ("kv_batch_stride", _i64),
+        ("T", _i32), ("B", _i32), ("eps", ctypes.c_float), ("index_eps", ctypes.c_float),
+    ]
+
+
+class ChunkArgs(ctypes.Structure):
+    """dsa_mla_chunk_args (include/dsa_chunk.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("q_stride_t", _i64), ("q_stride_h", _i64),
+        ("q_indptr", _vp), ("seq_lens", _vp),
+        ("kv_cache", _vp), ("kv_total_rows", _i64), ("kv_stride_row", _i64),
+        ("kv_format", _i32), ("block_size", _i32),
+        ("block_table", _vp), ("block_table_stride", _i64), ("kv_batch_stride", _i64),
+        ("out", _vp), ("o_stride_t", _i64), ("o_stride_h", _i64), ("lse", _vp),
+        ("table_blocks", _i32), ("T", _i32), ("B", _i32), ("H", _i32),
+        ("causal", _i32), ("max_kv_len", _i32), ("num_splits", _i32), ("sm_scale", ctypes.c_float),
+    ]
+
+
 class DsaError(RuntimeError):
     def __init__(self, code: int, where: str):
         self.code = code
@@ -239,6 +305,11 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.dsa_mla_prefill_v4_fp8.argtypes = [ctypes.POINTER(PrefillV4Fp8Args), _vp, ctypes.c_size_t, _vp]
     lib.dsa_kv_quantize_fp8.argtypes = [_vp, _i64, _i64, _vp, _i64, _vp, _vp]
     lib.dsa_topk_indices.argtypes = [_vp, _i64, _vp, _i32, _i32, _i32, _vp, _i64, _vp]
+    lib.dsa_qk_norm_rope.argtypes = [ctypes.POINTER(QkNormRopeArgs), _vp]
+    lib.dsa_kv_append.argtypes = [ctypes.POINTER(KvAppendArgs), _vp]
+    lib.dsa_mla_chunk_workspace_size.argtypes = [ctypes.POINTER(ChunkArgs), sz]
+    lib.dsa_mla_chunk_num_splits.argtypes = [ctypes.POINTER(ChunkArgs), ctypes.POINTER(_i32)]
+    lib.dsa_mla_chunk.argtypes = [ctypes.POINTER(ChunkArgs), _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_strerror.argtypes = [ctypes.c_int]
     lib.dsa_mla_strerror.restype = ctypes.c_char_p
     lib.dsa_mla_abi_version.argtypes = []

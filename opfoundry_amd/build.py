@@ -17,7 +17,8 @@ import sys
 from .abi import LIB_PATH, PKG_DIR
 
 SRC = os.path.join(PKG_DIR, "csrc", "dsa_mla.hip")
-SRCS = [SRC, os.path.join(PKG_DIR, "csrc", "dsa_topk.hip"), os.path.join(PKG_DIR, "csrc", "dsa_indexer.hip")]
+SRCS = [SRC] + [os.path.join(PKG_DIR, "csrc", f)
+                for f in ("dsa_topk.hip", "dsa_indexer.hip", "dsa_prep.hip", "dsa_chunk.hip")]
 PROBE_SRC = os.path.join(PKG_DIR, "csrc", "dsa_gather_floor.hip")
 PROBE_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libdsa_gather_floor.so")
 ISSUE_PROBE_SRC = os.path.join(PKG_DIR, "csrc", "dsa_issue_probe.hip")

@@ -122,3 +122,25 @@ __device__ __forceinline__ void lds_dma16_s(const void* sbase, unsigned voff, ld
 __device__ __forceinline__ void tile_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
+
+// The sequence of a chunk's token t (include/dsa_chunk.h): the count of entries 1..B of indptr that are <= t, or
+// NO_SEQ for a token of none.  A wave looks at 64 entries at a time: one read up
+// to 64 sequences, two up to 4096.  (The result is in [0, B) whatever the array
+// holds.)
+constexpr int32_t NO_SEQ = -1;
+__device__ __forceinline__ int32_t seq_of(const int32_t* indptr, int32_t B, int32_t t) {
+    const int lane = threadIdx.x & 63;
+    int32_t lo = 0, n = B;
+    while (n > 64) {
+        const int32_t step = (n + 63) / 64;
+        const int32_t at = (lane + 1) * step;
+        const bool below = at <= n && indptr[lo + (at <= n ? at : n)] <= t;
+        const int32_t c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
+        lo += c * step;
+        n = n - c * step < step - 1 ? n - c * step : step - 1;
+    }
+    const bool below = lane < n && indptr[lo + (lane < n ? lane + 1 : 0)] <= t;
+    const int32_t b = lo + __builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
+    if (b >= B || t < indptr[b]) return NO_SEQ;
+    return __builtin_amdgcn_readfirstlane(b);
+}

@@ -1,0 +1,66 @@
+// dsa_seq.h - which sequence and position a chunk's token has, and which cache
+// row a position has: the rules of include/dsa_chunk.h, for the kernels (device)
+// and their CPU test (host).
+//
+// hipcc compiles these for host and device; a host-only test defines
+// __host__ and __device__ as empty before including this file.
+#ifndef DSA_SEQ_H_
+#define DSA_SEQ_H_
+
+#include <stdint.h>
+
+namespace dsa_seq {
+
+// The pages of a call.  One cache row per (sequence, position).
+struct Pages {
+    const int32_t* table;      // NULL: flat
+    int64_t table_stride;
+    int64_t batch_stride;      // flat: rows of a sequence (0: every sequence starts at row 0)
+    int64_t limit;             // positions at or past it have no row
+    int32_t block_size, shift; // shift = log2(block_size) for a power of two, else -1
+};
+
+__host__ __device__ inline Pages make_pages(const int32_t* table, int64_t table_stride, int32_t table_blocks,
+                                            int32_t block_size, int64_t batch_stride) {
+    Pages g;
+    g.table = table;
+    g.table_stride = table_stride;
+    g.batch_stride = batch_stride;
+    g.block_size = block_size;
+    g.shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (block_size == (1 << s)) g.shift = s;
+    g.limit = table ? (int64_t)table_blocks * block_size : (batch_stride > 0 ? batch_stride : INT64_MAX);
+    return g;
+}
+
+// Cache row of position p of sequence b, or -1 where it has none inside [0, rows).
+__host__ __device__ inline int64_t row_of(const Pages& g, int32_t b, int64_t p, int64_t rows) {
+    if (p < 0 || p >= g.limit) return -1;
+    int64_t row;
+    if (g.table) {
+        const int32_t q = (int32_t)p;         // below table_blocks * block_size, which the host keeps in 31 bits
+        const int32_t blk = g.shift >= 0 ? q >> g.shift : q / g.block_size;
+        row = (int64_t)g.table[(int64_t)b * g.table_stride + blk] * g.block_size + (q - blk * g.block_size);
+    } else {
+        row = (int64_t)b * g.batch_stride + p;
+    }
+    return row >= 0 && row < rows ? row : -1;
+}
+
+// Position of token t (in sequence b) of the chunk.
+__host__ __device__ inline int64_t position_of(const int32_t* indptr, const int32_t* lens, int32_t b, int32_t t) {
+    return (int64_t)lens[b] - indptr[b + 1] + t;
+}
+
+// Blocks of `m` rows that a grid gives sequence b, whose tokens have H rows each:
+// sequence b starts at block_start(b), its own blocks come first among those up to
+// block_start(b + 1), and the grid has block_start(B) of them, which needs no count
+// of the sequences before it.  floor((a + n) / m) - floor(a / m) + 1 >= ceil(n / m).
+__host__ __device__ inline int64_t block_start(int64_t indptr_b, int32_t b, int32_t H, int32_t m) {
+    return indptr_b * H / m + b;
+}
+
+}  // namespace dsa_seq
+
+#endif  // DSA_SEQ_H_

@@ -602,3 +602,317 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
     a.B, a.s_q, a.H_I, a.n_cols, a.causal = B, s_q, H_I, n_cols, 1 if causal else 0
     check(load_library().dsa_indexer_scores(ctypes.byref(a), _stream(stream)), "dsa_indexer_scores")
     return scores
+
+
+# ------------------------------------------------------------------ a chunk of new tokens
+
+class _On:
+    """The device of a call's tensors and the stream it runs on.  Every tensor must lie on one
+    device, which need not be the current one.  What the call allocates is used on its stream:
+    when that is not the device's current stream, the allocator is told, so that the memory is
+    not handed out again while the call still runs."""
+
+    def __init__(self, device: torch.device, stream):
+        self.device = device
+        current = torch.cuda.current_stream(device)
+        if stream is None:
+            self.other = None
+            self.handle = current.cuda_stream
+        else:
+            self.handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            self.other = None
+            if self.handle != current.cuda_stream:
+                self.other = (stream if isinstance(stream, torch.cuda.Stream)
+                              else torch.cuda.ExternalStream(self.handle, device=device))
+
+    def empty(self, shape, dtype):
+        t = torch.empty(shape, dtype=dtype, device=self.device)
+        if self.other is not None:
+            # the memory may still be in use by the current stream's earlier work
+            self.other.wait_stream(torch.cuda.current_stream(self.device))
+            t.record_stream(self.other)
+        return t
+
+    def call(self, fn, where, *args):
+        if torch.cuda.current_device() == self.device.index:
+            check(fn(*args, self.handle), where)
+        else:
+            with torch.cuda.device(self.device):
+                check(fn(*args, self.handle), where)
+
+
+def _operand(t: Optional[torch.Tensor], dtype, name: str, device=None, shape=None):
+    """Address of an operand (None: no operand) after its checks: type, device, shape (-1: any) and a
+    dense last dim."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if shape is not None and (t.dim() != len(shape) or any(w >= 0 and n != w for n, w in zip(t.shape, shape))):
+        raise ValueError(f"{name} must have shape {['any' if w < 0 else w for w in shape]}, got {tuple(t.shape)}")
+    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a dense last dim")
+    return t.data_ptr()
+
+
+def _choice(table, value, name: str) -> int:
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"{name} must be one of {list(table)}, got {value!r}") from None
+
+
+def _chunk_fields(a, q_indptr, seq_lens, device):
+    """The chunk's own fields (q_indptr, seq_lens, B)."""
+    a.q_indptr = _operand(q_indptr, torch.int32, "q_indptr", device, (-1,))
+    a.seq_lens = _operand(seq_lens, torch.int32, "seq_lens", device, (-1,))
+    if q_indptr.shape[0] != seq_lens.shape[0] + 1:
+        raise ValueError("q_indptr must have one entry more than seq_lens")
+    a.B = seq_lens.shape[0]
+
+
+def _page_fields(a, block_table, block_size, kv_batch_stride, B, device):
+    if block_table is not None:
+        a.block_table = _operand(block_table, torch.int32, "block_table", device, (B, -1))
+        if block_size is None:
+            raise ValueError("block_size is required with a block table")
+        a.block_table_stride, a.table_blocks, a.block_size = block_table.stride(0), block_table.shape[1], int(block_size)
+    else:
+        a.kv_batch_stride = int(kv_batch_stride)
+
+
+def _angles(a, cos_sin, device):
+    if cos_sin is not None:
+        a.cos_sin = _operand(cos_sin, torch.float32, "cos_sin", device, (-1, abi.D_ROPE))
+        if not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be contiguous")
+        a.n_pos = cos_sin.shape[0]
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of t (all dims but the last count rows, one uniform stride apart)."""
+    rs = t.stride(-2) if t.dim() >= 2 and t.numel() else t.shape[-1]
+    expect = rs
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] > 1 and t.stride(d) != expect:
+            raise ValueError(f"{name}: rows must be one uniform stride apart")
+        expect *= t.shape[d]
+    return max(rs, t.shape[-1]) if t.numel() <= t.shape[-1] else rs
+
+
+def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, *, k: Optional[torch.Tensor] = None,
+                 q_norm: str = "none", k_norm: str = "none", q_weight: Optional[torch.Tensor] = None,
+                 q_bias: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 k_bias: Optional[torch.Tensor] = None, norm_dim: Optional[int] = None, eps: float = 1e-6,
+                 rot_off: Optional[int] = None, style: Optional[str] = "interleaved", inverse: bool = False,
+                 q_indptr: Optional[torch.Tensor] = None, seq_lens: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                 stream=None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Norms of queries and keys for each head with the position rotation in the same pass
+    (dsa_qk_norm_rope): q bf16 [T, H, D], k bf16 [T, Hk, D] (or None), D = 128, 512 or 576.
+
+    q_norm / k_norm "none", "rms" or "layer" over values 0 .. norm_dim - 1 (default: all, 512 of 576)
+    with fp32 weights and biases [norm_dim]; then values rot_off .. rot_off + 63 (default: the first 64
+    of 128, else the last 64) are rotated ("interleaved" pairs, "halves", or None), back when `inverse`.
+    cos_sin fp32 [n_pos, 64]: a position's 32 cosines, then its 32 sines.  The position of a row is
+    positions[t] (int32 [T]), or the chunk's (q_indptr, seq_lens), whose rows of no sequence are left as
+    allocated.  Returns (q_out, k_out); an output may be its input."""
+    T, H, D = q.shape if q.dim() == 3 else (-1, -1, -1)
+    dev = q.device
+    a = abi.QkNormRopeArgs()
+    a.T, a.D = T, D
+    a.norm_dim = min(D, 512) if norm_dim is None else int(norm_dim)
+    a.rot_off = (0 if D == 128 else D - abi.D_ROPE) if rot_off is None else int(rot_off)
+    a.rope = _choice(abi.ROPES, style, "style")
+    a.inverse, a.eps = (1 if inverse else 0), float(eps)
+    bf16 = torch.bfloat16
+    streams = [(a.q, q, q_norm, q_weight, q_bias, q_out, "q")]
+    if k is not None:
+        streams.append((a.k, k, k_norm, k_weight, k_bias, k_out, "k"))
+    elif k_norm != "none" or k_weight is not None or k_bias is not None or k_out is not None:
+        raise ValueError("k_norm, k_weight, k_bias and k_out need k")
+    for s, x, norm, w, b, o, name in streams:
+        s.x = _operand(x, bf16, name, dev, (T, -1, D))
+        s.H, s.norm = x.shape[1], _choice(abi.NORMS, norm, name + "_norm")
+        s.stride_t, s.stride_h = x.stride(0), x.stride(1)
+        s.weight = _operand(w, torch.float32, name + "_weight", dev, (a.norm_dim,))
+        s.bias = _operand(b, torch.float32, name + "_bias", dev, (a.norm_dim,))
+        if o is not None:
+            _operand(o, bf16, name + "_out", dev, (T, x.shape[1], D))
+    if a.rope:
+        if cos_sin is None:
+            raise ValueError("a rotation needs cos_sin")
+        _angles(a, cos_sin, dev)
+        if positions is None and q_indptr is None:
+            raise ValueError("a rotation needs positions, or q_indptr and seq_lens")
+    if positions is not None:
+        a.positions = _operand(positions, torch.int32, "positions", dev, (T,))
+    elif q_indptr is not None:
+        if seq_lens is None:
+            raise ValueError("q_indptr needs seq_lens")
+        _chunk_fields(a, q_indptr, seq_lens, dev)
+    on = _On(dev, stream)
+    outs = []
+    for s, x, _, _, _, o, _ in streams:
+        if o is None:
+            o = on.empty(x.shape, bf16)
+        s.out, s.out_stride_t, s.out_stride_h = o.data_ptr(), o.stride(0), o.stride(1)
+        outs.append(o)
+    on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", ctypes.byref(a))
+    return outs[0], outs[1] if k is not None else None
+
+
+def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
+              cos_sin: Optional[torch.Tensor] = None, *, block_table: Optional[torch.Tensor] = None,
+              block_size: Optional[int] = None, kv_batch_stride: int = 0, norm: Optional[str] = None,
+              weight: Optional[torch.Tensor] = None, eps: float = 1e-6, style: Optional[str] = "interleaved",
+              index_k: Optional[torch.Tensor] = None, index_cache: Optional[torch.Tensor] = None,
+              index_norm: str = "none", index_weight: Optional[torch.Tensor] = None,
+              index_bias: Optional[torch.Tensor] = None, index_eps: Optional[float] = None,
+              index_style: Optional[str] = "halves", stream=None) -> None:
+    """Append a chunk's latent rows, and index keys beside them, to their paged caches
+    (dsa_kv_append).
+
+    kv bf16 [T, 576] (or [T, 512] for V4 rows), normed over its first 512 values (norm "rms", the
+    default with a weight, or "none") and rotated in its last 64 (style None: as they are).  cache: bf16
+    [..., 576], uint8 [..., 656], bf16 [..., 512], (uint8 [..., 512], uint8 [..., 16], bf16 [..., 64])
+    for MXFP8 streams, or (uint8 [..., 512], bf16 [..., 64]) for V4 fp8 rows.  index_k bf16 [T, 128] goes
+    to the same row of index_cache bf16 [..., 128], after index_norm and a rotation of its first 64
+    values.  Pages as in mla_decode (block_size defaults to the cache's dim before its last two's last:
+    [blocks, block_size, row]); sequence b's tokens q_indptr[b] .. q_indptr[b + 1] - 1 are its last
+    positions below seq_lens[b].  kv or index_k may be None."""
+    bf16, u8 = torch.bfloat16, torch.uint8
+    dev = q_indptr.device
+    a = abi.KvAppendArgs()
+    _chunk_fields(a, q_indptr, seq_lens, dev)
+    paged_like = None
+    if kv is not None:
+        parts = tuple(cache) if isinstance(cache, (tuple, list)) else (cache,)
+        kinds = tuple((t.dtype, t.shape[-1]) for t in parts)
+        formats = {((bf16, 576),): (abi.KV_BF16, 576), ((u8, 656),): (abi.KV_FP8_656, 576),
+                   ((bf16, 512),): (abi.KV_BF16_D512, 512),
+                   ((u8, 512), (u8, 16), (bf16, 64)): (abi.KV_MXFP8, 576),
+                   ((u8, 512), (bf16, 64)): (abi.KV_MXFP8_V4, 512)}
+        if kinds not in formats:
+            raise ValueError(f"cache is of no known format: {kinds}")
+        a.kv_format, width = formats[kinds]
+        a.kv = _operand(kv, bf16, "kv", dev, (-1, width))
+        a.T, a.kv_stride_t = kv.shape[0], kv.stride(0)
+        rows = [t.numel() // t.shape[-1] for t in parts]
+        if len(set(rows)) != 1:
+            raise ValueError("the cache's streams must have the same rows")
+        a.cache_rows = rows[0]
+        ptrs = [_operand(t, t.dtype, "cache", dev) for t in parts]
+        strides = [_row_stride(t, "cache") for t in parts]
+        a.cache, a.stride_row = ptrs[0], strides[0]
+        if len(parts) > 1:
+            a.cache_rope, a.rope_stride_row = ptrs[-1], strides[-1]
+        if len(parts) == 3:
+            a.cache_scale, a.scale_stride_row = ptrs[1], strides[1]
+        a.norm = _choice({"none": 0, "rms": 1}, norm or ("rms" if weight is not None else "none"), "norm")
+        a.weight = _operand(weight, torch.float32, "weight", dev, (512,))
+        a.rope = _choice(abi.ROPES, style, "style")
+        paged_like = parts[0]
+    a.eps = float(eps)
+    a.index_eps = float(eps if index_eps is None else index_eps)
+    if index_k is not None:
+        if index_cache is None:
+            raise ValueError("index_k needs index_cache")
+        a.index_k = _operand(index_k, bf16, "index_k", dev, (-1, 128))
+        if kv is not None and index_k.shape[0] != kv.shape[0]:
+            raise ValueError("kv and index_k must have the same rows")
+        a.T, a.index_stride_t = index_k.shape[0], index_k.stride(0)
+        a.index_cache = _operand(index_cache, bf16, "index_cache", dev)
+        if index_cache.shape[-1] != 128:
+            raise ValueError("index_cache must be bf16 [..., 128]")
+        a.index_rows, a.index_stride_row = index_cache.numel() // 128, _row_stride(index_cache, "index_cache")
+        a.index_norm = _choice(abi.NORMS, index_norm, "index_norm")
+        a.index_weight = _operand(index_weight, torch.float32, "index_weight", dev, (128,))
+        a.index_bias = _operand(index_bias, torch.float32, "index_bias", dev, (128,))
+        a.index_rope = _choice(abi.ROPES, index_style, "index_style")
+        paged_like = index_cache if paged_like is None else paged_like
+    if a.rope or a.index_rope:
+        if cos_sin is None:
+            raise ValueError("a rotation needs cos_sin")
+        _angles(a, cos_sin, dev)
+    if block_table is not None and block_size is None and paged_like is not None and paged_like.dim() >= 3:
+        block_size = paged_like.shape[-2]
+    _page_fields(a, block_table, block_size, kv_batch_stride, a.B, dev)
+    _On(dev, stream).call(load_library().dsa_kv_append, "dsa_kv_append", ctypes.byref(a))
+
+
+def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, block_table=None, block_size=None,
+                    kv_batch_stride=0, causal=True, max_kv_len=None, num_splits=0):
+    dev = q.device
+    a = abi.ChunkArgs()
+    a.q = _operand(q, torch.bfloat16, "q", dev, (-1, -1, abi.D_QK))
+    a.T, a.H = q.shape[0], q.shape[1]
+    a.q_stride_t, a.q_stride_h = q.stride(0), q.stride(1)
+    _chunk_fields(a, q_indptr, seq_lens, dev)
+    a.kv_format, a.kv_total_rows, a.kv_stride_row = kv_format_of(kv_cache)
+    a.kv_cache = _operand(kv_cache, kv_cache.dtype, "kv_cache", dev)
+    if block_table is not None and block_size is None and kv_cache.dim() >= 3:
+        block_size = kv_cache.shape[-2]
+    _page_fields(a, block_table, block_size, kv_batch_stride, a.B, dev)
+    if max_kv_len is None:
+        max_kv_len = (block_table.shape[1] * int(block_size) if block_table is not None
+                      else int(kv_batch_stride) or a.kv_total_rows)
+    if out is not None:
+        a.out = _operand(out, torch.bfloat16, "out", dev, (a.T, a.H, abi.D_VO))
+        a.o_stride_t, a.o_stride_h = out.stride(0), out.stride(1)
+    if lse is not None:
+        a.lse = _operand(lse, torch.float32, "lse", dev, (a.T, a.H))
+        if not lse.is_contiguous():
+            raise ValueError("lse must be contiguous")
+    a.causal, a.max_kv_len, a.num_splits = (1 if causal else 0), int(max_kv_len), int(num_splits)
+    a.sm_scale = float(sm_scale)
+    return a
+
+
+def chunk_num_splits(args) -> int:
+    n = ctypes.c_int32(0)
+    check(load_library().dsa_mla_chunk_num_splits(ctypes.byref(args), ctypes.byref(n)), "dsa_mla_chunk_num_splits")
+    return n.value
+
+
+def chunk_workspace_size(args) -> int:
+    n = ctypes.c_size_t(0)
+    check(load_library().dsa_mla_chunk_workspace_size(ctypes.byref(args), ctypes.byref(n)),
+          "dsa_mla_chunk_workspace_size")
+    return n.value
+
+
+def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
+              sm_scale: float, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, *,
+              block_table: Optional[torch.Tensor] = None, block_size: Optional[int] = None,
+              kv_batch_stride: int = 0, causal: bool = True, max_kv_len: Optional[int] = None,
+              num_splits: int = 0, workspace: Optional[torch.Tensor] = None,
+              stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Dense attention of a chunk's tokens over the paged latent cache (dsa_mla_chunk); returns
+    (out bf16 [T, H, 512], lse fp32 [T, H]).
+
+    q bf16 [T, H, 576]; kv_cache bf16 [..., 576] or uint8 [..., 656]; sequence b's tokens
+    q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b] (their own rows already
+    in the cache) and attend positions up to their own (causal) or all.  Rows of no sequence are left as
+    allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold)."""
+    a = make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, block_table=block_table,
+                        block_size=block_size, kv_batch_stride=kv_batch_stride, causal=causal,
+                        max_kv_len=max_kv_len, num_splits=num_splits)
+    on = _On(q.device, stream)
+    if out is None:
+        out = on.empty((a.T, a.H, abi.D_VO), torch.bfloat16)
+        a.out, a.o_stride_t, a.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    if lse is None:
+        lse = on.empty((a.T, a.H), torch.float32)
+        a.lse = lse.data_ptr()
+    need = chunk_workspace_size(a)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = on.empty((need,), torch.uint8)
+    ws = _operand(workspace, workspace.dtype, "workspace", q.device) if need else None
+    on.call(load_library().dsa_mla_chunk, "dsa_mla_chunk", ctypes.byref(a), ws, need)
+    return out, lse
