@@ -171,7 +171,8 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  *     O   = sum_j exp(s_j) k_j[0:512] / sum_j exp(s_j),  LSE = ln sum_j exp(s_j)
  * over the positions j of the token's sequence with a row in the cache,
  * 0 <= j < seq_lens[b] and, when causal != 0, j <= p (the token's own position).
- * A token with none gets O = 0 and LSE = +inf.
+ * A token with none gets O = 0 and LSE = +inf.  A NaN or infinity in a row reaches
+ * the tokens that attend it and no others.  sm_scale must be positive and finite.
  * q        : bf16 [T, H, 576] addressed by q_stride_{t,h}
  * kv_cache : kv_format DSA_KV_BF16 or DSA_KV_FP8_656, rows kv_stride_row
  *            elements apart (0 = dense), kv_total_rows below 2^31

@@ -5,6 +5,7 @@
 #include <float.h>
 #include <stdint.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/dsa_chunk.h"
 #include "dsa_seq.h"
@@ -139,6 +140,517 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_row_kernel(const ChunkPara
     }
 }
 
+// ---------------------------------------------------------------------------
+// The tiled kernel: one workgroup per 128 rows and split.  A row is one head of
+// one token; a block holds 128 consecutive rows of one sequence (token-major), so
+// any head count fills it, and all its rows attend the same cache rows but for the
+// causal end.  The cache rows come in tiles of 32, three tile buffers deep:
+//   QK^T   wave w: S^T[32 positions x its 32 rows], 36 k-steps of 32x32x16, Q in registers
+//   P      exp2 against a fixed reference (the first tile's maximum of the row), 16 bits,
+//          exchanged through LDS
+//   PV     wave w: O^T[dims 128 w .. +127 x 128 rows] in 256 accumulation registers
+// Iteration i computes QK^T of tile i + 1, then PV of tile i with the exponentials of
+// tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 403 of a
+// CU's 512 KB of registers, which is why a workgroup is 128 rows and fills a CU.
+// ---------------------------------------------------------------------------
+constexpr int BLOCK = 128;                   // rows of a workgroup
+constexpr int SPAN = 2048;                   // positions resolved to cache rows at a time
+// A tile in LDS: NoPE row r at r * NOPE_STRIDE, its 16-byte piece c at c ^ nope_sw(r); RoPE
+// row r at ROPE_OFF + 128 r, piece c at c ^ rope_sw(r).  The pad moves every row by four
+// banks groups and the XOR parts rows four apart, so that the K reads (one piece of 16
+// rows) and the transposed V reads (four pieces of four rows) meet no bank twice.
+constexpr int NOPE_STRIDE = 1088;
+constexpr int ROPE_OFF = TILE * NOPE_STRIDE;
+constexpr int TILE_BYTES = ROPE_OFF + TILE * 128;
+constexpr int P_BYTES = 2 * NWAVE * 64 * 16;
+constexpr int KS_NOPE = 32, KS = 36;         // 16-deep k-steps of NoPE, and with RoPE
+constexpr int LPW = TILE / NWAVE + 1;        // loads of a wave and tile
+__device__ __forceinline__ int nope_sw(int r) { return (r >> 2) & 3; }
+__device__ __forceinline__ int rope_sw(int r) { return (r >> 1) & 7; }
+
+__device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// O += A B on an accumulation register tile; the wait states before it (a vector write of
+// an operand: two) and around accesses of O from outside (o_fence) are written out, since
+// the compiler does not see a matrix instruction here.
+__device__ __forceinline__ void mfma_o(f32x16& acc, u32x4 a, u32x4 b) {
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void o_fence(f32x16 (&o)[16]) {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
+                 : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]),
+                   "+a"(o[8]), "+a"(o[9]), "+a"(o[10]), "+a"(o[11]), "+a"(o[12]), "+a"(o[13]), "+a"(o[14]), "+a"(o[15]));
+}
+
+// A workgroup's rows: those of sequence b from row r0 (of its n * H) on.
+struct Block {
+    int32_t b, r0, rows;       // rows = 0: nothing to do
+    int32_t first;             // token of row 0 of the sequence
+    int32_t len, end;          // positions; token t is position len - end + t
+};
+__device__ __forceinline__ Block find_block(const ChunkParams& p, int64_t x, int32_t m) {
+    auto start = [&](int32_t i) { return dsa_seq::block_start(min(max(p.indptr[i], 0), p.T), i, p.H, m); };
+    Block k{};
+    k.b = count_upto(p.B, x, start);
+    if (k.b >= p.B) return k;
+    const int64_t local = x - start(k.b);
+    k.first = max(p.indptr[k.b], 0);
+    k.end = p.indptr[k.b + 1];
+    k.len = p.lens[k.b];
+    const int64_t left = (int64_t)(min(k.end, p.T) - k.first) * p.H - local * m;
+    if (local < 0 || left <= 0) return k;
+    k.r0 = (int32_t)(local * m);
+    k.rows = (int32_t)min(left, (int64_t)m);
+    return k;
+}
+// positions that token t (of the block's sequence) attends: [0, limit)
+__device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k, int32_t t) {
+    const int64_t own = (int64_t)k.len - k.end + t + 1;
+    return (int32_t)max((int64_t)0, p.causal ? min(own, (int64_t)k.len) : (int64_t)k.len);
+}
+
+// the kernel's argument block, in the constant address space
+typedef const __attribute__((address_space(4))) ChunkParams* Args;
+
+__global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(1, 1)))
+dsa_mla_chunk_tile_kernel(const ChunkParams p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[3 * TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * P_BYTES];
+    __shared__ __attribute__((aligned(16))) int32_t s_rows[SPAN];     // cache rows of a span's positions
+    __shared__ uint32_t s_skip[SPAN / TILE];                          // bit j: position j of the tile has no row
+    __shared__ uint32_t s_nan[SPAN / TILE];                           // bit j: its row holds a NaN or infinity
+    __shared__ int32_t s_misc[4];                                     // [0] a row that may be read, [1] restart
+    __shared__ float s_inv[BLOCK];
+    const lds_ptr T0 = (lds_ptr)s_tile, PX = (lds_ptr)s_p;
+    const LDS_AS int32_t* const rows_l = (const LDS_AS int32_t*)s_rows;
+    // The arguments as the code outside the tile loop reads them: anew where it needs them, so
+    // that none is kept in a register across the loop.
+    auto args = []() -> Args {
+        Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
+    };
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hi = lane >> 5, r32 = lane & 31;
+    const int split = blockIdx.y;
+    // last block first: later tokens attend more, and the long ones must not come last
+    const Block blk = find_block(p, (int64_t)gridDim.x - 1 - blockIdx.x, BLOCK);
+    if (blk.rows == 0) return;
+    const int t_lo = blk.first + blk.r0 / p.H, t_hi = blk.first + (blk.r0 + blk.rows - 1) / p.H;
+    const int lim_lo = limit_in(p, blk, t_lo), lim_hi = limit_in(p, blk, t_hi);
+    const bool too_long = blk.len > p.max_len;
+    const int k0 = split * p.per_split;        // (at most max_len + one split: below 2^31)
+    // (positions without a page end the sequence as far as its rows go)
+    const int k1 = too_long ? k0 : (int)min(min((int64_t)lim_hi, p.pages.limit), (int64_t)k0 + p.per_split);
+    // a split with no positions writes nothing: the combine does not read it
+    if (p.ns > 1 && k1 <= k0) return;
+
+    // this lane's row (rows past the block's end are computed on its last one and not stored)
+    const int row = blk.r0 + min(32 * wave + r32, blk.rows - 1);
+    const int tok = blk.first + row / p.H, head = row % p.H;
+    const int limit = limit_in(p, blk, tok);
+    u32x4 qf[KS];
+    {
+        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh + 8 * hi;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
+    }
+
+    // ---- positions [c0, c0 + SPAN) below k1 -> cache rows ----
+    // A position without a row, and those from k1 on, are read as some row that exists (every
+    // read is of the cache's own rows that the sequence attends) and masked.
+    int ntiles = 0;
+    auto resolve = [&](int c0) {
+        const Args a = args();
+        const int64_t rows = a->rows;
+        const int32_t bs = a->pages.block_size, shift = a->pages.shift;
+        const int32_t* const table = a->pages.table;
+        const int tid = 64 * wave + fresh_lane();
+        const int at = c0 + 8 * tid;
+        int32_t id[8];
+        // (positions past the end look up the last one's row: no branch splits the eight reads)
+        if (!table) {
+            const int64_t base = blk.b * a->pages.batch_stride;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t r = base + min(at + e, k1 - 1);
+                id[e] = r < rows ? (int32_t)r : -1;
+            }
+        } else {
+            const int32_t* const mine = table + blk.b * a->pages.table_stride;
+            int32_t blk_i[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int q = min(at + e, k1 - 1);
+                blk_i[e] = shift >= 0 ? q >> shift : q / bs;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) id[e] = mine[blk_i[e]];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t r = (int64_t)id[e] * bs + (min(at + e, k1 - 1) - blk_i[e] * bs);
+                id[e] = r >= 0 && r < rows ? (int32_t)r : -1;
+            }
+        }
+        uint32_t skip = 0;
+        int32_t some = -1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            skip |= at + e >= k1 || id[e] < 0 ? 1u << e : 0u;
+            some = max(some, id[e]);
+        }
+        __syncthreads();                       // the previous span is done with its rows and tiles
+        if (tid == 0) s_misc[0] = -1;
+        if (tid < SPAN / TILE) s_nan[tid] = 0;
+        __syncthreads();
+        if (some >= 0) s_misc[0] = some;       // any of them will do
+        __syncthreads();
+        const int32_t safe = __builtin_amdgcn_readfirstlane(s_misc[0]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) id[e] = id[e] < 0 ? max(safe, 0) : id[e];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+            *reinterpret_cast<int4*>(&s_rows[8 * tid + e]) = int4{id[e], id[e + 1], id[e + 2], id[e + 3]};
+        reinterpret_cast<unsigned char*>(s_skip)[tid] = (unsigned char)skip;
+        ntiles = safe < 0 ? 0 : (min(k1 - c0, SPAN) + TILE - 1) / TILE;
+        __syncthreads();
+    };
+
+    // ---- tile i of the span -> buffer `slot`: wave w rows 8 w .. 8 w + 7 and their RoPE ----
+    auto slot_of = [&](int s) -> lds_ptr { return T0 + s * TILE_BYTES; };
+    struct Rows {
+        int32_t r[8];
+        int32_t rope;
+    };
+    auto load_rows = [&](int i) -> Rows {
+        const LDS_AS int32_t* at = rows_l + i * TILE + 8 * wave;
+        const u32x4 a = lds_ld<u32x4>((lds_cptr)at), b = lds_ld<u32x4>((lds_cptr)(at + 4));
+        Rows g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            g.r[e] = __builtin_amdgcn_readfirstlane((int)a[e]);
+            g.r[4 + e] = __builtin_amdgcn_readfirstlane((int)b[e]);
+        }
+        g.rope = at[opaque(lane) >> 3];
+        return g;
+    };
+    auto issue = [&](const Rows& g, int slot) {
+        const int ln = opaque(lane);
+        const lds_ptr tb = slot_of(slot);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int r = 8 * wave + e;
+            const unsigned char* base = p.kv + (uint64_t)(uint32_t)g.r[e] * (uint32_t)p.row_bytes;
+            lds_dma16_s(base, 16u * (unsigned)(ln ^ nope_sw(r)), tb + r * NOPE_STRIDE);
+        }
+        const int r = 8 * wave + (ln >> 3);
+        lds_dma16(p.kv + (uint64_t)(uint32_t)g.rope * (uint32_t)p.row_bytes + 1024 + 16 * ((ln & 7) ^ rope_sw(r)),
+                  tb + ROPE_OFF + 8 * wave * 128);
+    };
+
+    // In a tile that some row of the block does not attend whole, a row of the cache may hold anything,
+    // and 0 x NaN is NaN: one with a NaN or infinity among its NoPE values is cleared, and the scores of
+    // those that do attend it become NaN.  (A wave looks at the rows that it loaded.)
+    auto scan = [&](int i, int slot) {
+        const int ln = opaque(lane);
+        const lds_ptr tb = slot_of(slot) + 8 * wave * NOPE_STRIDE + 16 * ln;
+        uint32_t bad = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const u32x4 v = lds_ld<u32x4>(tb + e * NOPE_STRIDE);
+            bool odd = false;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) odd |= (v[w] & 0x7F800000u) == 0x7F800000u || (v[w] & 0x7F80u) == 0x7F80u;
+            if (__builtin_amdgcn_ballot_w64(odd)) {
+                lds_st<u32x4>(tb + e * NOPE_STRIDE, u32x4{0, 0, 0, 0});
+                bad |= 1u << e;
+            }
+        }
+        if (bad && ln == 0) reinterpret_cast<unsigned char*>(s_nan)[4 * i + wave] = (unsigned char)bad;
+    };
+
+    auto landed = [&](auto keep) {
+        wait_vm<decltype(keep)::value>();
+        asm volatile("" ::: "memory");
+    };
+    const float c_s = p.scale_log2;
+    f32x16 o[16];
+    float m_ref = 0.0f, l_lane = 0.0f;
+    bool first_tile = true, any = false;
+
+    auto qk = [&](lds_cptr kt) -> f32x16 {
+        const int ln = lane, lhi = ln >> 5, lr = ln & 31;
+        const lds_cptr k_even = kt + lr * NOPE_STRIDE + 16 * (lhi ^ nope_sw(lr));
+        const lds_cptr k_odd = kt + lr * NOPE_STRIDE + 16 * ((2 + lhi) ^ nope_sw(lr));
+        const lds_cptr k_rope = kt + ROPE_OFF + 128 * lr;
+        const int rsw = rope_sw(lr);
+        constexpr int AHEAD = 6;
+        auto k_at = [&](int ks) -> lds_cptr {
+            return ks < KS_NOPE ? ((ks & 1) ? k_odd : k_even) + 64 * (ks >> 1) : k_rope + 16 * ((2 * (ks - KS_NOPE) + lhi) ^ rsw);
+        };
+        u32x4 kb[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kb[i] = lds_ld<u32x4>(k_at(i));
+        f32x16 acc = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            __builtin_amdgcn_sched_barrier(0);
+            acc = mfma_bf16(kb[ks % AHEAD], qf[ks], acc);
+            if (ks + AHEAD < KS) kb[ks % AHEAD] = lds_ld<u32x4>(k_at(ks + AHEAD));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return acc;
+    };
+    auto masked = [&](int i, int c0) { return c0 + (i + 1) * TILE > lim_lo || __builtin_amdgcn_readfirstlane(s_skip[i]) != 0; };
+    // lane (hi, r32), register r: position 8 (r / 4) + 4 hi + r % 4 of the tile, row r32 of the wave
+    auto mask = [&](f32x16& s, int i, int c0) {
+        const uint32_t skip = s_skip[i];
+        const int pos0 = c0 + i * TILE;
+        if (masked(i, c0)) {
+            asm volatile("");
+            const uint32_t nan = s_nan[i];
+            const int left = limit - pos0, h4 = 4 * opaque(hi);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = 8 * (r >> 2) + h4 + (r & 3);
+                const bool on = j < left && !((skip >> j) & 1);
+                any = any || on;
+                const float v = (nan >> j) & 1 ? __builtin_nanf("") : s[r];
+                s[r] = on ? v : -INFINITY;
+            }
+        } else {
+            any = true;
+        }
+    };
+    auto top_of = [&](const f32x16& s) -> float {
+        float m = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+        return fmaxf(m, __shfl_xor(m, 32, 64));
+    };
+    auto p_half = [&](const float* e, int u, lds_ptr px) {
+        const int ln = opaque(lane);
+        float lt = 0.0f;
+#pragma unroll
+        for (int r = 8 * u; r < 8 * u + 8; ++r) lt += e[r];
+        l_lane += lt;
+        const f32x8 a = {e[8 * u], e[8 * u + 1], e[8 * u + 2], e[8 * u + 3], e[8 * u + 4], e[8 * u + 5], e[8 * u + 6], e[8 * u + 7]};
+        lds_st<u32x4>(px + ((u * NWAVE + wave) * 64 + ln) * 16, __builtin_bit_cast(u32x4, __builtin_convertvector(a, bf16x8)));
+    };
+    auto p_first = [&](f32x16& s, lds_ptr px) {
+        if (first_tile) {
+            // no position of the first tile attended: any reference, checked at the end
+            const float top = top_of(s) * c_s;
+            m_ref = top == -INFINITY ? 0.0f : top;
+            first_tile = false;
+        }
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c_s, -m_ref));
+        p_half(e, 0, px);
+        p_half(e, 1, px);
+    };
+    auto pv = [&](lds_cptr vt, lds_cptr px, const f32x16& sn, float* en, auto with_exp) {
+        const int ln = lane, lhi = ln >> 5;
+        const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
+        const int vx = 2 * (g16 & 1) + (pp >> 1);
+        const lds_cptr v_a = vt + (4 * lhi + rr) * NOPE_STRIDE + 16 * (vx ^ lhi) + 8 * (pp & 1) + 256 * wave;
+        const lds_cptr v_b = vt + (4 * lhi + rr + 8) * NOPE_STRIDE + 16 * (vx ^ (lhi + 2)) + 8 * (pp & 1) + 256 * wave;
+        auto v_frag = [&](int u, int m) -> u32x4 {
+            const s16x4 va = lds_read_tr16(v_a + 16 * u * NOPE_STRIDE + 64 * m);
+            const s16x4 vb = lds_read_tr16(v_b + 16 * u * NOPE_STRIDE + 64 * m);
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            u32x4 pb[NWAVE];
+#pragma unroll
+            for (int h = 0; h < NWAVE; ++h) pb[h] = lds_ld<u32x4>(px + ((u * NWAVE + h) * 64 + ln) * 16);
+            u32x4 v_cur = v_frag(u, 0);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                __builtin_amdgcn_sched_barrier(0);
+                const u32x4 v_nxt = m + 1 < 4 ? v_frag(u, m + 1) : v_cur;
+#pragma unroll
+                for (int h = 0; h < NWAVE; ++h) mfma_o(o[4 * m + h], v_cur, pb[h]);
+                if constexpr (decltype(with_exp)::value) {
+                    const int r0 = 8 * u + 2 * m;
+                    en[r0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0], c_s, -m_ref));
+                    en[r0 + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0 + 1], c_s, -m_ref));
+                }
+                v_cur = v_nxt;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    const int nspans = k1 > k0 ? (k1 - k0 + SPAN - 1) / SPAN : 0;
+    // Pass 0; where its reference did not serve (rare): the largest score of every row, and the pass
+    // again with that as the reference.
+    for (bool again = false;;) {
+#pragma unroll
+        for (int m = 0; m < 16; ++m) o[m] = f32x16{};
+        o_fence(o);
+        l_lane = 0.0f;
+        for (int c = 0; c < nspans; ++c) {
+            const int c0 = k0 + c * SPAN;
+            resolve(c0);
+            if (ntiles == 0) continue;
+            issue(load_rows(0), 0);
+            if (ntiles > 1) issue(load_rows(1), 1);
+            Rows next = load_rows(min(2, ntiles - 1));
+            if (ntiles > 1) landed(std::integral_constant<int, LPW>{}); else landed(std::integral_constant<int, 0>{});
+            if (masked(0, c0)) scan(0, 0);
+            tile_barrier();
+            f32x16 s0 = qk(slot_of(0));
+            mask(s0, 0, c0);
+            p_first(s0, PX);
+            int cur = 0;
+            for (int i = 0; i + 1 < ntiles; ++i) {
+                const int nxt = cur == 2 ? 0 : cur + 1;
+                // tile i + 1, the only one in flight, has landed; the barrier shows every wave's P of
+                // tile i, and every wave is done with tile i - 1, whose buffer takes tile i + 2
+                landed(std::integral_constant<int, 0>{});
+                if (masked(i + 1, c0)) scan(i + 1, nxt);
+                tile_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 2 < ntiles) issue(next, nxt == 2 ? 0 : nxt + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16 sn = qk(slot_of(nxt));
+                if (i + 3 < ntiles) next = load_rows(i + 3);
+                mask(sn, i + 1, c0);
+                float en[16];
+                pv(slot_of(cur), PX + (i & 1) * P_BYTES, sn, en, std::true_type{});
+                const lds_ptr px = PX + ((i + 1) & 1) * P_BYTES;
+                p_half(en, 0, px);
+                p_half(en, 1, px);
+                cur = nxt;
+            }
+            tile_barrier();
+            float en[16];
+            pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{});
+        }
+        o_fence(o);
+        if (again) break;
+        // The reference served if the sum lies where fp32 and the 16-bit P hold it.  With the first
+        // tile's maximum it is at least 1; it grows past 2^100 only where later scores do.
+        const float l = l_lane + __shfl_xor(l_lane, 32, 64);
+        const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
+        __syncthreads();
+        if (wave == 0) s_misc[1] = 0;
+        __syncthreads();
+        if (have && !(l > 0x1p-40f && l < 0x1p100f)) s_misc[1] = 1;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
+        again = true;
+        float top = -INFINITY;
+        for (int c = 0; c < nspans; ++c) {
+            const int c0 = k0 + c * SPAN;
+            resolve(c0);
+            for (int i = 0; i < ntiles; ++i) {
+                issue(load_rows(i), 0);
+                landed(std::integral_constant<int, 0>{});
+                if (masked(i, c0)) scan(i, 0);
+                tile_barrier();
+                f32x16 s = qk(slot_of(0));
+                mask(s, i, c0);
+                top = fmaxf(top, top_of(s));
+                tile_barrier();
+            }
+        }
+        m_ref = top == -INFINITY ? 0.0f : top * c_s;
+    }
+
+    // ---- O / l, LSE ----
+    // (lane and wave numbers anew: none of what follows is kept through the tile loop)
+    const int ln = fresh_lane(), hi_ = ln >> 5, r_ = ln & 31;
+    int wv = wave;
+    asm volatile("" : "+s"(wv));
+    const Args a_ = args();
+    const int ns = a_->ns, H = a_->H;
+    const int64_t TH = (int64_t)a_->T * H;
+    const float l = l_lane + __shfl_xor(l_lane, 32, 64);
+    const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
+    const bool mine = 32 * wv + r_ < blk.rows;
+    const float lse = too_long ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l)) * LN2;
+    if (hi_ == 0) {
+        s_inv[32 * wv + r_] = too_long ? __builtin_nanf("") : (have ? 1.0f / l : 0.0f);
+        const int64_t at = (int64_t)blk.first * H + blk.r0 + 32 * wv + r_;      // rows are token-major
+        if (mine && ns > 1) a_->part_lse[split * TH + at] = have ? lse : -FLT_MAX;
+        else if (mine && a_->lse) a_->lse[at] = have || too_long ? lse : INFINITY;
+    }
+    __syncthreads();
+    float inv[NWAVE];
+#pragma unroll
+    for (int h = 0; h < NWAVE; ++h) inv[h] = s_inv[32 * h + r_];
+    const int d0 = 128 * wv + 4 * hi_;
+    if (ns == 1) {
+        const int64_t o_st = a_->o_st, o_sh = a_->o_sh;
+        __bf16* const out = a_->out;
+        // 32 rows at a time through LDS, so that a wave's store is one whole 1 KB row
+        constexpr int OUT_STRIDE = D_VO * 2 + 16;
+        static_assert(32 * OUT_STRIDE <= TILE_BYTES, "the stage fits a tile buffer");
+        const int st_w = opaque(r_ * OUT_STRIDE + 2 * d0);
+        const bool o16 = ((o_st | o_sh) & 7) == 0 && ((uintptr_t)out & 15) == 0;
+#pragma unroll
+        for (int h = 0; h < NWAVE; ++h) {
+            const lds_ptr stg = slot_of(h & 1);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16& a = o[4 * m + h];
+                    const f32x4 v = {a[4 * g] * inv[h], a[4 * g + 1] * inv[h], a[4 * g + 2] * inv[h], a[4 * g + 3] * inv[h]};
+                    lds_st<u32x2>(stg + st_w + 2 * (32 * m + 8 * g), __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4)));
+                }
+            }
+            __syncthreads();
+            for (int k = 0; k < 8; ++k) {
+                const int r = 32 * h + 8 * wv + k;
+                if (r >= blk.rows) break;
+                const int t = blk.first + (blk.r0 + r) / H, hh = (blk.r0 + r) % H;
+                const u32x4 v = lds_ld<u32x4>(stg + (8 * wv + k) * OUT_STRIDE + 16 * ln);
+                __bf16* const dst = out + t * o_st + hh * o_sh + 8 * ln;
+                if (o16) {
+                    *reinterpret_cast<u32x4*>(dst) = v;
+                } else {
+                    reinterpret_cast<u32x2*>(dst)[0] = u32x2{v[0], v[1]};
+                    reinterpret_cast<u32x2*>(dst)[1] = u32x2{v[2], v[3]};
+                }
+            }
+        }
+    } else {
+        // fp32 partials: the wave's 128 dims of two rows a store
+        constexpr int PST = D_VO + 16;
+        static_assert(4 * 32 * PST <= 3 * TILE_BYTES, "four waves' stages fit the tile buffers");
+        const lds_ptr stg = T0 + wv * 32 * PST;
+        const int st_w = opaque(r_ * PST + 16 * hi_);
+        float* const dst0 = a_->part_o + (split * TH + (int64_t)blk.first * H + blk.r0) * D_VO;
+#pragma unroll
+        for (int h = 0; h < NWAVE; ++h) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16& a = o[4 * m + h];
+                    const f32x4 v = {a[4 * g] * inv[h], a[4 * g + 1] * inv[h], a[4 * g + 2] * inv[h], a[4 * g + 3] * inv[h]};
+                    lds_st<f32x4>(stg + st_w + 4 * (32 * m + 8 * g), v);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int r = 2 * k + (ln >> 5);
+                const f32x4 v = lds_ld<f32x4>(stg + r * PST + 16 * (ln & 31));
+                if (32 * h + r < blk.rows)
+                    *reinterpret_cast<f32x4*>(dst0 + (int64_t)(32 * h + r) * D_VO + 128 * wv + 4 * (ln & 31)) = v;
+            }
+        }
+    }
+}
+
 // Joins the partials of a row's splits, one wave a row: a lane holds 8 of its 512
 // values.  Splits past the row's positions wrote nothing and are not read.
 __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const ChunkParams p) {
@@ -148,7 +660,7 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
     const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H);
     const int32_t b = seq_of(p.indptr, p.B, t);
     if (b == NO_SEQ) return;
-    const int64_t limit = limit_of(p, b, t);
+    const int64_t limit = min(limit_of(p, b, t), p.pages.limit);
     const int ns = (int)min((int64_t)p.ns, (limit + p.per_split - 1) / p.per_split);
     const int64_t step = (int64_t)p.T * p.H;
     const float mine = lane < ns ? p.part_lse[lane * step + row] : -FLT_MAX;     // at most 64 splits
@@ -217,6 +729,7 @@ int validate(const dsa_mla_chunk_args* a) {
     } else if (a->kv_batch_stride < 0) {
         return DSA_ERR_BAD_STRIDE;
     }
+    if (!(a->sm_scale > 0.0f && a->sm_scale <= FLT_MAX)) return DSA_ERR_UNSUPPORTED;
     if (a->T == 0 || a->B == 0) return DSA_OK;
     if (!a->q || !a->out || !a->q_indptr || !a->seq_lens || (a->kv_total_rows > 0 && !a->kv_cache))
         return DSA_ERR_NULL_POINTER;
@@ -274,8 +787,9 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
     const dim3 grid((unsigned)((int64_t)a->T * a->H), (unsigned)p.ns);
+    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, BLOCK), (unsigned)p.ns);
     if (a->kv_format == DSA_KV_BF16)
-        hipLaunchKernelGGL(dsa_mla_chunk_row_kernel<DSA_KV_BF16>, grid, dim3(NTHR), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
     else
         hipLaunchKernelGGL(dsa_mla_chunk_row_kernel<DSA_KV_FP8_656>, grid, dim3(NTHR), 0, (hipStream_t)stream, p);
     if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;

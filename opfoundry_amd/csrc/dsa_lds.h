@@ -123,24 +123,29 @@ __device__ __forceinline__ void tile_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The sequence of a chunk's token t (include/dsa_chunk.h): the count of entries 1..B of indptr that are <= t, or
-// NO_SEQ for a token of none.  A wave looks at 64 entries at a time: one read up
-// to 64 sequences, two up to 4096.  (The result is in [0, B) whatever the array
-// holds.)
-constexpr int32_t NO_SEQ = -1;
-__device__ __forceinline__ int32_t seq_of(const int32_t* indptr, int32_t B, int32_t t) {
+// The count of i in [1, n] with at(i) <= t, for an ascending at(); whatever at() gives,
+// the result is in [0, n] and at() is called for 0 .. n only.  A wave looks at 64 places
+// at a time: one round trip up to n = 64, two up to 4096.
+template <class F>
+__device__ __forceinline__ int32_t count_upto(int32_t n, int64_t t, F at) {
     const int lane = threadIdx.x & 63;
-    int32_t lo = 0, n = B;
+    int32_t lo = 0;
     while (n > 64) {
         const int32_t step = (n + 63) / 64;
-        const int32_t at = (lane + 1) * step;
-        const bool below = at <= n && indptr[lo + (at <= n ? at : n)] <= t;
+        const int64_t i = (int64_t)(lane + 1) * step;
+        const bool below = i <= n && at(lo + (int32_t)(i <= n ? i : n)) <= t;
         const int32_t c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
         lo += c * step;
         n = n - c * step < step - 1 ? n - c * step : step - 1;
     }
-    const bool below = lane < n && indptr[lo + (lane < n ? lane + 1 : 0)] <= t;
-    const int32_t b = lo + __builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
-    if (b >= B || t < indptr[b]) return NO_SEQ;
-    return __builtin_amdgcn_readfirstlane(b);
+    const bool below = lane < n && at(lo + (lane < n ? lane + 1 : 0)) <= t;
+    return __builtin_amdgcn_readfirstlane(lo + __builtin_popcountll(__builtin_amdgcn_ballot_w64(below)));
+}
+
+// The sequence of a chunk's token t (include/dsa_chunk.h), or NO_SEQ for a token of none;
+// in [0, B) whatever the array holds.
+constexpr int32_t NO_SEQ = -1;
+__device__ __forceinline__ int32_t seq_of(const int32_t* indptr, int32_t B, int32_t t) {
+    const int32_t b = count_upto(B, t, [&](int32_t i) { return (int64_t)indptr[i]; });
+    return b >= B || t < indptr[b] ? NO_SEQ : b;
 }

@@ -173,6 +173,42 @@ def test_scale_out_of_range_is_nan(dev, ns):
         check_chunk(c, out, lse, ref, True)
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("ns", [1, 2])
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
+def test_values_that_are_not_finite_stay_with_their_tokens(dev, fp8, ns, value):
+    """A row with a NaN or infinity, in NoPE or RoPE: the tokens of the same block of rows that do not
+    attend it are as if it were not there."""
+    g = gen(15, dev)
+    for place in (3, 515):
+        c = Chunk(g, [9, 4], [300, 70], 64)
+        q, kv = bf16(g, c.T, 16, 576), cache_of(g, c, fp8)
+        ref = attend64(c, q, kv, True)
+        hit = c.row(0, 295)                                     # tokens 4 .. 8 are positions 295 .. 299
+        if fp8 and place < 512:
+            kv[hit, place] = 0x7F                               # e4m3 has no infinity
+        else:
+            rope = kv[:, 528:].view(torch.bfloat16) if fp8 else kv
+            rope[hit, place - 512 if fp8 else place] = float(value)
+        out, lse = run(c, q, kv, num_splits=ns)
+        if value == "nan":
+            assert bool(torch.isnan(out[4:9]).all()) and bool(torch.isnan(lse[4:9]).all())
+        for x in ref[:2]:
+            x[4:9] = float("nan")
+        out[4:9], lse[4:9] = float("nan"), float("nan")
+        check_chunk(c, out, lse, ref, fp8, f"{place} {value}")
+
+
+def test_scale_must_be_positive_and_finite(dev):
+    g = gen(16, dev)
+    c = Chunk(g, [2], [70], 64)
+    q, kv = bf16(g, 2, 16, 576), cache_of(g, c, False)
+    for scale in (0.0, -0.1, math.inf, math.nan):
+        with pytest.raises(abi.DsaError) as e:
+            dsa.mla_chunk(q, kv, c.indptr, c.seq_lens, scale, **c.kw)
+        assert e.value.code == -3
+
+
 def test_cache_past_two_gigabytes(dev):
     """Rows whose byte offset passes 32 bits."""
     g = gen(11, dev)
