@@ -186,7 +186,7 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  *            (workspace: num_splits x T x H x 513 floats) a combine merges.
  * Scores and sums are fp32.  Probabilities are rounded to 16 bits for the
  * product with V (bf16; fp16 for DSA_KV_FP8_656).  656-byte rows: scores use
- * their exact values; V is rounded to fp16 and every scale must lie in [0, 128),
+ * their exact values; V is rounded to fp16 (its scale's mantissa first) and every scale must lie in [0, 128),
  * a token that attends a row with another scale getting NaN, as in dsa_mla.h.
  * The split count and so the last bits depend on the call's sizes alone; one
  * call repeats its bits.

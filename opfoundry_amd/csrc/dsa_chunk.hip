@@ -52,94 +52,6 @@ __device__ __forceinline__ int64_t limit_of(const ChunkParams& p, int32_t b, int
     return lim < 0 ? 0 : lim;
 }
 
-// One workgroup per (token, head, split): each wave takes every fourth position,
-// a lane 8 NoPE values and one RoPE value; the four waves' sums are joined in LDS.
-template <int FMT>
-__global__ void __launch_bounds__(NTHR) dsa_mla_chunk_row_kernel(const ChunkParams p) {
-    __shared__ float s_o[NWAVE][D_VO];
-    __shared__ float s_m[NWAVE], s_l[NWAVE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = (int)(blockIdx.x / (unsigned)p.H), h = (int)(blockIdx.x % (unsigned)p.H), split = blockIdx.y;
-    const int32_t b = seq_of(p.indptr, p.B, t);
-    if (b == NO_SEQ) return;
-    const int64_t limit = limit_of(p, b, t);
-    const bool too_long = p.lens[b] > p.max_len;
-    const int64_t k0 = (int64_t)split * p.per_split, k1 = min(limit, k0 + p.per_split);
-    float q[9], o[8] = {};
-    const __bf16* qp = p.q + (int64_t)t * p.q_st + (int64_t)h * p.q_sh;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = (float)qp[8 * lane + i];
-    q[8] = (float)qp[512 + lane];
-    float m = -INFINITY, l = 0.0f;
-    bool bad = false;
-    for (int64_t j = k0 + wave; j < k1; j += NWAVE) {
-        const int64_t row = dsa_seq::row_of(p.pages, b, j, p.rows);
-        if (row < 0) continue;
-        const unsigned char* r = p.kv + row * p.row_bytes;
-        float k[9];
-        if constexpr (FMT == DSA_KV_BF16) {
-            const __bf16* rb = (const __bf16*)r;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = (float)rb[8 * lane + i];
-            k[8] = (float)rb[512 + lane];
-        } else {
-            const u32x2 c = *reinterpret_cast<const u32x2*>(r + 8 * lane);
-            const float sc = *reinterpret_cast<const float*>(r + 512 + 4 * (lane >> 4));
-            bad |= __builtin_amdgcn_ballot_w64(__float_as_uint(sc) >= FP8_SCALE_LIMIT_BITS) != 0;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], true);
-                k[4 * w] = lo[0] * sc, k[4 * w + 1] = lo[1] * sc, k[4 * w + 2] = hi[0] * sc, k[4 * w + 3] = hi[1] * sc;
-            }
-            k[8] = (float)reinterpret_cast<const __bf16*>(r + 528)[lane];
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 9; ++i) s = __builtin_fmaf(q[i], k[i], s);
-        s = wave_sum(s) * p.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float a = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(s - mn);
-        l = l * a + e;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(e, k[i], o[i] * a);
-        m = mn;
-    }
-    const bool any = l != 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s_o[wave][8 * lane + i] = o[i];
-    if (lane == 0) s_m[wave] = any ? m : -INFINITY, s_l[wave] = bad || too_long ? __builtin_nanf("") : l;
-    __syncthreads();
-    float mm = -INFINITY, ll = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NWAVE; ++w) mm = fmaxf(mm, s_m[w]);
-    float f[NWAVE];
-#pragma unroll
-    for (int w = 0; w < NWAVE; ++w) {
-        f[w] = s_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w] - mm);
-        ll += s_l[w] * (s_l[w] == s_l[w] ? f[w] : 1.0f);
-    }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    const float lse = (mm + __builtin_amdgcn_logf(ll)) * LN2;
-    const int d = 2 * threadIdx.x;
-    float v[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NWAVE; ++w) x += f[w] == 0.0f ? 0.0f : s_o[w][d + i] * f[w];
-        v[i] = x * inv;
-    }
-    if (p.ns > 1) {
-        const int64_t at = ((int64_t)split * p.T + t) * p.H + h;
-        p.part_o[at * D_VO + d] = v[0], p.part_o[at * D_VO + d + 1] = v[1];
-        if (threadIdx.x == 0) p.part_lse[at] = ll == 0.0f ? -FLT_MAX : lse;
-    } else {
-        __bf16* op = p.out + (int64_t)t * p.o_st + (int64_t)h * p.o_sh;
-        op[d] = (__bf16)v[0], op[d + 1] = (__bf16)v[1];
-        if (threadIdx.x == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = ll == 0.0f ? INFINITY : lse;
-    }
-}
-
 // ---------------------------------------------------------------------------
 // The tiled kernel: one workgroup per 128 rows and split.  A row is one head of
 // one token; a block holds 128 consecutive rows of one sequence (token-major), so
@@ -165,6 +77,17 @@ constexpr int TILE_BYTES = ROPE_OFF + TILE * 128;
 constexpr int P_BYTES = 2 * NWAVE * 64 * 16;
 constexpr int KS_NOPE = 32, KS = 36;         // 16-deep k-steps of NoPE, and with RoPE
 constexpr int LPW = TILE / NWAVE + 1;        // loads of a wave and tile
+// 656-byte rows: the rows as they lie in the cache, back to back (41 pieces of 16 bytes each), three
+// tiles of them; V in two tiles of fp16 NoPE values in the layout above.
+constexpr int FP8_ROW = DSA_MLA_FP8_ROW_BYTES;
+constexpr int RAW_PIECES = TILE * FP8_ROW / 16;          // 1312
+constexpr int RAW_LOADS = (RAW_PIECES + 63) / 64;        // 21 loads of 1 KB
+constexpr int RAW_BYTES = RAW_LOADS * 1024;
+constexpr int RAW_LPW = (RAW_LOADS + NWAVE - 1) / NWAVE; // of wave 0 (6); the others 5
+static_assert(RAW_LOADS == NWAVE * (RAW_LPW - 1) + 1 && RAW_PIECES % 64 == 32, "the last load is wave 0's, half of it spare");
+constexpr int V_BYTES = TILE * NOPE_STRIDE;
+constexpr int K8S = 8;                                   // 64-deep k-steps of NoPE
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ int nope_sw(int r) { return (r >> 2) & 3; }
 __device__ __forceinline__ int rope_sw(int r) { return (r >> 1) & 7; }
 
@@ -174,9 +97,22 @@ __device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
 // O += A B on an accumulation register tile; the wait states before it (a vector write of
 // an operand: two) and around accesses of O from outside (o_fence) are written out, since
 // the compiler does not see a matrix instruction here.
+template <bool F16>
 __device__ __forceinline__ void mfma_o(f32x16& acc, u32x4 a, u32x4 b) {
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    if constexpr (F16)
+        asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    else
+        asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
+// e4m3 x e4m3, 32x32x64, B times 2^(eb - 127)
+__device__ __forceinline__ f32x16 mfma_fp8(i32x8 a, i32x8 b, f32x16 c, int eb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0x7F7F7F7F, 0, eb);
+}
+__device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
+    return __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ float bf16_lo(unsigned w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(unsigned w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ void o_fence(f32x16 (&o)[16]) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
                  : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]),
@@ -213,9 +149,12 @@ __device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k
 // the kernel's argument block, in the constant address space
 typedef const __attribute__((address_space(4))) ChunkParams* Args;
 
+template <int FMT>
 __global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(1, 1)))
 dsa_mla_chunk_tile_kernel(const ChunkParams p) {
-    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[3 * TILE_BYTES];
+    constexpr bool FP8 = FMT == DSA_KV_FP8_656;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[FP8 ? 2 * V_BYTES + 3 * RAW_BYTES : 3 * TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float s_scale[FP8 ? 2 * 4 * TILE : 4];    // [tile % 2][group][position]
     __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * P_BYTES];
     __shared__ __attribute__((aligned(16))) int32_t s_rows[SPAN];     // cache rows of a span's positions
     __shared__ uint32_t s_skip[SPAN / TILE];                          // bit j: position j of the tile has no row
@@ -252,11 +191,65 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int row = blk.r0 + min(32 * wave + r32, blk.rows - 1);
     const int tok = blk.first + row / p.H, head = row % p.H;
     const int limit = limit_in(p, blk, tok);
+    // bf16 rows: lane (hi, r32) holds dims 16 ks + 8 hi .. +7 of row r32 in qf[ks].
+    // 656-byte rows: NoPE in two e4m3 parts, q 2^-k = hi + lo / 16 with |q 2^-k| < 256: a bf16 value has 8
+    // significant bits and either part holds 4, so the two together are exact down to 2^-14 (2^-21 of the
+    // row's largest).  Dims 64 k8 + 32 hi .. +31: part hi in qf[2 k8], qf[2 k8 + 1], part lo 16 further on; the
+    // RoPE part, times 2^-k, in qf[32 ..].
     u32x4 qf[KS];
+    float c_s = p.scale_log2;
     {
-        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh + 8 * hi;
+        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh + (FP8 ? 32 : 8) * hi;
+        if constexpr (!FP8) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
+            for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
+        } else {
+            // (dims 64 k8 + 32 hi + 8 i in qf[4 k8 + i] first)
+#pragma unroll
+            for (int i = 0; i < KS_NOPE; ++i) qf[i] = *reinterpret_cast<const u32x4*>(qp + 64 * (i >> 2) + 8 * (i & 3));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qf[KS_NOPE + i] = *reinterpret_cast<const u32x4*>(qp - 24 * hi + 512 + 16 * i);
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            auto top = [&](int from, int to) {
+                u16x2 m = {0, 0};
+#pragma unroll
+                for (int i = from; i < to; ++i)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, qf[i][w] & 0x7FFF7FFFu));
+                const int e = max((int)m[0], (int)m[1]) >> 7;       // biased exponent of the largest
+                return max(e, __shfl_xor(e, 32, 64));
+            };
+            const int e_nope = top(0, KS_NOPE), e_rope = top(KS_NOPE, KS);
+            const int k = max(max(e_nope - 134, e_rope - 187), -100);
+            const float down = __uint_as_float((unsigned)(127 - k) << 23);
+            // (a row with an infinity or NaN among its values has NaN scores)
+            c_s = max(e_nope, e_rope) == 255 ? __builtin_nanf("") : c_s * __uint_as_float((unsigned)(127 + k) << 23);
+#pragma unroll
+            for (int i = KS_NOPE; i < KS; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const f32x2 v = {bf16_lo(qf[i][w]) * down, bf16_hi(qf[i][w]) * down};
+                    qf[i][w] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+                }
+            u32x4 part[KS_NOPE];
+#pragma unroll
+            for (int i = 0; i < KS_NOPE; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; w += 2) {
+                    float v[4] = {bf16_lo(qf[i][w]) * down, bf16_hi(qf[i][w]) * down, bf16_lo(qf[i][w + 1]) * down,
+                                  bf16_hi(qf[i][w + 1]) * down};
+                    int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+                    c = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], c, true);
+                    const f32x2 l = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), h = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+                    int d = __builtin_amdgcn_cvt_pk_fp8_f32((v[0] - l[0]) * 16.0f, (v[1] - l[1]) * 16.0f, 0, false);
+                    d = __builtin_amdgcn_cvt_pk_fp8_f32((v[2] - h[0]) * 16.0f, (v[3] - h[1]) * 16.0f, d, true);
+                    // bytes 8 i + 2 w .. of the lane's 256: word 2 i + w / 2
+                    part[(2 * i + (w >> 1)) >> 2][(2 * i + (w >> 1)) & 3] = (unsigned)c;
+                    part[16 + ((2 * i + (w >> 1)) >> 2)][(2 * i + (w >> 1)) & 3] = (unsigned)d;
+                }
+#pragma unroll
+            for (int i = 0; i < KS_NOPE; ++i) qf[i] = part[i];
+        }
     }
 
     // ---- positions [c0, c0 + SPAN) below k1 -> cache rows ----
@@ -319,66 +312,150 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         __syncthreads();
     };
 
-    // ---- tile i of the span -> buffer `slot`: wave w rows 8 w .. 8 w + 7 and their RoPE ----
-    auto slot_of = [&](int s) -> lds_ptr { return T0 + s * TILE_BYTES; };
+    // ---- tile i of the span -> buffer `slot`.  bf16: wave w rows 8 w .. 8 w + 7 and their RoPE;
+    // 656-byte rows: the tile's pieces, load k = w, w + 4, .. of wave w ----
+    auto slot_of = [&](int s) -> lds_ptr { return T0 + s * (FP8 ? V_BYTES : TILE_BYTES); };
+    auto raw_of = [&](int s) -> lds_ptr { return T0 + 2 * V_BYTES + s * RAW_BYTES; };
     struct Rows {
         int32_t r[8];
         int32_t rope;
     };
+    // 656-byte rows whose tile is one run of the cache (dense rows, pages of whole tiles): a load's source
+    // is the run's start plus its number and the lane
+    const bool runs = FP8 && p.row_bytes == FP8_ROW && (!p.pages.table || p.pages.block_size % TILE == 0);
     auto load_rows = [&](int i) -> Rows {
-        const LDS_AS int32_t* at = rows_l + i * TILE + 8 * wave;
-        const u32x4 a = lds_ld<u32x4>((lds_cptr)at), b = lds_ld<u32x4>((lds_cptr)(at + 4));
-        Rows g;
+        Rows g{};
+        if constexpr (!FP8) {
+            const LDS_AS int32_t* at = rows_l + i * TILE + 8 * wave;
+            const u32x4 a = lds_ld<u32x4>((lds_cptr)at), b = lds_ld<u32x4>((lds_cptr)(at + 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            g.r[e] = __builtin_amdgcn_readfirstlane((int)a[e]);
-            g.r[4 + e] = __builtin_amdgcn_readfirstlane((int)b[e]);
+            for (int e = 0; e < 4; ++e) {
+                g.r[e] = __builtin_amdgcn_readfirstlane((int)a[e]);
+                g.r[4 + e] = __builtin_amdgcn_readfirstlane((int)b[e]);
+            }
+            g.rope = at[opaque(lane) >> 3];
+        } else {
+            g.r[0] = runs && __builtin_amdgcn_readfirstlane(s_skip[i]) == 0 ? __builtin_amdgcn_readfirstlane(rows_l[i * TILE]) : -1;
+            g.r[1] = i;
         }
-        g.rope = at[opaque(lane) >> 3];
         return g;
     };
     auto issue = [&](const Rows& g, int slot) {
         const int ln = opaque(lane);
-        const lds_ptr tb = slot_of(slot);
+        if constexpr (!FP8) {
+            const lds_ptr tb = slot_of(slot);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int r = 8 * wave + e;
-            const unsigned char* base = p.kv + (uint64_t)(uint32_t)g.r[e] * (uint32_t)p.row_bytes;
-            lds_dma16_s(base, 16u * (unsigned)(ln ^ nope_sw(r)), tb + r * NOPE_STRIDE);
+            for (int e = 0; e < 8; ++e) {
+                const int r = 8 * wave + e;
+                const unsigned char* base = p.kv + (uint64_t)(uint32_t)g.r[e] * (uint32_t)p.row_bytes;
+                lds_dma16_s(base, 16u * (unsigned)(ln ^ nope_sw(r)), tb + r * NOPE_STRIDE);
+            }
+            const int r = 8 * wave + (ln >> 3);
+            lds_dma16(p.kv + (uint64_t)(uint32_t)g.rope * (uint32_t)p.row_bytes + 1024 + 16 * ((ln & 7) ^ rope_sw(r)),
+                      tb + ROPE_OFF + 8 * wave * 128);
+        } else {
+            // load k takes pieces 64 k .. +63; the last one's spare lanes repeat one of its pieces into the
+            // slot's padding
+            const lds_ptr rb = raw_of(slot) + 1024 * wave;
+            if (g.r[0] >= 0) {
+                const unsigned char* base = p.kv + (uint64_t)(uint32_t)g.r[0] * FP8_ROW + 1024 * wave;
+#pragma unroll
+                for (int e = 0; e < RAW_LPW - 1; ++e) lds_dma16_s(base + 1024 * NWAVE * e, 16u * ln, rb + 1024 * NWAVE * e);
+                if (wave == 0)
+                    lds_dma16_s(base + 1024 * (RAW_LOADS - 1), 16u * (ln & 31), rb + 1024 * (RAW_LOADS - 1));
+            } else {
+                // piece / 41 is its row in the tile
+                const int i = g.r[1];
+#pragma unroll 1
+                for (int k = wave; k < RAW_LOADS; k += NWAVE) {
+                    const unsigned piece = min(64u * k + ln, (unsigned)RAW_PIECES - 1), rt = piece / 41u;
+                    const uint32_t row = (uint32_t)rows_l[i * TILE + (int)rt];
+                    lds_dma16(p.kv + ((uint64_t)row * (uint32_t)p.row_bytes + 16u * (piece - 41u * rt)),
+                              raw_of(slot) + 1024 * k);
+                }
+            }
         }
-        const int r = 8 * wave + (ln >> 3);
-        lds_dma16(p.kv + (uint64_t)(uint32_t)g.rope * (uint32_t)p.row_bytes + 1024 + 16 * ((ln & 7) ^ rope_sw(r)),
-                  tb + ROPE_OFF + 8 * wave * 128);
     };
 
     // In a tile that some row of the block does not attend whole, a row of the cache may hold anything,
     // and 0 x NaN is NaN: one with a NaN or infinity among its NoPE values is cleared, and the scores of
-    // those that do attend it become NaN.  (A wave looks at the rows that it loaded.)
+    // those that do attend it become NaN.  (bf16: a wave looks at the rows that it loaded.)
     auto scan = [&](int i, int slot) {
         const int ln = opaque(lane);
-        const lds_ptr tb = slot_of(slot) + 8 * wave * NOPE_STRIDE + 16 * ln;
         uint32_t bad = 0;
+        if constexpr (!FP8) {
+            const lds_ptr tb = slot_of(slot) + 8 * wave * NOPE_STRIDE + 16 * ln;
+#pragma unroll 2
+            for (int e = 0; e < 8; ++e) {
+                const u32x4 v = lds_ld<u32x4>(tb + e * NOPE_STRIDE);
+                bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const u32x4 v = lds_ld<u32x4>(tb + e * NOPE_STRIDE);
-            bool odd = false;
+                for (int w = 0; w < 4; ++w) odd |= (v[w] & 0x7F800000u) == 0x7F800000u || (v[w] & 0x7F80u) == 0x7F80u;
+                if (__builtin_amdgcn_ballot_w64(odd)) {
+                    lds_st<u32x4>(tb + e * NOPE_STRIDE, u32x4{0, 0, 0, 0});
+                    bad |= 1u << e;
+                }
+            }
+        } else {
+            // two rows of 32 pieces a read: e4m3 has no infinity, and its NaN has all bits but the sign set
+            const lds_ptr tb = raw_of(slot) + (8 * wave + (ln >> 5)) * FP8_ROW + 16 * (ln & 31);
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const u32x4 v = lds_ld<u32x4>(tb + 2 * e * FP8_ROW);
+                unsigned odd = 0;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) odd |= (v[w] & 0x7F800000u) == 0x7F800000u || (v[w] & 0x7F80u) == 0x7F80u;
-            if (__builtin_amdgcn_ballot_w64(odd)) {
-                lds_st<u32x4>(tb + e * NOPE_STRIDE, u32x4{0, 0, 0, 0});
-                bad |= 1u << e;
+                for (int w = 0; w < 4; ++w) odd |= ((v[w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                const uint64_t who = __builtin_amdgcn_ballot_w64(odd != 0);
+                const bool lo = (uint32_t)who != 0, up = (who >> 32) != 0;
+                if (ln < 32 ? lo : up) lds_st<u32x4>(tb + 2 * e * FP8_ROW, u32x4{0, 0, 0, 0});
+                bad |= (lo ? 1u : 0u) << (2 * e) | (up ? 2u : 0u) << (2 * e);
             }
         }
         if (bad && ln == 0) reinterpret_cast<unsigned char*>(s_nan)[4 * i + wave] = (unsigned char)bad;
+    };
+
+    // ---- 656-byte rows: V of the raw tile -> fp16.  Piece g = 4 u + m of wave w is rows 16 u .. +15, dims
+    // 128 w + 32 m .. +31, the V block that its own PV group (u, m) reads: a buffer is refilled by its readers.
+    // v_cvt_scalef32 applies the power of two of the row's scale exactly, the product its mantissa (both in
+    // fp16).  The scales go to s_scale for the scores; one outside [0, 128) is NaN there, and its row 0 in V.
+    struct Piece {
+        u32x2 codes;
+        float scale;
+    };
+    auto deq_load = [&](lds_cptr rb, int g) -> Piece {
+        const int ln = opaque(lane);
+        const lds_cptr r = rb + (16 * (g >> 2) + (ln >> 2)) * FP8_ROW;
+        return Piece{lds_ld<u32x2>(r + 128 * wave + 32 * (g & 3) + 8 * (ln & 3)), lds_ld<float>(r + 512 + 4 * wave)};
+    };
+    auto deq_store = [&](lds_ptr vb, int par, int g, const Piece& d) {
+        const int ln = opaque(lane);
+        const int r = 16 * (g >> 2) + (ln >> 2), ch = 16 * wave + 4 * (g & 3) + (ln & 3);
+        const unsigned bits = __float_as_uint(d.scale);
+        const bool bad = bits >= FP8_SCALE_LIMIT_BITS;
+        const float sc = bad ? 0.0f : d.scale;
+        if ((g & 3) == 0 && (ln & 3) == 0)
+            *(LDS_AS float*)&s_scale[(4 * par + wave) * TILE + r] = bad ? __builtin_nanf("") : d.scale;
+        const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(sc) & 0x007FFFFFu) | 0x3F800000u);
+        const f16x2 mm = {m16, m16};
+        const u32x4 v = {
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[0], sc, false) * mm),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[0], sc, true) * mm),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[1], sc, false) * mm),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[1], sc, true) * mm)};
+        lds_st<u32x4>(vb + r * NOPE_STRIDE + 16 * (ch ^ nope_sw(r)), v);
+    };
+    auto dequant = [&](lds_cptr rb, lds_ptr vb, int par) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) deq_store(vb, par, g, deq_load(rb, g));
     };
 
     auto landed = [&](auto keep) {
         wait_vm<decltype(keep)::value>();
         asm volatile("" ::: "memory");
     };
-    const float c_s = p.scale_log2;
     f32x16 o[16];
     float m_ref = 0.0f, l_lane = 0.0f;
+    float p_top = 0.0f;          // 656-byte rows: the largest P (fp16 holds up to 2^16)
     bool first_tile = true, any = false;
 
     auto qk = [&](lds_cptr kt) -> f32x16 {
@@ -403,6 +480,50 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         }
         __builtin_amdgcn_sched_barrier(0);
         return acc;
+    };
+    // ---- 656-byte rows: S^T from the raw codes.  The scale of 128 dims is a position's own, so each group
+    // has a chain of its own: S = sum_g scale_g (K_g (hi + lo / 16)) + K_rope q_rope ----
+    auto qk8 = [&](lds_cptr raw, int par) -> f32x16 {
+        const int ln = opaque(lane), lhi = ln >> 5, lr = ln & 31;
+        const lds_cptr kn = raw + lr * FP8_ROW + 32 * lhi;
+        const lds_cptr kr = raw + lr * FP8_ROW + 528 + 16 * lhi;
+        const lds_cptr sc = (lds_cptr)(LDS_AS float*)&s_scale[4 * par * TILE] + 16 * lhi;
+        auto k_frag = [&](int k8) { return join8(lds_ld<u32x4>(kn + 64 * k8), lds_ld<u32x4>(kn + 64 * k8 + 16)); };
+        i32x8 kb[2] = {k_frag(0), k_frag(1)};
+        f32x16 s = {};
+        u32x4 rb[2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            f32x16 a = {};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k8 = 2 * g + h;
+                __builtin_amdgcn_sched_barrier(0);
+                a = mfma_fp8(kb[h], join8(qf[2 * k8], qf[2 * k8 + 1]), a, 127);
+                a = mfma_fp8(kb[h], join8(qf[16 + 2 * k8], qf[16 + 2 * k8 + 1]), a, 123);
+                if (k8 + 2 < K8S) kb[h] = k_frag(k8 + 2);
+                else rb[h] = lds_ld<u32x4>(kr + 32 * h);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const f32x4 f0 = lds_ld<f32x4>(sc + 4 * TILE * g + 32 * i), f1 = lds_ld<f32x4>(sc + 4 * TILE * g + 32 * i + 32);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[4 * i + r] = __builtin_fmaf(a[4 * i + r], f0[r], s[4 * i + r]);
+                    s[4 * i + 4 + r] = __builtin_fmaf(a[4 * i + 4 + r], f1[r], s[4 * i + 4 + r]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            s = mfma_bf16(rb[j & 1], qf[KS_NOPE + j], s);
+            if (j < 2) rb[j & 1] = lds_ld<u32x4>(kr + 32 * (j + 2));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return s;
     };
     auto masked = [&](int i, int c0) { return c0 + (i + 1) * TILE > lim_lo || __builtin_amdgcn_readfirstlane(s_skip[i]) != 0; };
     // lane (hi, r32), register r: position 8 (r / 4) + 4 hi + r % 4 of the tile, row r32 of the wave
@@ -437,6 +558,17 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 #pragma unroll
         for (int r = 8 * u; r < 8 * u + 8; ++r) lt += e[r];
         l_lane += lt;
+        if constexpr (FP8) {
+            u32x4 h;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const f16x2 v = {(_Float16)e[8 * u + 2 * w], (_Float16)e[8 * u + 2 * w + 1]};
+                h[w] = __builtin_bit_cast(unsigned, v);
+                p_top = fmaxf(p_top, fmaxf(e[8 * u + 2 * w], e[8 * u + 2 * w + 1]));
+            }
+            lds_st<u32x4>(px + ((u * NWAVE + wave) * 64 + ln) * 16, h);
+            return;
+        }
         const f32x8 a = {e[8 * u], e[8 * u + 1], e[8 * u + 2], e[8 * u + 3], e[8 * u + 4], e[8 * u + 5], e[8 * u + 6], e[8 * u + 7]};
         lds_st<u32x4>(px + ((u * NWAVE + wave) * 64 + ln) * 16, __builtin_bit_cast(u32x4, __builtin_convertvector(a, bf16x8)));
     };
@@ -453,8 +585,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         p_half(e, 0, px);
         p_half(e, 1, px);
     };
-    auto pv = [&](lds_cptr vt, lds_cptr px, const f32x16& sn, float* en, auto with_exp) {
-        const int ln = lane, lhi = ln >> 5;
+    // (656-byte rows, with_exp: the next tile but one, raw at draw, goes to V's own buffer, piece by piece)
+    auto pv = [&](lds_ptr vt, lds_cptr px, const f32x16& sn, float* en, auto with_exp, lds_cptr draw, int dpar) {
+        const int ln = FP8 ? opaque(lane) : lane, lhi = ln >> 5;
         const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
         const int vx = 2 * (g16 & 1) + (pp >> 1);
         const lds_cptr v_a = vt + (4 * lhi + rr) * NOPE_STRIDE + 16 * (vx ^ lhi) + 8 * (pp & 1) + 256 * wave;
@@ -474,13 +607,16 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             for (int m = 0; m < 4; ++m) {
                 __builtin_amdgcn_sched_barrier(0);
                 const u32x4 v_nxt = m + 1 < 4 ? v_frag(u, m + 1) : v_cur;
+                Piece d;
+                if constexpr (FP8 && decltype(with_exp)::value) d = deq_load(draw, 4 * u + m);
 #pragma unroll
-                for (int h = 0; h < NWAVE; ++h) mfma_o(o[4 * m + h], v_cur, pb[h]);
+                for (int h = 0; h < NWAVE; ++h) mfma_o<FP8>(o[4 * m + h], v_cur, pb[h]);
                 if constexpr (decltype(with_exp)::value) {
                     const int r0 = 8 * u + 2 * m;
                     en[r0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0], c_s, -m_ref));
                     en[r0 + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0 + 1], c_s, -m_ref));
                 }
+                if constexpr (FP8 && decltype(with_exp)::value) deq_store(vt, dpar, 4 * u + m, d);
                 v_cur = v_nxt;
             }
         }
@@ -491,14 +627,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // Pass 0; where its reference did not serve (rare): the largest score of every row, and the pass
     // again with that as the reference.
     for (bool again = false;;) {
+        // (0 x 0 + 0: cleared where they are, without the registers that zeros to copy would take)
+        const u32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < 16; ++m) o[m] = f32x16{};
+        for (int m = 0; m < 16; ++m)
+            asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(o[m]) : "v"(zero));
         o_fence(o);
         l_lane = 0.0f;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = k0 + c * SPAN;
             resolve(c0);
             if (ntiles == 0) continue;
+            if constexpr (!FP8) {
             issue(load_rows(0), 0);
             if (ntiles > 1) issue(load_rows(1), 1);
             Rows next = load_rows(min(2, ntiles - 1));
@@ -523,7 +663,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 if (i + 3 < ntiles) next = load_rows(i + 3);
                 mask(sn, i + 1, c0);
                 float en[16];
-                pv(slot_of(cur), PX + (i & 1) * P_BYTES, sn, en, std::true_type{});
+                pv(slot_of(cur), PX + (i & 1) * P_BYTES, sn, en, std::true_type{}, T0, 0);
                 const lds_ptr px = PX + ((i + 1) & 1) * P_BYTES;
                 p_half(en, 0, px);
                 p_half(en, 1, px);
@@ -531,7 +671,51 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             }
             tile_barrier();
             float en[16];
-            pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{});
+            pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{}, T0, 0);
+            } else {
+                // Iteration j: scores of tile j from raw slot j % 3; PV of tile j - 1 from V buffer (j - 1) % 2,
+                // with the exponentials of tile j and the conversion of tile j + 1 into that buffer.
+                auto ready = [&](int i) {          // tile i lies whole in its slot
+                    landed(std::integral_constant<int, 0>{});
+                    tile_barrier();
+                    if (i < ntiles && masked(i, c0)) {
+                        scan(i, i % 3);
+                        tile_barrier();
+                    }
+                };
+                issue(load_rows(0), 0);
+                ready(0);
+                if (ntiles > 1) issue(load_rows(1), 1);
+                dequant(raw_of(0), slot_of(0), 0);
+                Rows next = load_rows(min(2, ntiles - 1));
+                ready(1);
+                if (ntiles > 2) issue(next, 2);
+                f32x16 s0 = qk8(raw_of(0), 0);
+                next = load_rows(min(3, ntiles - 1));
+                mask(s0, 0, c0);
+                p_first(s0, PX);
+                if (ntiles > 1) dequant(raw_of(1), slot_of(1), 1);
+                for (int j = 1; j < ntiles; ++j) {
+                    // (the barrier also shows tile j's V and scales and tile j - 1's P, and every wave is
+                    // done with tile j - 1's raw slot, which takes tile j + 2)
+                    ready(j + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j + 2 < ntiles) issue(next, (j + 2) % 3);
+                    __builtin_amdgcn_sched_barrier(0);
+                    f32x16 sn = qk8(raw_of(j % 3), j & 1);
+                    if (j + 3 < ntiles) next = load_rows(j + 3);
+                    mask(sn, j, c0);
+                    float en[16];
+                    pv(slot_of((j - 1) & 1), PX + ((j - 1) & 1) * P_BYTES, sn, en, std::true_type{}, raw_of((j + 1) % 3),
+                       (j + 1) & 1);
+                    const lds_ptr px = PX + (j & 1) * P_BYTES;
+                    p_half(en, 0, px);
+                    p_half(en, 1, px);
+                }
+                tile_barrier();
+                float en[16];
+                pv(slot_of((ntiles - 1) & 1), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{}, T0, 0);
+            }
         }
         o_fence(o);
         if (again) break;
@@ -539,10 +723,12 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         // tile's maximum it is at least 1; it grows past 2^100 only where later scores do.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
         const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
+        const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
         __syncthreads();
         if (wave == 0) s_misc[1] = 0;
         __syncthreads();
-        if (have && !(l > 0x1p-40f && l < 0x1p100f)) s_misc[1] = 1;
+        const bool held = FP8 ? top_p >= 0.5f && top_p < 0x1p15f : l > 0x1p-40f;
+        if (have && !(held && l < 0x1p100f)) s_misc[1] = 1;
         __syncthreads();
         if (__builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
         again = true;
@@ -553,9 +739,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             for (int i = 0; i < ntiles; ++i) {
                 issue(load_rows(i), 0);
                 landed(std::integral_constant<int, 0>{});
-                if (masked(i, c0)) scan(i, 0);
-                tile_barrier();
-                f32x16 s = qk(slot_of(0));
+                f32x16 s;
+                if constexpr (FP8) {
+                    tile_barrier();
+                    if (masked(i, c0)) scan(i, 0);
+                    dequant(raw_of(0), slot_of(0), 0);
+                    tile_barrier();
+                    s = qk8(raw_of(0), 0);
+                } else {
+                    if (masked(i, c0)) scan(i, 0);
+                    tile_barrier();
+                    s = qk(slot_of(0));
+                }
                 mask(s, i, c0);
                 top = fmaxf(top, top_of(s));
                 tile_barrier();
@@ -786,12 +981,11 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
-    const dim3 grid((unsigned)((int64_t)a->T * a->H), (unsigned)p.ns);
     const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, BLOCK), (unsigned)p.ns);
     if (a->kv_format == DSA_KV_BF16)
-        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_BF16>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(dsa_mla_chunk_row_kernel<DSA_KV_FP8_656>, grid, dim3(NTHR), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
     if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;
     if (p.ns > 1) {
         const int64_t rows = (int64_t)a->T * a->H;

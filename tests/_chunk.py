@@ -146,11 +146,12 @@ def latent64(rows):
 
 
 def attend64(c: Chunk, q, kv, causal, sm_scale=SM_SCALE, max_len=None):
-    """(O, LSE, A, E) in float64: A = sum p |v| / sum p, and E the bound of a score's fp32 error times 2
-    (relative error of a probability): 64 additions of 2^-24 of sum |q k|, each row's largest."""
+    """(O, LSE, A, E, N) in float64: A = sum p |v| / sum p, E the bound of a score's fp32 error times 2
+    (relative error of a probability): 64 additions of 2^-24 of sum |q k|, each row's largest; N = sum |v|."""
     T, H, _ = q.shape
     dev = q.device
     o = torch.full((T, H, 512), float("nan"), dtype=torch.float64, device=dev)
+    N = torch.zeros_like(o)
     A, lse, E = torch.zeros_like(o), torch.full((T, H), float("nan"), dtype=torch.float64, device=dev), \
         torch.zeros((T, H), dtype=torch.float64, device=dev)
     t = c.first
@@ -172,26 +173,27 @@ def attend64(c: Chunk, q, kv, causal, sm_scale=SM_SCALE, max_len=None):
                 s = (x @ k[:m].t().contiguous()) * sm_scale
                 lse[t] = torch.logsumexp(s, 1)
                 p = torch.exp(s - lse[t][:, None])
+                N[t] = k[:m, :512].abs().sum(0)
                 o[t], A[t] = p @ k[:m, :512].contiguous(), p @ k[:m, :512].abs().contiguous()
                 big = (x.abs() @ k[:m].abs().t().contiguous()).amax(1) * abs(sm_scale)
                 E[t] = 2 * 64 * 2.0 ** -24 * big
             t += 1
-    return o, lse, A, E
+    return o, lse, A, E, N
 
 
 def check_chunk(c: Chunk, out, lse, ref, fp8, what=""):
-    """Bound of O: P rounded (2^-8; fp16 2^-11), V rounded to fp16 (656-byte rows: 2^-11 and 2^-25 below
-    fp16's normal range), the output rounded (2^-8 |O|), fp32 sums of up to 2^6 partial sums a split, the
-    scores' error E.  LSE: E and 2^-20 of itself and 1."""
-    o, l, A, E = ref
+    """Bound of O: P rounded (2^-8; fp16 2^-11), V rounded to fp16 (656-byte rows: the scale's mantissa and
+    its product with the code, 2^-11 each, and 2^-25 below fp16's normal range), the output rounded
+    (2^-8 |O|), fp32 sums of up to 2^6 partial sums a split, the scores' error E.  LSE: E and 2^-20 of itself and 1."""
+    o, l, A, E, N = ref
     own = torch.zeros(c.T, dtype=torch.bool, device=out.device)
     own[c.first:c.first + sum(c.new)] = True
     g, gl = out.double(), lse.double()
-    g, gl, o, l, A, E = g[own], gl[own], o[own], l[own], A[own], E[own]
+    g, gl, o, l, A, E, N = g[own], gl[own], o[own], l[own], A[own], E[own], N[own]
     assert torch.equal(torch.isnan(g), torch.isnan(o)), f"{what}: NaN where none is due, or none where one is"
     assert torch.equal(torch.isnan(gl), torch.isnan(l)) and torch.equal(torch.isinf(gl), torch.isinf(l)), what
-    rel = (2.0 ** -11 + 2.0 ** -11 if fp8 else 2.0 ** -8) + 2.0 ** -17
-    bound = (rel + E[..., None]) * A + 2.0 ** -8 * o.abs() + (2.0 ** -24 if fp8 else 0.0)
+    rel = (3 * 2.0 ** -11 if fp8 else 2.0 ** -8) + 2.0 ** -17
+    bound = (rel + E[..., None]) * A + 2.0 ** -8 * o.abs() + (2.0 ** -24 * (1 + N) if fp8 else 0.0)
     fin = torch.isfinite(o)
     over = ((g - o).abs() / bound.clamp(min=1e-300))[fin & (bound > 0)]
     assert over.numel() == 0 or float(over.max()) <= 1, f"{what}: O off by {float(over.max())} of its bound"

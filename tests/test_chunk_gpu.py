@@ -276,10 +276,10 @@ def test_agrees_with_the_sparse_decode_of_every_position(dev, fp8):
     # fp16 2^-11), fp16 V twice (656-byte rows), the fp32 error E of both scores, and for the sparse path's
     # K in fp16 scores off by up to 2^-11 of big = max_j sum |q k| sm_scale (E = 2^-17 big), which a
     # probability and its sum both carry.
-    o, l, A, E = ref
+    o, l, A, E, N = ref
     k16 = 2.0 ** -11 * E * 2.0 ** 17 if fp8 else torch.zeros_like(E)
     rel = 4 * 2.0 ** -11 if fp8 else 2 * 2.0 ** -8
-    bound = (rel + 2.0 ** -16 + 2 * E + 2 * k16)[..., None] * A + 2 * 2.0 ** -8 * o.abs() + 2.0 ** -23
+    bound = (rel + 2.0 ** -16 + 2 * E + 2 * k16)[..., None] * A + 2 * 2.0 ** -8 * o.abs() + 2.0 ** -23 * (1 + N)
     assert bool(((od.view(c.T, H, 512).double() - out.double()).abs() <= bound).all())
     assert bool(((ld.view(c.T, H).double() - lse.double()).abs() <= 2 * E + k16 + 2.0 ** -19 * (1 + l.abs())).all())
 
