@@ -86,8 +86,6 @@ constexpr int RAW_BYTES = RAW_LOADS * 1024;
 constexpr int RAW_LPW = (RAW_LOADS + NWAVE - 1) / NWAVE; // of wave 0 (6); the others 5
 static_assert(RAW_LOADS == NWAVE * (RAW_LPW - 1) + 1 && RAW_PIECES % 64 == 32, "the last load is wave 0's, half of it spare");
 constexpr int V_BYTES = TILE * NOPE_STRIDE;
-constexpr int K8S = 8;                                   // 64-deep k-steps of NoPE
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ int nope_sw(int r) { return (r >> 2) & 3; }
 __device__ __forceinline__ int rope_sw(int r) { return (r >> 1) & 7; }
 
@@ -104,15 +102,13 @@ __device__ __forceinline__ void mfma_o(f32x16& acc, u32x4 a, u32x4 b) {
     else
         asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
-// e4m3 x e4m3, 32x32x64, B times 2^(eb - 127)
-__device__ __forceinline__ f32x16 mfma_fp8(i32x8 a, i32x8 b, f32x16 c, int eb) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0x7F7F7F7F, 0, eb);
+// 8 e4m3 codes -> 8 bf16 (exact)
+__device__ __forceinline__ u32x4 codes_bf16(unsigned c0, unsigned c1) {
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c0, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c0, 1.0f, true)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c1, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c1, 1.0f, true))};
 }
-__device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
-    return __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-__device__ __forceinline__ float bf16_lo(unsigned w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(unsigned w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ void o_fence(f32x16 (&o)[16]) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
                  : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]),
@@ -191,64 +187,16 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int row = blk.r0 + min(32 * wave + r32, blk.rows - 1);
     const int tok = blk.first + row / p.H, head = row % p.H;
     const int limit = limit_in(p, blk, tok);
-    // bf16 rows: lane (hi, r32) holds dims 16 ks + 8 hi .. +7 of row r32 in qf[ks].
-    // 656-byte rows: NoPE in two e4m3 parts, q 2^-k = hi + lo / 16 with |q 2^-k| < 256: a bf16 value has 8
-    // significant bits and either part holds 4, so the two together are exact down to 2^-14 (2^-21 of the
-    // row's largest).  Dims 64 k8 + 32 hi .. +31: part hi in qf[2 k8], qf[2 k8 + 1], part lo 16 further on; the
-    // RoPE part, times 2^-k, in qf[32 ..].
+    // Q: lane (hi, r32) holds 8 dims of row r32 in qf[ks], the k-step's half `hi`: dims 16 ks + 8 hi .. +7; of
+    // 656-byte rows, whose codes come 16 to a read, dims 32 j + 16 hi .. +15 in qf[2 j] and qf[2 j + 1] (the order
+    // of the dims within a pair of k-steps is free as long as K has the same)
     u32x4 qf[KS];
-    float c_s = p.scale_log2;
     {
-        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh + (FP8 ? 32 : 8) * hi;
-        if constexpr (!FP8) {
+        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
-        } else {
-            // (dims 64 k8 + 32 hi + 8 i in qf[4 k8 + i] first)
-#pragma unroll
-            for (int i = 0; i < KS_NOPE; ++i) qf[i] = *reinterpret_cast<const u32x4*>(qp + 64 * (i >> 2) + 8 * (i & 3));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qf[KS_NOPE + i] = *reinterpret_cast<const u32x4*>(qp - 24 * hi + 512 + 16 * i);
-            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-            auto top = [&](int from, int to) {
-                u16x2 m = {0, 0};
-#pragma unroll
-                for (int i = from; i < to; ++i)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, qf[i][w] & 0x7FFF7FFFu));
-                const int e = max((int)m[0], (int)m[1]) >> 7;       // biased exponent of the largest
-                return max(e, __shfl_xor(e, 32, 64));
-            };
-            const int e_nope = top(0, KS_NOPE), e_rope = top(KS_NOPE, KS);
-            const int k = max(max(e_nope - 134, e_rope - 187), -100);
-            const float down = __uint_as_float((unsigned)(127 - k) << 23);
-            // (a row with an infinity or NaN among its values has NaN scores)
-            c_s = max(e_nope, e_rope) == 255 ? __builtin_nanf("") : c_s * __uint_as_float((unsigned)(127 + k) << 23);
-#pragma unroll
-            for (int i = KS_NOPE; i < KS; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const f32x2 v = {bf16_lo(qf[i][w]) * down, bf16_hi(qf[i][w]) * down};
-                    qf[i][w] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
-                }
-            u32x4 part[KS_NOPE];
-#pragma unroll
-            for (int i = 0; i < KS_NOPE; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; w += 2) {
-                    float v[4] = {bf16_lo(qf[i][w]) * down, bf16_hi(qf[i][w]) * down, bf16_lo(qf[i][w + 1]) * down,
-                                  bf16_hi(qf[i][w + 1]) * down};
-                    int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-                    c = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], c, true);
-                    const f32x2 l = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), h = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-                    int d = __builtin_amdgcn_cvt_pk_fp8_f32((v[0] - l[0]) * 16.0f, (v[1] - l[1]) * 16.0f, 0, false);
-                    d = __builtin_amdgcn_cvt_pk_fp8_f32((v[2] - h[0]) * 16.0f, (v[3] - h[1]) * 16.0f, d, true);
-                    // bytes 8 i + 2 w .. of the lane's 256: word 2 i + w / 2
-                    part[(2 * i + (w >> 1)) >> 2][(2 * i + (w >> 1)) & 3] = (unsigned)c;
-                    part[16 + ((2 * i + (w >> 1)) >> 2)][(2 * i + (w >> 1)) & 3] = (unsigned)d;
-                }
-#pragma unroll
-            for (int i = 0; i < KS_NOPE; ++i) qf[i] = part[i];
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = FP8 && ks < KS_NOPE ? 32 * (ks >> 1) + 16 * hi + 8 * (ks & 1) : 16 * ks + 8 * hi;
+            qf[ks] = *reinterpret_cast<const u32x4*>(qp + d);
         }
     }
 
@@ -449,6 +397,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         for (int g = 0; g < 8; ++g) deq_store(vb, par, g, deq_load(rb, g));
     };
 
+    const float c_s = p.scale_log2;
     auto landed = [&](auto keep) {
         wait_vm<decltype(keep)::value>();
         asm volatile("" ::: "memory");
@@ -481,28 +430,31 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         __builtin_amdgcn_sched_barrier(0);
         return acc;
     };
-    // ---- 656-byte rows: S^T from the raw codes.  The scale of 128 dims is a position's own, so each group
-    // has a chain of its own: S = sum_g scale_g (K_g (hi + lo / 16)) + K_rope q_rope ----
+    // ---- 656-byte rows: S^T from the raw codes, which bf16 holds exactly.  The scale of 128 dims is a
+    // position's own, so each group is a chain of its own: S = sum_g scale_g (K_g q_g) + K_rope q_rope.
+    // (The fp8 matrix instructions, with Q in two exact e4m3 parts, sum their products with 13 bits against the
+    // largest, scores off by 2^-15, and were no faster: two prompts of 1700 to 2048 tokens 1.40 ms, this 1.38.) ----
     auto qk8 = [&](lds_cptr raw, int par) -> f32x16 {
         const int ln = opaque(lane), lhi = ln >> 5, lr = ln & 31;
-        const lds_cptr kn = raw + lr * FP8_ROW + 32 * lhi;
-        const lds_cptr kr = raw + lr * FP8_ROW + 528 + 16 * lhi;
+        const lds_cptr kn = raw + lr * FP8_ROW + 16 * lhi;
+        const lds_cptr kr = kn + 528;
         const lds_cptr sc = (lds_cptr)(LDS_AS float*)&s_scale[4 * par * TILE] + 16 * lhi;
-        auto k_frag = [&](int k8) { return join8(lds_ld<u32x4>(kn + 64 * k8), lds_ld<u32x4>(kn + 64 * k8 + 16)); };
-        i32x8 kb[2] = {k_frag(0), k_frag(1)};
+        constexpr int AHEAD = 3;               // reads of 16 codes, each two k-steps
+        u32x4 kb[AHEAD];
+        auto k_frag = [&](int j) { return lds_ld<u32x4>(j < KS_NOPE / 2 ? kn + 32 * j : kr + 32 * (j - KS_NOPE / 2)); };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kb[i] = k_frag(i);
         f32x16 s = {};
-        u32x4 rb[2];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             f32x16 a = {};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k8 = 2 * g + h;
+            for (int j = 4 * g; j < 4 * g + 4; ++j) {
                 __builtin_amdgcn_sched_barrier(0);
-                a = mfma_fp8(kb[h], join8(qf[2 * k8], qf[2 * k8 + 1]), a, 127);
-                a = mfma_fp8(kb[h], join8(qf[16 + 2 * k8], qf[16 + 2 * k8 + 1]), a, 123);
-                if (k8 + 2 < K8S) kb[h] = k_frag(k8 + 2);
-                else rb[h] = lds_ld<u32x4>(kr + 32 * h);
+                const u32x4 c = kb[j % AHEAD];
+                a = mfma_bf16(codes_bf16(c[0], c[1]), qf[2 * j], a);
+                a = mfma_bf16(codes_bf16(c[2], c[3]), qf[2 * j + 1], a);
+                kb[j % AHEAD] = k_frag(j + AHEAD);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -519,8 +471,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            s = mfma_bf16(rb[j & 1], qf[KS_NOPE + j], s);
-            if (j < 2) rb[j & 1] = lds_ld<u32x4>(kr + 32 * (j + 2));
+            s = mfma_bf16(kb[(KS_NOPE / 2 + j) % AHEAD], qf[KS_NOPE + j], s);
+            if (j + AHEAD < 4) kb[(KS_NOPE / 2 + j) % AHEAD] = k_frag(KS_NOPE / 2 + j + AHEAD);
         }
         __builtin_amdgcn_sched_barrier(0);
         return s;
