@@ -366,35 +366,42 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // 128 w + 32 m .. +31, the V block that its own PV group (u, m) reads: a buffer is refilled by its readers.
     // v_cvt_scalef32 applies the power of two of the row's scale exactly, the product its mantissa (both in
     // fp16).  The scales go to s_scale for the scores; one outside [0, 128) is NaN there, and its row 0 in V.
-    struct Piece {
-        u32x2 codes;
-        float scale;
+    struct Scale {
+        float sc;          // 0 where the scale is out of range
+        f16x2 m;           // its mantissa, twice
     };
-    auto deq_load = [&](lds_cptr rb, int g) -> Piece {
+    auto deq_scale = [&](lds_cptr rb, int par, int u) -> Scale {
         const int ln = opaque(lane);
-        const lds_cptr r = rb + (16 * (g >> 2) + (ln >> 2)) * FP8_ROW;
-        return Piece{lds_ld<u32x2>(r + 128 * wave + 32 * (g & 3) + 8 * (ln & 3)), lds_ld<float>(r + 512 + 4 * wave)};
+        const int r = 16 * u + (ln >> 2);
+        const float s = lds_ld<float>(rb + r * FP8_ROW + 512 + 4 * wave);
+        const bool bad = __float_as_uint(s) >= FP8_SCALE_LIMIT_BITS;
+        if ((ln & 3) == 0) *(LDS_AS float*)&s_scale[(4 * par + wave) * TILE + r] = bad ? __builtin_nanf("") : s;
+        Scale d;
+        d.sc = bad ? 0.0f : s;
+        const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(d.sc) & 0x007FFFFFu) | 0x3F800000u);
+        d.m = f16x2{m16, m16};
+        return d;
     };
-    auto deq_store = [&](lds_ptr vb, int par, int g, const Piece& d) {
+    auto deq_load = [&](lds_cptr rb, int g) -> u32x2 {
+        const int ln = opaque(lane);
+        return lds_ld<u32x2>(rb + (16 * (g >> 2) + (ln >> 2)) * FP8_ROW + 128 * wave + 32 * (g & 3) + 8 * (ln & 3));
+    };
+    auto deq_store = [&](lds_ptr vb, int g, u32x2 c, const Scale& d) {
         const int ln = opaque(lane);
         const int r = 16 * (g >> 2) + (ln >> 2), ch = 16 * wave + 4 * (g & 3) + (ln & 3);
-        const unsigned bits = __float_as_uint(d.scale);
-        const bool bad = bits >= FP8_SCALE_LIMIT_BITS;
-        const float sc = bad ? 0.0f : d.scale;
-        if ((g & 3) == 0 && (ln & 3) == 0)
-            *(LDS_AS float*)&s_scale[(4 * par + wave) * TILE + r] = bad ? __builtin_nanf("") : d.scale;
-        const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(sc) & 0x007FFFFFu) | 0x3F800000u);
-        const f16x2 mm = {m16, m16};
-        const u32x4 v = {
-            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[0], sc, false) * mm),
-            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[0], sc, true) * mm),
-            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[1], sc, false) * mm),
-            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)d.codes[1], sc, true) * mm)};
+        const u32x4 v = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], d.sc, false) * d.m),
+                         __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], d.sc, true) * d.m),
+                         __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], d.sc, false) * d.m),
+                         __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], d.sc, true) * d.m)};
         lds_st<u32x4>(vb + r * NOPE_STRIDE + 16 * (ch ^ nope_sw(r)), v);
     };
     auto dequant = [&](lds_cptr rb, lds_ptr vb, int par) {
 #pragma unroll
-        for (int g = 0; g < 8; ++g) deq_store(vb, par, g, deq_load(rb, g));
+        for (int u = 0; u < 2; ++u) {
+            const Scale d = deq_scale(rb, par, u);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) deq_store(vb, 4 * u + m, deq_load(rb, 4 * u + m), d);
+        }
     };
 
     const float c_s = p.scale_log2;
@@ -448,6 +455,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             f32x16 a = {};
+            f32x4 f[4];
 #pragma unroll
             for (int j = 4 * g; j < 4 * g + 4; ++j) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -455,18 +463,14 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 a = mfma_bf16(codes_bf16(c[0], c[1]), qf[2 * j], a);
                 a = mfma_bf16(codes_bf16(c[2], c[3]), qf[2 * j + 1], a);
                 kb[j % AHEAD] = k_frag(j + AHEAD);
+                if (j == 4 * g + 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] = lds_ld<f32x4>(sc + 4 * TILE * g + 32 * i);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const f32x4 f0 = lds_ld<f32x4>(sc + 4 * TILE * g + 32 * i), f1 = lds_ld<f32x4>(sc + 4 * TILE * g + 32 * i + 32);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[4 * i + r] = __builtin_fmaf(a[4 * i + r], f0[r], s[4 * i + r]);
-                    s[4 * i + 4 + r] = __builtin_fmaf(a[4 * i + 4 + r], f1[r], s[4 * i + 4 + r]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(a[r], f[r >> 2][r & 3], s[r]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -555,12 +559,14 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 #pragma unroll
             for (int h = 0; h < NWAVE; ++h) pb[h] = lds_ld<u32x4>(px + ((u * NWAVE + h) * 64 + ln) * 16);
             u32x4 v_cur = v_frag(u, 0);
+            Scale ds;
+            if constexpr (FP8 && decltype(with_exp)::value) ds = deq_scale(draw, dpar, u);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 __builtin_amdgcn_sched_barrier(0);
                 const u32x4 v_nxt = m + 1 < 4 ? v_frag(u, m + 1) : v_cur;
-                Piece d;
-                if constexpr (FP8 && decltype(with_exp)::value) d = deq_load(draw, 4 * u + m);
+                u32x2 codes;
+                if constexpr (FP8 && decltype(with_exp)::value) codes = deq_load(draw, 4 * u + m);
 #pragma unroll
                 for (int h = 0; h < NWAVE; ++h) mfma_o<FP8>(o[4 * m + h], v_cur, pb[h]);
                 if constexpr (decltype(with_exp)::value) {
@@ -568,7 +574,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     en[r0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0], c_s, -m_ref));
                     en[r0 + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0 + 1], c_s, -m_ref));
                 }
-                if constexpr (FP8 && decltype(with_exp)::value) deq_store(vt, dpar, 4 * u + m, d);
+                if constexpr (FP8 && decltype(with_exp)::value) deq_store(vt, 4 * u + m, codes, ds);
                 v_cur = v_nxt;
             }
         }
