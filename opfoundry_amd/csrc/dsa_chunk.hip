@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
+#include <stdlib.h>
 #include <algorithm>
 #include <type_traits>
 
@@ -804,6 +805,489 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// The narrow kernel: 32 rows a workgroup, two workgroups a CU, for single tokens and
+// few heads, where the cache rows' way through memory counts and not the products.
+//   QK^T   wave w: 16 positions (half w % 2 of the tile) x 16 rows (half w / 2), 16x16x32
+//   P      as in the tiled kernel, one buffer: P of a tile is read before the next's is written
+//   PV     wave w: O^T[dims 128 w .. +127 x 32 rows] in 64 registers
+// Two barriers a tile; one workgroup's waits are the other's time.
+// ---------------------------------------------------------------------------
+constexpr int NARROW = 32;                   // rows of a workgroup
+constexpr int NSTRIDE = 1040;                // a tile's NoPE rows; piece c of row r at c ^ 4 (r % 4)
+constexpr int NROPE_OFF = TILE * NSTRIDE;
+constexpr int NTILE = NROPE_OFF + TILE * 128;
+constexpr int NLIST = 512;                   // entries of the row list
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return mfma_bf16(a, b, c);
+}
+
+// RUNS: a tile lies in one page (or in a flat cache), so that its rows follow its first one's
+template <int FMT, bool RUNS>
+__global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(2, 2)))
+dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
+    constexpr bool FP8 = FMT == DSA_KV_FP8_656;
+    constexpr int VT = TILE * NSTRIDE;                               // 656-byte rows: one V tile, two raw slots
+    constexpr int BYTES = FP8 ? VT + 2 * RAW_BYTES : 2 * NTILE;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[BYTES];
+    __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * 2 * 32 * 16];     // [u][hi][row] x 8 positions
+    __shared__ int32_t s_rows[NLIST];        // RUNS: the first row of every tile; else every position's
+    __shared__ float s_top[2][NARROW];
+    __shared__ uint32_t s_nan;               // bit j: position j's row holds a NaN or infinity
+    __shared__ int32_t s_misc[2];
+    const lds_ptr T0 = (lds_ptr)s_tile, PX = (lds_ptr)s_p;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.y;
+    // Blocks of one sequence follow one another and read the same rows: four at a time on one XCD
+    // (workgroups go to the eight in turn).
+    int64_t x = blockIdx.x;
+    if (x < (int64_t)(gridDim.x & ~31u)) x = (x & ~31) | (x & 7) << 2 | ((x >> 3) & 3);
+    const Block blk = find_block(p, (int64_t)gridDim.x - 1 - x, NARROW);
+    if (blk.rows == 0) return;
+    const int lim_lo = limit_in(p, blk, blk.first + blk.r0 / p.H);
+    const int lim_hi = limit_in(p, blk, blk.first + (blk.r0 + blk.rows - 1) / p.H);
+    const bool too_long = blk.len > p.max_len;
+    const int k0 = split * p.per_split;
+    const int k1 = too_long ? k0 : (int)min(min((int64_t)lim_hi, p.pages.limit), (int64_t)k0 + p.per_split);
+    if (p.ns > 1 && k1 <= k0) return;
+
+    // scores: this lane's row of the 16 of its wave, and its positions 16 half + 4 q .. +3 of a tile
+    const int half = wave & 1, q = lane >> 4;
+    const int my = 16 * (wave >> 1) + (lane & 15);
+    const int row = blk.r0 + min(my, blk.rows - 1);
+    const int tok = blk.first + row / p.H;
+    const int limit = limit_in(p, blk, tok);
+    u32x4 qf[KS / 2];
+    {
+        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)(row % p.H) * p.q_sh;
+#pragma unroll
+        for (int ks = 0; ks < KS / 2; ++ks) {
+            // (656-byte rows: 16 codes a read, the two k-steps of 64 dims share them)
+            const int d = FP8 && ks < 16 ? 64 * (ks >> 1) + 16 * q + 8 * (ks & 1) : 32 * ks + 8 * q;
+            qf[ks] = *reinterpret_cast<const u32x4*>(qp + d);
+        }
+    }
+
+    // ---- positions [c0, c0 + span) below k1 -> the row list; -1: no row ----
+    constexpr int STEP = RUNS ? TILE : 1;
+    constexpr int span = NLIST * STEP;
+    int ntiles = 0;
+    int32_t safe = -1;                       // a row that is there
+    auto resolve = [&](int c0) {
+        __syncthreads();
+        const int count = (min(k1 - c0, span) + STEP - 1) / STEP;
+        int32_t some = -1;
+        for (int e = threadIdx.x; e < NLIST; e += NTHR) {
+            int64_t r = -1;
+            if (e < count) r = dsa_seq::row_of(p.pages, blk.b, c0 + e * STEP, p.rows);
+            s_rows[e] = (int32_t)r;
+            some = max(some, (int32_t)r);
+        }
+        if (threadIdx.x == 0) s_misc[0] = -1;
+        __syncthreads();
+        if (some >= 0) s_misc[0] = some;
+        __syncthreads();
+        safe = __builtin_amdgcn_readfirstlane(s_misc[0]);
+        ntiles = safe < 0 ? 0 : (min(k1 - c0, span) + TILE - 1) / TILE;
+    };
+    // RUNS: a tile's first row, read ahead of its use
+    auto base_of = [&](int i) -> int32_t { return RUNS && i < NLIST ? s_rows[i] : 0; };
+    // a tile's positions that have a row (bit j clear: none, or past k1)
+    auto has_of = [&](int32_t base, int i, int c0) -> uint32_t {
+        const int left = k1 - (c0 + i * TILE);
+        if constexpr (RUNS) {
+            const int64_t n = base < 0 ? 0 : min((int64_t)left, p.rows - base);
+            return n >= TILE ? ~0u : (1u << n) - 1u;
+        } else {
+            const int j = lane & 31;
+            return (uint32_t)__builtin_amdgcn_ballot_w64(j < left && s_rows[i * TILE + j] >= 0);
+        }
+    };
+    // cache row of position j of tile i (some row that is there, for one without)
+    auto row_at = [&](int32_t base, uint32_t has, int i, int j) -> uint32_t {
+        const bool ok = (has >> j) & 1;
+        return (uint32_t)(ok ? (RUNS ? base + j : s_rows[i * TILE + j]) : safe);
+    };
+
+    auto slot_of = [&](int s) -> lds_ptr { return FP8 ? T0 + VT + s * RAW_BYTES : T0 + s * NTILE; };
+    auto issue = [&](int32_t base, uint32_t has, int i, int slot) {
+        const int ln = opaque(lane);
+        const lds_ptr tb = slot_of(slot);
+        if constexpr (!FP8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = 8 * wave + e;
+                const uint32_t at = __builtin_amdgcn_readfirstlane(row_at(base, has, i, r));
+                lds_dma16_s(p.kv + (uint64_t)at * (uint32_t)p.row_bytes, 16u * (unsigned)(ln ^ 4 * (r & 3)), tb + r * NSTRIDE);
+            }
+            const int r = 8 * wave + (ln >> 3);
+            lds_dma16(p.kv + (uint64_t)row_at(base, has, i, r) * (uint32_t)p.row_bytes + 1024 + 16 * ((ln & 7) ^ rope_sw(r)),
+                      tb + NROPE_OFF + 8 * wave * 128);
+        } else if (RUNS && has == ~0u && p.row_bytes == FP8_ROW) {
+            const unsigned char* from = p.kv + (uint64_t)(uint32_t)base * FP8_ROW + 1024 * wave;
+#pragma unroll
+            for (int e = 0; e < RAW_LPW - 1; ++e) lds_dma16_s(from + 1024 * NWAVE * e, 16u * ln, tb + 1024 * wave + 1024 * NWAVE * e);
+            if (wave == 0) lds_dma16_s(from + 1024 * (RAW_LOADS - 1), 16u * (ln & 31), tb + 1024 * (RAW_LOADS - 1));
+        } else {
+#pragma unroll 1
+            for (int k = wave; k < RAW_LOADS; k += NWAVE) {
+                const unsigned piece = min(64u * k + ln, (unsigned)RAW_PIECES - 1), rt = piece / 41u;
+                lds_dma16(p.kv + ((uint64_t)row_at(base, has, i, (int)rt) * (uint32_t)p.row_bytes + 16u * (piece - 41u * rt)), tb + 1024 * k);
+            }
+        }
+    };
+    // this wave's loads have landed, but for those of the newest tile where `one_more` is in flight
+    // (656-byte rows: RAW_LPW of wave 0, one fewer of the others)
+    auto landed = [&](bool one_more) {
+        if (FP8 && one_more) {
+            if (wave == 0) wait_vm<RAW_LPW>();
+            else wait_vm<RAW_LPW - 1>();
+        } else {
+            wait_vm<0>();
+        }
+        asm volatile("" ::: "memory");
+    };
+    // (as in the tiled kernel: rows that some row of the block does not attend must not reach it)
+    auto scan = [&](int slot) {
+        const int ln = opaque(lane);
+        uint32_t bad = 0;
+        if constexpr (!FP8) {
+            const lds_ptr tb = slot_of(slot) + 8 * wave * NSTRIDE + 16 * ln;
+#pragma unroll 2
+            for (int e = 0; e < 8; ++e) {
+                const u32x4 v = lds_ld<u32x4>(tb + e * NSTRIDE);
+                bool odd = false;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) odd |= (v[w] & 0x7F800000u) == 0x7F800000u || (v[w] & 0x7F80u) == 0x7F80u;
+                if (__builtin_amdgcn_ballot_w64(odd)) {
+                    lds_st<u32x4>(tb + e * NSTRIDE, u32x4{0, 0, 0, 0});
+                    bad |= 1u << e;
+                }
+            }
+        } else {
+            const lds_ptr tb = slot_of(slot) + (8 * wave + (ln >> 5)) * FP8_ROW + 16 * (ln & 31);
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const u32x4 v = lds_ld<u32x4>(tb + 2 * e * FP8_ROW);
+                unsigned odd = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) odd |= ((v[w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                const uint64_t who = __builtin_amdgcn_ballot_w64(odd != 0);
+                const bool lo = (uint32_t)who != 0, up = (who >> 32) != 0;
+                if (ln < 32 ? lo : up) lds_st<u32x4>(tb + 2 * e * FP8_ROW, u32x4{0, 0, 0, 0});
+                bad |= (lo ? 1u : 0u) << (2 * e) | (up ? 2u : 0u) << (2 * e);
+            }
+        }
+        if (ln == 0) reinterpret_cast<unsigned char*>(&s_nan)[wave] = (unsigned char)bad;
+    };
+
+    const float c_s = p.scale_log2;
+    f32x16 o[4];
+    float m_ref = 0.0f, l_lane = 0.0f, p_top = 0.0f;
+    bool any = false;
+
+    // S^T[4 positions of this lane x its row]
+    auto qk = [&](lds_cptr kt) -> f32x4 {
+        const int ln = opaque(lane), lq = ln >> 4, lr = 16 * half + (ln & 15);
+        if constexpr (!FP8) {
+            const lds_cptr kn = kt + lr * NSTRIDE, kr = kt + NROPE_OFF + 128 * lr;
+            // pieces 4 ks + lq, at their places: ks % 4 picks the two bits that the row flips
+            auto k_at = [&](int ks) -> lds_cptr {
+                return ks < 16 ? kn + 256 * (ks >> 2) + 16 * ((4 * (ks & 3) + lq) ^ 4 * (lr & 3)) : kr + 16 * ((4 * (ks - 16) + lq) ^ rope_sw(lr));
+            };
+            constexpr int AHEAD = 6;
+            u32x4 kb[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) kb[i] = lds_ld<u32x4>(k_at(i));
+            f32x4 a = {}, b = {};
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks) {
+                if (ks & 1) b = mfma16(kb[ks % AHEAD], qf[ks], b);
+                else a = mfma16(kb[ks % AHEAD], qf[ks], a);
+                if (ks + AHEAD < KS / 2) kb[ks % AHEAD] = lds_ld<u32x4>(k_at(ks + AHEAD));
+            }
+            return a + b;
+        } else {
+            const lds_cptr kn = kt + lr * FP8_ROW + 16 * lq;
+            u32x4 kb[10];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) kb[j] = lds_ld<u32x4>(kn + 64 * j);
+            kb[8] = lds_ld<u32x4>(kn + 528);
+            kb[9] = lds_ld<u32x4>(kn + 528 + 64);
+            // a position's four scales
+            f32x4 sc[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[r] = lds_ld<f32x4>(kt + (16 * half + 4 * lq + r) * FP8_ROW + 512);
+            f32x4 s = {}, g[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                g[i] = f32x4{};
+#pragma unroll
+                for (int j = 2 * i; j < 2 * i + 2; ++j) {
+                    g[i] = mfma16(codes_bf16(kb[j][0], kb[j][1]), qf[2 * j], g[i]);
+                    g[i] = mfma16(codes_bf16(kb[j][2], kb[j][3]), qf[2 * j + 1], g[i]);
+                }
+            }
+            s = mfma16(kb[8], qf[16], s);
+            s = mfma16(kb[9], qf[17], s);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = __float_as_uint(sc[r][i]) >= FP8_SCALE_LIMIT_BITS ? __builtin_nanf("") : sc[r][i];
+                    s[r] = __builtin_fmaf(g[i][r], f, s[r]);
+                }
+            return s;
+        }
+    };
+    auto masked = [&](uint32_t has, int i, int c0) { return c0 + (i + 1) * TILE > lim_lo || has != ~0u; };
+    auto mask = [&](f32x4& s, uint32_t has, int i, int c0) {
+        if (masked(has, i, c0)) {
+            const uint32_t nan = s_nan;
+            const int left = limit - (c0 + i * TILE);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * half + 4 * q + r;
+                const bool on = j < left && ((has >> j) & 1);
+                any = any || on;
+                const float v = (nan >> j) & 1 ? __builtin_nanf("") : s[r];
+                s[r] = on ? v : -INFINITY;
+            }
+        } else {
+            any = true;
+        }
+    };
+    // the largest of a row's scores in both halves of the tile
+    auto top_of = [&](const f32x4& s) -> float {
+        float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (q == 0) s_top[half][my] = m;
+        __syncthreads();
+        m = fmaxf(s_top[0][my], s_top[1][my]);
+        __syncthreads();
+        return m;
+    };
+    auto p_out = [&](const f32x4& s) {
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c_s, -m_ref));
+        l_lane += (e[0] + e[1]) + (e[2] + e[3]);
+        u32x2 w;
+        if constexpr (FP8) {
+            p_top = fmaxf(p_top, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
+            const f16x2 a = {(_Float16)e[0], (_Float16)e[1]}, b = {(_Float16)e[2], (_Float16)e[3]};
+            w = u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+        } else {
+            const f32x4 v = {e[0], e[1], e[2], e[3]};
+            w = __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
+        }
+        // (the order of a lane's eight positions in the product: 4 hi .. +3, then 8 + 4 hi .. +3)
+        lds_st<u32x2>(PX + ((2 * half + (q & 1)) * 32 + my) * 16 + 8 * (q >> 1), w);
+    };
+    // 656-byte rows: V of the raw tile as fp16, each wave the dims that it reads (as in the tiled kernel)
+    auto dequant = [&](lds_cptr rb) {
+        const int ln = opaque(lane);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = 16 * u + (ln >> 2);
+            const float s = lds_ld<float>(rb + r * FP8_ROW + 512 + 4 * wave);
+            const float sc = __float_as_uint(s) >= FP8_SCALE_LIMIT_BITS ? 0.0f : s;
+            const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(sc) & 0x007FFFFFu) | 0x3F800000u);
+            const f16x2 mm = {m16, m16};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const u32x2 c = lds_ld<u32x2>(rb + r * FP8_ROW + 128 * wave + 32 * m + 8 * (ln & 3));
+                const u32x4 v = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], sc, false) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], sc, true) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], sc, false) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], sc, true) * mm)};
+                lds_st<u32x4>(T0 + r * NSTRIDE + 256 * wave + 16 * ((4 * m + (ln & 3)) ^ 4 * (r & 3)), v);
+            }
+        }
+    };
+    auto pv = [&](lds_cptr vt) {
+        const int ln = opaque(lane), lhi = ln >> 5;
+        const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
+        const int vx = 2 * (g16 & 1) + (pp >> 1);
+        const lds_cptr v0 = vt + (4 * lhi + rr) * NSTRIDE + 256 * wave + 8 * (pp & 1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const u32x4 pb = lds_ld<u32x4>(PX + ((2 * u + lhi) * 32 + (ln & 31)) * 16);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const lds_cptr at = v0 + 16 * u * NSTRIDE + 16 * ((4 * m + vx) ^ 4 * rr);
+                const s16x4 va = lds_read_tr16(at), vb = lds_read_tr16(at + 8 * NSTRIDE);
+                o[m] = mfma32<FP8>(__builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[m]);
+            }
+        }
+    };
+
+    const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + span - 1) / span) : 0;
+    auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * span); };
+    bool first = true;
+    for (bool again = false;;) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) o[m] = f32x16{};
+        l_lane = 0.0f;
+        for (int c = 0; c < nspans; ++c) {
+            const int c0 = start_of(c);
+            resolve(c0);
+            if (ntiles == 0) continue;
+            auto at = [&](int i) { return __builtin_amdgcn_readfirstlane(base_of(i)); };
+            int32_t b0 = at(0), b1 = at(1);
+            uint32_t has = has_of(b0, 0, c0), has1 = ntiles > 1 ? has_of(b1, 1, c0) : 0;
+            issue(b0, has, 0, 0);
+            if (FP8 && ntiles > 1) issue(b1, has1, 1, 1);
+            for (int i = 0; i < ntiles; ++i) {
+                const int slot = i & 1;
+                // tile i, the older of those in flight, has landed
+                landed(i + 1 < ntiles);
+                const bool m = masked(has, i, c0);
+                if (!FP8 && m) scan(slot);
+                tile_barrier();
+                if (FP8 && m) {
+                    scan(slot);
+                    tile_barrier();
+                }
+                // bf16: every wave is done with tile i - 1, whose buffer takes tile i + 1
+                if (!FP8 && i + 1 < ntiles) issue(b1, has1, i + 1, slot ^ 1);
+                const int32_t ahead = base_of(i + 2);
+                f32x4 s = qk(slot_of(slot));
+                if constexpr (FP8) dequant(slot_of(slot));
+                mask(s, has, i, c0);
+                if (first) {
+                    const float top = top_of(s) * c_s;
+                    m_ref = top == -INFINITY ? 0.0f : top;
+                    first = false;
+                }
+                p_out(s);
+                const int32_t b2 = __builtin_amdgcn_readfirstlane(ahead);
+                const uint32_t has2 = i + 2 < ntiles ? has_of(b2, i + 2, c0) : 0;
+                tile_barrier();
+                // 656-byte rows: every wave is done with the raw slot, which takes tile i + 2
+                if (FP8 && i + 2 < ntiles) issue(b2, has2, i + 2, slot);
+                pv(FP8 ? (lds_cptr)T0 : (lds_cptr)slot_of(slot));
+                has = has1, b1 = b2, has1 = has2;
+            }
+        }
+        // row sums over the lanes and halves that share a row (s_top: free)
+        float l = l_lane, t = FP8 ? p_top : 0.0f;
+        l += __shfl_xor(l, 16, 64), l += __shfl_xor(l, 32, 64);
+        t = fmaxf(t, __shfl_xor(t, 16, 64)), t = fmaxf(t, __shfl_xor(t, 32, 64));
+        const uint64_t anys = __builtin_amdgcn_ballot_w64(any);
+        any = ((anys >> (lane & 15)) & 0x0001000100010001ull) != 0;
+        __syncthreads();
+        if (threadIdx.x == 0) s_misc[1] = 0;
+        if (q == 0) s_top[half][my] = any ? l : 0.0f;
+        __syncthreads();
+        l = s_top[0][my] + s_top[1][my];
+        __syncthreads();
+        if (q == 0) s_top[half][my] = any ? (FP8 ? t : 1.0f) : -1.0f;
+        __syncthreads();
+        t = fmaxf(s_top[0][my], s_top[1][my]);
+        any = t >= 0.0f;
+        const bool held = FP8 ? t >= 0.5f && t < 0x1p15f : l > 0x1p-40f;
+        if (!again && any && !(held && l < 0x1p100f)) s_misc[1] = 1;
+        l_lane = l;
+        __syncthreads();
+        if (again || __builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
+        again = true;
+        p_top = 0.0f;
+        float top = -INFINITY;
+        for (int c = 0; c < nspans; ++c) {
+            const int c0 = start_of(c);
+            resolve(c0);
+            for (int i = 0; i < ntiles; ++i) {
+                const int32_t base = __builtin_amdgcn_readfirstlane(base_of(i));
+                const uint32_t has = has_of(base, i, c0);
+                issue(base, has, i, 0);
+                landed(false);
+                tile_barrier();
+                if (masked(has, i, c0)) {
+                    scan(0);
+                    tile_barrier();
+                }
+                f32x4 s = qk(slot_of(0));
+                mask(s, has, i, c0);
+                top = fmaxf(top, top_of(s));       // (its barriers also end the slot's use)
+            }
+        }
+        m_ref = top == -INFINITY ? 0.0f : top * c_s;
+    }
+
+    // ---- O / l, LSE: rows' values from the scoring lanes to the lanes that hold O ----
+    const float lse = too_long ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l_lane)) * LN2;
+    __syncthreads();
+    if (q == 0 && half == 0) {
+        s_top[0][my] = too_long ? __builtin_nanf("") : (any ? 1.0f / l_lane : 0.0f);
+        const int64_t at = (int64_t)blk.first * p.H + blk.r0 + my;
+        if (my >= blk.rows) {
+        } else if (p.ns > 1) {
+            p.part_lse[(int64_t)split * p.T * p.H + at] = any ? lse : -FLT_MAX;
+        } else if (p.lse) {
+            p.lse[at] = any || too_long ? lse : INFINITY;
+        }
+    }
+    __syncthreads();
+    const int hi = lane >> 5, r32 = lane & 31;
+    const float inv = s_top[0][r32];
+    if (p.ns == 1) {
+        constexpr int OUT_STRIDE = D_VO * 2 + 16;
+        static_assert(32 * OUT_STRIDE <= BYTES, "the stage fits the tile buffers");
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = {o[m][4 * g] * inv, o[m][4 * g + 1] * inv, o[m][4 * g + 2] * inv, o[m][4 * g + 3] * inv};
+                lds_st<u32x2>(T0 + r32 * OUT_STRIDE + 2 * (128 * wave + 32 * m + 8 * g + 4 * hi),
+                              __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4)));
+            }
+        __syncthreads();
+        const bool o16 = ((p.o_st | p.o_sh) & 7) == 0 && ((uintptr_t)p.out & 15) == 0;
+        for (int k = 0; k < 8; ++k) {
+            const int r = 8 * wave + k;
+            if (r >= blk.rows) break;
+            const int t = blk.first + (blk.r0 + r) / p.H, h = (blk.r0 + r) % p.H;
+            const u32x4 v = lds_ld<u32x4>(T0 + r * OUT_STRIDE + 16 * lane);
+            __bf16* const dst = p.out + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * lane;
+            if (o16) {
+                *reinterpret_cast<u32x4*>(dst) = v;
+            } else {
+                reinterpret_cast<u32x2*>(dst)[0] = u32x2{v[0], v[1]};
+                reinterpret_cast<u32x2*>(dst)[1] = u32x2{v[2], v[3]};
+            }
+        }
+    } else {
+        constexpr int PST = D_VO + 16;
+        static_assert(4 * 32 * PST <= BYTES, "four waves' stages fit the tile buffers");
+        const lds_ptr stg = T0 + wave * 32 * PST;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = {o[m][4 * g] * inv, o[m][4 * g + 1] * inv, o[m][4 * g + 2] * inv, o[m][4 * g + 3] * inv};
+                lds_st<f32x4>(stg + r32 * PST + 4 * (32 * m + 8 * g + 4 * hi), v);
+            }
+        float* const dst0 = p.part_o + ((int64_t)split * p.T * p.H + (int64_t)blk.first * p.H + blk.r0) * D_VO;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int r = 2 * k + (lane >> 5);
+            const f32x4 v = lds_ld<f32x4>(stg + r * PST + 16 * (lane & 31));
+            if (r < blk.rows) *reinterpret_cast<f32x4*>(dst0 + (int64_t)r * D_VO + 128 * wave + 4 * (lane & 31)) = v;
+        }
+    }
+}
+
 // Joins the partials of a row's splits, one wave a row: a lane holds 8 of its 512
 // values.  Splits past the row's positions wrote nothing and are not read.
 __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const ChunkParams p) {
@@ -824,13 +1308,27 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
     const float w = mine == -FLT_MAX ? 0.0f : __builtin_amdgcn_exp2f((mine - top) * LOG2E);
     const float total = wave_sum(w);
     float o[8] = {};
-    for (int s = 0; s < ns; ++s) {
-        const float f = __shfl(w, s, 64);
-        if (f == 0.0f) continue;
-        const float* src = p.part_o + (s * step + row) * D_VO + 8 * lane;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
+    // eight splits' loads in flight at a time; the last one's again past it.  One of no weight is not added
+    // (its partial may hold anything).
+    const float* const src = p.part_o + row * D_VO + 8 * lane;
+    for (int s0 = 0; s0 < ns; s0 += 8) {
+        f32x4 x[8], y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(f, x[i], o[i]), o[4 + i] = __builtin_fmaf(f, y[i], o[4 + i]);
+        for (int s = 0; s < 8; ++s) {
+            const float* const at = src + min(s0 + s, ns - 1) * step * D_VO;
+            x[s] = *reinterpret_cast<const f32x4*>(at), y[s] = *reinterpret_cast<const f32x4*>(at + 4);
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const float f = __shfl(w, s0 + s, 64);          // 0 past the last
+            if (f != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = __builtin_fmaf(f, x[s][i], o[i]);
+                    o[4 + i] = __builtin_fmaf(f, y[s][i], o[4 + i]);
+                }
+            }
+        }
     }
     const float nan = p.lens[b] > p.max_len ? __builtin_nanf("") : 0.0f;
     const float inv = any ? 1.0f / total + nan : nan;
@@ -939,8 +1437,18 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
-    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, BLOCK), (unsigned)p.ns);
-    if (a->kv_format == DSA_KV_BF16)
+    const bool narrow = getenv("DSA_NARROW") != nullptr;
+    const bool runs = !a->block_table || a->block_size % TILE == 0;
+    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, narrow ? NARROW : BLOCK), (unsigned)p.ns);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
+    if (narrow && a->kv_format == DSA_KV_BF16) {
+        if (runs) launch(dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true>);
+        else launch(dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);
+    } else if (narrow) {
+        if (runs) launch(dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true>);
+        else launch(dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
+    }
+    else if (a->kv_format == DSA_KV_BF16)
         hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_BF16>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
     else
         hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);

@@ -605,58 +605,47 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
 
 
 # ------------------------------------------------------------------ a chunk of new tokens
+#
+# These calls are short (a decode step's kernels take a few microseconds), so their checks are written to
+# cost little: one look at a tensor's type, device, shape and strides, and argument structs filled at once.
 
-class _On:
-    """The device of a call's tensors and the stream it runs on.  Every tensor must lie on one
-    device, which need not be the current one.  What the call allocates is used on its stream:
-    when that is not the device's current stream, the allocator is told, so that the memory is
-    not handed out again while the call still runs."""
-
-    def __init__(self, device: torch.device, stream):
-        self.device = device
-        current = torch.cuda.current_stream(device)
-        if stream is None:
-            self.other = None
-            self.handle = current.cuda_stream
-        else:
-            self.handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-            self.other = None
-            if self.handle != current.cuda_stream:
-                self.other = (stream if isinstance(stream, torch.cuda.Stream)
-                              else torch.cuda.ExternalStream(self.handle, device=device))
-
-    def empty(self, shape, dtype):
-        t = torch.empty(shape, dtype=dtype, device=self.device)
-        if self.other is not None:
-            # the memory may still be in use by the current stream's earlier work
-            self.other.wait_stream(torch.cuda.current_stream(self.device))
-            t.record_stream(self.other)
-        return t
-
-    def call(self, fn, where, *args):
-        if torch.cuda.current_device() == self.device.index:
-            check(fn(*args, self.handle), where)
-        else:
-            with torch.cuda.device(self.device):
-                check(fn(*args, self.handle), where)
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
-def _operand(t: Optional[torch.Tensor], dtype, name: str, device=None, shape=None):
-    """Address of an operand (None: no operand) after its checks: type, device, shape (-1: any) and a
-    dense last dim."""
+def _bad(name: str, t, what: str):
+    raise ValueError(f"{name} must {what}, got {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _addr(t: torch.Tensor, dtype, name: str, dev: int) -> int:
+    """Address of a tensor of this type on device `dev`."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev or dev < 0:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor")
+        raise ValueError(f"{name} must be on device {dev}, got {t.device}")
+    return t.data_ptr()
+
+
+def _addr3(t: torch.Tensor, T: int, H: int, D: int, name: str, dev: int):
+    """(address, stride of a token, stride of a head) of a bf16 [T, H, D] with a dense last dim."""
+    p = _addr(t, _BF16, name, dev)
+    if t.shape != (T, H, D):
+        _bad(name, t, f"be [{T}, {H}, {D}]")
+    st = t.stride()
+    if st[2] != 1 and D > 1:
+        _bad(name, t, "have a dense last dim")
+    return p, st[0], st[1]
+
+
+def _vector(t: Optional[torch.Tensor], n: int, dtype, name: str, dev: int) -> Optional[int]:
+    """Address of an optional dense vector of n values."""
     if t is None:
         return None
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if shape is not None and (t.dim() != len(shape) or any(w >= 0 and n != w for n, w in zip(t.shape, shape))):
-        raise ValueError(f"{name} must have shape {['any' if w < 0 else w for w in shape]}, got {tuple(t.shape)}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must have a dense last dim")
-    return t.data_ptr()
+    p = _addr(t, dtype, name, dev)
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        _bad(name, t, f"be a dense vector of {n}")
+    return p
 
 
 def _choice(table, value, name: str) -> int:
@@ -666,42 +655,107 @@ def _choice(table, value, name: str) -> int:
         raise ValueError(f"{name} must be one of {list(table)}, got {value!r}") from None
 
 
-def _chunk_fields(a, q_indptr, seq_lens, device):
-    """The chunk's own fields (q_indptr, seq_lens, B)."""
-    a.q_indptr = _operand(q_indptr, torch.int32, "q_indptr", device, (-1,))
-    a.seq_lens = _operand(seq_lens, torch.int32, "seq_lens", device, (-1,))
-    if q_indptr.shape[0] != seq_lens.shape[0] + 1:
-        raise ValueError("q_indptr must have one entry more than seq_lens")
-    a.B = seq_lens.shape[0]
+def _sequences(q_indptr, seq_lens, dev: int):
+    """(q_indptr's address, seq_lens's, B)."""
+    B = seq_lens.numel()
+    return _vector(q_indptr, B + 1, _I32, "q_indptr", dev), _vector(seq_lens, B, _I32, "seq_lens", dev), B
 
 
-def _page_fields(a, block_table, block_size, kv_batch_stride, B, device):
-    if block_table is not None:
-        a.block_table = _operand(block_table, torch.int32, "block_table", device, (B, -1))
-        if block_size is None:
+def _pages(block_table, block_size, cache, B: int, dev: int):
+    """(address, stride, blocks of a row, rows of a block) of a block table; the block size defaults to
+    that of a cache [blocks, block_size, row]."""
+    if block_table is None:
+        return None, 0, 0, 0
+    p = _addr(block_table, _I32, "block_table", dev)
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        _bad("block_table", block_table, f"be [{B}, blocks]")
+    st = block_table.stride()
+    n = block_table.shape[1]
+    if n > 1 and st[1] != 1:
+        _bad("block_table", block_table, "have a dense last dim")
+    if block_size is None:
+        if cache is None or cache.dim() < 3:
             raise ValueError("block_size is required with a block table")
-        a.block_table_stride, a.table_blocks, a.block_size = block_table.stride(0), block_table.shape[1], int(block_size)
-    else:
-        a.kv_batch_stride = int(kv_batch_stride)
+        block_size = cache.shape[-2]
+    return p, st[0], n, int(block_size)
 
 
-def _angles(a, cos_sin, device):
-    if cos_sin is not None:
-        a.cos_sin = _operand(cos_sin, torch.float32, "cos_sin", device, (-1, abi.D_ROPE))
-        if not cos_sin.is_contiguous():
-            raise ValueError("cos_sin must be contiguous")
-        a.n_pos = cos_sin.shape[0]
+def _angles(cos_sin, dev: int):
+    """(address, positions) of a table of angles."""
+    if cos_sin is None:
+        raise ValueError("a rotation needs cos_sin")
+    p = _addr(cos_sin, _F32, "cos_sin", dev)
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != abi.D_ROPE or not cos_sin.is_contiguous():
+        _bad("cos_sin", cos_sin, "be a dense [positions, 64]")
+    return p, cos_sin.shape[0]
 
 
-def _row_stride(t: torch.Tensor, name: str) -> int:
-    """Elements between the rows of t (all dims but the last count rows, one uniform stride apart)."""
-    rs = t.stride(-2) if t.dim() >= 2 and t.numel() else t.shape[-1]
-    expect = rs
+def _rows(t: torch.Tensor, width: int, name: str):
+    """(rows, row stride; 0 = dense) of a tensor [..., width] whose rows are one uniform stride apart."""
+    n = t.numel() // width
+    if t.is_contiguous():
+        return n, 0
+    st = t.stride()
+    if st[-1] != 1:
+        _bad(name, t, "have a dense last dim")
+    rs = expect = st[-2] if t.dim() > 1 else width
     for d in range(t.dim() - 2, -1, -1):
-        if t.shape[d] > 1 and t.stride(d) != expect:
-            raise ValueError(f"{name}: rows must be one uniform stride apart")
+        if t.shape[d] > 1:
+            if st[d] != expect:
+                _bad(name, t, "have rows one uniform stride apart")
         expect *= t.shape[d]
-    return max(rs, t.shape[-1]) if t.numel() <= t.shape[-1] else rs
+    if n > 1 and t.shape[-2] == 1:
+        # (the rows are counted by a dim further out)
+        rs = next(st[d] for d in range(t.dim() - 2, -1, -1) if t.shape[d] > 1)
+    return n, (rs if n > 1 else 0)
+
+
+class _Stream:
+    """The stream of a call on device `dev` and what it allocates.  Memory used on a stream that is not the
+    device's current one is marked so for the allocator, which then does not hand it out while the call runs."""
+
+    __slots__ = ("dev", "handle", "other")
+
+    def __init__(self, dev: int, stream):
+        self.dev = dev
+        current = torch._C._cuda_getCurrentRawStream(dev)
+        self.other = None
+        if stream is None:
+            self.handle = current
+        else:
+            self.handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            if self.handle != current:
+                self.other = (stream if isinstance(stream, torch.cuda.Stream)
+                              else torch.cuda.ExternalStream(self.handle, device=dev))
+
+    def empty(self, like: torch.Tensor, shape, dtype) -> torch.Tensor:
+        t = like.new_empty(shape, dtype=dtype)
+        if self.other is not None:
+            # (the current stream's earlier work may still use that memory)
+            self.other.wait_stream(torch.cuda.current_stream(self.dev))
+            t.record_stream(self.other)
+        return t
+
+    def call(self, fn, where: str, *args) -> None:
+        if torch._C._cuda_getDevice() == self.dev:
+            rc = fn(*args, self.handle)
+        else:
+            with torch.cuda.device(self.dev):
+                rc = fn(*args, self.handle)
+        if rc:
+            check(rc, where)
+
+
+def _normed_rows(x, norm, w, b, out, T, D, norm_dim, name, dev, on):
+    """dsa_norm_rope_rows of one stream, and its output."""
+    H = x.shape[1]
+    px, st, sh = _addr3(x, T, H, D, name, dev)
+    if out is None:
+        out = on.empty(x, (T, H, D), _BF16)
+    po, ot, oh = _addr3(out, T, H, D, name + "_out", dev)
+    return abi.NormRopeRows(px, st, sh, po, ot, oh, _vector(w, norm_dim, _F32, name + "_weight", dev),
+                            _vector(b, norm_dim, _F32, name + "_bias", dev), H,
+                            _choice(abi.NORMS, norm, name + "_norm")), out
 
 
 def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
@@ -722,49 +776,48 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
     cos_sin fp32 [n_pos, 64]: a position's 32 cosines, then its 32 sines.  The position of a row is
     positions[t] (int32 [T]), or the chunk's (q_indptr, seq_lens), whose rows of no sequence are left as
     allocated.  Returns (q_out, k_out); an output may be its input."""
-    T, H, D = q.shape if q.dim() == 3 else (-1, -1, -1)
-    dev = q.device
-    a = abi.QkNormRopeArgs()
-    a.T, a.D = T, D
-    a.norm_dim = min(D, 512) if norm_dim is None else int(norm_dim)
-    a.rot_off = (0 if D == 128 else D - abi.D_ROPE) if rot_off is None else int(rot_off)
-    a.rope = _choice(abi.ROPES, style, "style")
-    a.inverse, a.eps = (1 if inverse else 0), float(eps)
-    bf16 = torch.bfloat16
-    streams = [(a.q, q, q_norm, q_weight, q_bias, q_out, "q")]
-    if k is not None:
-        streams.append((a.k, k, k_norm, k_weight, k_bias, k_out, "k"))
-    elif k_norm != "none" or k_weight is not None or k_bias is not None or k_out is not None:
-        raise ValueError("k_norm, k_weight, k_bias and k_out need k")
-    for s, x, norm, w, b, o, name in streams:
-        s.x = _operand(x, bf16, name, dev, (T, -1, D))
-        s.H, s.norm = x.shape[1], _choice(abi.NORMS, norm, name + "_norm")
-        s.stride_t, s.stride_h = x.stride(0), x.stride(1)
-        s.weight = _operand(w, torch.float32, name + "_weight", dev, (a.norm_dim,))
-        s.bias = _operand(b, torch.float32, name + "_bias", dev, (a.norm_dim,))
-        if o is not None:
-            _operand(o, bf16, name + "_out", dev, (T, x.shape[1], D))
-    if a.rope:
-        if cos_sin is None:
-            raise ValueError("a rotation needs cos_sin")
-        _angles(a, cos_sin, dev)
-        if positions is None and q_indptr is None:
-            raise ValueError("a rotation needs positions, or q_indptr and seq_lens")
+    if q.dim() != 3:
+        _bad("q", q, "be [T, H, D]")
+    T, _, D = q.shape
+    dev = q.get_device()
+    if dev < 0:
+        raise ValueError("q must be a device tensor")
+    norm_dim = min(D, 512) if norm_dim is None else int(norm_dim)
+    if rot_off is None:
+        rot_off = 0 if D == 128 else D - abi.D_ROPE
+    rope = _choice(abi.ROPES, style, "style")
+    pcs, n_pos = _angles(cos_sin, dev) if rope else (None, 0)
+    pp = pi = pl = None
+    B = 0
     if positions is not None:
-        a.positions = _operand(positions, torch.int32, "positions", dev, (T,))
+        pp = _vector(positions, T, _I32, "positions", dev)
     elif q_indptr is not None:
         if seq_lens is None:
             raise ValueError("q_indptr needs seq_lens")
-        _chunk_fields(a, q_indptr, seq_lens, dev)
-    on = _On(dev, stream)
-    outs = []
-    for s, x, _, _, _, o, _ in streams:
-        if o is None:
-            o = on.empty(x.shape, bf16)
-        s.out, s.out_stride_t, s.out_stride_h = o.data_ptr(), o.stride(0), o.stride(1)
-        outs.append(o)
+        pi, pl, B = _sequences(q_indptr, seq_lens, dev)
+    elif rope:
+        raise ValueError("a rotation needs positions, or q_indptr and seq_lens")
+    on = _Stream(dev, stream)
+    qs, q_out = _normed_rows(q, q_norm, q_weight, q_bias, q_out, T, D, norm_dim, "q", dev, on)
+    if k is not None:
+        if k.dim() != 3:
+            _bad("k", k, "be [T, H, D]")
+        ks, k_out = _normed_rows(k, k_norm, k_weight, k_bias, k_out, T, D, norm_dim, "k", dev, on)
+    else:
+        if k_norm != "none" or k_weight is not None or k_bias is not None or k_out is not None:
+            raise ValueError("k_norm, k_weight, k_bias and k_out need k")
+        ks = abi.NormRopeRows()
+    a = abi.QkNormRopeArgs(qs, ks, pcs, n_pos, pp, pi, pl, T, B, D, norm_dim, rot_off, rope, 1 if inverse else 0, eps)
     on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", ctypes.byref(a))
-    return outs[0], outs[1] if k is not None else None
+    return q_out, k_out
+
+
+# the tensors of a cache -> (kv_format, width of its latent rows)
+_CACHES = {((_BF16, 576),): (abi.KV_BF16, 576), ((_U8, 656),): (abi.KV_FP8_656, 576),
+           ((_BF16, 512),): (abi.KV_BF16_D512, 512),
+           ((_U8, 512), (_U8, 16), (_BF16, 64)): (abi.KV_MXFP8, 576),
+           ((_U8, 512), (_BF16, 64)): (abi.KV_MXFP8_V4, 512)}
+_KV_NORMS = {None: None, "none": 0, "rms": 1}
 
 
 def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
@@ -783,95 +836,98 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     [..., 576], uint8 [..., 656], bf16 [..., 512], (uint8 [..., 512], uint8 [..., 16], bf16 [..., 64])
     for MXFP8 streams, or (uint8 [..., 512], bf16 [..., 64]) for V4 fp8 rows.  index_k bf16 [T, 128] goes
     to the same row of index_cache bf16 [..., 128], after index_norm and a rotation of its first 64
-    values.  Pages as in mla_decode (block_size defaults to the cache's dim before its last two's last:
-    [blocks, block_size, row]); sequence b's tokens q_indptr[b] .. q_indptr[b + 1] - 1 are its last
-    positions below seq_lens[b].  kv or index_k may be None."""
-    bf16, u8 = torch.bfloat16, torch.uint8
-    dev = q_indptr.device
-    a = abi.KvAppendArgs()
-    _chunk_fields(a, q_indptr, seq_lens, dev)
-    paged_like = None
+    values.  Pages as in mla_decode (block_size defaults to that of a cache [blocks, block_size, row]);
+    sequence b's tokens q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b].  kv
+    or index_k may be None."""
+    dev = q_indptr.get_device()
+    pi, pl, B = _sequences(q_indptr, seq_lens, dev)
+    T = rope = irope = 0
+    paged_like = index_cache
+    kvp = kst = pw = None
+    kst = rows = stride = sstride = rstride = fmt = kind = 0
+    pc = psc = pr = None
     if kv is not None:
-        parts = tuple(cache) if isinstance(cache, (tuple, list)) else (cache,)
-        kinds = tuple((t.dtype, t.shape[-1]) for t in parts)
-        formats = {((bf16, 576),): (abi.KV_BF16, 576), ((u8, 656),): (abi.KV_FP8_656, 576),
-                   ((bf16, 512),): (abi.KV_BF16_D512, 512),
-                   ((u8, 512), (u8, 16), (bf16, 64)): (abi.KV_MXFP8, 576),
-                   ((u8, 512), (bf16, 64)): (abi.KV_MXFP8_V4, 512)}
-        if kinds not in formats:
-            raise ValueError(f"cache is of no known format: {kinds}")
-        a.kv_format, width = formats[kinds]
-        a.kv = _operand(kv, bf16, "kv", dev, (-1, width))
-        a.T, a.kv_stride_t = kv.shape[0], kv.stride(0)
-        rows = [t.numel() // t.shape[-1] for t in parts]
-        if len(set(rows)) != 1:
-            raise ValueError("the cache's streams must have the same rows")
-        a.cache_rows = rows[0]
-        ptrs = [_operand(t, t.dtype, "cache", dev) for t in parts]
-        strides = [_row_stride(t, "cache") for t in parts]
-        a.cache, a.stride_row = ptrs[0], strides[0]
+        parts = cache if isinstance(cache, (tuple, list)) else (cache,)
+        found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
+        if found is None:
+            raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
+        fmt, width = found
+        kvp = _addr(kv, _BF16, "kv", dev)
+        if kv.dim() != 2 or kv.shape[1] != width or kv.stride(1) != 1:
+            _bad("kv", kv, f"be [T, {width}] with a dense last dim")
+        T, kst = kv.shape[0], kv.stride(0)
+        paged_like = first = parts[0]
+        pc = _addr(first, first.dtype, "cache", dev)
+        rows, stride = _rows(first, first.shape[-1], "cache")
         if len(parts) > 1:
-            a.cache_rope, a.rope_stride_row = ptrs[-1], strides[-1]
-        if len(parts) == 3:
-            a.cache_scale, a.scale_stride_row = ptrs[1], strides[1]
-        a.norm = _choice({"none": 0, "rms": 1}, norm or ("rms" if weight is not None else "none"), "norm")
-        a.weight = _operand(weight, torch.float32, "weight", dev, (512,))
-        a.rope = _choice(abi.ROPES, style, "style")
-        paged_like = parts[0]
-    a.eps = float(eps)
-    a.index_eps = float(eps if index_eps is None else index_eps)
+            last = parts[-1]
+            pr = _addr(last, _BF16, "cache", dev)
+            more, rstride = _rows(last, 64, "cache")
+            if len(parts) == 3:
+                psc = _addr(parts[1], _U8, "cache", dev)
+                others, sstride = _rows(parts[1], 16, "cache")
+                more = more if others == rows else -1
+            if more != rows:
+                raise ValueError("the cache's streams must have the same rows")
+        kind = _choice(_KV_NORMS, norm, "norm")
+        if kind is None:
+            kind = 0 if weight is None else 1
+        pw = _vector(weight, 512, _F32, "weight", dev)
+        rope = _choice(abi.ROPES, style, "style")
+    ip = iw = ib = ic = None
+    ist = irows = istride = ikind = 0
     if index_k is not None:
         if index_cache is None:
             raise ValueError("index_k needs index_cache")
-        a.index_k = _operand(index_k, bf16, "index_k", dev, (-1, 128))
-        if kv is not None and index_k.shape[0] != kv.shape[0]:
+        ip = _addr(index_k, _BF16, "index_k", dev)
+        if index_k.dim() != 2 or index_k.shape[1] != 128 or index_k.stride(1) != 1:
+            _bad("index_k", index_k, "be [T, 128] with a dense last dim")
+        if kv is not None and index_k.shape[0] != T:
             raise ValueError("kv and index_k must have the same rows")
-        a.T, a.index_stride_t = index_k.shape[0], index_k.stride(0)
-        a.index_cache = _operand(index_cache, bf16, "index_cache", dev)
+        T, ist = index_k.shape[0], index_k.stride(0)
+        ic = _addr(index_cache, _BF16, "index_cache", dev)
         if index_cache.shape[-1] != 128:
-            raise ValueError("index_cache must be bf16 [..., 128]")
-        a.index_rows, a.index_stride_row = index_cache.numel() // 128, _row_stride(index_cache, "index_cache")
-        a.index_norm = _choice(abi.NORMS, index_norm, "index_norm")
-        a.index_weight = _operand(index_weight, torch.float32, "index_weight", dev, (128,))
-        a.index_bias = _operand(index_bias, torch.float32, "index_bias", dev, (128,))
-        a.index_rope = _choice(abi.ROPES, index_style, "index_style")
-        paged_like = index_cache if paged_like is None else paged_like
-    if a.rope or a.index_rope:
-        if cos_sin is None:
-            raise ValueError("a rotation needs cos_sin")
-        _angles(a, cos_sin, dev)
-    if block_table is not None and block_size is None and paged_like is not None and paged_like.dim() >= 3:
-        block_size = paged_like.shape[-2]
-    _page_fields(a, block_table, block_size, kv_batch_stride, a.B, dev)
-    _On(dev, stream).call(load_library().dsa_kv_append, "dsa_kv_append", ctypes.byref(a))
+            _bad("index_cache", index_cache, "be [..., 128]")
+        irows, istride = _rows(index_cache, 128, "index_cache")
+        ikind = _choice(abi.NORMS, index_norm, "index_norm")
+        iw = _vector(index_weight, 128, _F32, "index_weight", dev)
+        ib = _vector(index_bias, 128, _F32, "index_bias", dev)
+        irope = _choice(abi.ROPES, index_style, "index_style")
+    pcs, n_pos = _angles(cos_sin, dev) if rope or irope else (None, 0)
+    pt, tst, blocks, bs = _pages(block_table, block_size, paged_like, B, dev)
+    a = abi.KvAppendArgs(kvp, kst, pw, pc, psc, pr, rows, stride, sstride, rstride, fmt, kind, rope, ikind, irope,
+                         ip, ist, iw, ib, ic, irows, istride, pcs, n_pos, pi, pl, pt, tst, blocks, bs,
+                         kv_batch_stride, T, B, eps, eps if index_eps is None else index_eps)
+    _Stream(dev, stream).call(load_library().dsa_kv_append, "dsa_kv_append", ctypes.byref(a))
 
 
 def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, block_table=None, block_size=None,
                     kv_batch_stride=0, causal=True, max_kv_len=None, num_splits=0):
-    dev = q.device
-    a = abi.ChunkArgs()
-    a.q = _operand(q, torch.bfloat16, "q", dev, (-1, -1, abi.D_QK))
-    a.T, a.H = q.shape[0], q.shape[1]
-    a.q_stride_t, a.q_stride_h = q.stride(0), q.stride(1)
-    _chunk_fields(a, q_indptr, seq_lens, dev)
-    a.kv_format, a.kv_total_rows, a.kv_stride_row = kv_format_of(kv_cache)
-    a.kv_cache = _operand(kv_cache, kv_cache.dtype, "kv_cache", dev)
-    if block_table is not None and block_size is None and kv_cache.dim() >= 3:
-        block_size = kv_cache.shape[-2]
-    _page_fields(a, block_table, block_size, kv_batch_stride, a.B, dev)
+    dev = q.get_device()
+    if q.dim() != 3:
+        _bad("q", q, "be [T, H, 576]")
+    T, H, _ = q.shape
+    pq, qt, qh = _addr3(q, T, H, abi.D_QK, "q", dev)
+    pi, pl, B = _sequences(q_indptr, seq_lens, dev)
+    width = kv_cache.shape[-1]
+    fmt = _CACHES.get(((kv_cache.dtype, width),), (-1, 0))[0]
+    if fmt != abi.KV_BF16 and fmt != abi.KV_FP8_656:
+        raise ValueError(f"kv cache must be bf16 [..., 576] or uint8 [..., 656], got {kv_cache.dtype} "
+                         f"{tuple(kv_cache.shape)}")
+    pk = _addr(kv_cache, kv_cache.dtype, "kv_cache", dev)
+    rows, stride = _rows(kv_cache, width, "kv_cache")
+    pt, tst, blocks, bs = _pages(block_table, block_size, kv_cache, B, dev)
     if max_kv_len is None:
-        max_kv_len = (block_table.shape[1] * int(block_size) if block_table is not None
-                      else int(kv_batch_stride) or a.kv_total_rows)
-    if out is not None:
-        a.out = _operand(out, torch.bfloat16, "out", dev, (a.T, a.H, abi.D_VO))
-        a.o_stride_t, a.o_stride_h = out.stride(0), out.stride(1)
+        max_kv_len = blocks * bs if block_table is not None else int(kv_batch_stride) or rows
+    po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev) if out is not None else (None, 0, 0)
     if lse is not None:
-        a.lse = _operand(lse, torch.float32, "lse", dev, (a.T, a.H))
-        if not lse.is_contiguous():
-            raise ValueError("lse must be contiguous")
-    a.causal, a.max_kv_len, a.num_splits = (1 if causal else 0), int(max_kv_len), int(num_splits)
-    a.sm_scale = float(sm_scale)
-    return a
+        ps = _addr(lse, _F32, "lse", dev)
+        if lse.shape != (T, H) or not lse.is_contiguous():
+            _bad("lse", lse, f"be a dense [{T}, {H}]")
+    else:
+        ps = None
+    return abi.ChunkArgs(pq, qt, qh, pi, pl, pk, rows, stride, fmt, bs, pt, tst, kv_batch_stride, po, ot, oh, ps,
+                         blocks, T, B, H, 1 if causal else 0, max_kv_len, num_splits, sm_scale)
 
 
 def chunk_num_splits(args) -> int:
@@ -900,19 +956,25 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b] (their own rows already
     in the cache) and attend positions up to their own (causal) or all.  Rows of no sequence are left as
     allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold)."""
+    dev = q.get_device()
+    if dev < 0 or q.dim() != 3:
+        _bad("q", q, "be a device tensor [T, H, 576]")
+    on = _Stream(dev, stream)
+    T, H, _ = q.shape
+    if out is None:
+        out = on.empty(q, (T, H, abi.D_VO), _BF16)
+    if lse is None:
+        lse = on.empty(q, (T, H), _F32)
     a = make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, block_table=block_table,
                         block_size=block_size, kv_batch_stride=kv_batch_stride, causal=causal,
                         max_kv_len=max_kv_len, num_splits=num_splits)
-    on = _On(q.device, stream)
-    if out is None:
-        out = on.empty((a.T, a.H, abi.D_VO), torch.bfloat16)
-        a.out, a.o_stride_t, a.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    if lse is None:
-        lse = on.empty((a.T, a.H), torch.float32)
-        a.lse = lse.data_ptr()
     need = chunk_workspace_size(a)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = on.empty((need,), torch.uint8)
-    ws = _operand(workspace, workspace.dtype, "workspace", q.device) if need else None
+    ws = None
+    if need:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = on.empty(q, (need,), _U8)
+        elif not workspace.is_contiguous():
+            _bad("workspace", workspace, "be dense")
+        ws = _addr(workspace, workspace.dtype, "workspace", dev)
     on.call(load_library().dsa_mla_chunk, "dsa_mla_chunk", ctypes.byref(a), ws, need)
     return out, lse
