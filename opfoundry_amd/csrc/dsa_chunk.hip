@@ -814,7 +814,11 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 // Two barriers a tile; one workgroup's waits are the other's time.
 // ---------------------------------------------------------------------------
 constexpr int NARROW = 32;                   // rows of a workgroup
-constexpr int NSTRIDE = 1040;                // a tile's NoPE rows; piece c of row r at c ^ 4 (r % 4)
+// A tile in LDS: NoPE rows of 1 KB, piece c of row r at c ^ nsw(r), so that neither the K reads (one piece of
+// 16 rows: 16 values of nsw) nor the transposed V reads (four pieces of four rows: their pieces part at bit 2)
+// meet a bank twice; with 1040-byte rows and c ^ 4 (r % 4) conflicts took 400 of a tile's 880 LDS cycles.
+constexpr int NSTRIDE = 1024;
+__device__ __forceinline__ int nsw(int r) { return 4 * (r & 3) + ((r >> 2) & 3); }
 constexpr int NROPE_OFF = TILE * NSTRIDE;
 constexpr int NTILE = NROPE_OFF + TILE * 128;
 constexpr int NLIST = 512;                   // entries of the row list
@@ -841,7 +845,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     __shared__ int32_t s_rows[NLIST];        // RUNS: the first row of every tile; else every position's
     __shared__ float s_top[2][NARROW];
     __shared__ uint32_t s_nan;               // bit j: position j's row holds a NaN or infinity
-    __shared__ int32_t s_misc[2];
+    __shared__ int32_t s_misc[3];            // [0] a row that may be read, [1] again, [2] a scale out of range
     const lds_ptr T0 = (lds_ptr)s_tile, PX = (lds_ptr)s_p;
 
     const int lane = threadIdx.x & 63;
@@ -927,7 +931,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
             for (int e = 0; e < 8; ++e) {
                 const int r = 8 * wave + e;
                 const uint32_t at = __builtin_amdgcn_readfirstlane(row_at(base, has, i, r));
-                lds_dma16_s(p.kv + (uint64_t)at * (uint32_t)p.row_bytes, 16u * (unsigned)(ln ^ 4 * (r & 3)), tb + r * NSTRIDE);
+                lds_dma16_s(p.kv + (uint64_t)at * (uint32_t)p.row_bytes, 16u * (unsigned)(ln ^ nsw(r)), tb + r * NSTRIDE);
             }
             const int r = 8 * wave + (ln >> 3);
             lds_dma16(p.kv + (uint64_t)row_at(base, has, i, r) * (uint32_t)p.row_bytes + 1024 + 16 * ((ln & 7) ^ rope_sw(r)),
@@ -956,7 +960,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         }
         asm volatile("" ::: "memory");
     };
-    // (as in the tiled kernel: rows that some row of the block does not attend must not reach it)
+    // (as in the tiled kernel: rows that some row of the block does not attend must not reach it; of 656-byte
+    // rows one with a scale out of range too)
     auto scan = [&](int slot) {
         const int ln = opaque(lane);
         uint32_t bad = 0;
@@ -981,9 +986,15 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
                 unsigned odd = 0;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) odd |= ((v[w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                // (its scales, each by one lane)
+                const lds_ptr sp = slot_of(slot) + (8 * wave + 2 * e + (ln >> 5)) * FP8_ROW + 512 + 4 * (ln & 3);
+                if (lds_ld<unsigned>(sp) >= FP8_SCALE_LIMIT_BITS) odd = 1;
                 const uint64_t who = __builtin_amdgcn_ballot_w64(odd != 0);
                 const bool lo = (uint32_t)who != 0, up = (who >> 32) != 0;
-                if (ln < 32 ? lo : up) lds_st<u32x4>(tb + 2 * e * FP8_ROW, u32x4{0, 0, 0, 0});
+                if (ln < 32 ? lo : up) {
+                    lds_st<u32x4>(tb + 2 * e * FP8_ROW, u32x4{0, 0, 0, 0});
+                    lds_st<unsigned>(sp, 0u);
+                }
                 bad |= (lo ? 1u : 0u) << (2 * e) | (up ? 2u : 0u) << (2 * e);
             }
         }
@@ -994,15 +1005,18 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     f32x16 o[4];
     float m_ref = 0.0f, l_lane = 0.0f, p_top = 0.0f;
     bool any = false;
+    // 656-byte rows: a scale outside [0, 128) in a tile that every row of the block attends whole (in others
+    // scan() has seen to it): all of them are NaN
+    bool range_bad = false;
 
     // S^T[4 positions of this lane x its row]
     auto qk = [&](lds_cptr kt) -> f32x4 {
         const int ln = opaque(lane), lq = ln >> 4, lr = 16 * half + (ln & 15);
         if constexpr (!FP8) {
             const lds_cptr kn = kt + lr * NSTRIDE, kr = kt + NROPE_OFF + 128 * lr;
-            // pieces 4 ks + lq, at their places: ks % 4 picks the two bits that the row flips
+            const int sw = nsw(lr);
             auto k_at = [&](int ks) -> lds_cptr {
-                return ks < 16 ? kn + 256 * (ks >> 2) + 16 * ((4 * (ks & 3) + lq) ^ 4 * (lr & 3)) : kr + 16 * ((4 * (ks - 16) + lq) ^ rope_sw(lr));
+                return ks < 16 ? kn + 256 * (ks >> 2) + 16 * ((4 * (ks & 3) + lq) ^ sw) : kr + 16 * ((4 * (ks - 16) + lq) ^ rope_sw(lr));
             };
             constexpr int AHEAD = 6;
             u32x4 kb[AHEAD];
@@ -1011,41 +1025,69 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
             f32x4 a = {}, b = {};
 #pragma unroll
             for (int ks = 0; ks < KS / 2; ++ks) {
+                __builtin_amdgcn_sched_barrier(0);
                 if (ks & 1) b = mfma16(kb[ks % AHEAD], qf[ks], b);
                 else a = mfma16(kb[ks % AHEAD], qf[ks], a);
                 if (ks + AHEAD < KS / 2) kb[ks % AHEAD] = lds_ld<u32x4>(k_at(ks + AHEAD));
             }
             return a + b;
         } else {
-            const lds_cptr kn = kt + lr * FP8_ROW + 16 * lq;
-            u32x4 kb[10];
+            // With the scores, between their matrix instructions, V of the tile goes to T0 as fp16: each wave
+            // converts the dims that it reads, piece (u, m) = rows 16 u .. +15, dims 128 wave + 32 m .. +31 (as
+            // the tiled kernel does)
+            const int vr = ln >> 2;
+            u32x2 codes[8];
+            float vs[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) kb[j] = lds_ld<u32x4>(kn + 64 * j);
-            kb[8] = lds_ld<u32x4>(kn + 528);
-            kb[9] = lds_ld<u32x4>(kn + 528 + 64);
+            for (int u = 0; u < 2; ++u) {
+                const lds_cptr r = kt + (16 * u + vr) * FP8_ROW;
+                vs[u] = lds_ld<float>(r + 512 + 4 * wave);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) codes[4 * u + m] = lds_ld<u32x2>(r + 128 * wave + 32 * m + 8 * (ln & 3));
+            }
+            const lds_cptr kn = kt + lr * FP8_ROW + 16 * lq;
+            auto k_at = [&](int j) -> lds_cptr { return j < 8 ? kn + 64 * j : kn + 528 + 64 * (j - 8); };
+            constexpr int AHEAD = 4;
+            u32x4 kb[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) kb[j] = lds_ld<u32x4>(k_at(j));
             // a position's four scales
             f32x4 sc[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sc[r] = lds_ld<f32x4>(kt + (16 * half + 4 * lq + r) * FP8_ROW + 512);
             f32x4 s = {}, g[4];
+            f16x2 mm;
+            float vsc;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                g[i] = f32x4{};
+            for (int j = 0; j < 8; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                if ((j & 1) == 0) g[j >> 1] = f32x4{};
+                const u32x4 k = kb[j % AHEAD];
+                g[j >> 1] = mfma16(codes_bf16(k[0], k[1]), qf[2 * j], g[j >> 1]);
+                g[j >> 1] = mfma16(codes_bf16(k[2], k[3]), qf[2 * j + 1], g[j >> 1]);
+                if (j + AHEAD < 10) kb[j % AHEAD] = lds_ld<u32x4>(k_at(j + AHEAD));
+                if (j == 5) {
 #pragma unroll
-                for (int j = 2 * i; j < 2 * i + 2; ++j) {
-                    g[i] = mfma16(codes_bf16(kb[j][0], kb[j][1]), qf[2 * j], g[i]);
-                    g[i] = mfma16(codes_bf16(kb[j][2], kb[j][3]), qf[2 * j + 1], g[i]);
+                    for (int r = 0; r < 4; ++r) sc[r] = lds_ld<f32x4>(kt + (16 * half + 4 * lq + r) * FP8_ROW + 512);
                 }
+                if ((j & 3) == 0) {
+                    vsc = vs[j >> 2];
+                    range_bad |= __float_as_uint(vsc) >= FP8_SCALE_LIMIT_BITS;
+                    const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(vsc) & 0x007FFFFFu) | 0x3F800000u);
+                    mm = f16x2{m16, m16};
+                }
+                const u32x2 c = codes[j];
+                const u32x4 v = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], vsc, false) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], vsc, true) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], vsc, false) * mm),
+                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], vsc, true) * mm)};
+                const int r = 16 * (j >> 2) + vr;
+                lds_st<u32x4>(T0 + r * NSTRIDE + 256 * wave + 16 * ((4 * (j & 3) + (ln & 3)) ^ nsw(vr)), v);
             }
-            s = mfma16(kb[8], qf[16], s);
-            s = mfma16(kb[9], qf[17], s);
+            s = mfma16(kb[8 % AHEAD], qf[16], s);
+            s = mfma16(kb[9 % AHEAD], qf[17], s);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = __float_as_uint(sc[r][i]) >= FP8_SCALE_LIMIT_BITS ? __builtin_nanf("") : sc[r][i];
-                    s[r] = __builtin_fmaf(g[i][r], f, s[r]);
-                }
+                for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(g[i][r], sc[r][i], s[r]);
             return s;
         }
     };
@@ -1094,47 +1136,34 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         // (the order of a lane's eight positions in the product: 4 hi .. +3, then 8 + 4 hi .. +3)
         lds_st<u32x2>(PX + ((2 * half + (q & 1)) * 32 + my) * 16 + 8 * (q >> 1), w);
     };
-    // 656-byte rows: V of the raw tile as fp16, each wave the dims that it reads (as in the tiled kernel)
-    auto dequant = [&](lds_cptr rb) {
-        const int ln = opaque(lane);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = 16 * u + (ln >> 2);
-            const float s = lds_ld<float>(rb + r * FP8_ROW + 512 + 4 * wave);
-            const float sc = __float_as_uint(s) >= FP8_SCALE_LIMIT_BITS ? 0.0f : s;
-            const _Float16 m16 = (_Float16)__uint_as_float((__float_as_uint(sc) & 0x007FFFFFu) | 0x3F800000u);
-            const f16x2 mm = {m16, m16};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const u32x2 c = lds_ld<u32x2>(rb + r * FP8_ROW + 128 * wave + 32 * m + 8 * (ln & 3));
-                const u32x4 v = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], sc, false) * mm),
-                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[0], sc, true) * mm),
-                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], sc, false) * mm),
-                                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[1], sc, true) * mm)};
-                lds_st<u32x4>(T0 + r * NSTRIDE + 256 * wave + 16 * ((4 * m + (ln & 3)) ^ 4 * (r & 3)), v);
-            }
-        }
-    };
     auto pv = [&](lds_cptr vt) {
         const int ln = opaque(lane), lhi = ln >> 5;
         const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
         const int vx = 2 * (g16 & 1) + (pp >> 1);
         const lds_cptr v0 = vt + (4 * lhi + rr) * NSTRIDE + 256 * wave + 8 * (pp & 1);
+        auto v_frag = [&](int i) -> u32x4 {
+            const lds_cptr at = v0 + 16 * (i >> 2) * NSTRIDE;
+            const int c = (4 * (i & 3) + vx) ^ (4 * rr + lhi);                // row 8 further on: nsw + 2
+            const s16x4 va = lds_read_tr16(at + 16 * c), vb = lds_read_tr16(at + 8 * NSTRIDE + 16 * (c ^ 2));
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        u32x4 pb[2], v[3];
+        pb[0] = lds_ld<u32x4>(PX + (lhi * 32 + (ln & 31)) * 16);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const u32x4 pb = lds_ld<u32x4>(PX + ((2 * u + lhi) * 32 + (ln & 31)) * 16);
+        for (int i = 0; i < 3; ++i) v[i] = v_frag(i);
+        pb[1] = lds_ld<u32x4>(PX + ((2 + lhi) * 32 + (ln & 31)) * 16);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const lds_cptr at = v0 + 16 * u * NSTRIDE + 16 * ((4 * m + vx) ^ 4 * rr);
-                const s16x4 va = lds_read_tr16(at), vb = lds_read_tr16(at + 8 * NSTRIDE);
-                o[m] = mfma32<FP8>(__builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[m]);
-            }
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            o[i & 3] = mfma32<FP8>(v[i % 3], pb[i >> 2], o[i & 3]);
+            if (i + 3 < 8) v[i % 3] = v_frag(i + 3);
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + span - 1) / span) : 0;
     auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * span); };
-    bool first = true;
+    bool first = true, all_nan = false;
     for (bool again = false;;) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) o[m] = f32x16{};
@@ -1148,6 +1177,10 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
             uint32_t has = has_of(b0, 0, c0), has1 = ntiles > 1 ? has_of(b1, 1, c0) : 0;
             issue(b0, has, 0, 0);
             if (FP8 && ntiles > 1) issue(b1, has1, 1, 1);
+            // Q is waited for here, with the first tiles' loads in flight: left to its first use, the compiler's
+            // wait would stand in the loop and drain every tile's loads
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks) asm volatile("" : "+v"(qf[ks]));
             for (int i = 0; i < ntiles; ++i) {
                 const int slot = i & 1;
                 // tile i, the older of those in flight, has landed
@@ -1163,7 +1196,6 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
                 if (!FP8 && i + 1 < ntiles) issue(b1, has1, i + 1, slot ^ 1);
                 const int32_t ahead = base_of(i + 2);
                 f32x4 s = qk(slot_of(slot));
-                if constexpr (FP8) dequant(slot_of(slot));
                 mask(s, has, i, c0);
                 if (first) {
                     const float top = top_of(s) * c_s;
@@ -1187,7 +1219,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         const uint64_t anys = __builtin_amdgcn_ballot_w64(any);
         any = ((anys >> (lane & 15)) & 0x0001000100010001ull) != 0;
         __syncthreads();
-        if (threadIdx.x == 0) s_misc[1] = 0;
+        if (threadIdx.x == 0) s_misc[1] = 0, s_misc[2] = 0;
         if (q == 0) s_top[half][my] = any ? l : 0.0f;
         __syncthreads();
         l = s_top[0][my] + s_top[1][my];
@@ -1198,8 +1230,10 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         any = t >= 0.0f;
         const bool held = FP8 ? t >= 0.5f && t < 0x1p15f : l > 0x1p-40f;
         if (!again && any && !(held && l < 0x1p100f)) s_misc[1] = 1;
+        if (FP8 && range_bad) s_misc[2] = 1;
         l_lane = l;
         __syncthreads();
+        all_nan = too_long || s_misc[2] != 0;
         if (again || __builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
         again = true;
         p_top = 0.0f;
@@ -1226,16 +1260,16 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     }
 
     // ---- O / l, LSE: rows' values from the scoring lanes to the lanes that hold O ----
-    const float lse = too_long ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l_lane)) * LN2;
+    const float lse = all_nan ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l_lane)) * LN2;
     __syncthreads();
     if (q == 0 && half == 0) {
-        s_top[0][my] = too_long ? __builtin_nanf("") : (any ? 1.0f / l_lane : 0.0f);
+        s_top[0][my] = all_nan ? __builtin_nanf("") : (any ? 1.0f / l_lane : 0.0f);
         const int64_t at = (int64_t)blk.first * p.H + blk.r0 + my;
         if (my >= blk.rows) {
         } else if (p.ns > 1) {
-            p.part_lse[(int64_t)split * p.T * p.H + at] = any ? lse : -FLT_MAX;
+            p.part_lse[(int64_t)split * p.T * p.H + at] = any || all_nan ? lse : -FLT_MAX;
         } else if (p.lse) {
-            p.lse[at] = any || too_long ? lse : INFINITY;
+            p.lse[at] = any || all_nan ? lse : INFINITY;
         }
     }
     __syncthreads();
