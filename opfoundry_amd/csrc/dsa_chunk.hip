@@ -4,7 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
-#include <stdlib.h>
+#include <cmath>
 #include <algorithm>
 #include <type_traits>
 
@@ -36,6 +36,7 @@ struct ChunkParams {
     float* part_o;       // fp32 partials [split][t][h][512] and their LSE [split][t][h] (log2 units kept as ln)
     float* part_lse;
     int32_t T, B, H, causal, max_len, ns, per_split;
+    int32_t common;      // of H and the rows of a block (block_start)
     float scale_log2;
 };
 
@@ -123,7 +124,7 @@ struct Block {
     int32_t len, end;          // positions; token t is position len - end + t
 };
 __device__ __forceinline__ Block find_block(const ChunkParams& p, int64_t x, int32_t m) {
-    auto start = [&](int32_t i) { return dsa_seq::block_start(min(max(p.indptr[i], 0), p.T), i, p.H, m); };
+    auto start = [&](int32_t i) { return dsa_seq::block_start(min(max(p.indptr[i], 0), p.T), i, p.H, m, p.common); };
     Block k{};
     k.b = count_upto(p.B, x, start);
     if (k.b >= p.B) return k;
@@ -1376,17 +1377,67 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 
 // ------------------------------------------------------------------- host
 
-int splits_of(const dsa_mla_chunk_args* a, int32_t* per) {
-    int ns = a->num_splits;
-    if (ns == 0) {
-        // about two workgroups per CU, at least 256 positions each
-        const int64_t blocks = std::max<int64_t>(1, (int64_t)a->T * a->H / 32);
-        const int64_t want = std::max<int64_t>(1, 2 * CUS / blocks);
-        ns = (int)std::min<int64_t>({want, std::max(1, a->max_kv_len / 256), DSA_MLA_MAX_SPLITS});
+// The kernel and split count of a call: those of least expected time, from the call's sizes
+// alone.  A workgroup takes `start` us and `tile` us for each 32 positions (`pair` where two
+// share a CU); past one workgroup a CU (two of the narrow kernel) they run in rounds; the
+// cache's rows come at most at `BYTES_US` (splits of a sequence and blocks of rows find each
+// other's in the caches); a split writes and reads its fp32 partials.  Fitted to 3600 calls of
+// both kernels (1 to 200 sequences of 1 to 400 tokens, 1 to 128 heads, 64 to 60000 positions,
+// 1 to 64 splits): the choice is 1.9 % above the fastest candidate on average, 27 % at most
+// (15 tokens of 32 heads over 21979 bf16 rows, 75 us in 32 splits and 59 in 48).  Measured on
+// the two sides of it, us: one token of 128 heads over 1501 rows, 128-row blocks 25.2, 32-row 17.7;
+// 256 of 16 heads over 4096 302 and 217; 200 of 128 heads over 1000 78 and 120; 512 tokens of
+// 16 heads over the same 4096 rows 90 (4 splits) and 120.
+struct Kernel {
+    float start, tile, pair;
+};
+constexpr Kernel KERNELS[2][2] = {       // [656-byte rows][narrow]
+    {{6.3f, 1.83f, 0.0f}, {6.4f, 1.15f, 1.81f}},
+    {{10.6f, 2.47f, 0.0f}, {8.3f, 1.48f, 2.07f}},
+};
+constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f, PART_BYTES_US = 5.3e6f;
+constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+
+struct Plan {
+    bool narrow;
+    int ns;
+    int32_t per;         // positions of a split
+};
+
+float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int ns) {
+    const bool fp8 = a->kv_format == DSA_KV_FP8_656;
+    const Kernel& k = KERNELS[fp8][narrow];
+    const int64_t tiles = (a->max_kv_len + (int64_t)TILE - 1) / TILE, each = (tiles + ns - 1) / ns;
+    const float groups = (float)blocks * ns;
+    auto in_rounds = [](float us, float rounds) {
+        return us * (rounds <= 1.0f ? 1.0f : rounds <= 3.0f ? std::ceil(rounds) : rounds + 0.5f);
+    };
+    float us = narrow && groups > CUS ? in_rounds(k.start + each * k.pair, groups / (2 * CUS))
+                                      : in_rounds(k.start + each * k.tile, groups / CUS);
+    const float row = fp8 ? DSA_MLA_FP8_ROW_BYTES : DSA_MLA_BF16_ROW_BYTES;
+    us = std::max(us, FIRST_US + (float)a->B * a->max_kv_len * row / BYTES_US);
+    if (ns > 1) us += JOIN_US + (float)ns * a->T * a->H * (2 * 4 * (D_VO + 1)) / PART_BYTES_US;
+    return us;
+}
+
+Plan plan_of(const dsa_mla_chunk_args* a) {
+    Plan best{};
+    float least = INFINITY;
+    for (int n = 0; n < 2; ++n) {
+        const int32_t m = n ? NARROW : BLOCK;
+        const int64_t blocks = dsa_seq::block_start(a->T, a->B, a->H, m, dsa_seq::common(a->H, m));
+        for (const int c : COUNTS) {
+            const int ns = a->num_splits ? a->num_splits : c;
+            // (a split of fewer positions than a tile is none; 64 splits of a grid's y extent)
+            if (ns > 1 && !a->num_splits && (int64_t)a->max_kv_len < (int64_t)ns * TILE) break;
+            const float us = expected_us(a, n != 0, blocks, ns);
+            if (us < least) least = us, best.narrow = n != 0, best.ns = ns;
+            if (a->num_splits) break;
+        }
     }
-    const int64_t each = (a->max_kv_len + (int64_t)ns - 1) / ns;
-    *per = (int32_t)std::min<int64_t>(INT32_MAX - TILE + 1, std::max<int64_t>(TILE, (each + TILE - 1) / TILE * TILE));
-    return ns;
+    const int64_t each = (a->max_kv_len + (int64_t)best.ns - 1) / best.ns;
+    best.per = (int32_t)std::min<int64_t>(INT32_MAX - TILE + 1, std::max<int64_t>(TILE, (each + TILE - 1) / TILE * TILE));
+    return best;
 }
 
 size_t workspace_of(int ns, int64_t T, int64_t H) {
@@ -1433,8 +1484,7 @@ int dsa_mla_chunk_num_splits(const dsa_mla_chunk_args* a, int32_t* num_splits) {
     if (!num_splits) return DSA_ERR_NULL_POINTER;
     const int rc = validate(a);
     if (rc) return rc;
-    int32_t per;
-    *num_splits = splits_of(a, &per);
+    *num_splits = plan_of(a).ns;
     return DSA_OK;
 }
 
@@ -1442,8 +1492,7 @@ int dsa_mla_chunk_workspace_size(const dsa_mla_chunk_args* a, size_t* bytes) {
     if (!bytes) return DSA_ERR_NULL_POINTER;
     const int rc = validate(a);
     if (rc) return rc;
-    int32_t per;
-    *bytes = a->B == 0 ? 0 : workspace_of(splits_of(a, &per), a->T, a->H);
+    *bytes = a->T == 0 || a->B == 0 ? 0 : workspace_of(plan_of(a).ns, a->T, a->H);
     return DSA_OK;
 }
 
@@ -1452,7 +1501,9 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     if (rc) return rc;
     if (a->T == 0 || a->B == 0) return DSA_OK;
     ChunkParams p{};
-    p.ns = splits_of(a, &p.per_split);
+    const Plan plan = plan_of(a);
+    p.ns = plan.ns;
+    p.per_split = plan.per;
     const size_t need = workspace_of(p.ns, a->T, a->H);
     if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return DSA_ERR_WORKSPACE;
     p.q = (const __bf16*)a->q;
@@ -1471,21 +1522,16 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
-    const bool narrow = getenv("DSA_NARROW") != nullptr;
+    const bool narrow = plan.narrow;
     const bool runs = !a->block_table || a->block_size % TILE == 0;
-    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, narrow ? NARROW : BLOCK), (unsigned)p.ns);
+    const int32_t m = narrow ? NARROW : BLOCK;
+    p.common = dsa_seq::common(a->H, m);
+    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, m, p.common), (unsigned)p.ns);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
-    if (narrow && a->kv_format == DSA_KV_BF16) {
-        if (runs) launch(dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true>);
-        else launch(dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);
-    } else if (narrow) {
-        if (runs) launch(dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true>);
-        else launch(dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
-    }
-    else if (a->kv_format == DSA_KV_BF16)
-        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_BF16>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656>, blocks, dim3(NTHR), 0, (hipStream_t)stream, p);
+    const bool fp8 = a->kv_format == DSA_KV_FP8_656;
+    if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
+    else if (fp8) launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
+    else launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);
     if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;
     if (p.ns > 1) {
         const int64_t rows = (int64_t)a->T * a->H;

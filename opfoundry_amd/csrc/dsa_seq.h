@@ -53,12 +53,23 @@ __host__ __device__ inline int64_t position_of(const int32_t* indptr, const int3
     return (int64_t)lens[b] - indptr[b + 1] + t;
 }
 
-// Blocks of `m` rows that a grid gives sequence b, whose tokens have H rows each:
-// sequence b starts at block_start(b), its own blocks come first among those up to
-// block_start(b + 1), and the grid has block_start(B) of them, which needs no count
-// of the sequences before it.  floor((a + n) / m) - floor(a / m) + 1 >= ceil(n / m).
-__host__ __device__ inline int64_t block_start(int64_t indptr_b, int32_t b, int32_t H, int32_t m) {
-    return indptr_b * H / m + b;
+// Blocks of `m` rows that a grid gives sequence b, whose tokens have H rows each: sequence b
+// starts at block_start(b), its own blocks come first among those up to block_start(b + 1), and
+// the grid has block_start(B) of them, which needs no count of the sequences before it.  With
+// g = gcd(H, m) a sequence's rows are a multiple of g, so that it leaves at most m - g of its
+// last block unused, and that much is added for each: with A = indptr_b H + b (m - g),
+// floor((A + n H + m - g) / m) - floor(A / m) >= ceil(n H / m).  (A whole block for each would
+// leave every second block of single tokens with H = m empty, and with them every second XCD.)
+__host__ __device__ inline int32_t common(int32_t H, int32_t m) {
+    while (m) {
+        const int32_t r = H % m;
+        H = m;
+        m = r;
+    }
+    return H;
+}
+__host__ __device__ inline int64_t block_start(int64_t indptr_b, int32_t b, int32_t H, int32_t m, int32_t g) {
+    return (indptr_b * H + (int64_t)b * (m - g)) / m;
 }
 
 }  // namespace dsa_seq

@@ -154,30 +154,36 @@ def attend64(c: Chunk, q, kv, causal, sm_scale=SM_SCALE, max_len=None):
     N = torch.zeros_like(o)
     A, lse, E = torch.zeros_like(o), torch.full((T, H), float("nan"), dtype=torch.float64, device=dev), \
         torch.zeros((T, H), dtype=torch.float64, device=dev)
-    t = c.first
+    first = c.first
     for b, n in enumerate(c.new):
         L = c.lens[b]
-        rows = [c.row(b, j) for j in range(L)]
-        keep = torch.tensor([j for j, r in enumerate(rows) if r >= 0], dtype=torch.long, device=dev)
-        at = torch.tensor([r for r in rows if r >= 0], dtype=torch.long, device=dev)
-        k = latent64(kv[at]) if len(at) else torch.zeros((0, 576), dtype=torch.float64, device=dev)
-        for i in range(n):
-            lim = L - n + i if causal else L - 1
-            m = int((keep <= lim).sum())
-            x = q[t].double()
+        rows = torch.tensor([c.row(b, j) for j in range(L)], dtype=torch.long, device=dev)
+        keep = torch.nonzero(rows >= 0).flatten()
+        k = latent64(kv[rows[keep]]) if len(keep) else torch.zeros((0, 576), dtype=torch.float64, device=dev)
+        kt, v, va = k.t().contiguous(), k[:, :512].contiguous(), k[:, :512].abs().contiguous()
+        step = max(1, 60_000_000 // max(1, H * L))
+        for i in range(0, n, step):
+            m = min(step, n - i)
+            at = slice(first + i, first + i + m)
             if max_len is not None and L > max_len:
-                pass
-            elif m == 0:
-                o[t], lse[t] = 0.0, math.inf
-            else:
-                s = (x @ k[:m].t().contiguous()) * sm_scale
-                lse[t] = torch.logsumexp(s, 1)
-                p = torch.exp(s - lse[t][:, None])
-                N[t] = k[:m, :512].abs().sum(0)
-                o[t], A[t] = p @ k[:m, :512].contiguous(), p @ k[:m, :512].abs().contiguous()
-                big = (x.abs() @ k[:m].abs().t().contiguous()).amax(1) * abs(sm_scale)
-                E[t] = 2 * 64 * 2.0 ** -24 * big
-            t += 1
+                continue
+            x = q[at].double().reshape(m * H, 576)
+            limit = (L - n + i + torch.arange(m, device=dev)) if causal else torch.full((m,), L - 1, device=dev)
+            on = (keep[None, :] <= limit[:, None])[:, None, :]
+            s = ((x @ kt) * sm_scale).view(m, H, -1)
+            # (what a row that is not attended holds counts for nothing)
+            s = torch.where(on, s, -math.inf)
+            none = ~on.any(2).expand(m, H)
+            z = torch.where(none, math.inf, torch.logsumexp(s, 2)) if len(keep) else torch.full_like(E[at], math.inf)
+            p = torch.where(on, torch.exp(s - torch.where(none, 0.0, z)[..., None]), 0.0).view(m * H, -1)
+            fv = torch.where(torch.isfinite(v), v, 0.0)      # (NaN reaches O by p, which then is NaN)
+            o[at], A[at] = (p @ fv).view(m, H, 512), (p @ torch.where(torch.isfinite(va), va, 0.0)).view(m, H, 512)
+            lse[at] = z
+            N[at] = torch.where(torch.isfinite(va), va, 0.0).sum(0)
+            if len(keep):
+                big = ((x.abs() @ torch.where(torch.isfinite(kt), kt.abs(), 0.0)).view(m, H, -1) * on).amax(2)
+                E[at] = 2 * 64 * 2.0 ** -24 * big * abs(sm_scale)
+        first += n
     return o, lse, A, E, N
 
 

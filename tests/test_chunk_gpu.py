@@ -1,7 +1,10 @@
 """GPU parity of dsa_mla_chunk against a 64-bit reference (tests/_chunk.py): ragged chunks from one
 token on, empty sequences, rows before and behind the sequences, pages of every kind, positions
 without a row, causal and full masks, tokens that attend nothing, head counts that do and do not
-divide a block of rows, splits, strides, the largest offsets, streams and graphs."""
+divide a block of rows, splits, strides, the largest offsets, streams and graphs.
+
+Calls of few rows run in workgroups of 32 rows, calls of many in workgroups of 128 (more than 256 of
+them always do); `many` adds a sequence of enough tokens to a case, which so runs on the other kernel."""
 from __future__ import annotations
 
 import math
@@ -38,6 +41,12 @@ def run(c, q, kv, **kw):
     return out, lse
 
 
+def with_many(new, lens, H, many, n=None):
+    """The case with a sequence in front that fills over 300 blocks of 128 rows."""
+    n = n or -(-300 * 128 // H)
+    return ([n] + new, [n + 9] + lens) if many else (new, lens)
+
+
 CASES = [
     # new, lens, H, causal, block_size, num_splits, first, pad
     ([1], [1], 128, True, 64, 0, 0, 0),
@@ -63,7 +72,12 @@ CASES = [
 
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 @pytest.mark.parametrize("new,lens,H,causal,bs,ns,first,pad", CASES)
-def test_parity(dev, fp8, new, lens, H, causal, bs, ns, first, pad):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_parity(dev, fp8, new, lens, H, causal, bs, ns, first, pad, many):
+    if many and H < 16:
+        H, ns = H + 32, min(ns, 2)
+    ns = min(ns, 3) if many else ns
+    new, lens = with_many(new, lens, H, many)
     g = gen(len(new) * 1000 + H + sum(lens), dev)
     c = Chunk(g, new, lens, bs, first=first, pad=pad, spare=1)
     q, kv = bf16(g, c.T, H, 576), cache_of(g, c, fp8)
@@ -88,38 +102,43 @@ def test_many_sequences(dev, fp8):
 
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 @pytest.mark.parametrize("ns", [1, 3])
-def test_positions_without_a_row(dev, fp8, ns):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_positions_without_a_row(dev, fp8, ns, many):
     """Table entries outside the cache (the first page of one sequence, all of another, a middle page
     of a third) and sequences longer than their table row: skipped, never read."""
     g = gen(6, dev)
-    c = Chunk(g, [4, 3, 2, 5], [200, 150, 130, 400], 32)
-    c.blocks = 12                                   # 384 positions: the last sequence's end has no page
+    extra = [1700] if many else []                  # 1700 tokens of 24 heads over 384 positions that have pages
+    c = Chunk(g, [4, 3, 2, 5] + extra, [200, 150, 130, 400] + extra, 32)
+    c.blocks = 12                                   # 384 positions: the ends of the longer ones have no page
     c.table = c.table[:, :12].contiguous()
     c.table[0, 0], c.table[0, 5] = c.rows // 32, -1
     c.table[1, :] = 2 ** 31 - 1
     c.table[2, 1:4] = -(2 ** 31)
     c.kw["block_table"] = c.table
     q, kv = bf16(g, c.T, 24, 576), cache_of(g, c, fp8)
-    out, lse = run(c, q, kv, num_splits=ns, max_kv_len=400)
+    out, lse = run(c, q, kv, num_splits=ns, max_kv_len=max(c.lens))
     ref = attend64(c, q, kv, True)
     assert bool(torch.isinf(ref[1][4:7]).all())
     check_chunk(c, out, lse, ref, fp8)
 
 
 @pytest.mark.parametrize("ns", [1, 2])
-def test_longer_than_its_bound_is_nan(dev, ns):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_longer_than_its_bound_is_nan(dev, ns, many):
     g = gen(7, dev)
-    c = Chunk(g, [2, 2], [100, 300], 64)
+    new, lens = ([2, 2] + [1] * 2500, [100, 300] + [40] * 2500) if many else ([2, 2], [100, 300])
+    c = Chunk(g, new, lens, 64)
     q, kv = bf16(g, c.T, 16, 576), cache_of(g, c, False)
     out, lse = run(c, q, kv, num_splits=ns, max_kv_len=256)
     check_chunk(c, out, lse, attend64(c, q, kv, True, max_len=256), False)
 
 
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
-def test_flat_caches_and_strides(dev, fp8):
-    """Flat caches of padded rows, q and out with gaps, an 8-byte aligned out, one long sequence."""
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_flat_caches_and_strides(dev, fp8, many):
+    """Flat caches of padded rows, q and out with gaps, an 8-byte aligned out."""
     g = gen(8, dev)
-    c = Chunk(g, [3, 7], [90, 129], None, flat=129)
+    c = Chunk(g, *(([3, 7, 2000], [90, 129, 2001]) if many else ([3, 7], [90, 129])), None, flat=2001 if many else 129)
     q = bf16(g, c.T, 24, 640)[:, 2:22, 16:592]
     wide = fp8_rows(g, c.rows) if fp8 else bf16(g, c.rows, 576)
     kv = torch.full((c.rows, 704 if fp8 else 640), 0xFF if fp8 else float("nan"), dtype=wide.dtype, device=dev)
@@ -135,11 +154,12 @@ def test_flat_caches_and_strides(dev, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
-def test_scores_of_every_size(dev, fp8):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_scores_of_every_size(dev, fp8, many):
     """Scores that rise far above the first positions' (a running maximum that grows late), lie far below
     zero, differ by hundreds, and queries of every magnitude."""
     g = gen(9, dev)
-    c = Chunk(g, [40, 1], [700, 650], 64)
+    c = Chunk(g, *(([40, 1, 5000], [700, 650, 5000]) if many else ([40, 1], [700, 650])), 64)
     q, kv = bf16(g, c.T, 8, 576), cache_of(g, c, fp8)
     q[:, 0] *= 100
     q[:, 1] *= 1e-3
@@ -157,18 +177,19 @@ def test_scores_of_every_size(dev, fp8):
 
 
 @pytest.mark.parametrize("ns", [1, 2])
-def test_scale_out_of_range_is_nan(dev, ns):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_scale_out_of_range_is_nan(dev, ns, many):
     """A 656-byte row whose scale is 128 or more, negative or NaN: NaN for the tokens that attend it."""
     g = gen(10, dev)
     for bad in (128.0, -0.5, float("nan"), float("inf")):
-        c = Chunk(g, [6, 2], [300, 80], 64)
+        c = Chunk(g, *(([6, 2, 2400], [300, 80, 2400]) if many else ([6, 2], [300, 80])), 64)
         q, kv = bf16(g, c.T, 16, 576), cache_of(g, c, True)
+        ref = attend64(c, q, kv, True)
         kv[c.row(0, 296), 516:520] = torch.tensor([bad], device=dev).view(torch.uint8)
         out, lse = run(c, q, kv, num_splits=ns)
         hit = torch.zeros(c.T, dtype=torch.bool, device=dev)
         hit[2:6] = True                                     # tokens 2..5 are positions 296..299
         assert bool(torch.isnan(out[hit]).all()) and bool(torch.isnan(lse[hit]).all())
-        ref = attend64(c, q, kv, True)
         ref[0][hit], ref[1][hit] = float("nan"), float("nan")
         check_chunk(c, out, lse, ref, True)
 
@@ -176,12 +197,13 @@ def test_scale_out_of_range_is_nan(dev, ns):
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 @pytest.mark.parametrize("ns", [1, 2])
 @pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
-def test_values_that_are_not_finite_stay_with_their_tokens(dev, fp8, ns, value):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_values_that_are_not_finite_stay_with_their_tokens(dev, fp8, ns, value, many):
     """A row with a NaN or infinity, in NoPE or RoPE: the tokens of the same block of rows that do not
     attend it are as if it were not there."""
     g = gen(15, dev)
     for place in (3, 515):
-        c = Chunk(g, [9, 4], [300, 70], 64)
+        c = Chunk(g, *(([9, 4, 2400], [300, 70, 2400]) if many else ([9, 4], [300, 70])), 64)
         q, kv = bf16(g, c.T, 16, 576), cache_of(g, c, fp8)
         ref = attend64(c, q, kv, True)
         hit = c.row(0, 295)                                     # tokens 4 .. 8 are positions 295 .. 299
@@ -256,15 +278,16 @@ def test_repeats_its_bits_on_other_streams_and_in_graphs(dev):
 
 
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
-def test_agrees_with_the_sparse_decode_of_every_position(dev, fp8):
+@pytest.mark.parametrize("B", [3, 330])
+def test_agrees_with_the_sparse_decode_of_every_position(dev, fp8, B):
     """Contexts no longer than the top-k: mla_decode over a list of every position attends the same rows."""
     g = gen(13, dev)
-    B, H, s_q = 3, 128, 2
-    lens = [700, 64, 1025]
+    H, s_q = 128, 2
+    lens = [700, 64, 1025] if B == 3 else [2 + 7 * b % 300 for b in range(B)]
     c = Chunk(g, [s_q] * B, lens, 64)
     q, kv = bf16(g, c.T, H, 576), cache_of(g, c, fp8)
     out, lse = run(c, q, kv)
-    idx = torch.full((B, s_q, 1025), -1, dtype=torch.int32, device=dev)
+    idx = torch.full((B, s_q, max(lens)), -1, dtype=torch.int32, device=dev)
     for b in range(B):
         idx[b, :, :lens[b]] = torch.arange(lens[b], dtype=torch.int32, device=dev)
     od, ld = dsa.mla_decode(q.view(B, s_q, H, 576), kv, idx, SM_SCALE, seq_lens=c.seq_lens, causal=True, **c.kw)
