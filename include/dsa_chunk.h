@@ -183,13 +183,16 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  *            O and LSE are NaN.
  * num_splits: 0 = automatic, or 1 .. DSA_MLA_MAX_SPLITS parts of max_kv_len
  *            positions (rounded up to whole tiles of 32), whose fp32 partials
- *            (workspace: num_splits x T x H x 513 floats) a combine merges.
+ *            (workspace: num_splits x T x H x 513 floats and 16 bytes) a combine
+ *            merges.  Automatic: by the sizes, and for several sequences the
+ *            device deals their positions evenly, so that a sequence's parts go
+ *            by its length (dsa_mla_chunk_num_splits: the most that one has).
  * Scores and sums are fp32.  Probabilities are rounded to 16 bits for the
  * product with V (bf16; fp16 for DSA_KV_FP8_656).  656-byte rows: scores use
  * their exact values; V is rounded to fp16 (its scale's mantissa first) and every scale must lie in [0, 128),
  * a token that attends a row with another scale getting NaN, as in dsa_mla.h.
- * The split count and so the last bits depend on the call's sizes alone; one
- * call repeats its bits.
+ * The split and so the last bits depend on the call's sizes and, with
+ * num_splits = 0, on the lengths of all its sequences; one call repeats its bits.
  */
 typedef struct {
     const void* q;

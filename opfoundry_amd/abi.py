@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "_build", "libdsa_mla.so")
@@ -249,6 +250,23 @@ class ChunkArgs(ctypes.Structure):
     ]
 
 
+def packer(cls):
+    """A function of a struct's fields in order (nested structs' fields in their place; None: a null
+    pointer) that gives its bytes: filling a ctypes struct of 38 fields takes three times as long."""
+    codes = {_vp: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}
+
+    def flat(c):
+        return "".join(codes[t] if t in codes else flat(t) for _, t in c._fields_)
+
+    s = struct.Struct("@" + flat(cls))
+    if s.size != ctypes.sizeof(cls):
+        raise RuntimeError(f"{cls.__name__}: {s.size} packed bytes, {ctypes.sizeof(cls)} in C")
+    return s.pack
+
+
+pack_norm_rope, pack_append, pack_chunk = packer(QkNormRopeArgs), packer(KvAppendArgs), packer(ChunkArgs)
+
+
 class DsaError(RuntimeError):
     def __init__(self, code: int, where: str):
         self.code = code
@@ -305,11 +323,12 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.dsa_mla_prefill_v4_fp8.argtypes = [ctypes.POINTER(PrefillV4Fp8Args), _vp, ctypes.c_size_t, _vp]
     lib.dsa_kv_quantize_fp8.argtypes = [_vp, _i64, _i64, _vp, _i64, _vp, _vp]
     lib.dsa_topk_indices.argtypes = [_vp, _i64, _vp, _i32, _i32, _i32, _vp, _i64, _vp]
-    lib.dsa_qk_norm_rope.argtypes = [ctypes.POINTER(QkNormRopeArgs), _vp]
-    lib.dsa_kv_append.argtypes = [ctypes.POINTER(KvAppendArgs), _vp]
-    lib.dsa_mla_chunk_workspace_size.argtypes = [ctypes.POINTER(ChunkArgs), sz]
-    lib.dsa_mla_chunk_num_splits.argtypes = [ctypes.POINTER(ChunkArgs), ctypes.POINTER(_i32)]
-    lib.dsa_mla_chunk.argtypes = [ctypes.POINTER(ChunkArgs), _vp, ctypes.c_size_t, _vp]
+    # (argument blocks as a ctypes struct's address or as packed bytes)
+    lib.dsa_qk_norm_rope.argtypes = [_vp, _vp]
+    lib.dsa_kv_append.argtypes = [_vp, _vp]
+    lib.dsa_mla_chunk_workspace_size.argtypes = [_vp, sz]
+    lib.dsa_mla_chunk_num_splits.argtypes = [_vp, ctypes.POINTER(_i32)]
+    lib.dsa_mla_chunk.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_strerror.argtypes = [ctypes.c_int]
     lib.dsa_mla_strerror.restype = ctypes.c_char_p
     lib.dsa_mla_abi_version.argtypes = []

@@ -616,48 +616,65 @@ def _bad(name: str, t, what: str):
     raise ValueError(f"{name} must {what}, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _addr(t: torch.Tensor, dtype, name: str, dev: int) -> int:
-    """Address of a tensor of this type on device `dev`."""
+def _not_this(t, dtype, name: str, dev: int):
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.get_device() != dev or dev < 0:
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a device tensor")
-        raise ValueError(f"{name} must be on device {dev}, got {t.device}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    raise ValueError(f"{name} must be on device {dev}, got {t.device}")
+
+
+def _addr(t: torch.Tensor, dtype, name: str, dev: int) -> int:
+    """Address of a tensor of this type on device `dev`."""
+    if t.dtype is not dtype or t.get_device() != dev or dev < 0:
+        _not_this(t, dtype, name, dev)
     return t.data_ptr()
 
 
 def _addr3(t: torch.Tensor, T: int, H: int, D: int, name: str, dev: int):
     """(address, stride of a token, stride of a head) of a bf16 [T, H, D] with a dense last dim."""
-    p = _addr(t, _BF16, name, dev)
-    if t.shape != (T, H, D):
-        _bad(name, t, f"be [{T}, {H}, {D}]")
+    if t.dtype is not _BF16 or t.get_device() != dev or dev < 0:
+        _not_this(t, _BF16, name, dev)
     st = t.stride()
-    if st[2] != 1 and D > 1:
-        _bad(name, t, "have a dense last dim")
-    return p, st[0], st[1]
+    if t.shape != (T, H, D) or st[2] != 1:
+        _bad(name, t, f"be [{T}, {H}, {D}] with a dense last dim")
+    return t.data_ptr(), st[0], st[1]
 
 
-def _vector(t: Optional[torch.Tensor], n: int, dtype, name: str, dev: int) -> Optional[int]:
-    """Address of an optional dense vector of n values."""
+def _addr2(t: torch.Tensor, width: int, name: str, dev: int):
+    """(address, rows, row stride) of a bf16 [rows, width] with a dense last dim."""
+    if t.dtype is not _BF16 or t.get_device() != dev or dev < 0:
+        _not_this(t, _BF16, name, dev)
+    st = t.stride()
+    if len(st) != 2 or t.shape[1] != width or st[1] != 1:
+        _bad(name, t, f"be [T, {width}] with a dense last dim")
+    return t.data_ptr(), t.shape[0], st[0]
+
+
+def _vector(t: Optional[torch.Tensor], n: int, dtype, name: str, dev: int) -> int:
+    """Address of an optional dense vector of n values (0: none)."""
     if t is None:
-        return None
-    p = _addr(t, dtype, name, dev)
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        return 0
+    if t.dtype is not dtype or t.get_device() != dev or dev < 0:
+        _not_this(t, dtype, name, dev)
+    if t.numel() != n or t.dim() != 1 or not t.is_contiguous():
         _bad(name, t, f"be a dense vector of {n}")
-    return p
+    return t.data_ptr()
 
 
 def _choice(table, value, name: str) -> int:
-    try:
+    if value in table:
         return table[value]
-    except (KeyError, TypeError):
-        raise ValueError(f"{name} must be one of {list(table)}, got {value!r}") from None
+    raise ValueError(f"{name} must be one of {list(table)}, got {value!r}")
 
 
 def _sequences(q_indptr, seq_lens, dev: int):
     """(q_indptr's address, seq_lens's, B)."""
     B = seq_lens.numel()
+    if (q_indptr.dtype is _I32 and seq_lens.dtype is _I32 and q_indptr.get_device() == dev == seq_lens.get_device()
+            and q_indptr.shape == (B + 1,) and seq_lens.dim() == 1 and q_indptr.is_contiguous()
+            and seq_lens.is_contiguous()):
+        return q_indptr.data_ptr(), seq_lens.data_ptr(), B
     return _vector(q_indptr, B + 1, _I32, "q_indptr", dev), _vector(seq_lens, B, _I32, "seq_lens", dev), B
 
 
@@ -665,14 +682,14 @@ def _pages(block_table, block_size, cache, B: int, dev: int):
     """(address, stride, blocks of a row, rows of a block) of a block table; the block size defaults to
     that of a cache [blocks, block_size, row]."""
     if block_table is None:
-        return None, 0, 0, 0
+        return 0, 0, 0, 0
     p = _addr(block_table, _I32, "block_table", dev)
-    if block_table.dim() != 2 or block_table.shape[0] != B:
+    if block_table.dim() != 2:
         _bad("block_table", block_table, f"be [{B}, blocks]")
+    rows, n = block_table.shape
     st = block_table.stride()
-    n = block_table.shape[1]
-    if n > 1 and st[1] != 1:
-        _bad("block_table", block_table, "have a dense last dim")
+    if rows != B or (n > 1 and st[1] != 1):
+        _bad("block_table", block_table, f"be [{B}, blocks] with a dense last dim")
     if block_size is None:
         if cache is None or cache.dim() < 3:
             raise ValueError("block_size is required with a block table")
@@ -728,6 +745,9 @@ class _Stream:
                 self.other = (stream if isinstance(stream, torch.cuda.Stream)
                               else torch.cuda.ExternalStream(self.handle, device=dev))
 
+    def empty_like(self, like: torch.Tensor) -> torch.Tensor:
+        return torch.empty_like(like) if self.other is None else self.empty(like, like.shape, like.dtype)
+
     def empty(self, like: torch.Tensor, shape, dtype) -> torch.Tensor:
         t = like.new_empty(shape, dtype=dtype)
         if self.other is not None:
@@ -746,16 +766,31 @@ class _Stream:
             check(rc, where)
 
 
+def _launch(fn, where: str, dev: int, stream, *args) -> None:
+    """One call that allocates nothing on a stream."""
+    if stream is None and torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            check(rc, where)
+    else:
+        _Stream(dev, stream).call(fn, where, *args)
+
+
 def _normed_rows(x, norm, w, b, out, T, D, norm_dim, name, dev, on):
-    """dsa_norm_rope_rows of one stream, and its output."""
+    """The fields of dsa_norm_rope_rows of one stream, and its output."""
     H = x.shape[1]
     px, st, sh = _addr3(x, T, H, D, name, dev)
     if out is None:
-        out = on.empty(x, (T, H, D), _BF16)
-    po, ot, oh = _addr3(out, T, H, D, name + "_out", dev)
-    return abi.NormRopeRows(px, st, sh, po, ot, oh, _vector(w, norm_dim, _F32, name + "_weight", dev),
-                            _vector(b, norm_dim, _F32, name + "_bias", dev), H,
-                            _choice(abi.NORMS, norm, name + "_norm")), out
+        out = on.empty_like(x) if x.is_contiguous() else on.empty(x, (T, H, D), _BF16)
+        po, ot, oh = out.data_ptr(), H * D, D
+    else:
+        po, ot, oh = _addr3(out, T, H, D, name + "_out", dev)
+    return (px, st, sh, po, ot, oh, 0 if w is None else _vector(w, norm_dim, _F32, name + "_weight", dev),
+            0 if b is None else _vector(b, norm_dim, _F32, name + "_bias", dev), H,
+            _choice(abi.NORMS, norm, name + "_norm")), out
+
+
+_NO_ROWS = (0,) * 10
 
 
 def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
@@ -786,9 +821,8 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
     if rot_off is None:
         rot_off = 0 if D == 128 else D - abi.D_ROPE
     rope = _choice(abi.ROPES, style, "style")
-    pcs, n_pos = _angles(cos_sin, dev) if rope else (None, 0)
-    pp = pi = pl = None
-    B = 0
+    pcs, n_pos = _angles(cos_sin, dev) if rope else (0, 0)
+    pp = pi = pl = B = 0
     if positions is not None:
         pp = _vector(positions, T, _I32, "positions", dev)
     elif q_indptr is not None:
@@ -806,9 +840,9 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
     else:
         if k_norm != "none" or k_weight is not None or k_bias is not None or k_out is not None:
             raise ValueError("k_norm, k_weight, k_bias and k_out need k")
-        ks = abi.NormRopeRows()
-    a = abi.QkNormRopeArgs(qs, ks, pcs, n_pos, pp, pi, pl, T, B, D, norm_dim, rot_off, rope, 1 if inverse else 0, eps)
-    on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", ctypes.byref(a))
+        ks = _NO_ROWS
+    a = abi.pack_norm_rope(*qs, *ks, pcs, n_pos, pp, pi, pl, T, B, D, norm_dim, rot_off, rope, 1 if inverse else 0, eps)
+    on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", a)
     return q_out, k_out
 
 
@@ -843,23 +877,19 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     T = rope = irope = 0
     paged_like = index_cache
-    kvp = kst = pw = None
-    kst = rows = stride = sstride = rstride = fmt = kind = 0
-    pc = psc = pr = None
+    kvp = pw = kst = rows = stride = sstride = rstride = fmt = kind = pc = psc = pr = 0
     if kv is not None:
-        parts = cache if isinstance(cache, (tuple, list)) else (cache,)
+        several = isinstance(cache, (tuple, list))
+        paged_like = first = cache[0] if several else cache
+        parts = cache if several else (cache,)
         found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
         if found is None:
             raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
         fmt, width = found
-        kvp = _addr(kv, _BF16, "kv", dev)
-        if kv.dim() != 2 or kv.shape[1] != width or kv.stride(1) != 1:
-            _bad("kv", kv, f"be [T, {width}] with a dense last dim")
-        T, kst = kv.shape[0], kv.stride(0)
-        paged_like = first = parts[0]
+        kvp, T, kst = _addr2(kv, width, "kv", dev)
         pc = _addr(first, first.dtype, "cache", dev)
         rows, stride = _rows(first, first.shape[-1], "cache")
-        if len(parts) > 1:
+        if several and len(parts) > 1:
             last = parts[-1]
             pr = _addr(last, _BF16, "cache", dev)
             more, rstride = _rows(last, 64, "cache")
@@ -872,37 +902,38 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
         kind = _choice(_KV_NORMS, norm, "norm")
         if kind is None:
             kind = 0 if weight is None else 1
-        pw = _vector(weight, 512, _F32, "weight", dev)
+        if weight is not None:
+            pw = _vector(weight, 512, _F32, "weight", dev)
         rope = _choice(abi.ROPES, style, "style")
-    ip = iw = ib = ic = None
-    ist = irows = istride = ikind = 0
+    ip = iw = ib = ic = ist = irows = istride = ikind = 0
     if index_k is not None:
         if index_cache is None:
             raise ValueError("index_k needs index_cache")
-        ip = _addr(index_k, _BF16, "index_k", dev)
-        if index_k.dim() != 2 or index_k.shape[1] != 128 or index_k.stride(1) != 1:
-            _bad("index_k", index_k, "be [T, 128] with a dense last dim")
-        if kv is not None and index_k.shape[0] != T:
+        ip, n, ist = _addr2(index_k, 128, "index_k", dev)
+        if kv is not None and n != T:
             raise ValueError("kv and index_k must have the same rows")
-        T, ist = index_k.shape[0], index_k.stride(0)
+        T = n
         ic = _addr(index_cache, _BF16, "index_cache", dev)
         if index_cache.shape[-1] != 128:
             _bad("index_cache", index_cache, "be [..., 128]")
         irows, istride = _rows(index_cache, 128, "index_cache")
         ikind = _choice(abi.NORMS, index_norm, "index_norm")
-        iw = _vector(index_weight, 128, _F32, "index_weight", dev)
-        ib = _vector(index_bias, 128, _F32, "index_bias", dev)
+        if index_weight is not None:
+            iw = _vector(index_weight, 128, _F32, "index_weight", dev)
+        if index_bias is not None:
+            ib = _vector(index_bias, 128, _F32, "index_bias", dev)
         irope = _choice(abi.ROPES, index_style, "index_style")
-    pcs, n_pos = _angles(cos_sin, dev) if rope or irope else (None, 0)
+    pcs, n_pos = _angles(cos_sin, dev) if rope or irope else (0, 0)
     pt, tst, blocks, bs = _pages(block_table, block_size, paged_like, B, dev)
-    a = abi.KvAppendArgs(kvp, kst, pw, pc, psc, pr, rows, stride, sstride, rstride, fmt, kind, rope, ikind, irope,
+    a = abi.pack_append(kvp, kst, pw, pc, psc, pr, rows, stride, sstride, rstride, fmt, kind, rope, ikind, irope,
                          ip, ist, iw, ib, ic, irows, istride, pcs, n_pos, pi, pl, pt, tst, blocks, bs,
                          kv_batch_stride, T, B, eps, eps if index_eps is None else index_eps)
-    _Stream(dev, stream).call(load_library().dsa_kv_append, "dsa_kv_append", ctypes.byref(a))
+    _launch(load_library().dsa_kv_append, "dsa_kv_append", dev, stream, a)
 
 
 def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, block_table=None, block_size=None,
-                    kv_batch_stride=0, causal=True, max_kv_len=None, num_splits=0):
+                    kv_batch_stride=0, causal=True, max_kv_len=None, num_splits=0) -> bytes:
+    """dsa_mla_chunk_args, as the library's calls take them."""
     dev = q.get_device()
     if q.dim() != 3:
         _bad("q", q, "be [T, H, 576]")
@@ -919,27 +950,26 @@ def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, bloc
     pt, tst, blocks, bs = _pages(block_table, block_size, kv_cache, B, dev)
     if max_kv_len is None:
         max_kv_len = blocks * bs if block_table is not None else int(kv_batch_stride) or rows
-    po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev) if out is not None else (None, 0, 0)
+    po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev) if out is not None else (0, 0, 0)
     if lse is not None:
         ps = _addr(lse, _F32, "lse", dev)
         if lse.shape != (T, H) or not lse.is_contiguous():
             _bad("lse", lse, f"be a dense [{T}, {H}]")
     else:
-        ps = None
-    return abi.ChunkArgs(pq, qt, qh, pi, pl, pk, rows, stride, fmt, bs, pt, tst, kv_batch_stride, po, ot, oh, ps,
+        ps = 0
+    return abi.pack_chunk(pq, qt, qh, pi, pl, pk, rows, stride, fmt, bs, pt, tst, kv_batch_stride, po, ot, oh, ps,
                          blocks, T, B, H, 1 if causal else 0, max_kv_len, num_splits, sm_scale)
 
 
 def chunk_num_splits(args) -> int:
     n = ctypes.c_int32(0)
-    check(load_library().dsa_mla_chunk_num_splits(ctypes.byref(args), ctypes.byref(n)), "dsa_mla_chunk_num_splits")
+    check(load_library().dsa_mla_chunk_num_splits(args, ctypes.byref(n)), "dsa_mla_chunk_num_splits")
     return n.value
 
 
 def chunk_workspace_size(args) -> int:
     n = ctypes.c_size_t(0)
-    check(load_library().dsa_mla_chunk_workspace_size(ctypes.byref(args), ctypes.byref(n)),
-          "dsa_mla_chunk_workspace_size")
+    check(load_library().dsa_mla_chunk_workspace_size(args, ctypes.byref(n)), "dsa_mla_chunk_workspace_size")
     return n.value
 
 
@@ -976,5 +1006,5 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
         elif not workspace.is_contiguous():
             _bad("workspace", workspace, "be dense")
         ws = _addr(workspace, workspace.dtype, "workspace", dev)
-    on.call(load_library().dsa_mla_chunk, "dsa_mla_chunk", ctypes.byref(a), ws, need)
+    on.call(load_library().dsa_mla_chunk, "dsa_mla_chunk", a, ws, need)
     return out, lse
