@@ -1355,20 +1355,50 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     }
 }
 
-// Joins the partials of a row's splits, one wave a row: a lane holds 8 of its 512
-// values.  Splits past the row's positions wrote nothing and are not read.
+// Joins the partials of a row's splits, SHARES waves a row: a lane holds 8 of its 512 values,
+// wave i takes splits i, i + SHARES, ...  Splits past the row's positions wrote nothing and add nothing.
+template <int SHARES>
 __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const ChunkParams p) {
+    __shared__ __attribute__((aligned(16))) float s_o[SHARES > 1 ? SHARES * D_VO : 4];
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * NWAVE + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= (int64_t)p.T * p.H) return;
-    const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H);
-    const int32_t b = seq_of(p.indptr, p.B, t);
-    if (b == NO_SEQ) return;
-    const int64_t limit = min(limit_of(p, b, t), p.pages.limit);
-    const int32_t per = p.target ? *p.dealt : p.per_split;
-    const int ns = (int)min((int64_t)p.ns, (limit + per - 1) / per);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int share = SHARES > 1 ? wave : 0;
+    const int64_t row = (int64_t)blockIdx.x * (NWAVE / SHARES) + wave / SHARES;
     const int64_t step = (int64_t)p.T * p.H;
-    const float mine = lane < ns ? p.part_lse[lane * step + row] : -FLT_MAX;     // at most 64 splits
+    if (row >= step) return;
+    const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H);
+    // Requested at once, before it is known which of them are needed: the sequences' bounds, every
+    // split's sum and (where a row has four waves) a wave's first eight partials.
+    const int32_t i0 = min(lane, p.B - 1);
+    const int32_t start_l = p.indptr[i0], end_l = p.indptr[i0 + 1], len_l = p.lens[i0];
+    const int32_t per = p.target ? *p.dealt : p.per_split;
+    const float lse_l = p.part_lse[min(lane, p.ns - 1) * step + row];
+    const float* const src = p.part_o + row * D_VO + 8 * lane;
+    f32x4 x[8], y[8];
+    auto fetch = [&](int s0, int last) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const float* const at = src + min(s0 + s * SHARES, last) * step * D_VO;
+            x[s] = *reinterpret_cast<const f32x4*>(at), y[s] = *reinterpret_cast<const f32x4*>(at + 4);
+        }
+    };
+    if constexpr (SHARES > 1) fetch(share, p.ns - 1);
+    int64_t limit;
+    int32_t len;
+    if (p.B <= 64) {
+        const int32_t b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < p.B && end_l <= t));
+        if (b >= p.B || t < __builtin_amdgcn_readlane(start_l, b)) return;
+        len = __builtin_amdgcn_readlane(len_l, b);
+        const int64_t own = (int64_t)len - __builtin_amdgcn_readlane(end_l, b) + t + 1;
+        limit = max((int64_t)0, p.causal ? min(own, (int64_t)len) : (int64_t)len);
+    } else {
+        const int32_t b = seq_of(p.indptr, p.B, t);
+        if (b == NO_SEQ) return;
+        len = p.lens[b];
+        limit = limit_of(p, b, t);
+    }
+    const int ns = (int)min((int64_t)p.ns, (min(limit, p.pages.limit) + per - 1) / per);
+    const float mine = lane < ns ? lse_l : -FLT_MAX;
     float top = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -1378,17 +1408,11 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
     float o[8] = {};
     // eight splits' loads in flight at a time; the last one's again past it.  One of no weight is not added
     // (its partial may hold anything).
-    const float* const src = p.part_o + row * D_VO + 8 * lane;
-    for (int s0 = 0; s0 < ns; s0 += 8) {
-        f32x4 x[8], y[8];
+    for (int s0 = share; s0 < ns; s0 += 8 * SHARES) {
+        if (SHARES == 1 || s0 != share) fetch(s0, ns - 1);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            const float* const at = src + min(s0 + s, ns - 1) * step * D_VO;
-            x[s] = *reinterpret_cast<const f32x4*>(at), y[s] = *reinterpret_cast<const f32x4*>(at + 4);
-        }
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const float f = __shfl(w, s0 + s, 64);          // 0 past the last
+            const float f = __shfl(w, s0 + s * SHARES, 64);          // 0 past the last
             if (f != 0.0f) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -1398,14 +1422,29 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
             }
         }
     }
-    const float nan = p.lens[b] > p.max_len ? __builtin_nanf("") : 0.0f;
+    const float nan = len > p.max_len ? __builtin_nanf("") : 0.0f;
     const float inv = any ? 1.0f / total + nan : nan;
-    const f32x8 r = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
-    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_convertvector(r, bf16x8));
-    u32x2* const dst = reinterpret_cast<u32x2*>(p.out + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * lane);
-    dst[0] = u32x2{v[0], v[1]};
-    dst[1] = u32x2{v[2], v[3]};
-    if (lane == 0 && p.lse) p.lse[row] = nan != 0.0f ? nan : (any ? top + __builtin_amdgcn_logf(total) * LN2 : INFINITY);
+    __bf16* const dst = p.out + (int64_t)t * p.o_st + (int64_t)h * p.o_sh;
+    if constexpr (SHARES == 1) {
+        const f32x8 r = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_convertvector(r, bf16x8));
+        u32x2* const d = reinterpret_cast<u32x2*>(dst + 8 * lane);
+        d[0] = u32x2{v[0], v[1]};
+        d[1] = u32x2{v[2], v[3]};
+    } else {
+        f32x4* const mine_o = reinterpret_cast<f32x4*>(s_o + share * D_VO + 8 * lane);
+        mine_o[0] = f32x4{o[0], o[1], o[2], o[3]};
+        mine_o[1] = f32x4{o[4], o[5], o[6], o[7]};
+        __syncthreads();
+        static_assert(D_VO == 2 * NTHR);
+        float a = 0.0f, c = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SHARES; ++i) a += s_o[i * D_VO + 2 * threadIdx.x], c += s_o[i * D_VO + 2 * threadIdx.x + 1];
+        const f32x2 r = {a * inv, c * inv};
+        *reinterpret_cast<uint32_t*>(dst + 2 * threadIdx.x) = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+    }
+    if (lane == 0 && share == 0 && p.lse)
+        p.lse[row] = nan != 0.0f ? nan : (any ? top + __builtin_amdgcn_logf(total) * LN2 : INFINITY);
 }
 
 // ------------------------------------------------------------------- host
@@ -1430,6 +1469,12 @@ constexpr Kernel KERNELS[2][2] = {       // [656-byte rows][narrow]
 };
 constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f, PART_BYTES_US = 5.3e6f;
 constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+
+// Four waves join a row where there are few rows of many splits, one wave elsewhere.  A call with one
+// and with four, us: 16 rows of 48 splits 22.7 and 17.4; 128 of 32 27.0 and 23.6, of 8 20.4 and 19.6, of 2
+// 19.9 and 19.9; 512 of 16 30.3 and 28.5, of 4 21.4 and 22.0; 1024 of 8 26.4 and 27.2; 4096 of 4 34.2 and 39.0.
+constexpr int64_t FEW_ROWS = 512;
+constexpr int FOUR_FROM = 5;
 
 struct Plan {
     bool narrow;
@@ -1578,8 +1623,11 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;
     if (p.ns > 1) {
         const int64_t rows = (int64_t)a->T * a->H;
-        hipLaunchKernelGGL(dsa_mla_chunk_combine_kernel, dim3((unsigned)((rows + NWAVE - 1) / NWAVE)), dim3(NTHR), 0,
-                           (hipStream_t)stream, p);
+        if (rows <= FEW_ROWS && p.ns >= FOUR_FROM)
+            hipLaunchKernelGGL(dsa_mla_chunk_combine_kernel<4>, dim3((unsigned)rows), dim3(NTHR), 0, (hipStream_t)stream, p);
+        else
+            hipLaunchKernelGGL(dsa_mla_chunk_combine_kernel<1>, dim3((unsigned)((rows + NWAVE - 1) / NWAVE)), dim3(NTHR),
+                               0, (hipStream_t)stream, p);
         if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;
     }
     return DSA_OK;
