@@ -22,6 +22,12 @@ constexpr int CUS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr unsigned FP8_SCALE_LIMIT_BITS = 0x43000000u;   // 128.0f
 
+constexpr int NARROW = 32;                   // rows of a workgroup of the kernel for few rows
+// What a workgroup of a kernel takes, us: `start`, and `tile` for each 32 positions (`pair` where two
+// share a CU).
+struct Kernel {
+    float start, tile, pair;
+};
 struct ChunkParams {
     const __bf16* q;
     int64_t q_st, q_sh;
@@ -37,9 +43,10 @@ struct ChunkParams {
     float* part_lse;
     int32_t T, B, H, causal, max_len, ns, per_split;
     int32_t common;      // of H and the rows of a block (block_start)
-    int32_t target;      // workgroups that the positions are dealt to (0: splits of per_split positions)
-    int32_t* dealt;      // where the dealt split's positions are kept for the combine
+    int32_t* dealt;      // where the positions of a split that the device chose are kept for the join (null:
+                         // splits of per_split positions)
     float scale_log2;
+    Kernel kernel;
 };
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -131,10 +138,10 @@ __device__ __forceinline__ Block find_block(const ChunkParams& p, int64_t x, int
     k.b = count_upto(p.B, x, start);
     if (k.b >= p.B) return k;
     const int64_t local = x - start(k.b);
-    k.first = max(p.indptr[k.b], 0);
+    k.first = min(max(p.indptr[k.b], 0), p.T);
     k.end = p.indptr[k.b + 1];
     k.len = p.lens[k.b];
-    const int64_t left = (int64_t)(min(k.end, p.T) - k.first) * p.H - local * m;
+    const int64_t left = (int64_t)(min(max(k.end, 0), p.T) - k.first) * p.H - local * m;
     if (local < 0 || left <= 0) return k;
     k.r0 = (int32_t)(local * m);
     k.rows = (int32_t)min(left, (int64_t)m);
@@ -146,32 +153,123 @@ __device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k
     return (int32_t)max((int64_t)0, p.causal ? min(own, (int64_t)k.len) : (int64_t)k.len);
 }
 
-// Positions of a split.  The host knows a bound of the lengths alone; where it left the split to
-// the device, the positions of all blocks together are dealt evenly to `target` workgroups, so that
-// short sequences take few and long ones many (16 sequences of 6670 to 20011 positions and 16
-// heads: 81 us by the bound, 70 dealt).  Every wave finds the same value.
-__device__ __forceinline__ int32_t split_of(const ChunkParams& p, int32_t m) {
-    if (p.target == 0) return p.per_split;
-    const int lane = threadIdx.x & 63;
-    int64_t all = 0;
-    int32_t most = 0;
-    for (int b = lane; b < p.B; b += 64) {
-        const int64_t rows = (int64_t)max(0, min(p.indptr[b + 1], p.T) - max(p.indptr[b], 0)) * p.H;
-        const int32_t len = (int32_t)min((int64_t)min(max(p.lens[b], 0), p.max_len), p.pages.limit);
-        const int32_t tiles = rows > 0 ? (len + TILE - 1) / TILE : 0;
-        all += (rows + m - 1) / m * tiles;
-        most = max(most, tiles);
-    }
+constexpr float PART_BYTES_US = 5.3e6f;            // at which splits' partials are written and read again
+constexpr float JOIN_SPLIT_US = 0.1f;              // and what the join's wait for one more split costs
+
+// Reductions and a running sum over a wave's lanes by moves within and between its rows of 16.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t moved(int32_t v, int32_t none) {
+    return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
+}
+template <class T, class F>
+__device__ __forceinline__ T scan(T v, T none, F op) {
+    auto step = [&](auto ctrl, auto rows) {
+        v = op(v, __builtin_bit_cast(T, moved<decltype(ctrl)::value, decltype(rows)::value>(
+                      __builtin_bit_cast(int32_t, v), __builtin_bit_cast(int32_t, none))));
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});        // from 1, 2, 4, 8 lanes below
+    step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});        // row 0's last lane to row 1, 2's to 3
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});        // lane 31 to rows 2 and 3
+    return v;
+}
+template <class T, class F>
+__device__ __forceinline__ T over_lanes(T v, T none, F op) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, scan(v, none, op)), 63));
+}
+
+// ceil(a / b) of 0 <= a < 2^31 and 1 <= b <= 2^26: exact where it is below 2^20, else at least that and at
+// most 2^-19 more.  (The product is off by less than 2^-21 of itself; an integer division takes ten times
+// the code, which a workgroup's first waves fetch.)
+__device__ __forceinline__ int32_t parts(int32_t a, int32_t b) {
+    uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+    q += q >> 20;
+    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
+    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
+    return (int32_t)q;
+}
+
+// The block, the split and the positions of a split of a workgroup.  The host knows a bound of the
+// lengths alone.  Where it leaves the splits to the device (`dealt`, at most 64 sequences: a lane holds
+// one), each lane prices one split size about the even share of a workgroup's place on the chip
+// (`places`: one a CU, or two) and the cheapest is taken: the longest split where all workgroups have a
+// place, else their sum with half of a split at the end; and what the partials and their join cost.
+// The workgroups are then numbered without gaps, and a sequence's splits are even: workgroups with nothing
+// to do between the others make the dispatcher, which hands them to XCDs and shader engines in turn,
+// leave CUs idle while others hold three.  16 sequences of 7130 to 19272 bf16 rows, 16 heads: 66 us, of
+// 506 workgroups (77 in 16 splits by the bound of the lengths, 366 of them with work); 66 too where that
+// bound is four times as much (173).  7 sequences of 1994 to 4772 rows and 28 to 258 tokens of 40 heads:
+// 383 us (402 in 2).  Finding it out takes 1.5 us: one token of 128 heads over 1483 656-byte rows 19.1
+// and, in 20 splits by the caller's count, 17.3.  Of 50 ragged calls it was 4 % above the best of 13
+// counts on average (23 % below to 17 % above).
+struct Work {
+    Block blk;
+    int32_t split, per;
+};
+__device__ __forceinline__ Work find_work(const ChunkParams& p, int32_t m, int32_t places) {
+    // Blocks of one sequence follow one another and read the same rows: four at a time on one XCD
+    // (workgroups go to the eight in turn).
+    uint32_t x = blockIdx.x;
+    if (x < (gridDim.x & ~31u) && (p.dealt || m == NARROW)) x = (x & ~31u) | (x & 7) << 2 | ((x >> 3) & 3);
+    // (the last block first: later tokens attend more, and the long ones must not come last)
+    if (!p.dealt) return {find_block(p, (int64_t)gridDim.x - 1 - x, m), (int32_t)blockIdx.y, p.per_split};
+    const int lane = threadIdx.x & 63, i = min(lane, p.B - 1);
+    const int32_t first = min(max(p.indptr[i], 0), p.T), end = p.indptr[i + 1], len = p.lens[i];
+    const int64_t rows = lane < p.B ? (int64_t)max(0, min(max(end, 0), p.T) - first) * p.H : 0;
+    const int32_t blocks = (int32_t)((rows + m - 1) / m);
+    const int32_t tiles = rows > 0 ? (int32_t)((min((int64_t)min(max(len, 0), p.max_len), p.pages.limit) + TILE - 1) / TILE) : 0;
+    const float all = over_lanes((float)blocks * (float)tiles, 0.0f, [](float u, float v) { return u + v; });
+    const int32_t most = over_lanes(max(tiles, 1), 1, [](int32_t u, int32_t v) { return max(u, v); });
+    const int32_t least = parts(most, p.ns);          // no more than ns splits of any
+    const float want = all / (float)places * __builtin_amdgcn_exp2f((float)(lane - 15) * 0.1f);
+    const int32_t size = lane == 63 ? most : max(least, min(most, (int32_t)fminf(want, 1.0e9f) + 1));
+    const float inv = 0.99999f * __builtin_amdgcn_rcpf((float)size);
+    float groups = 0.0f;
+    const float blocks_f = (float)blocks, tiles_f = (float)tiles;
+    for (int j0 = 0; j0 < p.B; j0 += 4)               // (lanes past the last hold no blocks)
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        all += __shfl_xor(all, off, 64);
-        most = max(most, __shfl_xor(most, off, 64));
+        for (int j = 0; j < 4; ++j) {
+            auto at = [&](float v) {
+                return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, v), j0 + j));
+            };
+            groups = __builtin_fmaf(at(blocks_f), __builtin_ceilf(at(tiles_f) * inv), groups);
+        }
+    const Kernel k = p.kernel;
+    const float room = (float)places, tile = groups > (float)CUS && k.pair > 0.0f ? k.pair : k.tile;
+    float us = groups <= room ? k.start + tile * (float)size
+                              : (tile * all + k.start * groups) / room + 0.5f * tile * (float)size;
+    us += groups * (float)m * (2.0f * 4.0f * (D_VO + 1) / PART_BYTES_US) + JOIN_SPLIT_US * (float)most * inv;
+    if (lane != 63 && groups > (float)gridDim.x) us = FLT_MAX;
+    const float best = over_lanes(us, FLT_MAX, [](float u, float v) { return fminf(u, v); });
+    const uint64_t at = __builtin_amdgcn_ballot_w64(us == best);
+    int32_t per = __builtin_amdgcn_readlane(size, at ? __builtin_ctzll(at) : 63);
+    // the workgroups up to and with a sequence's; whole sequences where the estimate was too low
+    uint32_t upto;
+    int32_t splits;
+    while (true) {
+        splits = parts(tiles, per);
+        upto = scan((uint32_t)min((int64_t)blocks * splits, ((int64_t)1 << 26) - 1), 0u,
+                    [](uint32_t u, uint32_t v) { return u + v; });
+        if (per == most || __builtin_amdgcn_ballot_w64(upto > gridDim.x) == 0) break;
+        per = most;
     }
-    const int64_t even = (all + p.target - 1) / p.target;
-    const int64_t least = ((int64_t)most + p.ns - 1) / p.ns;          // no more than ns splits of any
-    const int32_t per = TILE * (int32_t)max((int64_t)1, max(even, least));
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.dealt = per;
-    return __builtin_amdgcn_readfirstlane(per);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.dealt = per;
+    Work w{};
+    const int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= x));
+    if (b >= p.B) return w;
+    const int32_t nb = __builtin_amdgcn_readlane(blocks, b), ns = __builtin_amdgcn_readlane(splits, b);
+    const int32_t local = (int32_t)(x - ((uint32_t)__builtin_amdgcn_readlane(upto, b) - (uint32_t)nb * ns));
+    w.split = __builtin_amdgcn_readfirstlane(parts(local + 1, nb) - 1);
+    w.per = TILE * parts(__builtin_amdgcn_readlane(tiles, b), ns);
+    w.blk.b = b;
+    w.blk.first = __builtin_amdgcn_readlane(first, b), w.blk.end = __builtin_amdgcn_readlane(end, b);
+    w.blk.len = __builtin_amdgcn_readlane(len, b);
+    w.blk.r0 = __builtin_amdgcn_readfirstlane((nb - 1 - (local - w.split * nb)) * m);
+    w.blk.rows = (int32_t)min((int64_t)(min(max(w.blk.end, 0), p.T) - w.blk.first) * p.H - w.blk.r0, (int64_t)m);
+    return w;
 }
 
 // the kernel's argument block, in the constant address space
@@ -202,10 +300,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hi = lane >> 5, r32 = lane & 31;
-    const int split = blockIdx.y;
-    // last block first: later tokens attend more, and the long ones must not come last
-    const Block blk = find_block(p, (int64_t)gridDim.x - 1 - blockIdx.x, BLOCK);
-    const int32_t per = split_of(p, BLOCK);
+    const Work work = find_work(p, BLOCK, CUS);
+    const Block& blk = work.blk;
+    const int split = work.split, per = work.per;
     if (blk.rows == 0) return;
     const int t_lo = blk.first + blk.r0 / p.H, t_hi = blk.first + (blk.r0 + blk.rows - 1) / p.H;
     const int lim_lo = limit_in(p, blk, t_lo), lim_hi = limit_in(p, blk, t_hi);
@@ -845,7 +942,6 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 //   PV     wave w: O^T[dims 128 w .. +127 x 32 rows] in 64 registers
 // Two barriers a tile; one workgroup's waits are the other's time.
 // ---------------------------------------------------------------------------
-constexpr int NARROW = 32;                   // rows of a workgroup
 // A tile in LDS: NoPE rows of 1 KB, piece c of row r at c ^ nsw(r), so that neither the K reads (one piece of
 // 16 rows: 16 values of nsw) nor the transposed V reads (four pieces of four rows: their pieces part at bit 2)
 // meet a bank twice; with 1040-byte rows and c ^ 4 (r % 4) conflicts took 400 of a tile's 880 LDS cycles.
@@ -882,13 +978,9 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.y;
-    // Blocks of one sequence follow one another and read the same rows: four at a time on one XCD
-    // (workgroups go to the eight in turn).
-    int64_t x = blockIdx.x;
-    if (x < (int64_t)(gridDim.x & ~31u)) x = (x & ~31) | (x & 7) << 2 | ((x >> 3) & 3);
-    const Block blk = find_block(p, (int64_t)gridDim.x - 1 - x, NARROW);
-    const int32_t per = split_of(p, NARROW);
+    const Work work = find_work(p, NARROW, 2 * CUS);
+    const Block& blk = work.blk;
+    const int split = work.split, per = work.per;
     if (blk.rows == 0) return;
     const int lim_lo = limit_in(p, blk, blk.first + blk.r0 / p.H);
     const int lim_hi = limit_in(p, blk, blk.first + (blk.r0 + blk.rows - 1) / p.H);
@@ -1371,7 +1463,7 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
     // split's sum and (where a row has four waves) a wave's first eight partials.
     const int32_t i0 = min(lane, p.B - 1);
     const int32_t start_l = p.indptr[i0], end_l = p.indptr[i0 + 1], len_l = p.lens[i0];
-    const int32_t per = p.target ? *p.dealt : p.per_split;
+    const int32_t dealt = p.dealt ? *p.dealt : 0;
     const float lse_l = p.part_lse[min(lane, p.ns - 1) * step + row];
     const float* const src = p.part_o + row * D_VO + 8 * lane;
     f32x4 x[8], y[8];
@@ -1396,6 +1488,12 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
         if (b == NO_SEQ) return;
         len = p.lens[b];
         limit = limit_of(p, b, t);
+    }
+    int32_t per = p.per_split;
+    if (p.dealt) {
+        // (as find_work has it; 1 where there is no position, and no split is read)
+        const int32_t tiles = (int32_t)((min((int64_t)min(max(len, 1), p.max_len), p.pages.limit) + TILE - 1) / TILE);
+        per = TILE * max(1, parts(tiles, max(1, parts(tiles, dealt))));
     }
     const int ns = (int)min((int64_t)p.ns, (min(limit, p.pages.limit) + per - 1) / per);
     const float mine = lane < ns ? lse_l : -FLT_MAX;
@@ -1460,14 +1558,11 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 // the two sides of it, us: one token of 128 heads over 1501 rows, 128-row blocks 25.2, 32-row 17.7;
 // 256 of 16 heads over 4096 302 and 217; 200 of 128 heads over 1000 78 and 120; 512 tokens of
 // 16 heads over the same 4096 rows 90 (4 splits) and 120.
-struct Kernel {
-    float start, tile, pair;
-};
 constexpr Kernel KERNELS[2][2] = {       // [656-byte rows][narrow]
     {{6.3f, 1.83f, 0.0f}, {6.4f, 1.15f, 1.81f}},
     {{10.6f, 2.47f, 0.0f}, {8.3f, 1.48f, 2.07f}},
 };
-constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f, PART_BYTES_US = 5.3e6f;
+constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f;
 constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64};
 
 // Four waves join a row where there are few rows of many splits, one wave elsewhere.  A call with one
@@ -1480,7 +1575,7 @@ struct Plan {
     bool narrow;
     int ns;              // at most
     int32_t per;         // positions of a split
-    int32_t target;      // workgroups to deal to (0: ns splits of `per` positions)
+    bool deal;           // the device chooses the split's positions
 };
 
 float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int ns) {
@@ -1510,16 +1605,13 @@ Plan plan_of(const dsa_mla_chunk_args* a) {
             // (a split of fewer positions than a tile is none; 64 splits of a grid's y extent)
             if (ns > 1 && !a->num_splits && (int64_t)a->max_kv_len < (int64_t)ns * TILE) break;
             const float us = expected_us(a, n != 0, blocks, ns);
-            if (us < least) {
-                least = us, best.narrow = n != 0, best.ns = ns;
-                best.target = (int32_t)std::min<int64_t>(INT32_MAX, blocks * ns);
-            }
+            if (us < least) least = us, best.narrow = n != 0, best.ns = ns;
             if (a->num_splits) break;
         }
     }
-    // several sequences, split by the device: up to twice as many splits of those twice as long as the mean
-    if (a->num_splits || best.ns == 1 || a->B == 1) best.target = 0;
-    else best.ns = std::min(2 * best.ns, (int)DSA_MLA_MAX_SPLITS);
+    // up to twice as many splits, of the size that the lengths ask for
+    best.deal = !a->num_splits && best.ns > 1 && a->B <= 64;
+    if (best.deal) best.ns = std::min(2 * best.ns, (int)DSA_MLA_MAX_SPLITS);
     const int64_t each = (a->max_kv_len + (int64_t)best.ns - 1) / best.ns;
     best.per = (int32_t)std::min<int64_t>(INT32_MAX - TILE + 1, std::max<int64_t>(TILE, (each + TILE - 1) / TILE * TILE));
     return best;
@@ -1606,15 +1698,18 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.lse = a->lse;
     p.part_o = (float*)ws;
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
-    p.dealt = (int32_t*)(p.part_lse + (size_t)p.ns * a->T * a->H);
-    p.target = plan.target;
+    p.dealt = plan.deal ? (int32_t*)(p.part_lse + (size_t)p.ns * a->T * a->H) : nullptr;
+    p.kernel = KERNELS[a->kv_format == DSA_KV_FP8_656][plan.narrow];
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
     const bool narrow = plan.narrow;
     const bool runs = !a->block_table || a->block_size % TILE == 0;
     const int32_t m = narrow ? NARROW : BLOCK;
     p.common = dsa_seq::common(a->H, m);
-    const dim3 blocks((unsigned)dsa_seq::block_start(a->T, a->B, a->H, m, p.common), (unsigned)p.ns);
+    const int64_t most = dsa_seq::block_start(a->T, a->B, a->H, m, p.common);
+    const int64_t places = plan.narrow ? 2 * CUS : CUS;
+    const dim3 blocks((unsigned)(plan.deal ? std::min(most * p.ns, most <= places / 4 ? places : 3 * places + most) : most),
+                      plan.deal ? 1u : (unsigned)p.ns);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
     const bool fp8 = a->kv_format == DSA_KV_FP8_656;
     if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
