@@ -128,8 +128,8 @@ int dsa_qk_norm_rope(const dsa_qk_norm_rope_args* args, void* stream);
  *            n_pos are NaN.
  * A call must not name one cache row twice.  Flat caches of several sequences
  * need kv_batch_stride > 0.
- * Alignment: 16 bytes for pointers to rows, cos_sin, weights (4 for cache_scale: 16
- * bytes too); bf16 strides multiples of 8, byte strides of 16.
+ * Alignment: 16 bytes for pointers to rows, cos_sin, weights and biases; bf16
+ * strides multiples of 8, byte strides of 16.
  */
 typedef struct {
     const void* kv;
@@ -184,13 +184,18 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  * num_splits: 0 = automatic, or 1 .. DSA_MLA_MAX_SPLITS parts of max_kv_len
  *            positions (rounded up to whole tiles of 32), whose fp32 partials
  *            (workspace: num_splits x T x H x 513 floats and 16 bytes) a combine
- *            merges.  Automatic: by the sizes, and for several sequences the
- *            device deals their positions evenly, so that a sequence's parts go
- *            by its length (dsa_mla_chunk_num_splits: the most that one has).
+ *            merges.  Automatic: whether to split by the call's sizes, and up to
+ *            64 sequences the size of a split by their lengths, on the device
+ *            (dsa_mla_chunk_num_splits: the most that one sequence has).
  * Scores and sums are fp32.  Probabilities are rounded to 16 bits for the
  * product with V (bf16; fp16 for DSA_KV_FP8_656).  656-byte rows: scores use
- * their exact values; V is rounded to fp16 (its scale's mantissa first) and every scale must lie in [0, 128),
- * a token that attends a row with another scale getting NaN, as in dsa_mla.h.
+ * their exact values; V is rounded to fp16 (its scale's mantissa first), and
+ * every scale must lie in [0, 128), a token that attends a row with another
+ * scale getting NaN, as in dsa_mla.h.
+ * Limits: T x H + 128 B, kv_total_rows and block_size x table_blocks below 2^31,
+ * max_kv_len at most DSA_MLA_MAX_LIST.
+ * Alignment: q and kv_cache 16 bytes, out 8; q's strides multiples of 8, out's of
+ * 4 and at least 512, cache rows of 16 bytes and below 4 GiB.
  * The split and so the last bits depend on the call's sizes and, with
  * num_splits = 0, on the lengths of all its sequences; one call repeats its bits.
  */

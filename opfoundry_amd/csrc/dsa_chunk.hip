@@ -181,15 +181,10 @@ __device__ __forceinline__ T over_lanes(T v, T none, F op) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, scan(v, none, op)), 63));
 }
 
-// ceil(a / b) of 0 <= a < 2^31 and 1 <= b <= 2^26: exact where it is below 2^20, else at least that and at
-// most 2^-19 more.  (The product is off by less than 2^-21 of itself; an integer division takes ten times
-// the code, which a workgroup's first waves fetch.)
+// Parts of at most b that `a` has (an integer division takes ten times the code, which a workgroup's first
+// waves fetch).
 __device__ __forceinline__ int32_t parts(int32_t a, int32_t b) {
-    uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
-    q += q >> 20;
-    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
-    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
-    return (int32_t)q;
+    return dsa_seq::parts_by(a, b, __builtin_amdgcn_rcpf((float)b));
 }
 
 // The block, the split and the positions of a split of a workgroup.  The host knows a bound of the
@@ -1647,6 +1642,7 @@ int validate(const dsa_mla_chunk_args* a) {
     if (a->T == 0 || a->B == 0) return DSA_OK;
     if (!a->q || !a->out || !a->q_indptr || !a->seq_lens || (a->kv_total_rows > 0 && !a->kv_cache))
         return DSA_ERR_NULL_POINTER;
+    if ((a->H > 1 && a->o_stride_h < D_VO) || (a->T > 1 && a->o_stride_t < D_VO)) return DSA_ERR_BAD_STRIDE;
     if (a->q_stride_t < 0 || a->q_stride_h < 0 || (a->q_stride_t % 8) || (a->q_stride_h % 8) || a->o_stride_t < 0 ||
         a->o_stride_h < 0 || (a->o_stride_t % 4) || (a->o_stride_h % 4))
         return DSA_ERR_BAD_STRIDE;

@@ -72,6 +72,18 @@ __host__ __device__ inline int64_t block_start(int64_t indptr_b, int32_t b, int3
     return (indptr_b * H + (int64_t)b * (m - g)) / m;
 }
 
+// ceil(a / b) of 0 <= a < 2^31 and 1 <= b <= 2^26 by a reciprocal of b that is off by at most 2^-23 of
+// itself: exact where it is below 2^20, else at least that and at most 2^-19 more.  (Rounding a, b, the
+// reciprocal and the product moves the quotient by less than 2^-21 of itself: below 2^20 its floor is then
+// off by one at most, and two steps reach the ceiling; above, the share added first outweighs it.)
+__host__ __device__ inline int32_t parts_by(int32_t a, int32_t b, float reciprocal) {
+    uint32_t q = (uint32_t)((float)a * reciprocal);
+    q += q >> 20;
+    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
+    q += q * (uint32_t)b < (uint32_t)a ? 1 : 0;
+    return (int32_t)q;
+}
+
 }  // namespace dsa_seq
 
 #endif  // DSA_SEQ_H_

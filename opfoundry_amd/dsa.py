@@ -874,6 +874,8 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     sequence b's tokens q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b].  kv
     or index_k may be None."""
     dev = q_indptr.get_device()
+    if dev < 0:
+        raise ValueError("q_indptr must be a device tensor")
     pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     T = rope = irope = 0
     paged_like = index_cache
