@@ -163,6 +163,36 @@ __device__ __forceinline__ void norm8(V8& x, int kind, bool in, float inv_n, flo
     }
 }
 
+// Sequences and positions of the N tokens from t on (include/dsa_chunk.h); NO_SEQ for one of none.  Up to
+// 64 sequences are read at once, a lane each, so that a token waits for one load and not for three in turn.
+template <int N>
+struct Located {
+    int32_t b[N];
+    int64_t pos[N];
+};
+template <int N>
+__device__ __forceinline__ Located<N> locate(const int32_t* indptr, const int32_t* lens, int32_t B, int32_t t) {
+    Located<N> r;
+    if (B <= 64) {
+        const int lane = threadIdx.x & 63, i = min(lane, B - 1);
+        const int32_t start = indptr[i], end = indptr[i + 1], len = lens[i];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int32_t b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < B && end <= t + k));
+            const int32_t at = min(b, B - 1);
+            r.b[k] = b < B && t + k >= __builtin_amdgcn_readlane(start, at) ? b : NO_SEQ;
+            r.pos[k] = (int64_t)__builtin_amdgcn_readlane(len, at) - __builtin_amdgcn_readlane(end, at) + t + k;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            r.b[k] = seq_of(indptr, B, t + k);
+            r.pos[k] = r.b[k] == NO_SEQ ? -1 : dsa_seq::position_of(indptr, lens, r.b[k], t + k);
+        }
+    }
+    return r;
+}
+
 // ---------------------------------------------------------------------------
 // Norms and rotation of queries and keys.  A wave takes GROUP heads of one
 // token of one stream: their loads are all in flight before the first is used,
@@ -205,9 +235,9 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_qk_norm_rope_kernel(const dsa_
     if (p.positions) {
         pos = p.positions[t];
     } else if (ROPE != DSA_ROPE_NONE || p.q_indptr) {
-        const int32_t b = seq_of(p.q_indptr, p.B, t);
-        if (b == NO_SEQ) return;
-        pos = dsa_seq::position_of(p.q_indptr, p.seq_lens, b, t);
+        const Located<1> at = locate<1>(p.q_indptr, p.seq_lens, p.B, t);
+        if (at.b[0] == NO_SEQ) return;
+        pos = at.pos[0];
     } else {
         pos = 0;
     }
@@ -296,12 +326,12 @@ __device__ __forceinline__ void append_latent(const AppendParams& p, int t) {
     V8 w{};
     if (a.weight) w = load8f(a.weight + 8 * lane);
 
-    const int32_t b = seq_of(a.q_indptr, a.B, t);
-    if (b == NO_SEQ) return;
-    const int64_t pos = dsa_seq::position_of(a.q_indptr, a.seq_lens, b, t);
-    const int64_t row = dsa_seq::row_of(p.pages, b, pos, a.cache_rows);
+    const Located<1> at = locate<1>(a.q_indptr, a.seq_lens, a.B, t);
+    if (at.b[0] == NO_SEQ) return;
+    const int64_t pos = at.pos[0];
+    const Turn turn = load_turn<ROPE>(a.cos_sin, a.n_pos, pos, lane & 7, false);      // in flight beside the page's
+    const int64_t row = dsa_seq::row_of(p.pages, at.b[0], pos, a.cache_rows);
     if (row < 0) return;
-    const Turn turn = load_turn<ROPE>(a.cos_sin, a.n_pos, pos, lane & 7, false);
     V8 v = unpack8(raw), tail = unpack8(raw_tail);
     norm8<64>(v, a.norm, true, 1.0f / 512.0f, a.eps, a.weight != nullptr, w, false, w);
     if (wide) turn8<ROPE>(tail, turn, true);
@@ -352,16 +382,11 @@ __device__ __forceinline__ void append_index(const AppendParams& p, int t0) {
     V8 w{}, bias{};
     if (a.index_weight) w = load8f(a.index_weight + 8 * piece);
     if (a.index_bias) bias = load8f(a.index_bias + 8 * piece);
-    int64_t row = -1, pos = -1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (t0 + i >= a.T) break;
-        const int32_t b = seq_of(a.q_indptr, a.B, t0 + i);
-        if (b == NO_SEQ) continue;
-        const int64_t at = dsa_seq::position_of(a.q_indptr, a.seq_lens, b, t0 + i);
-        const int64_t r = dsa_seq::row_of(p.pages, b, at, a.index_rows);
-        if ((lane >> 4) == i) row = r, pos = at;
-    }
+    const Located<4> at = locate<4>(a.q_indptr, a.seq_lens, a.B, t0);
+    const int k = lane >> 4;
+    const int32_t b = there ? (k & 2 ? (k & 1 ? at.b[3] : at.b[2]) : (k & 1 ? at.b[1] : at.b[0])) : NO_SEQ;
+    const int64_t pos = k & 2 ? (k & 1 ? at.pos[3] : at.pos[2]) : (k & 1 ? at.pos[1] : at.pos[0]);
+    const int64_t row = b == NO_SEQ ? -1 : dsa_seq::row_of(p.pages, b, pos, a.index_rows);
     const Turn turn = load_turn<ROPE>(a.cos_sin, a.n_pos, pos, piece & 7, false);
     V8 v = unpack8(raw);
     norm8<16>(v, a.index_norm, true, 1.0f / 128.0f, a.index_eps, a.index_weight != nullptr, w,
