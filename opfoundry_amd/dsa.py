@@ -610,6 +610,9 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
 # cost little: one look at a tensor's type, device, shape and strides, and argument structs filled at once.
 
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+# (absent from a torch without devices, where every call ends before it needs them)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _bad(name: str, t, what: str):
@@ -662,9 +665,7 @@ def _vector(t: Optional[torch.Tensor], n: int, dtype, name: str, dev: int) -> in
     return t.data_ptr()
 
 
-def _choice(table, value, name: str) -> int:
-    if value in table:
-        return table[value]
+def _no_choice(table, value, name: str):
     raise ValueError(f"{name} must be one of {list(table)}, got {value!r}")
 
 
@@ -727,6 +728,10 @@ def _rows(t: torch.Tensor, width: int, name: str):
     return n, (rs if n > 1 else 0)
 
 
+def _empty_like(like: torch.Tensor, shape, dtype) -> torch.Tensor:
+    return like.new_empty(shape, dtype=dtype)
+
+
 class _Stream:
     """The stream of a call on device `dev` and what it allocates.  Memory used on a stream that is not the
     device's current one is marked so for the allocator, which then does not hand it out while the call runs."""
@@ -735,7 +740,7 @@ class _Stream:
 
     def __init__(self, dev: int, stream):
         self.dev = dev
-        current = torch._C._cuda_getCurrentRawStream(dev)
+        current = _raw_stream(dev)
         self.other = None
         if stream is None:
             self.handle = current
@@ -757,7 +762,7 @@ class _Stream:
         return t
 
     def call(self, fn, where: str, *args) -> None:
-        if torch._C._cuda_getDevice() == self.dev:
+        if _current_device() == self.dev:
             rc = fn(*args, self.handle)
         else:
             with torch.cuda.device(self.dev):
@@ -768,8 +773,8 @@ class _Stream:
 
 def _launch(fn, where: str, dev: int, stream, *args) -> None:
     """One call that allocates nothing on a stream."""
-    if stream is None and torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if stream is None and _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
         if rc:
             check(rc, where)
     else:
@@ -777,17 +782,23 @@ def _launch(fn, where: str, dev: int, stream, *args) -> None:
 
 
 def _normed_rows(x, norm, w, b, out, T, D, norm_dim, name, dev, on):
-    """The fields of dsa_norm_rope_rows of one stream, and its output."""
+    """The fields of dsa_norm_rope_rows of one stream, and its output (on: None where the call runs on the
+    current stream of the current device)."""
     H = x.shape[1]
     px, st, sh = _addr3(x, T, H, D, name, dev)
     if out is None:
-        out = on.empty_like(x) if x.is_contiguous() else on.empty(x, (T, H, D), _BF16)
+        if not x.is_contiguous():
+            out = (on or _Stream(dev, None)).empty(x, (T, H, D), _BF16)
+        else:
+            out = torch.empty_like(x) if on is None else on.empty_like(x)
         po, ot, oh = out.data_ptr(), H * D, D
     else:
         po, ot, oh = _addr3(out, T, H, D, name + "_out", dev)
+    kind = abi.NORMS.get(norm)
+    if kind is None:
+        _no_choice(abi.NORMS, norm, name + "_norm")
     return (px, st, sh, po, ot, oh, 0 if w is None else _vector(w, norm_dim, _F32, name + "_weight", dev),
-            0 if b is None else _vector(b, norm_dim, _F32, name + "_bias", dev), H,
-            _choice(abi.NORMS, norm, name + "_norm")), out
+            0 if b is None else _vector(b, norm_dim, _F32, name + "_bias", dev), H, kind), out
 
 
 _NO_ROWS = (0,) * 10
@@ -820,7 +831,9 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
     norm_dim = min(D, 512) if norm_dim is None else int(norm_dim)
     if rot_off is None:
         rot_off = 0 if D == 128 else D - abi.D_ROPE
-    rope = _choice(abi.ROPES, style, "style")
+    rope = abi.ROPES.get(style)
+    if rope is None:
+        _no_choice(abi.ROPES, style, "style")
     pcs, n_pos = _angles(cos_sin, dev) if rope else (0, 0)
     pp = pi = pl = B = 0
     if positions is not None:
@@ -831,7 +844,7 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
         pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     elif rope:
         raise ValueError("a rotation needs positions, or q_indptr and seq_lens")
-    on = _Stream(dev, stream)
+    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
     qs, q_out = _normed_rows(q, q_norm, q_weight, q_bias, q_out, T, D, norm_dim, "q", dev, on)
     if k is not None:
         if k.dim() != 3:
@@ -842,16 +855,21 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
             raise ValueError("k_norm, k_weight, k_bias and k_out need k")
         ks = _NO_ROWS
     a = abi.pack_norm_rope(*qs, *ks, pcs, n_pos, pp, pi, pl, T, B, D, norm_dim, rot_off, rope, 1 if inverse else 0, eps)
-    on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", a)
+    if on is None:
+        rc = load_library().dsa_qk_norm_rope(a, _raw_stream(dev))
+        if rc:
+            check(rc, "dsa_qk_norm_rope")
+    else:
+        on.call(load_library().dsa_qk_norm_rope, "dsa_qk_norm_rope", a)
     return q_out, k_out
 
 
-# the tensors of a cache -> (kv_format, width of its latent rows)
-_CACHES = {((_BF16, 576),): (abi.KV_BF16, 576), ((_U8, 656),): (abi.KV_FP8_656, 576),
-           ((_BF16, 512),): (abi.KV_BF16_D512, 512),
-           ((_U8, 512), (_U8, 16), (_BF16, 64)): (abi.KV_MXFP8, 576),
-           ((_U8, 512), (_BF16, 64)): (abi.KV_MXFP8_V4, 512)}
-_KV_NORMS = {None: None, "none": 0, "rms": 1}
+# the tensors of a cache -> (kv_format, width of its latent rows, width of the first tensor's rows)
+_CACHE = {(_BF16, 576): (abi.KV_BF16, 576, 576), (_U8, 656): (abi.KV_FP8_656, 576, 656),
+          (_BF16, 512): (abi.KV_BF16_D512, 512, 512)}
+_CACHES = {((_U8, 512), (_U8, 16), (_BF16, 64)): (abi.KV_MXFP8, 576, 512),
+           ((_U8, 512), (_BF16, 64)): (abi.KV_MXFP8_V4, 512, 512)}
+_KV_NORMS = {"none": 0, "rms": 1}
 
 
 def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
@@ -881,17 +899,19 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     paged_like = index_cache
     kvp = pw = kst = rows = stride = sstride = rstride = fmt = kind = pc = psc = pr = 0
     if kv is not None:
-        several = isinstance(cache, (tuple, list))
-        paged_like = first = cache[0] if several else cache
-        parts = cache if several else (cache,)
-        found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
+        parts = cache if isinstance(cache, (tuple, list)) else (cache,)
+        paged_like = first = parts[0]
+        if len(parts) == 1:
+            found = _CACHE.get((first.dtype, first.shape[-1]))
+        else:
+            found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
         if found is None:
             raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
-        fmt, width = found
+        fmt, width, own = found
         kvp, T, kst = _addr2(kv, width, "kv", dev)
         pc = _addr(first, first.dtype, "cache", dev)
-        rows, stride = _rows(first, first.shape[-1], "cache")
-        if several and len(parts) > 1:
+        rows, stride = (first.numel() // own, 0) if first.is_contiguous() else _rows(first, own, "cache")
+        if len(parts) > 1:
             last = parts[-1]
             pr = _addr(last, _BF16, "cache", dev)
             more, rstride = _rows(last, 64, "cache")
@@ -901,12 +921,17 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
                 more = more if others == rows else -1
             if more != rows:
                 raise ValueError("the cache's streams must have the same rows")
-        kind = _choice(_KV_NORMS, norm, "norm")
-        if kind is None:
+        if norm is None:
             kind = 0 if weight is None else 1
+        elif norm in _KV_NORMS:
+            kind = _KV_NORMS[norm]
+        else:
+            _no_choice(_KV_NORMS, norm, "norm")
         if weight is not None:
             pw = _vector(weight, 512, _F32, "weight", dev)
-        rope = _choice(abi.ROPES, style, "style")
+        rope = abi.ROPES.get(style)
+        if rope is None:
+            _no_choice(abi.ROPES, style, "style")
     ip = iw = ib = ic = ist = irows = istride = ikind = 0
     if index_k is not None:
         if index_cache is None:
@@ -918,13 +943,20 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
         ic = _addr(index_cache, _BF16, "index_cache", dev)
         if index_cache.shape[-1] != 128:
             _bad("index_cache", index_cache, "be [..., 128]")
-        irows, istride = _rows(index_cache, 128, "index_cache")
-        ikind = _choice(abi.NORMS, index_norm, "index_norm")
+        if index_cache.is_contiguous():
+            irows = index_cache.numel() // 128
+        else:
+            irows, istride = _rows(index_cache, 128, "index_cache")
+        ikind = abi.NORMS.get(index_norm)
+        if ikind is None:
+            _no_choice(abi.NORMS, index_norm, "index_norm")
         if index_weight is not None:
             iw = _vector(index_weight, 128, _F32, "index_weight", dev)
         if index_bias is not None:
             ib = _vector(index_bias, 128, _F32, "index_bias", dev)
-        irope = _choice(abi.ROPES, index_style, "index_style")
+        irope = abi.ROPES.get(index_style)
+        if irope is None:
+            _no_choice(abi.ROPES, index_style, "index_style")
     pcs, n_pos = _angles(cos_sin, dev) if rope or irope else (0, 0)
     pt, tst, blocks, bs = _pages(block_table, block_size, paged_like, B, dev)
     a = abi.pack_append(kvp, kst, pw, pc, psc, pr, rows, stride, sstride, rstride, fmt, kind, rope, ikind, irope,
@@ -943,12 +975,13 @@ def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, bloc
     pq, qt, qh = _addr3(q, T, H, abi.D_QK, "q", dev)
     pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     width = kv_cache.shape[-1]
-    fmt = _CACHES.get(((kv_cache.dtype, width),), (-1, 0))[0]
-    if fmt != abi.KV_BF16 and fmt != abi.KV_FP8_656:
+    found = _CACHE.get((kv_cache.dtype, width))
+    if found is None or found[0] == abi.KV_BF16_D512:
         raise ValueError(f"kv cache must be bf16 [..., 576] or uint8 [..., 656], got {kv_cache.dtype} "
                          f"{tuple(kv_cache.shape)}")
+    fmt = found[0]
     pk = _addr(kv_cache, kv_cache.dtype, "kv_cache", dev)
-    rows, stride = _rows(kv_cache, width, "kv_cache")
+    rows, stride = (kv_cache.numel() // width, 0) if kv_cache.is_contiguous() else _rows(kv_cache, width, "kv_cache")
     pt, tst, blocks, bs = _pages(block_table, block_size, kv_cache, B, dev)
     if max_kv_len is None:
         max_kv_len = blocks * bs if block_table is not None else int(kv_batch_stride) or rows
@@ -991,12 +1024,14 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     dev = q.get_device()
     if dev < 0 or q.dim() != 3:
         _bad("q", q, "be a device tensor [T, H, 576]")
-    on = _Stream(dev, stream)
+    # (None: the current stream of the current device, the usual call)
+    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
+    empty = _empty_like if on is None else on.empty
     T, H, _ = q.shape
     if out is None:
-        out = on.empty(q, (T, H, abi.D_VO), _BF16)
+        out = empty(q, (T, H, abi.D_VO), _BF16)
     if lse is None:
-        lse = on.empty(q, (T, H), _F32)
+        lse = empty(q, (T, H), _F32)
     a = make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, block_table=block_table,
                         block_size=block_size, kv_batch_stride=kv_batch_stride, causal=causal,
                         max_kv_len=max_kv_len, num_splits=num_splits)
@@ -1004,9 +1039,15 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     ws = None
     if need:
         if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = on.empty(q, (need,), _U8)
+            workspace = empty(q, (need,), _U8)
         elif not workspace.is_contiguous():
             _bad("workspace", workspace, "be dense")
         ws = _addr(workspace, workspace.dtype, "workspace", dev)
-    on.call(load_library().dsa_mla_chunk, "dsa_mla_chunk", a, ws, need)
+    fn = load_library().dsa_mla_chunk
+    if on is None:
+        rc = fn(a, ws, need, _raw_stream(dev))
+        if rc:
+            check(rc, "dsa_mla_chunk")
+    else:
+        on.call(fn, "dsa_mla_chunk", a, ws, need)
     return out, lse
