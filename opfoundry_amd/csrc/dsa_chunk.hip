@@ -75,6 +75,13 @@ __device__ __forceinline__ int64_t limit_of(const ChunkParams& p, int32_t b, int
 // Iteration i computes QK^T of tile i + 1, then PV of tile i with the exponentials of
 // tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 403 of a
 // CU's 512 KB of registers, which is why a workgroup is 128 rows and fills a CU.
+// Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 2.05 ms, 1.21 PFLOP/s, 89 % of what
+// a product of two 16384 x 16384 matrices reaches here; 1.79 us a tile and workgroup, matrix units busy
+// 54 % of the cycles at the 1.8 to 2.2 GHz that the card holds under them (reading the first operands of
+// PV ahead, in the last steps of the scores, changes nothing).  656-byte rows (two prompts of 1915 and
+// 1782 tokens): 1.30 ms, 733 TFLOP/s, 2.44 us a tile: every wave converts the whole tile's codes for its
+// scores (8 vector instructions to a matrix instruction, matrix units busy 30 %).  A shared tile of
+// converted codes has no room beside V's two and the three raw ones.
 // ---------------------------------------------------------------------------
 constexpr int BLOCK = 128;                   // rows of a workgroup
 constexpr int SPAN = 2048;                   // positions resolved to cache rows at a time
@@ -936,10 +943,14 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 //   P      as in the tiled kernel, one buffer: P of a tile is read before the next's is written
 //   PV     wave w: O^T[dims 128 w .. +127 x 32 rows] in 64 registers
 // Two barriers a tile; one workgroup's waits are the other's time.
+// Measured (16 sequences of 7130 to 19272 bf16 rows, 1 to 4 tokens of 16 heads): 59 us, 290 MB read at
+// 4.9 TB/s, 96 % of a large copy's rate.  One token of 128 heads over 1483 656-byte rows: 14.4 us in
+// 64 workgroups of 3 tiles, a chain of memory round trips (1.5 us to the split, then pages, rows, partials).
 // ---------------------------------------------------------------------------
-// A tile in LDS: NoPE rows of 1 KB, piece c of row r at c ^ nsw(r), so that neither the K reads (one piece of
-// 16 rows: 16 values of nsw) nor the transposed V reads (four pieces of four rows: their pieces part at bit 2)
-// meet a bank twice; with 1040-byte rows and c ^ 4 (r % 4) conflicts took 400 of a tile's 880 LDS cycles.
+// A tile in LDS: NoPE rows of 1 KB, piece c of row r at c ^ nsw(r): the K reads (one piece of 16 rows) find 16
+// values of nsw, the transposed V reads (four pieces of four rows) pieces that part at bit 2.  Conflicts take
+// 270 of a tile's 790 LDS cycles (1040-byte rows and c ^ 4 (r % 4): 400 of 880, and 233 us where this is 202:
+// 256 single tokens of 16 heads over 4096 656-byte rows).
 constexpr int NSTRIDE = 1024;
 __device__ __forceinline__ int nsw(int r) { return 4 * (r & 3) + ((r >> 2) & 3); }
 constexpr int NROPE_OFF = TILE * NSTRIDE;
@@ -1444,6 +1455,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
 
 // Joins the partials of a row's splits, SHARES waves a row: a lane holds 8 of its 512 values,
 // wave i takes splits i, i + SHARES, ...  Splits past the row's positions wrote nothing and add nothing.
+// Bound by a chain of memory round trips where there are few rows (128 rows of 16 splits 4.1 us, 6.8 with one
+// wave a row and the loads in turn), by the partials' bytes where there are many (40040 rows of 1 to 3 splits 39 us).
 template <int SHARES>
 __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const ChunkParams p) {
     __shared__ __attribute__((aligned(16))) float s_o[SHARES > 1 ? SHARES * D_VO : 4];
@@ -1562,8 +1575,9 @@ constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 4
 
 // Four waves join a row where there are few rows of many splits, one wave elsewhere.  A call with one
 // and with four, us: 16 rows of 48 splits 22.7 and 17.4; 128 of 32 27.0 and 23.6, of 8 20.4 and 19.6, of 2
-// 19.9 and 19.9; 512 of 16 30.3 and 28.5, of 4 21.4 and 22.0; 1024 of 8 26.4 and 27.2; 4096 of 4 34.2 and 39.0.
-constexpr int64_t FEW_ROWS = 512;
+// 19.9 and 19.9; 512 of 16 30.3 and 28.5, of 4 21.4 and 22.0; 1024 of 32 38.0 and 37.2, of 8 26.4 and 27.2;
+// 2048 of 8 35.0 and 36.7; 4096 of 4 34.2 and 39.0.
+constexpr int64_t FEW_ROWS = 1024;
 constexpr int FOUR_FROM = 5;
 
 struct Plan {
