@@ -85,6 +85,8 @@ typedef struct {
  * norm_dim : a multiple of 8, 8 .. min(D, 512)
  * rot_off  : a multiple of 64, 0 .. D - 64
  * Alignment: x, out, cos_sin, weight and bias 16 bytes, strides multiples of 8.
+ * Limit: T x (ceil(q.H / g) + ceil(k.H / g)) at most 2^26 - 4, with g = 16 for
+ * D = 128, else 8.
  */
 typedef struct {
     dsa_norm_rope_rows q, k;
@@ -126,6 +128,7 @@ int dsa_qk_norm_rope(const dsa_qk_norm_rope_args* args, void* stream);
  *            the token's row of index_cache (the same row number).
  * cos_sin  : as in dsa_qk_norm_rope.  The rotated values of a token at or past
  *            n_pos are NaN.
+ * T, with index keys T + ceil(T / 4), is at most 2^26 - 4.
  * A call must not name one cache row twice.  Flat caches of several sequences
  * need kv_batch_stride > 0.
  * Alignment: 16 bytes for pointers to rows, cos_sin, weights and biases; bf16
@@ -192,8 +195,9 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  * their exact values; V is rounded to fp16 (its scale's mantissa first), and
  * every scale must lie in [0, 128), a token that attends a row with another
  * scale getting NaN, as in dsa_mla.h.
- * Limits: T x H + 128 B, kv_total_rows and block_size x table_blocks below 2^31,
- * max_kv_len at most DSA_MLA_MAX_LIST.
+ * Limits: T x H + 32 B at most 2^29 - 32 (split calls: T x H at most 2^26 - 4),
+ * kv_total_rows and block_size x table_blocks below 2^31, max_kv_len at most
+ * DSA_MLA_MAX_LIST; beyond them DSA_ERR_BAD_SHAPE.
  * Alignment: q and kv_cache 16 bytes, out 8; q's strides multiples of 8, out's of
  * 4 and at least 512, cache rows of 16 bytes and below 4 GiB.
  * The split and so the last bits depend on the call's sizes and, with

@@ -204,7 +204,7 @@ __device__ __forceinline__ int32_t parts(int32_t a, int32_t b) {
 // leave CUs idle while others hold three.  16 sequences of 7130 to 19272 bf16 rows, 16 heads: 66 us, of
 // 506 workgroups (77 in 16 splits by the bound of the lengths, 366 of them with work); 66 too where that
 // bound is four times as much (173).  7 sequences of 1994 to 4772 rows and 28 to 258 tokens of 40 heads:
-// 383 us (402 in 2).  Finding it out takes 1.5 us: one token of 128 heads over 1483 656-byte rows 19.1
+// 378 us (402 in 2).  Finding it out takes 1.5 us: one token of 128 heads over 1483 656-byte rows 19.1
 // and, in 20 splits by the caller's count, 17.3.  Of 50 ragged calls it was 4 % above the best of 13
 // counts on average (23 % below to 17 % above).
 struct Work {
@@ -1573,6 +1573,8 @@ constexpr Kernel KERNELS[2][2] = {       // [656-byte rows][narrow]
 constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f;
 constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64};
 
+constexpr int64_t MAX_GROUPS = ((int64_t)1 << 32) / NTHR - 1, MAX_SPLIT_ROWS = MAX_GROUPS * NWAVE;
+
 // Four waves join a row where there are few rows of many splits, one wave elsewhere.  A call with one
 // and with four, us: 16 rows of 48 splits 22.7 and 17.4; 128 of 32 27.0 and 23.6, of 8 20.4 and 19.6, of 2
 // 19.9 and 19.9; 512 of 16 30.3 and 28.5, of 4 21.4 and 22.0; 1024 of 32 38.0 and 37.2, of 8 26.4 and 27.2;
@@ -1613,6 +1615,7 @@ Plan plan_of(const dsa_mla_chunk_args* a) {
             const int ns = a->num_splits ? a->num_splits : c;
             // (a split of fewer positions than a tile is none; 64 splits of a grid's y extent)
             if (ns > 1 && !a->num_splits && (int64_t)a->max_kv_len < (int64_t)ns * TILE) break;
+            if (ns > 1 && (int64_t)a->T * a->H > MAX_SPLIT_ROWS) break;
             const float us = expected_us(a, n != 0, blocks, ns);
             if (us < least) least = us, best.narrow = n != 0, best.ns = ns;
             if (a->num_splits) break;
@@ -1638,8 +1641,10 @@ int validate(const dsa_mla_chunk_args* a) {
         return DSA_ERR_BAD_SHAPE;
     if (a->max_kv_len > DSA_MLA_MAX_LIST) return DSA_ERR_BAD_SHAPE;
     if (a->num_splits < 0 || a->num_splits > DSA_MLA_MAX_SPLITS) return DSA_ERR_BAD_SPLITS;
-    // (rows of queries, with a block of each sequence's own, stay below 2^31)
-    if ((int64_t)a->T * a->H + (int64_t)128 * a->B > INT32_MAX) return DSA_ERR_BAD_SHAPE;
+    // (a grid holds below 2^32 threads: workgroups of 32 rows, and the join's of 4)
+    const int64_t rows = (int64_t)a->T * a->H;
+    if (rows + (int64_t)NARROW * a->B > MAX_GROUPS * NARROW) return DSA_ERR_BAD_SHAPE;
+    if (a->num_splits > 1 && rows > MAX_SPLIT_ROWS) return DSA_ERR_BAD_SHAPE;
     const int64_t least = a->kv_format == DSA_KV_BF16 ? D_QK : DSA_MLA_FP8_ROW_BYTES;
     const int64_t unit = a->kv_format == DSA_KV_BF16 ? 2 : 1;
     if (a->kv_stride_row != 0 &&

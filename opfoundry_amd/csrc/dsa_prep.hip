@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_kv_append_kernel(const AppendP
 }
 
 // ------------------------------------------------------------------- host
-constexpr int64_t MAX_JOBS = (int64_t)INT32_MAX - 4 * WAVES;
+constexpr int64_t MAX_JOBS = (((int64_t)1 << 32) / (64 * WAVES) - 1) * WAVES;      // a grid holds below 2^32 threads
 
 bool kind_ok(int v) { return v >= 0 && v <= 2; }
 bool ptr16(const void* q) { return ((uintptr_t)q & 15) == 0; }

@@ -716,16 +716,19 @@ def _rows(t: torch.Tensor, width: int, name: str):
     st = t.stride()
     if st[-1] != 1:
         _bad(name, t, "have a dense last dim")
-    rs = expect = st[-2] if t.dim() > 1 else width
+    rs = expect = None
     for d in range(t.dim() - 2, -1, -1):
         if t.shape[d] > 1:
+            if rs is None:
+                rs = expect = st[d]
             if st[d] != expect:
                 _bad(name, t, "have rows one uniform stride apart")
-        expect *= t.shape[d]
-    if n > 1 and t.shape[-2] == 1:
-        # (the rows are counted by a dim further out)
-        rs = next(st[d] for d in range(t.dim() - 2, -1, -1) if t.shape[d] > 1)
-    return n, (rs if n > 1 else 0)
+            expect *= t.shape[d]
+    if rs is None:
+        return n, 0
+    if rs < width:
+        _bad(name, t, "have rows that do not overlap")
+    return n, rs
 
 
 def _empty_like(like: torch.Tensor, shape, dtype) -> torch.Tensor:
@@ -1020,7 +1023,8 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     q bf16 [T, H, 576]; kv_cache bf16 [..., 576] or uint8 [..., 656]; sequence b's tokens
     q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b] (their own rows already
     in the cache) and attend positions up to their own (causal) or all.  Rows of no sequence are left as
-    allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold)."""
+    allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold).  workspace:
+    a dense tensor for the partials of a split call (chunk_workspace_size bytes; a smaller one is not used)."""
     dev = q.get_device()
     if dev < 0 or q.dim() != 3:
         _bad("q", q, "be a device tensor [T, H, 576]")

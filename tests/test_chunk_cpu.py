@@ -221,6 +221,7 @@ PREP_BAD = [
     ({"k.H": 1}, NULL), ({"k.H": 1, "k.norm": 7}, UNSUPPORTED), ({"cos_sin": 0}, NULL), ({"cos_sin": 0x4008}, STRIDE),
     ({"positions": 0, "B": 1}, NULL), ({"positions": 0, "B": 1, "q_indptr": 0x6000}, NULL),
     ({"positions": 0, "B": 1, "seq_lens": 0x6000}, NULL), ({"T": 2 ** 31 - 1, "q.H": 2 ** 20}, SHAPE),
+    ({"T": 2 ** 25 + 1, "q.H": 16}, SHAPE),
 ]
 
 
@@ -262,6 +263,7 @@ APPEND_BAD = [
     ({**MX, "cache_rope": 0xa008}, STRIDE), ({**INDEX, "index_cache": 0}, NULL), ({**INDEX, "index_stride_row": 120}, STRIDE),
     ({**INDEX, "index_stride_row": 132}, STRIDE), ({**INDEX, "index_stride_t": -8}, STRIDE), ({**INDEX, "index_stride_t": 4}, STRIDE),
     ({**INDEX, "index_k": 0x7008}, STRIDE), ({**INDEX, "index_cache": 0x8008}, STRIDE),
+    (dict(T=2 ** 26), SHAPE), ({**INDEX, "T": 2 ** 26 - 2 ** 20}, SHAPE),
     ({**INDEX, "index_norm": 2, "index_weight": 0x14}, STRIDE), ({**INDEX, "index_norm": 2, "index_bias": 0x14}, STRIDE),
 ]
 
@@ -290,7 +292,8 @@ CHUNK_BAD = [
     (dict(kv_format=abi.KV_BF16_D512), FORMAT), (dict(kv_format=abi.KV_MXFP8), FORMAT), (dict(kv_format=-1), FORMAT),
     (dict(T=-1), SHAPE), (dict(B=-1), SHAPE), (dict(H=0), SHAPE), (dict(max_kv_len=-1), SHAPE), (dict(max_kv_len=2 ** 31 - 1), SHAPE),
     (dict(kv_total_rows=-1), SHAPE), (dict(kv_total_rows=2 ** 31), SHAPE), (dict(num_splits=-1), SPLITS), (dict(num_splits=65), SPLITS),
-    (dict(T=2 ** 27), SHAPE), (dict(B=2 ** 24), SHAPE), (dict(kv_stride_row=568), STRIDE), (dict(kv_stride_row=580), STRIDE),
+    (dict(T=2 ** 27), SHAPE), (dict(B=2 ** 24), SHAPE), (dict(T=2 ** 25, num_splits=1), SHAPE), (dict(T=2 ** 25), SHAPE),
+    (dict(T=2 ** 22, num_splits=2), SHAPE), (dict(kv_stride_row=568), STRIDE), (dict(kv_stride_row=580), STRIDE),
     (dict(kv_stride_row=2 ** 31), STRIDE), (dict(kv_format=abi.KV_FP8_656, kv_stride_row=664), STRIDE), (dict(block_size=0), SHAPE),
     (dict(table_blocks=-1), SHAPE), (dict(block_size=2 ** 20, table_blocks=2 ** 12), SHAPE), (dict(block_table_stride=-1), STRIDE),
     (dict(block_table=0, kv_batch_stride=-1), STRIDE), (dict(sm_scale=0.0), UNSUPPORTED), (dict(sm_scale=-1.0), UNSUPPORTED),
@@ -340,7 +343,7 @@ def test_chunk_workspace(lib):
 @pytest.mark.parametrize("fmt", [abi.KV_BF16, abi.KV_FP8_656])
 @pytest.mark.parametrize("T,B,H,longest", [(1, 1, 1, 0), (1, 1, 128, 1), (1, 1, 128, 33), (1, 1, 128, 100000), (64, 64, 16, 9000),
                                            (65, 65, 16, 9000), (4096, 2, 128, 4096), (2 ** 20, 1, 16, 2 ** 20),
-                                           (1, 1, 1, 2147481599), (2 ** 24, 1, 127, 64), (0, 0, 1, 0)])
+                                           (1, 1, 1, 2147481599), (2 ** 22, 1, 127, 64), (0, 0, 1, 0)])
 def test_chunk_automatic_splits(lib, fmt, T, B, H, longest):
     """From 1 to 64, no more than there are tiles of 32 positions (twice the planned ones, where the device
     deals them), with a workspace that goes by them; an unsplit call needs none."""
@@ -365,6 +368,22 @@ def test_host_tensors_are_refused():
         dsa.qk_norm_rope(q, torch.zeros(9, 64), torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="q_indptr must be a device tensor"):
         dsa.kv_append(q[:, 0], kv, indptr, lens, torch.zeros(9, 64), block_table=table)
+
+
+def test_rows_of_caches():
+    """(rows, stride; 0 = dense) of a cache; rows that lie on one another or unevenly are refused, not taken
+    for dense ones (whose memory would end past the tensor's)."""
+    t = torch.zeros(6, 4, 576)
+    assert dsa._rows(t, 576, "cache") == (24, 0)
+    assert dsa._rows(torch.zeros(6, 4, 640)[..., :576], 576, "cache") == (24, 640)
+    assert dsa._rows(torch.zeros(6, 2, 1, 576)[:, 0], 576, "cache") == (6, 1152)
+    assert dsa._rows(torch.zeros(1, 576).expand(1, 576), 576, "cache") == (1, 0)
+    for bad in (torch.zeros(1, 576).expand(100, 576), torch.zeros(1, 1, 576).expand(100, 1, 576),
+                torch.zeros(1, 4, 576).expand(6, 4, 576), torch.zeros(6, 1, 576).expand(6, 4, 576),
+                t[:, :3], t.transpose(0, 1), torch.zeros(6 * 576).as_strided((6, 576), (64, 1)),
+                torch.zeros(576, 6).t()):
+        with pytest.raises(ValueError, match="cache must"):
+            dsa._rows(bad, 576, "cache")
 
 
 def test_shapes_are_refused_before_the_device():
