@@ -810,7 +810,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         o_fence(o);
         if (again) break;
         // The reference served if the sum lies where fp32 and the 16-bit P hold it.  With the first
-        // tile's maximum it is at least 1; it grows past 2^100 only where later scores do.
+        // tile's maximum it is at least 1; it grows past 2^40 only where later scores do, and the products with V stay finite below.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
         const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
         const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
@@ -818,7 +818,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         if (wave == 0) s_misc[1] = 0;
         __syncthreads();
         const bool held = FP8 ? top_p >= 0.5f && top_p < 0x1p15f : l > 0x1p-40f;
-        if (have && !(held && l < 0x1p100f)) s_misc[1] = 1;
+        if (have && !(held && l < 0x1p40f)) s_misc[1] = 1;
         __syncthreads();
         if (__builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
         again = true;
@@ -1360,7 +1360,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         t = fmaxf(s_top[0][my], s_top[1][my]);
         any = t >= 0.0f;
         const bool held = FP8 ? t >= 0.5f && t < 0x1p15f : l > 0x1p-40f;
-        if (!again && any && !(held && l < 0x1p100f)) s_misc[1] = 1;
+        if (!again && any && !(held && l < 0x1p40f)) s_misc[1] = 1;
         if (FP8 && range_bad) s_misc[2] = 1;
         l_lane = l;
         __syncthreads();

@@ -114,3 +114,26 @@ def test_lengths_that_grow_under_a_graph(dev):
         assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1]), now
         c.lens = now
         check_chunk(c, out, lse, attend64(c, q, kv, True), True, str(now))
+
+
+@pytest.mark.parametrize("tokens", [2, 3000], ids=["few", "many"])
+@pytest.mark.parametrize("ns", [1, 2])
+def test_large_values_behind_a_low_first_tile(dev, tokens, ns):
+    """Scores that rise by 55 (2^80) after the first tile, values of 2^60: the answer is of 2^60, and a sum
+    kept against the first tile's maximum would pass the range of fp32."""
+    g = gen(34, dev)
+    c = Chunk(g, [tokens], [tokens + 200], 64)
+    H = 16
+    q = torch.zeros((c.T, H, 576), dtype=torch.bfloat16, device=dev)
+    q[..., 512:] = 8.0
+    kv = bf16(g, c.rows, 576, scale=2.0 ** 60)
+    kv[:, 512:] = 0.0
+    late = torch.tensor([c.row(0, j) for j in range(100, c.lens[0])], device=dev)
+    kv[late, 512:] = 1.5
+    out, lse = run(c, q, kv, num_splits=ns)
+    assert bool(torch.isfinite(out).all())
+    o, l, A, E, N = attend64(c, q, kv, True)
+    # (fp32 sums of values of both signs: 2^-24 a term of sum p |v|, which attends all of them alike)
+    rel = 2.0 ** -8 + 2.0 ** -17 + E[..., None]
+    assert bool(((out.double() - o).abs() <= rel * A + 2.0 ** -8 * o.abs()).all())
+    assert bool(((lse.double() - l).abs() <= E + 2.0 ** -20 * (1 + l.abs())).all())
