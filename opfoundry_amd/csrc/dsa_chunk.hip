@@ -322,14 +322,45 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // Q: lane (hi, r32) holds 8 dims of row r32 in qf[ks], the k-step's half `hi`: dims 16 ks + 8 hi .. +7; of
     // 656-byte rows, whose codes come 16 to a read, dims 32 j + 16 hi .. +15 in qf[2 j] and qf[2 j + 1] (the order
     // of the dims within a pair of k-steps is free as long as K has the same)
+    // They come by way of the tile buffers, 12 k-steps at a time and two such parts in flight: a load of a wave
+    // takes 1 KB of one row after the other, where fragments read from memory touch 64 places (7 us a workgroup).
+    // In LDS row r of a part is at 384 r, its 16-byte piece c at c ^ (r >> 1) % 8.
     u32x4 qf[KS];
     {
-        const __bf16* qp = p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh;
+        constexpr int PART = 12, LINE = 32 * PART, BYTES = 32 * LINE;
+        static_assert(NWAVE * 2 * BYTES <= sizeof(s_tile) && KS == 3 * PART);
+        const uint64_t mine = (uint64_t)(p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh);
+        const lds_ptr qb = T0 + wave * 2 * BYTES;
+        uint64_t src[PART];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d = FP8 && ks < KS_NOPE ? 32 * (ks >> 1) + 16 * hi + 8 * (ks & 1) : 16 * ks + 8 * hi;
-            qf[ks] = *reinterpret_cast<const u32x4*>(qp + d);
+        for (int k = 0; k < PART; ++k) {
+            const int at = 64 * (k % 3) + lane, r8 = at / 24, r = 8 * (k / 3) + r8;        // piece 64 k + lane
+            src[k] = __shfl(mine, r, 64) + 16 * ((at - 24 * r8) ^ ((r >> 1) & 7));
         }
+        auto request = [&](int part) {
+#pragma unroll
+            for (int k = 0; k < PART; ++k)
+                lds_dma16((const void*)(src[k] + part * LINE), qb + (part & 1) * BYTES + 1024 * k);
+        };
+        auto take = [&](int part) {
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < PART; ++j) {
+                const int ks = PART * part + j;
+                const int c = FP8 && ks < KS_NOPE ? 4 * (j >> 1) + 2 * hi + (j & 1) : 2 * j + hi;
+                qf[ks] = lds_ld<u32x4>(qb + (part & 1) * BYTES + r32 * LINE + 16 * (c ^ ((r32 >> 1) & 7)));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        };
+        request(0);
+        request(1);
+        wait_vm<PART>();
+        take(0);
+        request(2);
+        wait_vm<PART>();
+        take(1);
+        wait_vm<0>();
+        take(2);
     }
 
     // ---- positions [c0, c0 + SPAN) below k1 -> cache rows ----
@@ -893,18 +924,24 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 }
             }
             __syncthreads();
+            // the wave's eight rows, read together
+            u32x4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = lds_ld<u32x4>(stg + (8 * wv + k) * OUT_STRIDE + 16 * ln);
+            const int r0 = 32 * h + 8 * wv;
+            int t = (blk.r0 + r0) / H, hh = (blk.r0 + r0) - t * H;
+            t += blk.first;
+#pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const int r = 32 * h + 8 * wv + k;
-                if (r >= blk.rows) break;
-                const int t = blk.first + (blk.r0 + r) / H, hh = (blk.r0 + r) % H;
-                const u32x4 v = lds_ld<u32x4>(stg + (8 * wv + k) * OUT_STRIDE + 16 * ln);
+                if (r0 + k >= blk.rows) break;
                 __bf16* const dst = out + t * o_st + hh * o_sh + 8 * ln;
                 if (o16) {
-                    *reinterpret_cast<u32x4*>(dst) = v;
+                    *reinterpret_cast<u32x4*>(dst) = v[k];
                 } else {
-                    reinterpret_cast<u32x2*>(dst)[0] = u32x2{v[0], v[1]};
-                    reinterpret_cast<u32x2*>(dst)[1] = u32x2{v[2], v[3]};
+                    reinterpret_cast<u32x2*>(dst)[0] = u32x2{v[k][0], v[k][1]};
+                    reinterpret_cast<u32x2*>(dst)[1] = u32x2{v[k][2], v[k][3]};
                 }
+                if (++hh == H) hh = 0, ++t;
             }
         }
     } else {
