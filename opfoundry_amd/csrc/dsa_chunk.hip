@@ -75,13 +75,15 @@ __device__ __forceinline__ int64_t limit_of(const ChunkParams& p, int32_t b, int
 // Iteration i computes QK^T of tile i + 1, then PV of tile i with the exponentials of
 // tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 403 of a
 // CU's 512 KB of registers, which is why a workgroup is 128 rows and fills a CU.
-// Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 2.05 ms, 1.21 PFLOP/s, 89 % of what
+// Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 2.02 ms, 1.23 PFLOP/s, 90 % of what
 // a product of two 16384 x 16384 matrices reaches here; 1.79 us a tile and workgroup, matrix units busy
 // 54 % of the cycles at the 1.8 to 2.2 GHz that the card holds under them (reading the first operands of
 // PV ahead, in the last steps of the scores, changes nothing).  656-byte rows (two prompts of 1915 and
-// 1782 tokens): 1.30 ms, 733 TFLOP/s, 2.44 us a tile: every wave converts the whole tile's codes for its
+// 1782 tokens): 1.29 ms, 740 TFLOP/s, 2.44 us a tile: every wave converts the whole tile's codes for its
 // scores (8 vector instructions to a matrix instruction, matrix units busy 30 %).  A shared tile of
-// converted codes has no room beside V's two and the three raw ones.
+// converted codes has no room beside V's two and the three raw ones.  A workgroup's Q and O pass through
+// memory once, 8 us each and 16 before and after its tiles together; the next workgroup's Q read ahead
+// from within the loop gave that time back there (the loads are waited for in order).
 // ---------------------------------------------------------------------------
 constexpr int BLOCK = 128;                   // rows of a workgroup
 constexpr int SPAN = 2048;                   // positions resolved to cache rows at a time
@@ -323,8 +325,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // 656-byte rows, whose codes come 16 to a read, dims 32 j + 16 hi .. +15 in qf[2 j] and qf[2 j + 1] (the order
     // of the dims within a pair of k-steps is free as long as K has the same)
     // They come by way of the tile buffers, 12 k-steps at a time and two such parts in flight: a load of a wave
-    // takes 1 KB of one row after the other, where fragments read from memory touch 64 places (7 us a workgroup).
-    // In LDS row r of a part is at 384 r, its 16-byte piece c at c ^ (r >> 1) % 8.
+    // takes 1 KB of one row after the other, where fragments read from memory touch 64 places (1024 tokens of 128
+    // heads over 8192 bf16 rows: 2019 us, 2045 by fragments).  In LDS row r of a part is at 384 r, its 16-byte
+    // piece c at c ^ (r >> 1) % 8.
     u32x4 qf[KS];
     {
         constexpr int PART = 12, LINE = 32 * PART, BYTES = 32 * LINE;
@@ -841,7 +844,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         o_fence(o);
         if (again) break;
         // The reference served if the sum lies where fp32 and the 16-bit P hold it.  With the first
-        // tile's maximum it is at least 1; it grows past 2^40 only where later scores do, and the products with V stay finite below.
+        // tile's maximum it is at least 1; it grows past 2^40 only where later scores do, and below that the
+        // products with V stay finite.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
         const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
         const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
