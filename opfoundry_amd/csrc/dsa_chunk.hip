@@ -75,15 +75,14 @@ __device__ __forceinline__ int64_t limit_of(const ChunkParams& p, int32_t b, int
 // Iteration i computes QK^T of tile i + 1, then PV of tile i with the exponentials of
 // tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 403 of a
 // CU's 512 KB of registers, which is why a workgroup is 128 rows and fills a CU.
-// Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 2.02 ms, 1.23 PFLOP/s, 90 % of what
-// a product of two 16384 x 16384 matrices reaches here; 1.79 us a tile and workgroup, matrix units busy
-// 54 % of the cycles at the 1.8 to 2.2 GHz that the card holds under them (reading the first operands of
-// PV ahead, in the last steps of the scores, changes nothing).  656-byte rows (two prompts of 1915 and
-// 1782 tokens): 1.29 ms, 740 TFLOP/s, 2.44 us a tile: every wave converts the whole tile's codes for its
+// Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 1.98 ms, 1.25 PFLOP/s, 92 % of what
+// a product of two 16384 x 16384 matrices reaches here (2.06 ms in sessions where the card holds a lower
+// clock); matrix units busy 54 % of the cycles at 1.8 to 2.2 GHz.  656-byte rows (two prompts of 1915 and
+// 1782 tokens): 1.27 ms, 750 TFLOP/s, 2.4 us a tile: every wave converts the whole tile's codes for its
 // scores (8 vector instructions to a matrix instruction, matrix units busy 30 %).  A shared tile of
 // converted codes has no room beside V's two and the three raw ones.  A workgroup's Q and O pass through
-// memory once, 8 us each and 16 before and after its tiles together; the next workgroup's Q read ahead
-// from within the loop gave that time back there (the loads are waited for in order).
+// memory once, 8 us each; the next workgroup's Q read ahead from within the loop, whose loads are waited
+// for in order, cost more there than it saved (1296 -> 1367 us).
 // ---------------------------------------------------------------------------
 constexpr int BLOCK = 128;                   // rows of a workgroup
 constexpr int SPAN = 2048;                   // positions resolved to cache rows at a time
@@ -206,7 +205,7 @@ __device__ __forceinline__ int32_t parts(int32_t a, int32_t b) {
 // leave CUs idle while others hold three.  16 sequences of 7130 to 19272 bf16 rows, 16 heads: 66 us, of
 // 506 workgroups (77 in 16 splits by the bound of the lengths, 366 of them with work); 66 too where that
 // bound is four times as much (173).  7 sequences of 1994 to 4772 rows and 28 to 258 tokens of 40 heads:
-// 378 us (402 in 2).  Finding it out takes 1.5 us: one token of 128 heads over 1483 656-byte rows 19.1
+// 374 us (402 in 2).  Finding it out takes 1.5 us: one token of 128 heads over 1483 656-byte rows 19.1
 // and, in 20 splits by the caller's count, 17.3.  Of 50 ragged calls it was 4 % above the best of 13
 // counts on average (23 % below to 17 % above).
 struct Work {
@@ -325,9 +324,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // 656-byte rows, whose codes come 16 to a read, dims 32 j + 16 hi .. +15 in qf[2 j] and qf[2 j + 1] (the order
     // of the dims within a pair of k-steps is free as long as K has the same)
     // They come by way of the tile buffers, 12 k-steps at a time and two such parts in flight: a load of a wave
-    // takes 1 KB of one row after the other, where fragments read from memory touch 64 places (1024 tokens of 128
-    // heads over 8192 bf16 rows: 2019 us, 2045 by fragments).  In LDS row r of a part is at 384 r, its 16-byte
-    // piece c at c ^ (r >> 1) % 8.
+    // takes 1 KB of one row after the other, where fragments read from memory touch 64 places (with the epilogue's
+    // rows stored together 2002 -> 1999 us for 1024 tokens over 8192 bf16 rows, 1302 -> 1292 for the two prompts).
+    // In LDS row r of a part is at 384 r, its 16-byte piece c at c ^ (r >> 1) % 8.
     u32x4 qf[KS];
     {
         constexpr int PART = 12, LINE = 32 * PART, BYTES = 32 * LINE;
@@ -580,7 +579,29 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     float p_top = 0.0f;          // 656-byte rows: the largest P (fp16 holds up to 2^16)
     bool first_tile = true, any = false;
 
-    auto qk = [&](lds_cptr kt) -> f32x16 {
+    // PV's first operands of a tile (bf16 rows): read in the last steps of the scores before it (1024 tokens of
+    // 128 heads over 8192 rows 2000 -> 1978 us; 656-byte rows, whose scores leave no idle reads: 1294 -> 1307)
+    struct First {
+        u32x4 p[NWAVE], v;
+    };
+    // V^T block m of the wave's dims, positions 16 u .. +15 (transposed reads of rows 4 hi .. +3 and 8 further)
+    auto v_block = [&](lds_cptr vt, int ln, int u, int m) -> u32x4 {
+        const int lhi = ln >> 5, g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
+        const int vx = 2 * (g16 & 1) + (pp >> 1);
+        const lds_cptr v_a = vt + (4 * lhi + rr) * NOPE_STRIDE + 16 * (vx ^ lhi) + 8 * (pp & 1) + 256 * wave;
+        const lds_cptr v_b = vt + (4 * lhi + rr + 8) * NOPE_STRIDE + 16 * (vx ^ (lhi + 2)) + 8 * (pp & 1) + 256 * wave;
+        const s16x4 va = lds_read_tr16(v_a + 16 * u * NOPE_STRIDE + 64 * m);
+        const s16x4 vb = lds_read_tr16(v_b + 16 * u * NOPE_STRIDE + 64 * m);
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto p_block = [&](lds_cptr px, int ln, int u, int h) -> u32x4 { return lds_ld<u32x4>(px + ((u * NWAVE + h) * 64 + ln) * 16); };
+    auto read_first = [&](First& f, int i, lds_cptr vt, lds_cptr px) {
+        if (i < NWAVE) f.p[i] = p_block(px, lane, 0, i);
+        else f.v = v_block(vt, lane, 0, 0);
+    };
+    auto none = [](int) {};
+    // (last(i), i = 0 .. 4, is called in the last five steps)
+    auto qk = [&](lds_cptr kt, auto&& last) -> f32x16 {
         const int ln = lane, lhi = ln >> 5, lr = ln & 31;
         const lds_cptr k_even = kt + lr * NOPE_STRIDE + 16 * (lhi ^ nope_sw(lr));
         const lds_cptr k_odd = kt + lr * NOPE_STRIDE + 16 * ((2 + lhi) ^ nope_sw(lr));
@@ -599,6 +620,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             __builtin_amdgcn_sched_barrier(0);
             acc = mfma_bf16(kb[ks % AHEAD], qf[ks], acc);
             if (ks + AHEAD < KS) kb[ks % AHEAD] = lds_ld<u32x4>(k_at(ks + AHEAD));
+            if (ks >= KS - 5) last(ks - (KS - 5));
         }
         __builtin_amdgcn_sched_barrier(0);
         return acc;
@@ -708,33 +730,32 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         p_half(e, 1, px);
     };
     // (656-byte rows, with_exp: the next tile but one, raw at draw, goes to V's own buffer, piece by piece)
-    auto pv = [&](lds_ptr vt, lds_cptr px, const f32x16& sn, float* en, auto with_exp, lds_cptr draw, int dpar) {
-        const int ln = FP8 ? opaque(lane) : lane, lhi = ln >> 5;
-        const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
-        const int vx = 2 * (g16 & 1) + (pp >> 1);
-        const lds_cptr v_a = vt + (4 * lhi + rr) * NOPE_STRIDE + 16 * (vx ^ lhi) + 8 * (pp & 1) + 256 * wave;
-        const lds_cptr v_b = vt + (4 * lhi + rr + 8) * NOPE_STRIDE + 16 * (vx ^ (lhi + 2)) + 8 * (pp & 1) + 256 * wave;
-        auto v_frag = [&](int u, int m) -> u32x4 {
-            const s16x4 va = lds_read_tr16(v_a + 16 * u * NOPE_STRIDE + 64 * m);
-            const s16x4 vb = lds_read_tr16(v_b + 16 * u * NOPE_STRIDE + 64 * m);
-            return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
+    auto pv = [&](lds_ptr vt, lds_cptr px, First& f, const f32x16& sn, float* en, auto with_exp, lds_cptr draw, int dpar) {
+        const int ln = FP8 ? opaque(lane) : lane;
+        u32x4 v_cur = {};
+        if constexpr (!FP8) v_cur = f.v;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            u32x4 pb[NWAVE];
+            if constexpr (FP8) {
 #pragma unroll
-            for (int h = 0; h < NWAVE; ++h) pb[h] = lds_ld<u32x4>(px + ((u * NWAVE + h) * 64 + ln) * 16);
-            u32x4 v_cur = v_frag(u, 0);
+                for (int h = 0; h < NWAVE; ++h) f.p[h] = p_block(px, ln, u, h);
+                v_cur = v_block(vt, ln, u, 0);
+            }
             Scale ds;
             if constexpr (FP8 && decltype(with_exp)::value) ds = deq_scale(draw, dpar, u);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 __builtin_amdgcn_sched_barrier(0);
-                const u32x4 v_nxt = m + 1 < 4 ? v_frag(u, m + 1) : v_cur;
+                u32x4 v_nxt = v_cur;
+                if (m + 1 < 4) v_nxt = v_block(vt, ln, u, m + 1);
+                else if (!FP8 && u == 0) v_nxt = v_block(vt, ln, 1, 0);
                 u32x2 codes;
                 if constexpr (FP8 && decltype(with_exp)::value) codes = deq_load(draw, 4 * u + m);
 #pragma unroll
-                for (int h = 0; h < NWAVE; ++h) mfma_o<FP8>(o[4 * m + h], v_cur, pb[h]);
+                for (int h = 0; h < NWAVE; ++h) {
+                    mfma_o<FP8>(o[4 * m + h], v_cur, f.p[h]);
+                    if (!FP8 && u == 0 && m == 3) f.p[h] = p_block(px, ln, 1, h);
+                }
                 if constexpr (decltype(with_exp)::value) {
                     const int r0 = 8 * u + 2 * m;
                     en[r0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0], c_s, -m_ref));
@@ -769,7 +790,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             if (ntiles > 1) landed(std::integral_constant<int, LPW>{}); else landed(std::integral_constant<int, 0>{});
             if (masked(0, c0)) scan(0, 0);
             tile_barrier();
-            f32x16 s0 = qk(slot_of(0));
+            f32x16 s0 = qk(slot_of(0), none);
             mask(s0, 0, c0);
             p_first(s0, PX);
             int cur = 0;
@@ -783,11 +804,12 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 __builtin_amdgcn_sched_barrier(0);
                 if (i + 2 < ntiles) issue(next, nxt == 2 ? 0 : nxt + 1);
                 __builtin_amdgcn_sched_barrier(0);
-                f32x16 sn = qk(slot_of(nxt));
+                First f;
+                f32x16 sn = qk(slot_of(nxt), [&](int k) { read_first(f, k, slot_of(cur), PX + (i & 1) * P_BYTES); });
                 if (i + 3 < ntiles) next = load_rows(i + 3);
                 mask(sn, i + 1, c0);
                 float en[16];
-                pv(slot_of(cur), PX + (i & 1) * P_BYTES, sn, en, std::true_type{}, T0, 0);
+                pv(slot_of(cur), PX + (i & 1) * P_BYTES, f, sn, en, std::true_type{}, T0, 0);
                 const lds_ptr px = PX + ((i + 1) & 1) * P_BYTES;
                 p_half(en, 0, px);
                 p_half(en, 1, px);
@@ -795,7 +817,10 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             }
             tile_barrier();
             float en[16];
-            pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{}, T0, 0);
+            First f;
+#pragma unroll
+            for (int k = 0; k < 5; ++k) read_first(f, k, slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES);
+            pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f, f32x16{}, en, std::false_type{}, T0, 0);
             } else {
                 // Iteration j: scores of tile j from raw slot j % 3; PV of tile j - 1 from V buffer (j - 1) % 2,
                 // with the exponentials of tile j and the conversion of tile j + 1 into that buffer.
@@ -830,7 +855,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     if (j + 3 < ntiles) next = load_rows(j + 3);
                     mask(sn, j, c0);
                     float en[16];
-                    pv(slot_of((j - 1) & 1), PX + ((j - 1) & 1) * P_BYTES, sn, en, std::true_type{}, raw_of((j + 1) % 3),
+                    First f;
+                    pv(slot_of((j - 1) & 1), PX + ((j - 1) & 1) * P_BYTES, f, sn, en, std::true_type{}, raw_of((j + 1) % 3),
                        (j + 1) & 1);
                     const lds_ptr px = PX + (j & 1) * P_BYTES;
                     p_half(en, 0, px);
@@ -838,7 +864,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 }
                 tile_barrier();
                 float en[16];
-                pv(slot_of((ntiles - 1) & 1), PX + ((ntiles - 1) & 1) * P_BYTES, f32x16{}, en, std::false_type{}, T0, 0);
+                First f;
+                pv(slot_of((ntiles - 1) & 1), PX + ((ntiles - 1) & 1) * P_BYTES, f, f32x16{}, en, std::false_type{}, T0, 0);
             }
         }
         o_fence(o);
@@ -874,7 +901,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 } else {
                     if (masked(i, c0)) scan(i, 0);
                     tile_barrier();
-                    s = qk(slot_of(0));
+                    s = qk(slot_of(0), none);
                 }
                 mask(s, i, c0);
                 top = fmaxf(top, top_of(s));
