@@ -121,8 +121,9 @@ int dsa_qk_norm_rope(const dsa_qk_norm_rope_args* args, void* stream);
  *              other bytes stay as they were), cache_rope = 64 bf16 values
  *            E8M0: per 32 values the least power of two 2^e >= amax / 448, e at
  *            least -126 (e = 0 for 32 zeros), byte e + 127.
- *            A NaN value becomes a NaN code.  Row strides in elements of each
- *            stream (bytes for codes and scales); 0 = dense.
+ *            A NaN value becomes a NaN code in every format, also where its group
+ *            holds nothing else (scale 0, or E8M0 127).  Row strides in elements of
+ *            each stream (bytes for codes and scales); 0 = dense.
  * index_k  : bf16 [T, 128]; NULL: no index keys.  index_norm over all 128
  *            values, then the first 64 rotated (index_rope), written as bf16 to
  *            the token's row of index_cache (the same row number).

@@ -504,9 +504,10 @@ int dsa_mla_prefill_v4_fp8(const dsa_mla_prefill_v4_fp8_args* args, void* worksp
  * src_stride elements) into 656-byte DSA_KV_FP8_656 rows.  Destination row
  * of source row r is dst_rows[r] (int64 physical cache row) or r when
  * dst_rows is NULL; negative destinations are skipped.  scale_g =
- * amax_g / 448 (IEEE division), code = e4m3fn(x / scale_g) with round to
- * nearest even and saturation to +-448; an all-zero group stores scale 0 and
- * zero codes.  The reference leaves cache writing to its caller
+ * amax_g / 448 (IEEE division, amax_g over the values that are no NaN), code
+ * = e4m3fn(x / scale_g) with round to nearest even, saturation to +-448 and
+ * NaN for a NaN or infinity; a group without a value above zero stores scale 0,
+ * zero codes and its NaNs' codes.  The reference leaves cache writing to its caller
  * (opus_attn/dsa_v32/README.md:99); the codec follows float_to_fp8_e4m3,
  * opus_attn/dsa_v32/common/defs.h:11-38.
  */

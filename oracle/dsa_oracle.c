@@ -123,8 +123,9 @@ void oracle_bf16_round_n(const float* x, uint16_t* out, int64_t n) {
 
 /*
  * 656-byte row writer: src is 576 fp32 values (the bf16 latent widened).
- * scale_g = amax_g / 448 (IEEE division), code = e4m3(x / scale_g); an
- * all-zero group stores scale 0 and zero codes.  RoPE is rounded to bf16.
+ * scale_g = amax_g / 448 (IEEE division, amax_g over the values that are no
+ * NaN), code = e4m3(x / scale_g); a group whose amax is 0 stores scale 0, zero
+ * codes and its NaNs' codes.  RoPE is rounded to bf16.
  */
 void oracle_quantize_row_656(const float* src, uint8_t* dst) {
     for (int g = 0; g < 4; ++g) {
@@ -135,8 +136,10 @@ void oracle_quantize_row_656(const float* src, uint8_t* dst) {
         }
         const float scale = amax / 448.0f;
         memcpy(dst + 512 + 4 * g, &scale, 4);
-        for (int i = 0; i < 128; ++i)
-            dst[128 * g + i] = (scale > 0.0f) ? oracle_fp8_e4m3_encode(src[128 * g + i] / scale) : 0;
+        for (int i = 0; i < 128; ++i) {
+            const float x = src[128 * g + i];
+            dst[128 * g + i] = scale > 0.0f ? oracle_fp8_e4m3_encode(x / scale) : isnan(x) ? oracle_fp8_e4m3_encode(x) : 0;
+        }
     }
     for (int i = 0; i < D_ROPE; ++i) {
         const uint16_t h = oracle_f32_to_bf16(src[D_NOPE + i]);
