@@ -192,7 +192,9 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  *            64 sequences the size of a split by their lengths, on the device
  *            (dsa_mla_chunk_num_splits: the most that one sequence has).
  * Scores and sums are fp32.  Probabilities are rounded to 16 bits for the
- * product with V (bf16; fp16 for DSA_KV_FP8_656).  656-byte rows: scores use
+ * product with V (bf16; fp16 for DSA_KV_FP8_656, where those below fp16's normal
+ * range are off by at most 2^-10 of the largest |V| together, up to 2^28 positions
+ * a split).  656-byte rows: scores use
  * their exact values; V is rounded to fp16 (its scale's mantissa first), and
  * every scale must lie in [0, 128), a token that attends a row with another
  * scale getting NaN, as in dsa_mla.h.

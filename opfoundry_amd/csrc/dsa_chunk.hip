@@ -161,6 +161,13 @@ __device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k
     return (int32_t)max((int64_t)0, p.causal ? min(own, (int64_t)k.len) : (int64_t)k.len);
 }
 
+// 656-byte rows: P in fp16 loses up to 2^-25 where it is below 2^-14, which n positions could add up to n 2^-25
+// of a row's sum.  Past 2^14 positions the first tile's maximum stands for P = 2^lift instead of 1, so that the
+// loss stays below 2^-11 of it; P may then grow by 15 - lift powers of two before the row starts again.
+__device__ __forceinline__ int lift_of(int32_t n) {
+    return n <= 1 << 14 ? 0 : min(14, 32 - 14 - __builtin_clz((unsigned)n - 1));
+}
+
 constexpr float PART_BYTES_US = 5.3e6f;            // at which splits' partials are written and read again
 constexpr float JOIN_SPLIT_US = 0.1f;              // and what the join's wait for one more split costs
 
@@ -721,6 +728,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             // no position of the first tile attended: any reference, checked at the end
             const float top = top_of(s) * c_s;
             m_ref = top == -INFINITY ? 0.0f : top;
+            if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
             first_tile = false;
         }
         float e[16];
@@ -870,17 +878,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         }
         o_fence(o);
         if (again) break;
-        // The reference served if the sum lies where fp32 and the 16-bit P hold it.  With the first
-        // tile's maximum it is at least 1; it grows past 2^40 only where later scores do, and below that the
-        // products with V stay finite.
+        // The reference served if the sum (bf16 P, which has the range of fp32) or the largest P (fp16) lies where
+        // its type holds it.  With the first tile's maximum the sum is at least 1; it grows past 2^40 only where
+        // later scores do, and below that the products with V stay finite.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
         const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
         const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
         __syncthreads();
         if (wave == 0) s_misc[1] = 0;
         __syncthreads();
-        const bool held = FP8 ? top_p >= 0.5f && top_p < 0x1p15f : l > 0x1p-40f;
-        if (have && !(held && l < 0x1p40f)) s_misc[1] = 1;
+        const bool held = FP8 ? top_p >= __builtin_ldexpf(0.5f, lift_of(k1 - k0)) && top_p < 0x1p15f
+                              : l > 0x1p-40f && l < 0x1p40f;
+        if (have && !held) s_misc[1] = 1;
         __syncthreads();
         if (__builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
         again = true;
@@ -909,6 +918,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             }
         }
         m_ref = top == -INFINITY ? 0.0f : top * c_s;
+        if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
     }
 
     // ---- O / l, LSE ----
@@ -1399,6 +1409,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
                 if (first) {
                     const float top = top_of(s) * c_s;
                     m_ref = top == -INFINITY ? 0.0f : top;
+                    if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
                     first = false;
                 }
                 p_out(s);
@@ -1427,8 +1438,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         __syncthreads();
         t = fmaxf(s_top[0][my], s_top[1][my]);
         any = t >= 0.0f;
-        const bool held = FP8 ? t >= 0.5f && t < 0x1p15f : l > 0x1p-40f;
-        if (!again && any && !(held && l < 0x1p40f)) s_misc[1] = 1;
+        const bool held = FP8 ? t >= __builtin_ldexpf(0.5f, lift_of(k1 - k0)) && t < 0x1p15f : l > 0x1p-40f && l < 0x1p40f;
+        if (!again && any && !held) s_misc[1] = 1;
         if (FP8 && range_bad) s_misc[2] = 1;
         l_lane = l;
         __syncthreads();
@@ -1456,6 +1467,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
             }
         }
         m_ref = top == -INFINITY ? 0.0f : top * c_s;
+        if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
     }
 
     // ---- O / l, LSE: rows' values from the scoring lanes to the lanes that hold O ----
