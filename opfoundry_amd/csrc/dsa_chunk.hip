@@ -161,11 +161,18 @@ __device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k
     return (int32_t)max((int64_t)0, p.causal ? min(own, (int64_t)k.len) : (int64_t)k.len);
 }
 
+// The power of two that P of a row's reference score stands for, of a split of n positions.
 // 656-byte rows: P in fp16 loses up to 2^-25 where it is below 2^-14, which n positions could add up to n 2^-25
-// of a row's sum.  Past 2^14 positions the first tile's maximum stands for P = 2^lift instead of 1, so that the
-// loss stays below 2^-11 of it; P may then grow by 15 - lift powers of two before the row starts again.
-__device__ __forceinline__ int lift_of(int32_t n) {
-    return n <= 1 << 14 ? 0 : min(14, 32 - 14 - __builtin_clz((unsigned)n - 1));
+// of a row's sum.  Past 2^14 positions the first tile's maximum is 2^lift instead of 1, so that the loss stays below
+// 2^-11 of it; P may then grow by 15 - lift powers of two before the row starts again.
+// bf16 rows, whose values and P have the range of fp32: O passes it where a sum of P above 1 meets values near the
+// largest.  With the maximum at 2^-15 most rows' sums stay below 1/2, and O below the largest value; for the others O
+// is looked at, and a row starts again with its exact maximum so low that n of them add up to 1/2 at most.
+template <bool FP8>
+__device__ __forceinline__ int lift_of(int32_t n, bool again) {
+    const int bits = n <= 1 ? 0 : 32 - __builtin_clz((unsigned)n - 1);         // ceil(log2 n)
+    if (FP8) return max(0, min(14, bits - 14));
+    return again ? -1 - bits : -15;
 }
 
 constexpr float PART_BYTES_US = 5.3e6f;            // at which splits' partials are written and read again
@@ -295,7 +302,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     __shared__ __attribute__((aligned(16))) int32_t s_rows[SPAN];     // cache rows of a span's positions
     __shared__ uint32_t s_skip[SPAN / TILE];                          // bit j: position j of the tile has no row
     __shared__ uint32_t s_nan[SPAN / TILE];                           // bit j: its row holds a NaN or infinity
-    __shared__ int32_t s_misc[4];                                     // [0] a row that may be read, [1] restart
+    __shared__ int32_t s_misc[4];                                     // [0] a row that may be read, [1] restart, [2] O may
+                                                                      // have passed fp32, [3] and has
     __shared__ float s_inv[BLOCK];
     const lds_ptr T0 = (lds_ptr)s_tile, PX = (lds_ptr)s_p;
     const LDS_AS int32_t* const rows_l = (const LDS_AS int32_t*)s_rows;
@@ -728,7 +736,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             // no position of the first tile attended: any reference, checked at the end
             const float top = top_of(s) * c_s;
             m_ref = top == -INFINITY ? 0.0f : top;
-            if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
+            m_ref -= (float)lift_of<FP8>(k1 - k0, false);
             first_tile = false;
         }
         float e[16];
@@ -779,7 +787,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int nspans = k1 > k0 ? (k1 - k0 + SPAN - 1) / SPAN : 0;
     // Pass 0; where its reference did not serve (rare): the largest score of every row, and the pass
     // again with that as the reference.
-    for (bool again = false;;) {
+    bool again = false;
+    while (true) {
         // (0 x 0 + 0: cleared where they are, without the registers that zeros to copy would take)
         const u32x4 zero = {0, 0, 0, 0};
 #pragma unroll
@@ -879,19 +888,36 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         o_fence(o);
         if (again) break;
         // The reference served if the sum (bf16 P, which has the range of fp32) or the largest P (fp16) lies where
-        // its type holds it.  With the first tile's maximum the sum is at least 1; it grows past 2^40 only where
-        // later scores do, and below that the products with V stay finite.
+        // its type holds it, and if O, which is at most the sum times the largest value, did not pass fp32.  The sum
+        // is at least the first tile's maximum, 2^lift; it grows past 2^40 times that only where later scores do.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
         const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
         const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
         __syncthreads();
-        if (wave == 0) s_misc[1] = 0;
+        if (wave == 0) s_misc[1] = 0, s_misc[2] = 0, s_misc[3] = 0;
         __syncthreads();
-        const bool held = FP8 ? top_p >= __builtin_ldexpf(0.5f, lift_of(k1 - k0)) && top_p < 0x1p15f
-                              : l > 0x1p-40f && l < 0x1p40f;
+        const int lift = lift_of<FP8>(k1 - k0, false);
+        const bool held = FP8 ? top_p >= __builtin_ldexpf(0.5f, lift) && top_p < 0x1p15f
+                              : l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
         if (have && !held) s_misc[1] = 1;
+        if (!FP8 && have && l >= 0.5f) s_misc[2] = 1;
         __syncthreads();
-        if (__builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
+        bool served = __builtin_amdgcn_readfirstlane(s_misc[1]) == 0;
+        if (!FP8 && __builtin_expect(served && __builtin_amdgcn_readfirstlane(s_misc[2]) != 0, false)) {
+            // (0 times what is not finite is NaN; tile after tile, without copies of all of O)
+            float t = 0.0f;
+#pragma unroll
+            for (int m = 0; m < 16; ++m) {
+                asm volatile("" : "+a"(o[m]), "+v"(t));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t = __builtin_fmaf(o[m][r], 0.0f, t);
+            }
+            asm volatile("" : "+v"(t));
+            if (t != 0.0f) s_misc[3] = 1;
+            __syncthreads();
+            served = __builtin_amdgcn_readfirstlane(s_misc[3]) == 0;
+        }
+        if (served) break;
         again = true;
         float top = -INFINITY;
         for (int c = 0; c < nspans; ++c) {
@@ -918,7 +944,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             }
         }
         m_ref = top == -INFINITY ? 0.0f : top * c_s;
-        if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
+        m_ref -= (float)lift_of<FP8>(k1 - k0, true);
     }
 
     // ---- O / l, LSE ----
@@ -932,7 +958,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const float l = l_lane + __shfl_xor(l_lane, 32, 64);
     const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
     const bool mine = 32 * wv + r_ < blk.rows;
-    const float lse = too_long ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l)) * LN2;
+    const int lift = lift_of<FP8>(k1 - k0, again);
+    const float lse = too_long ? __builtin_nanf("")
+                               : (m_ref + (float)lift + __builtin_amdgcn_logf(__builtin_ldexpf(l, -lift))) * LN2;
     if (hi_ == 0) {
         s_inv[32 * wv + r_] = too_long ? __builtin_nanf("") : (have ? 1.0f / l : 0.0f);
         const int64_t at = (int64_t)blk.first * H + blk.r0 + 32 * wv + r_;      // rows are token-major
@@ -1057,7 +1085,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     __shared__ int32_t s_rows[NLIST];        // RUNS: the first row of every tile; else every position's
     __shared__ float s_top[2][NARROW];
     __shared__ uint32_t s_nan;               // bit j: position j's row holds a NaN or infinity
-    __shared__ int32_t s_misc[3];            // [0] a row that may be read, [1] again, [2] a scale out of range
+    __shared__ int32_t s_misc[4];            // [0] a row that may be read, [1] again, [2] a scale out of range
+                                             // (bf16: O may have passed fp32), [3] it has
     const lds_ptr T0 = (lds_ptr)s_tile, PX = (lds_ptr)s_p;
 
     const int lane = threadIdx.x & 63;
@@ -1373,7 +1402,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + span - 1) / span) : 0;
     auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * span); };
     bool first = true, all_nan = false;
-    for (bool again = false;;) {
+    bool again = false;
+    while (true) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) o[m] = f32x16{};
         l_lane = 0.0f;
@@ -1409,7 +1439,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
                 if (first) {
                     const float top = top_of(s) * c_s;
                     m_ref = top == -INFINITY ? 0.0f : top;
-                    if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
+                    m_ref -= (float)lift_of<FP8>(k1 - k0, false);
                     first = false;
                 }
                 p_out(s);
@@ -1429,7 +1459,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         const uint64_t anys = __builtin_amdgcn_ballot_w64(any);
         any = ((anys >> (lane & 15)) & 0x0001000100010001ull) != 0;
         __syncthreads();
-        if (threadIdx.x == 0) s_misc[1] = 0, s_misc[2] = 0;
+        if (threadIdx.x == 0) s_misc[1] = 0, s_misc[2] = 0, s_misc[3] = 0;
         if (q == 0) s_top[half][my] = any ? l : 0.0f;
         __syncthreads();
         l = s_top[0][my] + s_top[1][my];
@@ -1438,13 +1468,26 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         __syncthreads();
         t = fmaxf(s_top[0][my], s_top[1][my]);
         any = t >= 0.0f;
-        const bool held = FP8 ? t >= __builtin_ldexpf(0.5f, lift_of(k1 - k0)) && t < 0x1p15f : l > 0x1p-40f && l < 0x1p40f;
+        const int lift = lift_of<FP8>(k1 - k0, false);
+        const bool held = FP8 ? t >= __builtin_ldexpf(0.5f, lift) && t < 0x1p15f
+                              : l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
         if (!again && any && !held) s_misc[1] = 1;
-        if (FP8 && range_bad) s_misc[2] = 1;
+        if (FP8 ? range_bad : any && l >= 0.5f) s_misc[2] = 1;
         l_lane = l;
         __syncthreads();
-        all_nan = too_long || s_misc[2] != 0;
-        if (again || __builtin_amdgcn_readfirstlane(s_misc[1]) == 0) break;
+        all_nan = too_long || (FP8 && s_misc[2] != 0);
+        bool served = again || __builtin_amdgcn_readfirstlane(s_misc[1]) == 0;
+        if (!FP8 && !again && __builtin_expect(served && __builtin_amdgcn_readfirstlane(s_misc[2]) != 0, false)) {
+            float z = 0.0f;                    // (as in the tiled kernel)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[m][r], 0.0f, z);
+            if (z != 0.0f) s_misc[3] = 1;
+            __syncthreads();
+            served = __builtin_amdgcn_readfirstlane(s_misc[3]) == 0;
+        }
+        if (served) break;
         again = true;
         p_top = 0.0f;
         float top = -INFINITY;
@@ -1467,11 +1510,13 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
             }
         }
         m_ref = top == -INFINITY ? 0.0f : top * c_s;
-        if constexpr (FP8) m_ref -= (float)lift_of(k1 - k0);
+        m_ref -= (float)lift_of<FP8>(k1 - k0, true);
     }
 
     // ---- O / l, LSE: rows' values from the scoring lanes to the lanes that hold O ----
-    const float lse = all_nan ? __builtin_nanf("") : (m_ref + __builtin_amdgcn_logf(l_lane)) * LN2;
+    const int lift = lift_of<FP8>(k1 - k0, again);
+    const float lse = all_nan ? __builtin_nanf("")
+                              : (m_ref + (float)lift + __builtin_amdgcn_logf(__builtin_ldexpf(l_lane, -lift))) * LN2;
     __syncthreads();
     if (q == 0 && half == 0) {
         s_top[0][my] = all_nan ? __builtin_nanf("") : (any ? 1.0f / l_lane : 0.0f);
@@ -1589,7 +1634,8 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
     const bool any = __builtin_amdgcn_ballot_w64(mine != -FLT_MAX) != 0;
-    const float w = mine == -FLT_MAX ? 0.0f : __builtin_amdgcn_exp2f((mine - top) * LOG2E);
+    // (a weight of 1 is 2^-7 here, so that 64 partials near the largest value stay in fp32 together)
+    const float w = mine == -FLT_MAX ? 0.0f : 0x1p-7f * __builtin_amdgcn_exp2f((mine - top) * LOG2E);
     const float total = wave_sum(w);
     float o[8] = {};
     // eight splits' loads in flight at a time; the last one's again past it.  One of no weight is not added
@@ -1630,7 +1676,7 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
         *reinterpret_cast<uint32_t*>(dst + 2 * threadIdx.x) = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
     }
     if (lane == 0 && share == 0 && p.lse)
-        p.lse[row] = nan != 0.0f ? nan : (any ? top + __builtin_amdgcn_logf(total) * LN2 : INFINITY);
+        p.lse[row] = nan != 0.0f ? nan : (any ? top + __builtin_amdgcn_logf(0x1p7f * total) * LN2 : INFINITY);
 }
 
 // ------------------------------------------------------------------- host
