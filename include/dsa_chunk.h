@@ -56,7 +56,10 @@ typedef enum {
 } dsa_rope;
 
 /* Rows of a stream: bf16 x [T, H, D] and out [T, H, D], last dim dense.  out may
- * be x itself (same pointer and strides); otherwise the two must not overlap.
+ * be x itself (same pointer and strides).  Rows of out that overlap one another, x
+ * otherwise, or the other stream's x or out are refused (DSA_ERR_BAD_STRIDE), and so
+ * are two that lie among one another with different strides: slices of one buffer
+ * need the same stride_t and, with several heads each that take turns, stride_h.
  * weight and bias (fp32 [norm_dim]; either may be NULL) follow the norm; they
  * must be NULL without one.  H == 0: no such stream. */
 typedef struct {
@@ -202,7 +205,8 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  * kv_total_rows and block_size x table_blocks below 2^31, max_kv_len at most
  * DSA_MLA_MAX_LIST; beyond them DSA_ERR_BAD_SHAPE.
  * Alignment: q and kv_cache 16 bytes, out 8; q's strides multiples of 8, out's of
- * 4 and at least 512, cache rows of 16 bytes and below 4 GiB.
+ * 4, cache rows of 16 bytes and below 4 GiB.  Rows of out that overlap one another
+ * are refused (DSA_ERR_BAD_STRIDE); out must not overlap the cache, q, or lse.
  * The split and so the last bits depend on the call's sizes and, with
  * num_splits = 0, on the lengths of all its sequences; one call repeats its bits.
  */

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "../../include/dsa_chunk.h"
+#include "dsa_overlap.h"
 #include "dsa_seq.h"
 
 namespace {
@@ -1787,7 +1788,7 @@ int validate(const dsa_mla_chunk_args* a) {
     if (a->T == 0 || a->B == 0) return DSA_OK;
     if (!a->q || !a->out || !a->q_indptr || !a->seq_lens || (a->kv_total_rows > 0 && !a->kv_cache))
         return DSA_ERR_NULL_POINTER;
-    if ((a->H > 1 && a->o_stride_h < D_VO) || (a->T > 1 && a->o_stride_t < D_VO)) return DSA_ERR_BAD_STRIDE;
+    if (dsa_overlap::within({a->T, a->H, a->o_stride_t, a->o_stride_h, D_VO})) return DSA_ERR_BAD_STRIDE;
     if (a->q_stride_t < 0 || a->q_stride_h < 0 || (a->q_stride_t % 8) || (a->q_stride_h % 8) || a->o_stride_t < 0 ||
         a->o_stride_h < 0 || (a->o_stride_t % 4) || (a->o_stride_h % 4))
         return DSA_ERR_BAD_STRIDE;

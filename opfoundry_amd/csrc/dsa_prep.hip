@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "../../include/dsa_chunk.h"
+#include "dsa_overlap.h"
 #include "dsa_seq.h"
 
 namespace {
@@ -438,12 +439,43 @@ int check_rows(const dsa_norm_rope_rows& s, int T, int D, int rope) {
     return DSA_OK;
 }
 
+// Rows of an output share memory with one another, with the other output's, or with an input's other than
+// their own in place.
+bool outputs_overlap(const dsa_qk_norm_rope_args& a) {
+    using dsa_overlap::Rows;
+    using dsa_overlap::wide;
+    struct Part {
+        Rows rows;
+        int64_t at;            // address, in elements (all are 16-byte aligned)
+        wide end;
+    };
+    auto part = [&](const dsa_norm_rope_rows& s, const void* p, int64_t st, int64_t sh) {
+        const Rows r{a.T, s.H, st, sh, a.D};
+        const int64_t at = (int64_t)((uintptr_t)p >> 1);
+        return Part{r, at, at + dsa_overlap::extent(r)};
+    };
+    auto overlap = [](const Part& x, const Part& o) {
+        return x.at < o.end && o.at < x.end && dsa_overlap::between(x.rows, o.rows, o.at - x.at);
+    };
+    Part x[2], o[2];
+    int n = 0;
+    for (const dsa_norm_rope_rows* s : {&a.q, &a.k}) {
+        if (s->H == 0) continue;
+        x[n] = part(*s, s->x, s->stride_t, s->stride_h);
+        o[n] = part(*s, s->out, s->out_stride_t, s->out_stride_h);
+        if (dsa_overlap::within(o[n].rows) || (s->x != s->out && overlap(x[n], o[n]))) return true;
+        ++n;
+    }
+    return n == 2 && (overlap(x[0], o[1]) || overlap(x[1], o[0]) || overlap(o[0], o[1]));
+}
+
 template <int D>
 int launch_norm_rope(const dsa_qk_norm_rope_args* a, hipStream_t stream) {
     const int qg = (a->q.H + GROUP<D> - 1) / GROUP<D>, kg = (a->k.H + GROUP<D> - 1) / GROUP<D>;
     const int64_t jobs = (int64_t)a->T * (qg + kg);
     if (jobs == 0) return DSA_OK;
     if (jobs > MAX_JOBS) return DSA_ERR_BAD_SHAPE;
+    if (outputs_overlap(*a)) return DSA_ERR_BAD_STRIDE;
     const dim3 grid((unsigned)((jobs + WAVES - 1) / WAVES)), block(64 * WAVES);
     if (a->rope == DSA_ROPE_INTERLEAVED)
         hipLaunchKernelGGL((dsa_qk_norm_rope_kernel<D, DSA_ROPE_INTERLEAVED>), grid, block, 0, stream, *a, qg, qg + kg);
