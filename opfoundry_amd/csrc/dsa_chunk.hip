@@ -21,6 +21,7 @@ constexpr int NWAVE = 4, NTHR = 64 * NWAVE;
 constexpr int TILE = 32;
 constexpr int CUS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
+constexpr float FP16_MAX = 65504.0f;
 constexpr unsigned FP8_SCALE_LIMIT_BITS = 0x43000000u;   // 128.0f
 
 constexpr int NARROW = 32;                   // rows of a workgroup of the kernel for few rows
@@ -165,7 +166,7 @@ __device__ __forceinline__ int32_t limit_in(const ChunkParams& p, const Block& k
 // The power of two that P of a row's reference score stands for, of a split of n positions.
 // 656-byte rows: P in fp16 loses up to 2^-25 where it is below 2^-14, which n positions could add up to n 2^-25
 // of a row's sum.  Past 2^14 positions the first tile's maximum is 2^lift instead of 1, so that the loss stays below
-// 2^-11 of it; P may then grow by 15 - lift powers of two before the row starts again.
+// 2^-11 of it; P may then grow by 16 - lift powers of two before the row starts again.
 // bf16 rows, whose values and P have the range of fp32: O passes it where a sum of P above 1 meets values near the
 // largest.  With the maximum at 2^-15 most rows' sums stay below 1/2, and O below the largest value; for the others O
 // is looked at, and a row starts again with its exact maximum so low that n of them add up to 1/2 at most.
@@ -898,7 +899,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         if (wave == 0) s_misc[1] = 0, s_misc[2] = 0, s_misc[3] = 0;
         __syncthreads();
         const int lift = lift_of<FP8>(k1 - k0, false);
-        const bool held = FP8 ? top_p >= __builtin_ldexpf(0.5f, lift) && top_p < 0x1p15f
+        const bool held = FP8 ? top_p >= __builtin_ldexpf(0.5f, lift) && top_p <= FP16_MAX
                               : l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
         if (have && !held) s_misc[1] = 1;
         if (!FP8 && have && l >= 0.5f) s_misc[2] = 1;
@@ -1470,7 +1471,7 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
         t = fmaxf(s_top[0][my], s_top[1][my]);
         any = t >= 0.0f;
         const int lift = lift_of<FP8>(k1 - k0, false);
-        const bool held = FP8 ? t >= __builtin_ldexpf(0.5f, lift) && t < 0x1p15f
+        const bool held = FP8 ? t >= __builtin_ldexpf(0.5f, lift) && t <= FP16_MAX
                               : l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
         if (!again && any && !held) s_misc[1] = 1;
         if (FP8 ? range_bad : any && l >= 0.5f) s_misc[2] = 1;

@@ -81,6 +81,8 @@ LONG = [
     (1 << 11, 1, 16.0),
     ((1 << 8) + 1, 200, 10.0),          # just past 2^14 positions
     (1 << 8, 1, 17.0),                  # and at them
+    (1 << 8, 200, 10.8),                # P grows to 2^15.6, which fp16 holds
+    (1 << 8, 200, 11.2),                # ... and to 2^16.2, which it does not
 ]
 
 
