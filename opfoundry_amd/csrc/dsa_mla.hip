@@ -3837,9 +3837,15 @@ dsa_kv_quantize_kernel(const __bf16* __restrict__ src, int64_t src_stride, int64
     unsigned w0 = 0, w1 = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // (scale 0: zeros, and the NaNs, which the largest value does not see)
-        const unsigned c = scale > 0.0f ? e4m3_encode(v[i] / scale) : v[i] != v[i] ? e4m3_encode(v[i]) : 0u;
+        const unsigned c = scale > 0.0f ? e4m3_encode(v[i] / scale) : 0u;
         if (i < 4) w0 |= c << (8 * i); else w1 |= c << (8 * (i - 4));
+    }
+    if (!(scale > 0.0f)) {                     // zeros, and the NaNs, which the largest value does not see
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned c = v[i] != v[i] ? 0x7Fu | ((__float_as_uint(v[i]) >> 24) & 0x80u) : 0u;
+            if (i < 4) w0 |= c << (8 * i); else w1 |= c << (8 * (i - 4));
+        }
     }
     unsigned char* d = dst + dr * DSA_MLA_FP8_ROW_BYTES;
     *reinterpret_cast<u32x2*>(d + 8 * lane) = u32x2{w0, w1};

@@ -353,10 +353,13 @@ __device__ __forceinline__ void append_latent(const AppendParams& p, int t) {
     } else if (fmt == DSA_KV_FP8_656) {
         const float amax = all16(amax8(v), max_abs);
         const float scale = amax / 448.0f;
-        // (scale 0: zeros, and the NaNs, which the largest value does not see)
         V8 c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c.v[i] = scale > 0.0f ? v.v[i] / scale : v.v[i] != v.v[i] ? v.v[i] : 0.0f;
+        for (int i = 0; i < 8; ++i) c.v[i] = v.v[i] / scale;
+        if (!(scale > 0.0f)) {                 // zeros, and the NaNs, which the largest value does not see
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c.v[i] = v.v[i] != v.v[i] ? v.v[i] : 0.0f;
+        }
         *reinterpret_cast<u32x2*>(dst + 8 * lane) = e4m3x8(c);
         if ((lane & 15) == 0) *reinterpret_cast<float*>(dst + 512 + 4 * (lane >> 4)) = scale;
         if (lane < 8) *reinterpret_cast<u32x4*>(dst + 528 + 16 * lane) = pack8(tail);
