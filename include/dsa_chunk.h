@@ -193,7 +193,9 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  *            (workspace: num_splits x T x H x 513 floats and 16 bytes) a combine
  *            merges.  Automatic: whether to split by the call's sizes, and up to
  *            64 sequences the size of a split by their lengths, on the device
- *            (dsa_mla_chunk_num_splits: the most that one sequence has).
+ *            (dsa_mla_chunk_num_splits: the most that one sequence has).  Of more
+ *            sequences a split is an even part of max_kv_len, which should then be
+ *            near their lengths: with a bound far above them most parts are empty.
  * Scores and sums are fp32.  Probabilities are rounded to 16 bits for the
  * product with V (bf16; fp16 for DSA_KV_FP8_656, where those below fp16's normal
  * range are off by at most 2^-10 of the largest |V| together, up to 2^28 positions

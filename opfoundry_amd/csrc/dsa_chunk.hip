@@ -71,11 +71,11 @@ __device__ __forceinline__ int64_t limit_of(const ChunkParams& p, int32_t b, int
 // any head count fills it, and all its rows attend the same cache rows but for the
 // causal end.  The cache rows come in tiles of 32, three tile buffers deep:
 //   QK^T   wave w: S^T[32 positions x its 32 rows], 36 k-steps of 32x32x16, Q in registers
-//   P      exp2 against a fixed reference (the first tile's maximum of the row), 16 bits,
-//          exchanged through LDS
+//   P      exp2 against a fixed reference (the first tile's maximum of the row, which stands
+//          for 2^lift), 16 bits, exchanged through LDS
 //   PV     wave w: O^T[dims 128 w .. +127 x 128 rows] in 256 accumulation registers
 // Iteration i computes QK^T of tile i + 1, then PV of tile i with the exponentials of
-// tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 403 of a
+// tile i + 1 between its matrix instructions: one barrier a tile.  Q and O are 400 of a
 // CU's 512 KB of registers, which is why a workgroup is 128 rows and fills a CU.
 // Measured (1024 tokens of 128 heads, 8192 bf16 rows before them): 1.98 ms, 1.25 PFLOP/s, 92 % of what
 // a product of two 16384 x 16384 matrices reaches here (2.06 ms in sessions where the card holds a lower
@@ -787,8 +787,11 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     };
 
     const int nspans = k1 > k0 ? (k1 - k0 + SPAN - 1) / SPAN : 0;
-    // Pass 0; where its reference did not serve (rare): the largest score of every row, and the pass
-    // again with that as the reference.
+    // Pass 0; where its reference did not serve one of the rows: the largest score of every row, and the pass
+    // again with that as the reference.  A row of 656-byte rows needs it whose later scores pass its first tile's by
+    // 11 (16 powers of two), one of bf16 rows by 28 less the logarithm of how many do; its whole block then takes
+    // 2.7 times as long (1024 tokens of 128 heads over 8192 rows, all blocks: bf16 1.96 -> 5.33 ms, 656-byte rows
+    // 2.75 -> 7.84; the 32-row kernel on 32 tokens of 16 heads 41 -> 83 us and 41 -> 76).
     bool again = false;
     while (true) {
         // (0 x 0 + 0: cleared where they are, without the registers that zeros to copy would take)

@@ -201,8 +201,10 @@ __device__ __forceinline__ Located<N> locate(const int32_t* indptr, const int32_
 // and 576: a row of 64 lanes (and, for 576, the last 64 values of 8 rows in one
 // further load); D = 128: four rows of 16 lanes.
 // Bound by memory: 4096 tokens of 129 rows of 512, 1.08 GB in 195 us, 5.6 TB/s (a 1 GiB copy: 5.1); 1531 tokens
-// of 65 rows of 128, 51 MB in 12 us, 4.2 TB/s.  Two tokens of 129 rows of 576 take 6 us, a launch and a chain of
-// two loads.
+// of 65 rows of 128, 51 MB in 12 us, 4.2 TB/s; 3000 of 129 rows of 576, 892 MB in 158 us, 5.6 TB/s.  Two tokens of
+// 129 rows of 576 take 6.2 us: 3.1 for one row without a norm, a launch and its chain of two loads, 1.6 more for 8 rows
+// each in 16 waves a token, 1.6 more for the key's norm, which runs over all 8 places of its wave where one is taken
+// (one row with a norm 5.2, eight 5.6).
 // ---------------------------------------------------------------------------
 template <int D>
 constexpr int GROUP = D == 128 ? 16 : 8;

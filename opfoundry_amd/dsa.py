@@ -824,7 +824,7 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
     of 128, else the last 64) are rotated ("interleaved" pairs, "halves", or None), back when `inverse`.
     cos_sin fp32 [n_pos, 64]: a position's 32 cosines, then its 32 sines.  The position of a row is
     positions[t] (int32 [T]), or the chunk's (q_indptr, seq_lens), whose rows of no sequence are left as
-    allocated.  Returns (q_out, k_out); an output may be its input."""
+    allocated.  Returns (q_out, k_out); an output may be its input, and must not overlap one otherwise."""
     if q.dim() != 3:
         _bad("q", q, "be [T, H, D]")
     T, _, D = q.shape
@@ -1023,7 +1023,8 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     q bf16 [T, H, 576]; kv_cache bf16 [..., 576] or uint8 [..., 656]; sequence b's tokens
     q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b] (their own rows already
     in the cache) and attend positions up to their own (causal) or all.  Rows of no sequence are left as
-    allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold).  workspace:
+    allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold; past
+    64 sequences a bound near the lengths is faster).  workspace:
     a dense tensor for the partials of a split call (chunk_workspace_size bytes; a smaller one is not used)."""
     dev = q.get_device()
     if dev < 0 or q.dim() != 3:
