@@ -123,6 +123,11 @@ __device__ __forceinline__ void mfma_o(f32x16& acc, u32x4 a, u32x4 b) {
     else
         asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
+// This lane's v or that of the lane 32 further (a ballot, which every lane takes part in, whatever its own v)
+__device__ __forceinline__ bool either(bool v) {
+    const uint64_t all = __builtin_amdgcn_ballot_w64(v);
+    return (((uint32_t)all | (uint32_t)(all >> 32)) >> (threadIdx.x & 31)) & 1;
+}
 // 8 e4m3 codes -> 8 bf16 (exact)
 __device__ __forceinline__ u32x4 codes_bf16(unsigned c0, unsigned c1) {
     return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c0, 1.0f, false)),
@@ -896,7 +901,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         // its type holds it, and if O, which is at most the sum times the largest value, did not pass fp32.  The sum
         // is at least the first tile's maximum, 2^lift; it grows past 2^40 times that only where later scores do.
         const float l = l_lane + __shfl_xor(l_lane, 32, 64);
-        const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
+        const bool have = either(any);
         const float top_p = FP8 ? fmaxf(p_top, __shfl_xor(p_top, 32, 64)) : 0.0f;
         __syncthreads();
         if (wave == 0) s_misc[1] = 0, s_misc[2] = 0, s_misc[3] = 0;
@@ -961,7 +966,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int ns = a_->ns, H = a_->H;
     const int64_t TH = (int64_t)a_->T * H;
     const float l = l_lane + __shfl_xor(l_lane, 32, 64);
-    const bool have = any || __shfl_xor((int)any, 32, 64) != 0;
+    const bool have = either(any);
     const bool mine = 32 * wv + r_ < blk.rows;
     const int lift = lift_of<FP8>(k1 - k0, again);
     const float lse = too_long ? __builtin_nanf("")
