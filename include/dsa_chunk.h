@@ -1,9 +1,10 @@
 /*
  * dsa_chunk.h - C ABI of the operators on a chunk of new tokens in libdsa_mla.so:
  * norms of queries and keys with the position rotation (dsa_qk_norm_rope), the
- * write of latent rows and index keys into the paged caches (dsa_kv_append), and
- * dense attention of the chunk's tokens over the paged latent cache
- * (dsa_mla_chunk).  They fill and read the caches that dsa_mla_decode,
+ * write of latent rows and index keys into the paged caches (dsa_kv_append), the
+ * rows of a paged cache read back as bf16 (dsa_kv_read), and dense attention of
+ * the chunk's tokens over the paged latent cache (dsa_mla_chunk).  They fill and
+ * read the caches that dsa_mla_decode,
  * dsa_mla_prefill and dsa_indexer_scores use; where a context is no longer than
  * the top-k, every position is selected and dsa_mla_chunk takes the place of the
  * scorer, the selection and the sparse attention.
@@ -109,7 +110,7 @@ int dsa_qk_norm_rope(const dsa_qk_norm_rope_args* args, void* stream);
 
 /*
  * Append a chunk's latent rows and index keys to their paged caches.
- * kv       : bf16 [T, 576] (DSA_KV_BF16, DSA_KV_FP8_656, DSA_KV_MXFP8) or
+ * kv       : bf16 [T, 576] (DSA_KV_BF16, DSA_KV_FP8_656, DSA_KV_MXFP8, DSA_KV_MXFP4) or
  *            [T, 512] (DSA_KV_BF16_D512, DSA_KV_MXFP8_V4); NULL: no latent rows.
  *            norm (NONE or RMS, weight fp32 [512] or NULL) covers values 0..511,
  *            then the last 64 values are rotated (rope) by the token's position.
@@ -124,9 +125,16 @@ int dsa_qk_norm_rope(const dsa_qk_norm_rope_args* args, void* stream);
  *              other bytes stay as they were), cache_rope = 64 bf16 values
  *            E8M0: per 32 values the least power of two 2^e >= amax / 448, e at
  *            least -126 (e = 0 for 32 zeros), byte e + 127.
- *            A NaN value becomes a NaN code in every format, also where its group
- *            holds nothing else (scale 0, or E8M0 127).  Row strides in elements of
- *            each stream (bytes for codes and scales); 0 = dense.
+ *            A NaN value becomes a NaN code in every format that has one, also where
+ *            its group holds nothing else (scale 0, or E8M0 127).
+ *            DSA_KV_MXFP4: 400-byte rows; per 32 values the least power of two
+ *              2^e >= amax / 6, e at least -125 (e = 0 for 32 zeros), byte e + 127;
+ *              code = x / 2^e rounded to the nearest e2m1 value, ties to the even
+ *              code.  (Values past 3.5 * 2^126, which could round to 2^128, become
+ *              3 * 2^126.)  A group with a NaN or infinity gets scale byte 255 and
+ *              codes 0: its 32 values are NaN.
+ *            Row strides in elements of each stream (bytes for codes and scales,
+ *            and for 656- and 400-byte rows); 0 = dense.
  * index_k  : bf16 [T, 128]; NULL: no index keys.  index_norm over all 128
  *            values, then the first 64 rotated (index_rope), written as bf16 to
  *            the token's row of index_cache (the same row number).
@@ -173,6 +181,41 @@ typedef struct {
 int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
 
 /*
+ * Rows of a paged latent cache read back as bf16: row t of out becomes the cache
+ * row of token t's position (the chunk's rule above: a whole context is n_b =
+ * seq_lens[b] tokens, positions s .. e - 1 are n_b = e - s with seq_lens[b] = e;
+ * the order of the pages does not matter).  A position without a row reads as
+ * zeros.  Rows of out that belong to no sequence are left as they were.
+ * cache    : the streams of kv_format as in dsa_kv_append; every value is the
+ *            code's times its scale, in fp32 and rounded once to bf16 (exact for
+ *            MXFP8, V4 fp8 and MXFP4 rows), NaN for a NaN code and for E8M0 255
+ * out      : bf16 [T, 576], of DSA_KV_BF16_D512 and DSA_KV_MXFP8_V4 [T, 512], rows
+ *            out_stride_t elements apart.  Rows that overlap one another, or
+ *            memory of the cache, are refused (DSA_ERR_BAD_STRIDE).
+ * T at most 2^29 - 32 (DSA_ERR_BAD_SHAPE).  Alignment as in dsa_kv_append.
+ */
+typedef struct {
+    const void* cache;
+    const void* cache_scale;
+    const void* cache_rope;
+    int64_t cache_rows;
+    int64_t stride_row, scale_stride_row, rope_stride_row;   /* 0 = dense */
+    int32_t kv_format;
+    int32_t T;
+    void* out;
+    int64_t out_stride_t;
+    const int32_t* q_indptr;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    int64_t block_table_stride;
+    int32_t table_blocks, block_size;
+    int64_t kv_batch_stride;
+    int32_t B;
+} dsa_kv_read_args;
+
+int dsa_kv_read(const dsa_kv_read_args* args, void* stream);
+
+/*
  * Dense attention of a chunk's tokens over the paged latent cache.
  *     s_j = (q[t, h] . k_j) * sm_scale
  *     O   = sum_j exp(s_j) k_j[0:512] / sum_j exp(s_j),  LSE = ln sum_j exp(s_j)
@@ -181,8 +224,9 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  * A token with none gets O = 0 and LSE = +inf.  A NaN or infinity in a row reaches
  * the tokens that attend it and no others.  sm_scale must be positive and finite.
  * q        : bf16 [T, H, 576] addressed by q_stride_{t,h}
- * kv_cache : kv_format DSA_KV_BF16 or DSA_KV_FP8_656, rows kv_stride_row
- *            elements apart (0 = dense), kv_total_rows below 2^31
+ * kv_cache : kv_format DSA_KV_BF16, DSA_KV_FP8_656 or DSA_KV_MXFP4, rows
+ *            kv_stride_row elements apart (bytes for 656- and 400-byte rows; 0 =
+ *            dense), kv_total_rows below 2^31
  * out      : bf16 [T, H, 512] addressed by o_stride_{t,h}
  * lse      : fp32 [T, H] dense (may be NULL)
  * max_kv_len: an upper bound of seq_lens (the host cannot read them; it sizes

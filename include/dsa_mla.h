@@ -22,6 +22,18 @@
  *   or non-finite one, gets NaN O and LSE (a defined signal, never a silently
  *   wrong attention).  Rows the cache writer produces from bf16 inputs with
  *   group amax below 57344 always qualify.
+ *   DSA_KV_MXFP4   : [0,256)   512 x e2m1 NoPE codes, value 2 i in the low half of
+ *                              byte i (1 sign, 2 exponent, 1 mantissa bits:
+ *                              0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *                    [256,272) 16 x E8M0 scales, byte g covers NoPE dims
+ *                              [32g, 32g+32) and stands for 2^(byte - 127), 255
+ *                              for NaN
+ *                    [272,400) 64 x bf16 RoPE                    =  400 B
+ *   Dequantised value of NoPE dim d = e2m1(code_d) * 2^(scale[d / 32] - 127),
+ *   which bf16 holds exactly: the kernels compute these rows as bf16 rows of
+ *   those values.  dsa_mla_decode, dsa_mla_decode_noalloc, dsa_mla_prefill and
+ *   the chunk operators (dsa_chunk.h) take them; a NaN or infinity among an
+ *   attended row's values reaches the tokens that attend it.
  *
  * Index semantics (top-k form).  indices[b][t][k] is a logical position j in
  * sequence b.  It is valid iff 0 <= j < seq_lens[b] and, when causal != 0,
@@ -80,6 +92,7 @@ extern "C" {
 #define DSA_MLA_D_VO 512
 #define DSA_MLA_FP8_ROW_BYTES 656
 #define DSA_MLA_BF16_ROW_BYTES 1152
+#define DSA_MLA_FP4_ROW_BYTES 400
 #define DSA_MLA_MAX_SPLITS 64
 /* num_splits of the CSR entries: the workspace already holds the work plan
  * of these lists (dsa_mla_csr_plan) */
@@ -95,8 +108,9 @@ typedef enum {
     DSA_KV_FP8_656 = 1,
     DSA_KV_BF16_D512 = 2,      /* 512 x bf16 rows (V4 prefill only) */
     DSA_KV_MXFP8 = 3,          /* MXFP8 split streams (dsa_mla_decode_mxfp8 only) */
-    DSA_KV_MXFP8_V4 = 4        /* V4 fp8 rows: 448 e4m3 + 14 E8M0 + pad | 64 bf16 RoPE
+    DSA_KV_MXFP8_V4 = 4,       /* V4 fp8 rows: 448 e4m3 + 14 E8M0 + pad | 64 bf16 RoPE
                                   (dsa_mla_prefill_v4_fp8 only) */
+    DSA_KV_MXFP4 = 5           /* 400-byte rows: 512 e2m1 + 16 E8M0 + 64 bf16 RoPE (not the CSR form) */
 } dsa_kv_format;
 
 enum {

@@ -14,7 +14,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "_build", "libdsa_mla.so")
 
 D_QK, D_NOPE, D_ROPE, D_VO = 576, 512, 64, 512
-FP8_ROW_BYTES, BF16_ROW_BYTES = 656, 1152
+FP8_ROW_BYTES, BF16_ROW_BYTES, FP4_ROW_BYTES = 656, 1152, 400
 MAX_SPLITS = 64
 SPLITS_PLANNED = -1               # DSA_MLA_SPLITS_PLANNED: CSR plan already in the workspace
 MAX_LIST = 2 ** 31 - 1 - 2048      # DSA_MLA_MAX_LIST: longest top-k / max_kv_len / max_rows
@@ -24,6 +24,7 @@ KV_FP8_656 = 1
 KV_BF16_D512 = 2
 KV_MXFP8 = 3
 KV_MXFP8_V4 = 4
+KV_MXFP4 = 5
 V4_NOPE = 448
 D_V4 = 512
 
@@ -66,6 +67,7 @@ EXPORTED_SYMBOLS = (
     "dsa_mla_abi_version",
     "dsa_qk_norm_rope",
     "dsa_kv_append",
+    "dsa_kv_read",
     "dsa_mla_chunk_workspace_size",
     "dsa_mla_chunk_num_splits",
     "dsa_mla_chunk",
@@ -235,6 +237,21 @@ class KvAppendArgs(ctypes.Structure):
     ]
 
 
+class KvReadArgs(ctypes.Structure):
+    """dsa_kv_read_args (include/dsa_chunk.h)."""
+
+    _fields_ = [
+        ("cache", _vp), ("cache_scale", _vp), ("cache_rope", _vp), ("cache_rows", _i64),
+        ("stride_row", _i64), ("scale_stride_row", _i64), ("rope_stride_row", _i64),
+        ("kv_format", _i32), ("T", _i32),
+        ("out", _vp), ("out_stride_t", _i64),
+        ("q_indptr", _vp), ("seq_lens", _vp),
+        ("block_table", _vp), ("block_table_stride", _i64), ("table_blocks", _i32), ("block_size", _i32),
+        ("kv_batch_stride", _i64),
+        ("B", _i32),
+    ]
+
+
 class ChunkArgs(ctypes.Structure):
     """dsa_mla_chunk_args (include/dsa_chunk.h)."""
 
@@ -258,13 +275,15 @@ def packer(cls):
     def flat(c):
         return "".join(codes[t] if t in codes else flat(t) for _, t in c._fields_)
 
-    s = struct.Struct("@" + flat(cls))
+    # (0q: the padding at a struct's end)
+    s = struct.Struct("@" + flat(cls) + "0q")
     if s.size != ctypes.sizeof(cls):
         raise RuntimeError(f"{cls.__name__}: {s.size} packed bytes, {ctypes.sizeof(cls)} in C")
     return s.pack
 
 
 pack_norm_rope, pack_append, pack_chunk = packer(QkNormRopeArgs), packer(KvAppendArgs), packer(ChunkArgs)
+pack_read = packer(KvReadArgs)
 
 
 class DsaError(RuntimeError):
@@ -326,6 +345,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     # (argument blocks as a ctypes struct's address or as packed bytes)
     lib.dsa_qk_norm_rope.argtypes = [_vp, _vp]
     lib.dsa_kv_append.argtypes = [_vp, _vp]
+    lib.dsa_kv_read.argtypes = [_vp, _vp]
     lib.dsa_mla_chunk_workspace_size.argtypes = [_vp, sz]
     lib.dsa_mla_chunk_num_splits.argtypes = [_vp, ctypes.POINTER(_i32)]
     lib.dsa_mla_chunk.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]

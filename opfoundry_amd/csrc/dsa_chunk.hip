@@ -1,5 +1,6 @@
 // dsa_chunk.hip - gfx950 kernels of dsa_mla_chunk (include/dsa_chunk.h): dense
-// attention of a chunk's tokens over the paged latent cache.
+// attention of a chunk's tokens over the paged latent cache; and of attention over
+// lists of positions where the cache's rows are 4-bit ones (dsa_list.h).
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -9,12 +10,15 @@
 #include <type_traits>
 
 #include "../../include/dsa_chunk.h"
+#include "dsa_list.h"
 #include "dsa_overlap.h"
+#include "dsa_rows.h"
 #include "dsa_seq.h"
 
 namespace {
 
 #include "dsa_lds.h"
+#include "dsa_fp4.h"
 
 constexpr int D_QK = DSA_MLA_D_QK, D_VO = DSA_MLA_D_VO;
 constexpr int NWAVE = 4, NTHR = 64 * NWAVE;
@@ -49,6 +53,11 @@ struct ChunkParams {
                          // splits of per_split positions)
     float scale_log2;
     Kernel kernel;
+    // calls over lists (B * s_q = T tokens; lens may be null: list_len)
+    const int32_t* indices;
+    int64_t idx_sb, idx_st, q_sb, o_sb;
+    int64_t list_len, causal_offset;
+    int32_t s_q, topk;
 };
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -1588,6 +1597,8 @@ dsa_mla_chunk_narrow_kernel(const ChunkParams p) {
     }
 }
 
+#include "dsa_chunk_fp4.h"
+
 // Joins the partials of a row's splits, SHARES waves a row: a lane holds 8 of its 512 values,
 // wave i takes splits i, i + SHARES, ...  Splits past the row's positions wrote nothing and add nothing.
 // Bound by a chain of memory round trips where there are few rows (128 rows of 16 splits 4.1 us, 6.8 with one
@@ -1702,10 +1713,13 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 // the two sides of it, us: one token of 128 heads over 1501 rows, 128-row blocks 25.2, 32-row 17.7;
 // 256 of 16 heads over 4096 302 and 217; 200 of 128 heads over 1000 78 and 120; 512 tokens of
 // 16 heads over the same 4096 rows 90 (4 splits) and 120.
-constexpr Kernel KERNELS[2][2] = {       // [656-byte rows][narrow]
+constexpr Kernel KERNELS[3][2] = {       // [bf16, 656-byte, 400-byte rows][narrow]
     {{6.3f, 1.83f, 0.0f}, {6.4f, 1.15f, 1.81f}},
     {{10.6f, 2.47f, 0.0f}, {8.3f, 1.48f, 2.07f}},
+    {{6.3f, 1.83f, 0.0f}, {6.4f, 1.0f, 1.3f}},
 };
+int kind_of(int fmt) { return fmt == DSA_KV_BF16 ? 0 : fmt == DSA_KV_FP8_656 ? 1 : 2; }
+constexpr int ROW_BYTES[] = {DSA_MLA_BF16_ROW_BYTES, DSA_MLA_FP8_ROW_BYTES, DSA_MLA_FP4_ROW_BYTES};
 constexpr float BYTES_US = 8.5e6f, FIRST_US = 10.7f, JOIN_US = 3.7f;
 constexpr int COUNTS[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64};
 
@@ -1726,8 +1740,7 @@ struct Plan {
 };
 
 float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int ns) {
-    const bool fp8 = a->kv_format == DSA_KV_FP8_656;
-    const Kernel& k = KERNELS[fp8][narrow];
+    const Kernel& k = KERNELS[kind_of(a->kv_format)][narrow];
     const int64_t tiles = (a->max_kv_len + (int64_t)TILE - 1) / TILE, each = (tiles + ns - 1) / ns;
     const float groups = (float)blocks * ns;
     auto in_rounds = [](float us, float rounds) {
@@ -1735,7 +1748,7 @@ float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int 
     };
     float us = narrow && groups > CUS ? in_rounds(k.start + each * k.pair, groups / (2 * CUS))
                                       : in_rounds(k.start + each * k.tile, groups / CUS);
-    const float row = fp8 ? DSA_MLA_FP8_ROW_BYTES : DSA_MLA_BF16_ROW_BYTES;
+    const float row = ROW_BYTES[kind_of(a->kv_format)];
     us = std::max(us, FIRST_US + (float)a->B * a->max_kv_len * row / BYTES_US);
     if (ns > 1) us += JOIN_US + (float)ns * a->T * a->H * (2 * 4 * (D_VO + 1)) / PART_BYTES_US;
     return us;
@@ -1744,7 +1757,7 @@ float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int 
 Plan plan_of(const dsa_mla_chunk_args* a) {
     Plan best{};
     float least = INFINITY;
-    for (int n = 0; n < 2; ++n) {
+    for (int n = a->kv_format == DSA_KV_MXFP4 ? 1 : 0; n < 2; ++n) {
         const int32_t m = n ? NARROW : BLOCK;
         const int64_t blocks = dsa_seq::block_start(a->T, a->B, a->H, m, dsa_seq::common(a->H, m));
         for (const int c : COUNTS) {
@@ -1772,7 +1785,8 @@ size_t workspace_of(int ns, int64_t T, int64_t H) {
 
 int validate(const dsa_mla_chunk_args* a) {
     if (!a) return DSA_ERR_NULL_POINTER;
-    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8_656) return DSA_ERR_BAD_FORMAT;
+    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8_656 && a->kv_format != DSA_KV_MXFP4)
+        return DSA_ERR_BAD_FORMAT;
     if (a->T < 0 || a->B < 0 || a->H < 1 || a->max_kv_len < 0 || a->kv_total_rows < 0 || a->kv_total_rows > INT32_MAX)
         return DSA_ERR_BAD_SHAPE;
     if (a->max_kv_len > DSA_MLA_MAX_LIST) return DSA_ERR_BAD_SHAPE;
@@ -1781,8 +1795,7 @@ int validate(const dsa_mla_chunk_args* a) {
     const int64_t rows = (int64_t)a->T * a->H;
     if (rows + (int64_t)NARROW * a->B > MAX_GROUPS * NARROW) return DSA_ERR_BAD_SHAPE;
     if (a->num_splits > 1 && rows > MAX_SPLIT_ROWS) return DSA_ERR_BAD_SHAPE;
-    const int64_t least = a->kv_format == DSA_KV_BF16 ? D_QK : DSA_MLA_FP8_ROW_BYTES;
-    const int64_t unit = a->kv_format == DSA_KV_BF16 ? 2 : 1;
+    const int64_t unit = a->kv_format == DSA_KV_BF16 ? 2 : 1, least = ROW_BYTES[kind_of(a->kv_format)] / unit;
     if (a->kv_stride_row != 0 &&
         (a->kv_stride_row < least || (a->kv_stride_row * unit) % 16 || a->kv_stride_row * unit > UINT32_MAX))
         return DSA_ERR_BAD_STRIDE;
@@ -1806,6 +1819,27 @@ int validate(const dsa_mla_chunk_args* a) {
 }
 
 }  // namespace
+
+int dsa_list::launch(const Call& c, bool tiled, hipStream_t stream) {
+    ChunkParams p{};
+    p.q = (const __bf16*)c.q;
+    p.q_sb = c.q_sb, p.q_st = c.q_st, p.q_sh = c.q_sh;
+    p.lens = c.seq_lens, p.list_len = c.len;
+    p.kv = (const unsigned char*)c.kv;
+    p.rows = c.rows, p.row_bytes = c.row_bytes;
+    p.pages = dsa_seq::make_pages(c.block_table, c.table_stride, 0, c.block_size, c.batch_stride);
+    p.indices = c.indices, p.idx_sb = c.idx_sb, p.idx_st = c.idx_st;
+    p.out = (__bf16*)c.out;
+    p.o_sb = c.o_sb, p.o_st = c.o_st, p.o_sh = c.o_sh;
+    p.lse = c.lse, p.part_o = c.part_o, p.part_lse = c.part_lse;
+    p.B = c.B, p.s_q = c.s_q, p.T = c.B * c.s_q, p.H = c.H, p.topk = c.topk;
+    p.causal = c.causal, p.causal_offset = c.causal_offset, p.scale_log2 = c.scale_log2;
+    p.ns = c.ns, p.per_split = c.per_split;
+    const int32_t m = NARROW;
+    const dim3 grid((unsigned)((int64_t)p.T * ((c.H + m - 1) / m)), (unsigned)c.ns);
+    hipLaunchKernelGGL(dsa_mla_fp4_narrow_kernel<true>, grid, dim3(NTHR), 0, stream, p);
+    return hipGetLastError() == hipSuccess ? DSA_OK : DSA_ERR_HIP;
+}
 
 extern "C" {
 
@@ -1840,8 +1874,7 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.indptr = a->q_indptr, p.lens = a->seq_lens;
     p.kv = (const unsigned char*)a->kv_cache;
     p.rows = a->kv_total_rows;
-    p.row_bytes = a->kv_format == DSA_KV_BF16 ? 2 * (a->kv_stride_row ? a->kv_stride_row : D_QK)
-                                              : (a->kv_stride_row ? a->kv_stride_row : DSA_MLA_FP8_ROW_BYTES);
+    p.row_bytes = a->kv_stride_row ? a->kv_stride_row * (a->kv_format == DSA_KV_BF16 ? 2 : 1) : ROW_BYTES[kind_of(a->kv_format)];
     p.pages = dsa_seq::make_pages(a->block_table, a->block_table_stride, a->table_blocks, a->block_size,
                                   a->kv_batch_stride);
     p.out = (__bf16*)a->out;
@@ -1850,7 +1883,7 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.part_o = (float*)ws;
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
     p.dealt = plan.deal ? (int32_t*)(p.part_lse + (size_t)p.ns * a->T * a->H) : nullptr;
-    p.kernel = KERNELS[a->kv_format == DSA_KV_FP8_656][plan.narrow];
+    p.kernel = KERNELS[kind_of(a->kv_format)][plan.narrow];
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
     const bool narrow = plan.narrow;
@@ -1863,7 +1896,8 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
                       plan.deal ? 1u : (unsigned)p.ns);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
     const bool fp8 = a->kv_format == DSA_KV_FP8_656;
-    if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
+    if (a->kv_format == DSA_KV_MXFP4) launch(dsa_mla_fp4_narrow_kernel<false>);
+    else if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
     else if (fp8) launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
     else launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);
     if (hipGetLastError() != hipSuccess) return DSA_ERR_HIP;

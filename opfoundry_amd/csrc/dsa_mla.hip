@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "../../include/dsa_mla.h"
+#include "dsa_list.h"
 #include "dsa_rows.h"
 
 namespace {
@@ -3893,9 +3894,9 @@ bool is_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
 // -1 when the stride is shorter than a row or not a multiple of 16 bytes
 // (every gather load is 16 bytes).
 int64_t row_stride_bytes(int fmt, int64_t stride) {
-    const int64_t dense = fmt == DSA_KV_FP8_656 ? FP8_ROW : BF16_ROW;
+    const int64_t dense = fmt == DSA_KV_FP8_656 ? FP8_ROW : fmt == DSA_KV_MXFP4 ? DSA_MLA_FP4_ROW_BYTES : BF16_ROW;
     if (stride == 0) return dense;
-    const int64_t bytes = fmt == DSA_KV_FP8_656 ? stride : 2 * stride;
+    const int64_t bytes = fmt == DSA_KV_BF16 ? 2 * stride : stride;
     // (below 4 GiB: the kernels form a row's byte offset as a 32 x 32-bit product)
     return stride < 0 || bytes < dense || (bytes % 16) != 0 || bytes > 0xFFFFFFF0ll ? -1 : bytes;
 }
@@ -3975,6 +3976,8 @@ constexpr KernTime KERN_TIME[][4] = {
     // DSA_KV_MXFP8_V4 (no NARROW kernel)
     {{13.8f, 2.23f, 0, 0, 2.7f, 0.40f, 0}, {},
      {10.4f, 2.14f, 11.9f, 2.65f, 1.6f, 0.36f, 0}, {10.8f, 2.41f, 11.8f, 3.06f, 2.0f, 0.32f, 0}},
+    // DSA_KV_MXFP4 (128 heads a workgroup, or 32 and two workgroups per CU)
+    {{13.5f, 1.83f, 0, 0, 3.2f, 0.38f, 0}, {}, {8.3f, 1.0f, 9.0f, 1.3f, 2.6f, 0.39f, 0}, {}},
 };
 double kern_time(int fmt, Kern k, int64_t tokens, int32_t H, int64_t list, int ns) {
     const KernTime& c = KERN_TIME[fmt][k];
@@ -4010,7 +4013,9 @@ struct Choice {
     Kern kern;
     int ns;
 };
+Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len);
 Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
+    if (fmt == DSA_KV_MXFP4) return choose_fp4(tokens, H, list, requested, by_len);
     Choice best{WIDE, requested > 0 ? requested : one_round_splits(tokens * head_groups(H), by_len)};
     if (tokens <= 0 || !narrow_path(fmt, tokens, H, best.ns)) return best;
     double least = -1.0;
@@ -4025,6 +4030,23 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
             if (k == NARROW && wgs * ns > CUS) continue;
             if (k == PAIR && H > 64 && wgs * ns <= CUS) continue;
             const double t = kern_time(fmt, k, tokens, H, list, ns);
+            if (least >= 0 && t >= least) continue;
+            least = t;
+            best = Choice{k, ns};
+        }
+    }
+    return best;
+}
+// MXFP4 rows
+Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
+    Choice best{PAIR, requested > 0 ? requested : 1};
+    double least = -1.0;
+    for (Kern k : {PAIR}) {
+        const int64_t wgs = tokens * groups_of(k, H);
+        const int counts[] = {1, one_round_splits(wgs, by_len), one_round_splits(wgs, by_len, k == PAIR ? 2 * CUS : CUS)};
+        for (int ns : counts) {
+            if (requested > 0) ns = requested;
+            const double t = kern_time(DSA_KV_MXFP4, k, tokens, H, list, ns);
             if (least >= 0 && t >= least) continue;
             least = t;
             best = Choice{k, ns};
@@ -4057,11 +4079,20 @@ int noalloc_splits(const dsa_mla_decode_args* a) {
     return (int)std::min<int64_t>(std::min<int64_t>((CUS + wgs - 1) / wgs, by_len), DSA_MLA_MAX_SPLITS);
 }
 
+// formats of the top-k and prefill forms
+bool list_format(int fmt) { return fmt == DSA_KV_BF16 || fmt == DSA_KV_FP8_656 || fmt == DSA_KV_MXFP4; }
+// MXFP4 rows: a grid holds below 2^32 threads, of workgroups of 32 heads
+bool fp4_call_ok(int fmt, int64_t tokens, int32_t H) {
+    return fmt != DSA_KV_MXFP4 || tokens * narrow_groups(H) < ((int64_t)1 << 32) / NTHR;
+}
+
 int validate_decode(const dsa_mla_decode_args* a, DecodePlan* plan) {
     if (!a) return DSA_ERR_NULL_POINTER;
     if (a->B < 0 || a->s_q <= 0 || a->topk < 0 || a->topk > MAX_LIST) return DSA_ERR_BAD_SHAPE;
     if (!heads_ok(a->H, a->B)) return DSA_ERR_BAD_SHAPE;
-    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8_656) return DSA_ERR_BAD_FORMAT;
+    if (!list_format(a->kv_format)) return DSA_ERR_BAD_FORMAT;
+    if (!fp4_call_ok(a->kv_format, (int64_t)a->B * a->s_q, a->H)) return DSA_ERR_BAD_SHAPE;
+    if (a->kv_format == DSA_KV_MXFP4 && !(a->sm_scale > 0.0f && a->sm_scale <= FLT_MAX)) return DSA_ERR_UNSUPPORTED;
     if (a->kv_total_rows < 0 || a->kv_total_rows > INT32_MAX) return DSA_ERR_BAD_SHAPE;
     if (a->block_table && a->block_size <= 0) return DSA_ERR_BAD_SHAPE;
     if (row_stride_bytes(a->kv_format, a->kv_stride_row) < 0) return DSA_ERR_BAD_STRIDE;
@@ -4087,7 +4118,25 @@ size_t decode_ws_bytes(const dsa_mla_decode_args* a, int ns) {
     return (size_t)ns * rows * (D_VO + 1) * sizeof(float) + 256;
 }
 
+// MXFP4 rows: the kernels over lists of dsa_chunk.hip
+int launch_fp4(const FwdParams& fp, int ns, hipStream_t st, Kern kern) {
+    dsa_list::Call c{};
+    c.q = fp.q, c.q_sb = fp.q_sb, c.q_st = fp.q_st, c.q_sh = fp.q_sh;
+    c.kv = fp.kv, c.rows = fp.kv_total_rows, c.row_bytes = fp.row_bytes;
+    c.block_table = fp.block_table, c.table_stride = fp.bt_stride, c.block_size = fp.block_size;
+    c.batch_stride = fp.kv_batch_stride;
+    c.seq_lens = fp.seq_lens, c.len = fp.seq_len_default;
+    c.indices = fp.indices, c.idx_sb = fp.idx_sb, c.idx_st = fp.idx_st;
+    c.out = fp.out, c.o_sb = fp.o_sb, c.o_st = fp.o_st, c.o_sh = fp.o_sh;
+    c.lse = fp.lse, c.part_o = fp.part_o, c.part_lse = fp.part_lse;
+    c.B = fp.B, c.s_q = fp.s_q, c.H = fp.H, c.topk = fp.topk;
+    c.causal = fp.causal, c.causal_offset = fp.causal_offset, c.scale_log2 = fp.scale_log2;
+    c.ns = ns, c.per_split = fp.chunk;
+    return dsa_list::launch(c, kern == WIDE, st);
+}
+
 int launch_fwd(const FwdParams& fp, int fmt, int B, int s_q, int ns, hipStream_t st, Kern kern = WIDE) {
+    if (fmt == DSA_KV_MXFP4) return launch_fp4(fp, ns, st, kern);
     dim3 grid((unsigned)((int64_t)B * fp.hgroups), s_q, ns), block(NTHR);
     if (kern == PAIR || kern == PAIR64) {
         auto pick = [&](auto hg) {
@@ -4302,7 +4351,9 @@ int validate_prefill(const dsa_mla_prefill_args* a, int* ns_out) {
     if (!a) return DSA_ERR_NULL_POINTER;
     if (a->N < 0 || a->topk < 0 || a->kv_rows < 0 || a->kv_rows > INT32_MAX) return DSA_ERR_BAD_SHAPE;
     if (!heads_ok(a->H, a->N)) return DSA_ERR_BAD_SHAPE;
-    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8_656) return DSA_ERR_BAD_FORMAT;
+    if (!list_format(a->kv_format)) return DSA_ERR_BAD_FORMAT;
+    if (!fp4_call_ok(a->kv_format, a->N, a->H)) return DSA_ERR_BAD_SHAPE;
+    if (a->kv_format == DSA_KV_MXFP4 && !(a->sm_scale > 0.0f && a->sm_scale <= FLT_MAX)) return DSA_ERR_UNSUPPORTED;
     if (row_stride_bytes(a->kv_format, a->kv_stride_row) < 0) return DSA_ERR_BAD_STRIDE;
     if (a->topk > MAX_LIST) return DSA_ERR_BAD_SHAPE;
     if (a->num_splits < 0 || a->num_splits > DSA_MLA_MAX_SPLITS) return DSA_ERR_BAD_SPLITS;

@@ -1,9 +1,9 @@
 // dsa_prep.hip - gfx950 kernels in front of the attention: norms of queries and
-// keys with the position rotation (dsa_qk_norm_rope), and the write of latent
-// rows and index keys into the paged caches (dsa_kv_append), of
-// include/dsa_chunk.h.
+// keys with the position rotation (dsa_qk_norm_rope), the write of latent rows
+// and index keys into the paged caches (dsa_kv_append), and their rows read back
+// (dsa_kv_read), of include/dsa_chunk.h.
 //
-// Both are one pass over memory: a row lives in the registers of one wave, 8
+// All are one pass over memory: a row lives in the registers of one wave, 8
 // values (16 bytes) a lane, between its load and its store.
 
 #include <hip/hip_runtime.h>
@@ -17,6 +17,7 @@
 namespace {
 
 #include "dsa_lds.h"
+#include "dsa_fp4.h"
 
 constexpr int WAVES = 4;                 // waves of a workgroup
 constexpr int ROT = DSA_MLA_D_ROPE;      // rotated values of a row
@@ -323,12 +324,35 @@ __device__ __forceinline__ int scale_exponent(float amax) {
     return max(-126, min(127, e));
 }
 
+// The largest |x| by its bits, so that a NaN is above infinity and both above every value
+__device__ __forceinline__ float max_bits(float a, float b) {
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+}
+__device__ __forceinline__ float amax_any8(const V8& x) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max_bits(a, fabsf(x.v[i]));
+    return a;
+}
+// e2m1 codes of 8 values / 2^e: the conversion rounds to nearest, ties to the even code, and saturates at 6.
+// (At e = 126 a code of 4 would be 2^128: those values take 3.)
+__device__ __forceinline__ unsigned e2m1x8(const V8& x, int e) {
+    const float top = e >= 126 ? 3.0f : 6.0f;
+    float c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(ldexpf(x.v[i], -e), -top), top);
+    unsigned w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, c[0], c[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[2], c[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[4], c[5], 1.0f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[6], c[7], 1.0f, 3);
+}
+
 template <int ROPE>
 __device__ __forceinline__ void append_latent(const AppendParams& p, int t) {
     const dsa_kv_append_args& a = p.a;
     const int lane = threadIdx.x & 63;
     const int fmt = a.kv_format;
-    const bool wide = fmt == DSA_KV_BF16 || fmt == DSA_KV_FP8_656 || fmt == DSA_KV_MXFP8;   // 576 values
+    const bool wide = fmt != DSA_KV_BF16_D512 && fmt != DSA_KV_MXFP8_V4;      // 576 values
     const __bf16* x = (const __bf16*)a.kv + (int64_t)t * a.kv_stride_t;
     const u32x4 raw = *reinterpret_cast<const u32x4*>(x + 8 * lane);
     u32x4 raw_tail = {};
@@ -365,6 +389,13 @@ __device__ __forceinline__ void append_latent(const AppendParams& p, int t) {
         *reinterpret_cast<u32x2*>(dst + 8 * lane) = e4m3x8(c);
         if ((lane & 15) == 0) *reinterpret_cast<float*>(dst + 512 + 4 * (lane >> 4)) = scale;
         if (lane < 8) *reinterpret_cast<u32x4*>(dst + 528 + 16 * lane) = pack8(tail);
+    } else if (fmt == DSA_KV_MXFP4) {
+        const float amax = all4(amax_any8(v), max_bits);
+        const bool nan = __float_as_uint(amax) >= 0x7F800000u;
+        const int e = nan ? 128 : fp4_exponent(amax);
+        *reinterpret_cast<unsigned*>(dst + 4 * lane) = nan ? 0u : e2m1x8(v, e);
+        if ((lane & 3) == 0) dst[FP4_SCALE_OFF + (lane >> 2)] = (unsigned char)(e + 127);
+        if (lane < 8) *reinterpret_cast<u32x4*>(dst + FP4_ROPE_OFF + 16 * lane) = pack8(tail);
     } else {
         const int e = scale_exponent(all4(amax8(v), max_abs));
         V8 c;
@@ -422,6 +453,103 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_kv_append_kernel(const AppendP
     }
 }
 
+// ---------------------------------------------------------------------------
+// Rows read back: a wave takes READ_ROWS tokens.  Their cache rows are looked up a
+// lane each, then every load of all of them goes out before the first is used.
+// ---------------------------------------------------------------------------
+constexpr int READ_ROWS = 8;
+struct ReadParams {
+    dsa_kv_read_args a;
+    dsa_seq::Pages pages;
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(64 * WAVES) dsa_kv_read_kernel(const ReadParams p) {
+    constexpr bool WIDE = FMT != DSA_KV_BF16_D512 && FMT != DSA_KV_MXFP8_V4;       // 576 values
+    constexpr bool BF16 = FMT == DSA_KV_BF16 || FMT == DSA_KV_BF16_D512;
+    constexpr bool STREAMS = FMT == DSA_KV_MXFP8 || FMT == DSA_KV_MXFP8_V4;
+    const dsa_kv_read_args& a = p.a;
+    const int lane = threadIdx.x & 63;
+    const int t0 = ((int)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * READ_ROWS;
+    if (t0 >= a.T) return;
+    const Located<READ_ROWS> at = locate<READ_ROWS>(a.q_indptr, a.seq_lens, a.B, t0);
+    // lane k: the cache row of token t0 + k; -1: none, NONE: no sequence's
+    constexpr int32_t NONE = INT32_MIN;
+    int32_t b = NO_SEQ;
+    int64_t pos = -1;
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k)
+        if ((lane & (READ_ROWS - 1)) == k) b = at.b[k], pos = at.pos[k];
+    int32_t mine = NONE;
+    if (b != NO_SEQ && t0 + (lane & (READ_ROWS - 1)) < a.T) mine = (int32_t)dsa_seq::row_of(p.pages, b, pos, a.cache_rows);
+    int32_t row[READ_ROWS];
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k) row[k] = __builtin_amdgcn_readlane(mine, k);
+
+    const unsigned char* const cache = (const unsigned char*)a.cache;
+    const unsigned char* const rope = (const unsigned char*)a.cache_rope;
+    const int64_t unit = BF16 ? 2 : 1;
+    u32x4 v[READ_ROWS];                 // the codes (or values) of this lane's 8 values
+    unsigned sc[READ_ROWS];             // their scale
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k) {
+        v[k] = u32x4{0, 0, 0, 0};
+        sc[k] = 0;
+        if (row[k] < 0) continue;
+        const unsigned char* const r = cache + (int64_t)row[k] * a.stride_row * unit;
+        if constexpr (BF16) {
+            v[k] = *reinterpret_cast<const u32x4*>(r + 16 * lane);
+        } else if constexpr (FMT == DSA_KV_MXFP4) {
+            v[k][0] = *reinterpret_cast<const unsigned*>(r + 4 * lane);
+            sc[k] = r[FP4_SCALE_OFF + (lane >> 2)];
+        } else if (WIDE || lane < 56) {
+            const u32x2 c = *reinterpret_cast<const u32x2*>(r + 8 * lane);
+            v[k][0] = c[0], v[k][1] = c[1];
+            if constexpr (FMT == DSA_KV_FP8_656) sc[k] = *reinterpret_cast<const unsigned*>(r + 512 + 4 * (lane >> 4));
+            else if constexpr (FMT == DSA_KV_MXFP8) sc[k] = ((const unsigned char*)a.cache_scale)[(int64_t)row[k] * a.scale_stride_row + (lane >> 2)];
+            else sc[k] = r[DSA_MLA_V4_NOPE + (lane >> 2)];
+        } else {
+            v[k] = *reinterpret_cast<const u32x4*>(rope + (int64_t)row[k] * a.rope_stride_row * 2 + 16 * (lane - 56));
+        }
+    }
+    // the last 64 values of all rows: lane 8 k + i has piece i of row k's
+    u32x4 tail = {0, 0, 0, 0};
+    static_assert(READ_ROWS == 8, "a piece a lane");
+    const int32_t trow = __shfl(mine, lane >> 3, 64);
+    if constexpr (WIDE)
+        if (trow >= 0) {
+            if constexpr (STREAMS) tail = *reinterpret_cast<const u32x4*>(rope + (int64_t)trow * a.rope_stride_row * 2 + 16 * (lane & 7));
+            else tail = *reinterpret_cast<const u32x4*>(cache + (int64_t)trow * a.stride_row * unit + (BF16 ? 1024 : FMT == DSA_KV_FP8_656 ? 528 : FP4_ROPE_OFF) + 16 * (lane & 7));
+        }
+
+    __bf16* const out = (__bf16*)a.out + (int64_t)t0 * a.out_stride_t;
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k) {
+        if (row[k] == NONE) continue;
+        u32x4 o = v[k];
+        if (row[k] < 0) o = u32x4{0, 0, 0, 0};
+        else if constexpr (FMT == DSA_KV_MXFP4) o = fp4_to_bf16(v[k][0], sc[k]);
+        else if constexpr (!BF16) {
+            if (WIDE || lane < 56) {
+                // (a power of two by its exponent: byte 0 is below fp32's normal range, 255 is NaN)
+                const float s = FMT == DSA_KV_FP8_656 ? __uint_as_float(sc[k])
+                                                      : sc[k] == 255 ? __builtin_nanf("") : ldexpf(1.0f, (int)sc[k] - 127);
+                V8 x;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[k][h], false);
+                    const f32x2 up = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[k][h], true);
+                    x.v[4 * h] = lo[0] * s, x.v[4 * h + 1] = lo[1] * s, x.v[4 * h + 2] = up[0] * s, x.v[4 * h + 3] = up[1] * s;
+                }
+                o = pack8(x);
+            }
+        }
+        *reinterpret_cast<u32x4*>(out + (int64_t)k * a.out_stride_t + 8 * lane) = o;
+    }
+    if constexpr (WIDE)
+        if (trow != NONE) *reinterpret_cast<u32x4*>(out + (int64_t)(lane >> 3) * a.out_stride_t + 512 + 8 * (lane & 7)) = tail;
+}
+
 // ------------------------------------------------------------------- host
 constexpr int64_t MAX_JOBS = (((int64_t)1 << 32) / (64 * WAVES) - 1) * WAVES;      // a grid holds below 2^32 threads
 
@@ -472,6 +600,42 @@ bool outputs_overlap(const dsa_qk_norm_rope_args& a) {
         ++n;
     }
     return n == 2 && (overlap(x[0], o[1]) || overlap(x[1], o[0]) || overlap(o[0], o[1]));
+}
+
+// The pages and the cache's streams of an append or a read; strides of 0 become those of dense rows.
+template <class A>
+int check_pages(const A& a) {
+    if (a.block_table) {
+        if (a.block_size < 1 || a.table_blocks < 0 || (int64_t)a.block_size * a.table_blocks > INT32_MAX)
+            return DSA_ERR_BAD_SHAPE;
+        if (a.block_table_stride < 0) return DSA_ERR_BAD_STRIDE;
+    } else if (a.kv_batch_stride < 0) {
+        return DSA_ERR_BAD_STRIDE;
+    }
+    return DSA_OK;
+}
+struct Streams {
+    bool bf16, rope, scales;
+};
+Streams streams_of(int fmt) {
+    return {fmt == DSA_KV_BF16 || fmt == DSA_KV_BF16_D512, fmt == DSA_KV_MXFP8 || fmt == DSA_KV_MXFP8_V4, fmt == DSA_KV_MXFP8};
+}
+int64_t least_stride(int fmt) {
+    return fmt == DSA_KV_BF16 ? 576 : fmt == DSA_KV_FP8_656 ? DSA_MLA_FP8_ROW_BYTES : fmt == DSA_KV_MXFP4 ? FP4_ROW : 512;
+}
+template <class A>
+int check_cache(A& a) {
+    const Streams s = streams_of(a.kv_format);
+    const int64_t least = least_stride(a.kv_format);
+    if (a.stride_row == 0) a.stride_row = least;
+    if (a.scale_stride_row == 0) a.scale_stride_row = 16;
+    if (a.rope_stride_row == 0) a.rope_stride_row = ROT;
+    if (a.cache_rows > 0 && (!a.cache || (s.rope && !a.cache_rope) || (s.scales && !a.cache_scale))) return DSA_ERR_NULL_POINTER;
+    if (a.stride_row < least || a.stride_row % (s.bf16 ? 8 : 16)) return DSA_ERR_BAD_STRIDE;
+    if (s.rope && (a.rope_stride_row < ROT || a.rope_stride_row % 8)) return DSA_ERR_BAD_STRIDE;
+    if (s.scales && (a.scale_stride_row < 16 || a.scale_stride_row % 16)) return DSA_ERR_BAD_STRIDE;
+    if (!ptr16(a.cache) || (s.rope && !ptr16(a.cache_rope)) || (s.scales && !ptr16(a.cache_scale))) return DSA_ERR_BAD_STRIDE;
+    return DSA_OK;
 }
 
 template <int D>
@@ -532,37 +696,19 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream) {
     if (a.norm != DSA_NORM_NONE && a.norm != DSA_NORM_RMS) return DSA_ERR_UNSUPPORTED;
     if (a.norm == DSA_NORM_NONE && a.weight) return DSA_ERR_UNSUPPORTED;
     if (a.index_norm == DSA_NORM_NONE && (a.index_weight || a.index_bias)) return DSA_ERR_UNSUPPORTED;
-    if (a.kv_format < DSA_KV_BF16 || a.kv_format > DSA_KV_MXFP8_V4) return DSA_ERR_BAD_FORMAT;
+    if (a.kv_format < DSA_KV_BF16 || a.kv_format > DSA_KV_MXFP4) return DSA_ERR_BAD_FORMAT;
     if (!(a.eps >= 0.0f) || !(a.index_eps >= 0.0f)) return DSA_ERR_BAD_SHAPE;
-    if (a.block_table) {
-        if (a.block_size < 1 || a.table_blocks < 0 || (int64_t)a.block_size * a.table_blocks > INT32_MAX)
-            return DSA_ERR_BAD_SHAPE;
-        if (a.block_table_stride < 0) return DSA_ERR_BAD_STRIDE;
-    } else {
-        if (a.kv_batch_stride < 0 || (a.kv_batch_stride == 0 && a.B > 1)) return DSA_ERR_BAD_STRIDE;
-    }
+    if (const int rc = check_pages(a)) return rc;
+    if (!a.block_table && a.kv_batch_stride == 0 && a.B > 1) return DSA_ERR_BAD_STRIDE;
     if (a.T == 0 || a.B == 0 || (!a.kv && !a.index_k)) return DSA_OK;
     if (!a.q_indptr || !a.seq_lens) return DSA_ERR_NULL_POINTER;
     const bool rotates = (a.kv && a.rope != DSA_ROPE_NONE) || (a.index_k && a.index_rope != DSA_ROPE_NONE);
     if (rotates && a.n_pos > 0 && !a.cos_sin) return DSA_ERR_NULL_POINTER;
     if (!ptr16(a.cos_sin)) return DSA_ERR_BAD_STRIDE;
     if (a.kv) {
-        const bool bf16 = a.kv_format == DSA_KV_BF16 || a.kv_format == DSA_KV_BF16_D512;
-        const bool streams = a.kv_format == DSA_KV_MXFP8 || a.kv_format == DSA_KV_MXFP8_V4;
-        const bool scales = a.kv_format == DSA_KV_MXFP8;
-        const int64_t least = a.kv_format == DSA_KV_BF16 ? 576 : a.kv_format == DSA_KV_FP8_656 ? 656 : 512;
-        if (a.stride_row == 0) a.stride_row = least;
-        if (a.scale_stride_row == 0) a.scale_stride_row = 16;
-        if (a.rope_stride_row == 0) a.rope_stride_row = ROT;
-        if (a.cache_rows > 0 && (!a.cache || (streams && !a.cache_rope) || (scales && !a.cache_scale)))
-            return DSA_ERR_NULL_POINTER;
-        if (a.stride_row < least || a.stride_row % (bf16 ? 8 : 16)) return DSA_ERR_BAD_STRIDE;
-        if (streams && (a.rope_stride_row < ROT || a.rope_stride_row % 8)) return DSA_ERR_BAD_STRIDE;
-        if (scales && (a.scale_stride_row < 16 || a.scale_stride_row % 16)) return DSA_ERR_BAD_STRIDE;
+        if (const int rc = check_cache(a)) return rc;
         if (a.kv_stride_t < 0 || a.kv_stride_t % 8) return DSA_ERR_BAD_STRIDE;
-        if (!ptr16(a.kv) || !ptr16(a.weight) || !ptr16(a.cache) || (streams && !ptr16(a.cache_rope)) ||
-            (scales && !ptr16(a.cache_scale)))
-            return DSA_ERR_BAD_STRIDE;
+        if (!ptr16(a.kv) || !ptr16(a.weight)) return DSA_ERR_BAD_STRIDE;
     }
     if (a.index_k) {
         if (a.index_stride_row == 0) a.index_stride_row = 128;
@@ -578,6 +724,46 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream) {
     if (jobs > MAX_JOBS) return DSA_ERR_BAD_SHAPE;
     hipLaunchKernelGGL(dsa_kv_append_kernel, dim3((unsigned)((jobs + WAVES - 1) / WAVES)), dim3(64 * WAVES), 0,
                        (hipStream_t)stream, p, latent);
+    return hipGetLastError() == hipSuccess ? DSA_OK : DSA_ERR_HIP;
+}
+
+int dsa_kv_read(const dsa_kv_read_args* args, void* stream) {
+    if (!args) return DSA_ERR_NULL_POINTER;
+    ReadParams p;
+    p.a = *args;
+    dsa_kv_read_args& a = p.a;
+    if (a.T < 0 || a.T > MAX_JOBS * READ_ROWS || a.B < 0 || a.cache_rows < 0 || a.cache_rows > INT32_MAX) return DSA_ERR_BAD_SHAPE;
+    if (a.kv_format < DSA_KV_BF16 || a.kv_format > DSA_KV_MXFP4) return DSA_ERR_BAD_FORMAT;
+    if (const int rc = check_pages(a)) return rc;
+    if (a.T == 0 || a.B == 0) return DSA_OK;
+    if (!a.q_indptr || !a.seq_lens || !a.out) return DSA_ERR_NULL_POINTER;
+    if (const int rc = check_cache(a)) return rc;
+    const Streams s = streams_of(a.kv_format);
+    const int64_t width = a.kv_format == DSA_KV_BF16_D512 || a.kv_format == DSA_KV_MXFP8_V4 ? 512 : 576;
+    if (!ptr16(a.out) || a.out_stride_t % 8 || a.out_stride_t < 0 || (a.T > 1 && a.out_stride_t < width)) return DSA_ERR_BAD_STRIDE;
+    // (bytes of n rows, whatever their stride)
+    typedef dsa_overlap::wide wide;
+    const wide o0 = (uintptr_t)a.out, o1 = o0 + 2 * ((wide)(a.T - 1) * a.out_stride_t + width);
+    auto meets = [&](const void* q, int64_t stride, int64_t bytes) {
+        const wide c0 = (uintptr_t)q, c1 = c0 + (wide)(a.cache_rows - 1) * stride + bytes;
+        return a.cache_rows > 0 && o0 < c1 && c0 < o1;
+    };
+    const int64_t unit = s.bf16 ? 2 : 1;
+    if (meets(a.cache, a.stride_row * unit, least_stride(a.kv_format) * unit) ||
+        (s.rope && meets(a.cache_rope, 2 * a.rope_stride_row, 2 * ROT)) || (s.scales && meets(a.cache_scale, a.scale_stride_row, 16)))
+        return DSA_ERR_BAD_STRIDE;
+    p.pages = dsa_seq::make_pages(a.block_table, a.block_table_stride, a.table_blocks, a.block_size, a.kv_batch_stride);
+    const int64_t jobs = ((int64_t)a.T + READ_ROWS - 1) / READ_ROWS;
+    const dim3 grid((unsigned)((jobs + WAVES - 1) / WAVES)), block(64 * WAVES);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, p); };
+    switch (a.kv_format) {
+        case DSA_KV_BF16: launch(dsa_kv_read_kernel<DSA_KV_BF16>); break;
+        case DSA_KV_FP8_656: launch(dsa_kv_read_kernel<DSA_KV_FP8_656>); break;
+        case DSA_KV_BF16_D512: launch(dsa_kv_read_kernel<DSA_KV_BF16_D512>); break;
+        case DSA_KV_MXFP8: launch(dsa_kv_read_kernel<DSA_KV_MXFP8>); break;
+        case DSA_KV_MXFP8_V4: launch(dsa_kv_read_kernel<DSA_KV_MXFP8_V4>); break;
+        default: launch(dsa_kv_read_kernel<DSA_KV_MXFP4>); break;
+    }
     return hipGetLastError() == hipSuccess ? DSA_OK : DSA_ERR_HIP;
 }
 

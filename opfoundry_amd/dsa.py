@@ -29,15 +29,17 @@ def _stream(stream) -> Optional[int]:
 
 
 def kv_format_of(kv: torch.Tensor) -> Tuple[int, int, int]:
-    """(kv_format, total_rows, row_stride) of a cache tensor: bf16 [..., 576] or uint8
-    [..., 656] with a dense last dim.  Rows may be padded (a view of wider rows): row_stride
+    """(kv_format, total_rows, row_stride) of a cache tensor: bf16 [..., 576], uint8
+    [..., 656] or uint8 [..., 400] (MXFP4) with a dense last dim.  Rows may be padded (a view of wider rows): row_stride
     is the element distance between rows, 0 when they are dense."""
     if kv.dtype == torch.bfloat16 and kv.shape[-1] == abi.D_QK:
         fmt, width = abi.KV_BF16, abi.D_QK
     elif kv.dtype == torch.uint8 and kv.shape[-1] == abi.FP8_ROW_BYTES:
         fmt, width = abi.KV_FP8_656, abi.FP8_ROW_BYTES
+    elif kv.dtype == torch.uint8 and kv.shape[-1] == abi.FP4_ROW_BYTES:
+        fmt, width = abi.KV_MXFP4, abi.FP4_ROW_BYTES
     else:
-        raise ValueError(f"kv cache must be bf16 [..., 576] or uint8 [..., 656], got {kv.dtype} "
+        raise ValueError(f"kv cache must be bf16 [..., 576], uint8 [..., 656] or uint8 [..., 400], got {kv.dtype} "
                          f"{tuple(kv.shape)}")
     if kv.stride(-1) != 1:
         raise ValueError("kv cache rows must have a dense last dim")
@@ -869,10 +871,38 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
 
 # the tensors of a cache -> (kv_format, width of its latent rows, width of the first tensor's rows)
 _CACHE = {(_BF16, 576): (abi.KV_BF16, 576, 576), (_U8, 656): (abi.KV_FP8_656, 576, 656),
-          (_BF16, 512): (abi.KV_BF16_D512, 512, 512)}
+          (_U8, 400): (abi.KV_MXFP4, 576, 400), (_BF16, 512): (abi.KV_BF16_D512, 512, 512)}
 _CACHES = {((_U8, 512), (_U8, 16), (_BF16, 64)): (abi.KV_MXFP8, 576, 512),
            ((_U8, 512), (_BF16, 64)): (abi.KV_MXFP8_V4, 512, 512)}
 _KV_NORMS = {"none": 0, "rms": 1}
+
+
+def _streams(cache, dev: int):
+    """(first tensor, kv_format, values of a row, addresses of rows, scales and RoPE, rows, their strides) of a
+    cache: a tensor, or the tuple of its streams."""
+    parts = cache if isinstance(cache, (tuple, list)) else (cache,)
+    first = parts[0]
+    if len(parts) == 1:
+        found = _CACHE.get((first.dtype, first.shape[-1]))
+    else:
+        found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
+    if found is None:
+        raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
+    fmt, width, own = found
+    psc = pr = sstride = rstride = 0
+    pc = _addr(first, first.dtype, "cache", dev)
+    rows, stride = (first.numel() // own, 0) if first.is_contiguous() else _rows(first, own, "cache")
+    if len(parts) > 1:
+        last = parts[-1]
+        pr = _addr(last, _BF16, "cache", dev)
+        more, rstride = _rows(last, 64, "cache")
+        if len(parts) == 3:
+            psc = _addr(parts[1], _U8, "cache", dev)
+            others, sstride = _rows(parts[1], 16, "cache")
+            more = more if others == rows else -1
+        if more != rows:
+            raise ValueError("the cache's streams must have the same rows")
+    return first, fmt, width, pc, psc, pr, rows, stride, sstride, rstride
 
 
 def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
@@ -888,7 +918,7 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
 
     kv bf16 [T, 576] (or [T, 512] for V4 rows), normed over its first 512 values (norm "rms", the
     default with a weight, or "none") and rotated in its last 64 (style None: as they are).  cache: bf16
-    [..., 576], uint8 [..., 656], bf16 [..., 512], (uint8 [..., 512], uint8 [..., 16], bf16 [..., 64])
+    [..., 576], uint8 [..., 656] (fp8), uint8 [..., 400] (MXFP4), bf16 [..., 512], (uint8 [..., 512], uint8 [..., 16], bf16 [..., 64])
     for MXFP8 streams, or (uint8 [..., 512], bf16 [..., 64]) for V4 fp8 rows.  index_k bf16 [T, 128] goes
     to the same row of index_cache bf16 [..., 128], after index_norm and a rotation of its first 64
     values.  Pages as in mla_decode (block_size defaults to that of a cache [blocks, block_size, row]);
@@ -902,28 +932,8 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     paged_like = index_cache
     kvp = pw = kst = rows = stride = sstride = rstride = fmt = kind = pc = psc = pr = 0
     if kv is not None:
-        parts = cache if isinstance(cache, (tuple, list)) else (cache,)
-        paged_like = first = parts[0]
-        if len(parts) == 1:
-            found = _CACHE.get((first.dtype, first.shape[-1]))
-        else:
-            found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
-        if found is None:
-            raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
-        fmt, width, own = found
+        paged_like, fmt, width, pc, psc, pr, rows, stride, sstride, rstride = _streams(cache, dev)
         kvp, T, kst = _addr2(kv, width, "kv", dev)
-        pc = _addr(first, first.dtype, "cache", dev)
-        rows, stride = (first.numel() // own, 0) if first.is_contiguous() else _rows(first, own, "cache")
-        if len(parts) > 1:
-            last = parts[-1]
-            pr = _addr(last, _BF16, "cache", dev)
-            more, rstride = _rows(last, 64, "cache")
-            if len(parts) == 3:
-                psc = _addr(parts[1], _U8, "cache", dev)
-                others, sstride = _rows(parts[1], 16, "cache")
-                more = more if others == rows else -1
-            if more != rows:
-                raise ValueError("the cache's streams must have the same rows")
         if norm is None:
             kind = 0 if weight is None else 1
         elif norm in _KV_NORMS:
@@ -968,6 +978,40 @@ def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_len
     _launch(load_library().dsa_kv_append, "dsa_kv_append", dev, stream, a)
 
 
+def kv_read(cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor, rows: Optional[int] = None, *,
+            out: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
+            block_size: Optional[int] = None, kv_batch_stride: int = 0, stream=None) -> torch.Tensor:
+    """Rows of a paged latent cache read back as bf16 [rows, 576] (V4 rows: 512) (dsa_kv_read).
+
+    cache: of any format that kv_append writes.  Rows q_indptr[b] .. q_indptr[b + 1] - 1 of the result are
+    sequence b's last positions below seq_lens[b]; a whole context is as many rows as it is long.  A
+    position without a row reads as zeros; rows of no sequence are left as allocated.  rows: how many rows
+    the result has (the last of q_indptr, which the host does not read; default: those of `out`)."""
+    dev = q_indptr.get_device()
+    if dev < 0:
+        raise ValueError("q_indptr must be a device tensor")
+    pi, pl, B = _sequences(q_indptr, seq_lens, dev)
+    first, fmt, width, pc, psc, pr, n, stride, sstride, rstride = _streams(cache, dev)
+    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
+    if out is None:
+        if rows is None:
+            raise ValueError("rows is required without out")
+        out = (_empty_like if on is None else on.empty)(first, (int(rows), width), _BF16)
+    po, T, ot = _addr2(out, width, "out", dev)
+    if rows is not None and T != rows:
+        _bad("out", out, f"have {rows} rows")
+    pt, tst, blocks, bs = _pages(block_table, block_size, first, B, dev)
+    a = abi.pack_read(pc, psc, pr, n, stride, sstride, rstride, fmt, T, po, ot, pi, pl, pt, tst, blocks, bs,
+                      kv_batch_stride, B)
+    if on is None:
+        rc = load_library().dsa_kv_read(a, _raw_stream(dev))
+        if rc:
+            check(rc, "dsa_kv_read")
+    else:
+        on.call(load_library().dsa_kv_read, "dsa_kv_read", a)
+    return out
+
+
 def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, block_table=None, block_size=None,
                     kv_batch_stride=0, causal=True, max_kv_len=None, num_splits=0) -> bytes:
     """dsa_mla_chunk_args, as the library's calls take them."""
@@ -980,7 +1024,7 @@ def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, bloc
     width = kv_cache.shape[-1]
     found = _CACHE.get((kv_cache.dtype, width))
     if found is None or found[0] == abi.KV_BF16_D512:
-        raise ValueError(f"kv cache must be bf16 [..., 576] or uint8 [..., 656], got {kv_cache.dtype} "
+        raise ValueError(f"kv cache must be bf16 [..., 576], uint8 [..., 656] or uint8 [..., 400], got {kv_cache.dtype} "
                          f"{tuple(kv_cache.shape)}")
     fmt = found[0]
     pk = _addr(kv_cache, kv_cache.dtype, "kv_cache", dev)
