@@ -116,6 +116,10 @@ constexpr int RAW_BYTES = RAW_LOADS * 1024;
 constexpr int RAW_LPW = (RAW_LOADS + NWAVE - 1) / NWAVE; // of wave 0 (6); the others 5
 static_assert(RAW_LOADS == NWAVE * (RAW_LPW - 1) + 1 && RAW_PIECES % 64 == 32, "the last load is wave 0's, half of it spare");
 constexpr int V_BYTES = TILE * NOPE_STRIDE;
+// 400-byte rows: a tile's codes (256 bytes a row) and scales (16 a row) as they come, in two slots; its values go
+// into a tile buffer, as those of bf16 rows, which its RoPE values are loaded into.
+constexpr int RAW4_SCALES = TILE * 256, RAW4_BYTES = RAW4_SCALES + TILE * 16;
+constexpr int RAW4_LPW = 4;                  // loads of a wave and tile: two of codes, one each of scales and RoPE
 __device__ __forceinline__ int nope_sw(int r) { return (r >> 2) & 3; }
 __device__ __forceinline__ int rope_sw(int r) { return (r >> 1) & 7; }
 
@@ -305,14 +309,17 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int32_t m, int32
     return w;
 }
 
+#include "dsa_chunk_list.h"
+
 // the kernel's argument block, in the constant address space
 typedef const __attribute__((address_space(4))) ChunkParams* Args;
 
-template <int FMT>
+// LIST: a block is 128 heads of one token, its positions the valid entries of the token's list
+template <int FMT, bool LIST = false>
 __global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(1, 1)))
 dsa_mla_chunk_tile_kernel(const ChunkParams p) {
-    constexpr bool FP8 = FMT == DSA_KV_FP8_656;
-    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[FP8 ? 2 * V_BYTES + 3 * RAW_BYTES : 3 * TILE_BYTES];
+    constexpr bool FP8 = FMT == DSA_KV_FP8_656, FP4 = FMT == DSA_KV_MXFP4;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[FP8 ? 2 * V_BYTES + 3 * RAW_BYTES : 3 * TILE_BYTES + (FP4 ? 2 * RAW4_BYTES : 0)];
     __shared__ __attribute__((aligned(16))) float s_scale[FP8 ? 2 * 4 * TILE : 4];    // [tile % 2][group][position]
     __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * P_BYTES];
     __shared__ __attribute__((aligned(16))) int32_t s_rows[SPAN];     // cache rows of a span's positions
@@ -334,23 +341,25 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hi = lane >> 5, r32 = lane & 31;
-    const Work work = find_work(p, BLOCK, CUS);
+    Work work;
+    if constexpr (LIST) work = list_work(p, BLOCK);
+    else work = find_work(p, BLOCK, CUS);
     const Block& blk = work.blk;
     const int split = work.split, per = work.per;
     if (blk.rows == 0) return;
     const int t_lo = blk.first + blk.r0 / p.H, t_hi = blk.first + (blk.r0 + blk.rows - 1) / p.H;
-    const int lim_lo = limit_in(p, blk, t_lo), lim_hi = limit_in(p, blk, t_hi);
-    const bool too_long = blk.len > p.max_len;
+    const int lim_lo = LIST ? p.topk : limit_in(p, blk, t_lo), lim_hi = LIST ? p.topk : limit_in(p, blk, t_hi);
+    const bool too_long = !LIST && blk.len > p.max_len;
     const int k0 = (int)min((int64_t)split * per, (int64_t)lim_hi);
     // (positions without a page end the sequence as far as its rows go)
-    const int k1 = too_long ? k0 : (int)min(min((int64_t)lim_hi, p.pages.limit), (int64_t)k0 + per);
-    // a split with no positions writes nothing: the combine does not read it
-    if (p.ns > 1 && k1 <= k0) return;
+    const int k1 = too_long ? k0 : (int)min(LIST ? (int64_t)lim_hi : min((int64_t)lim_hi, p.pages.limit), (int64_t)k0 + per);
+    // a split with no positions writes nothing: the combine does not read it (that of lists reads all)
+    if (!LIST && p.ns > 1 && k1 <= k0) return;
 
     // this lane's row (rows past the block's end are computed on its last one and not stored)
     const int row = blk.r0 + min(32 * wave + r32, blk.rows - 1);
     const int tok = blk.first + row / p.H, head = row % p.H;
-    const int limit = limit_in(p, blk, tok);
+    const int limit = LIST ? 0 : limit_in(p, blk, tok);
     // Q: lane (hi, r32) holds 8 dims of row r32 in qf[ks], the k-step's half `hi`: dims 16 ks + 8 hi .. +7; of
     // 656-byte rows, whose codes come 16 to a read, dims 32 j + 16 hi .. +15 in qf[2 j] and qf[2 j + 1] (the order
     // of the dims within a pair of k-steps is free as long as K has the same)
@@ -362,7 +371,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     {
         constexpr int PART = 12, LINE = 32 * PART, BYTES = 32 * LINE;
         static_assert(NWAVE * 2 * BYTES <= sizeof(s_tile) && KS == 3 * PART);
-        const uint64_t mine = (uint64_t)(p.q + (int64_t)tok * p.q_st + (int64_t)head * p.q_sh);
+        const uint64_t mine = (uint64_t)(p.q + (LIST ? token_at(tok, p.s_q, p.q_sb, p.q_st) : (int64_t)tok * p.q_st) + (int64_t)head * p.q_sh);
         const lds_ptr qb = T0 + wave * 2 * BYTES;
         uint64_t src[PART];
 #pragma unroll
@@ -399,8 +408,13 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // ---- positions [c0, c0 + SPAN) below k1 -> cache rows ----
     // A position without a row, and those from k1 on, are read as some row that exists (every
     // read is of the cache's own rows that the sequence attends) and masked.
-    int ntiles = 0;
+    int ntiles = 0, n_valid = 0;
     auto resolve = [&](int c0) {
+        if constexpr (LIST) {
+            n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc);
+            ntiles = (n_valid + TILE - 1) / TILE;
+            return;
+        }
         const Args a = args();
         const int64_t rows = a->rows;
         const int32_t bs = a->pages.block_size, shift = a->pages.shift;
@@ -467,9 +481,17 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     // 656-byte rows whose tile is one run of the cache (dense rows, pages of whole tiles): a load's source
     // is the run's start plus its number and the lane
     const bool runs = FP8 && p.row_bytes == FP8_ROW && (!p.pages.table || p.pages.block_size % TILE == 0);
+    // (400-byte rows: the lane's rows of its two loads of codes, of RoPE and of scales, each of the wave's own eight)
     auto load_rows = [&](int i) -> Rows {
         Rows g{};
-        if constexpr (!FP8) {
+        if constexpr (FP4) {
+            const LDS_AS int32_t* at = rows_l + i * TILE + 8 * wave;
+            const int ln = opaque(lane);
+            g.r[0] = at[ln >> 4];
+            g.r[1] = at[4 + (ln >> 4)];
+            g.r[2] = at[ln & 7];
+            g.rope = at[ln >> 3];
+        } else if constexpr (!FP8) {
             const LDS_AS int32_t* at = rows_l + i * TILE + 8 * wave;
             const u32x4 a = lds_ld<u32x4>((lds_cptr)at), b = lds_ld<u32x4>((lds_cptr)(at + 4));
 #pragma unroll
@@ -484,9 +506,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         }
         return g;
     };
-    auto issue = [&](const Rows& g, int slot) {
+    auto raw4_of = [&](int s) -> lds_ptr { return T0 + 3 * TILE_BYTES + s * RAW4_BYTES; };
+    auto issue = [&](const Rows& g, int slot, int raw4 = 0) {
         const int ln = opaque(lane);
-        if constexpr (!FP8) {
+        if constexpr (FP4) {
+            const lds_ptr rb = raw4_of(raw4);
+            auto from = [&](int32_t row, unsigned at) { return p.kv + ((uint64_t)(uint32_t)row * (uint32_t)p.row_bytes + at); };
+#pragma unroll
+            for (int k = 0; k < 2; ++k) lds_dma16(from(g.r[k], 16u * (ln & 15)), rb + 2048 * wave + 1024 * k);
+            const int r = 8 * wave + (ln >> 3);
+            lds_dma16(from(g.rope, FP4_ROPE_OFF + 16u * ((ln & 7) ^ rope_sw(r))), slot_of(slot) + ROPE_OFF + 8 * wave * 128);
+            if (ln < 8) lds_dma16(from(g.r[2], FP4_SCALE_OFF), rb + RAW4_SCALES + 128 * wave);
+        } else if constexpr (!FP8) {
             const lds_ptr tb = slot_of(slot);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -600,6 +631,23 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         }
     };
 
+    // ---- 400-byte rows: a wave converts the eight rows that it loaded, one at a time, 8 codes a lane ----
+    struct Codes {
+        unsigned c, e;
+    };
+    auto fp4_load = [&](lds_cptr rb, int k) -> Codes {
+        const int ln = opaque(lane), r = 8 * wave + k;
+        return {lds_ld<unsigned>(rb + 256 * r + 4 * ln), lds_ld<unsigned char>(rb + RAW4_SCALES + 16 * r + (ln >> 2))};
+    };
+    auto fp4_store = [&](lds_ptr tb, int k, const Codes& x) {
+        const int ln = opaque(lane), r = 8 * wave + k;
+        lds_st<u32x4>(tb + r * NOPE_STRIDE + 16 * (ln ^ nope_sw(r)), fp4_to_bf16(x.c, x.e));
+    };
+    auto fp4_convert = [&](lds_cptr rb, lds_ptr tb) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) fp4_store(tb, k, fp4_load(rb, k));
+    };
+
     const float c_s = p.scale_log2;
     auto landed = [&](auto keep) {
         wait_vm<decltype(keep)::value>();
@@ -700,15 +748,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         __builtin_amdgcn_sched_barrier(0);
         return s;
     };
-    auto masked = [&](int i, int c0) { return c0 + (i + 1) * TILE > lim_lo || __builtin_amdgcn_readfirstlane(s_skip[i]) != 0; };
+    auto masked = [&](int i, int c0) -> bool {
+        if constexpr (LIST) return (i + 1) * TILE > n_valid;
+        else return c0 + (i + 1) * TILE > lim_lo || __builtin_amdgcn_readfirstlane(s_skip[i]) != 0;
+    };
     // lane (hi, r32), register r: position 8 (r / 4) + 4 hi + r % 4 of the tile, row r32 of the wave
     auto mask = [&](f32x16& s, int i, int c0) {
-        const uint32_t skip = s_skip[i];
+        const uint32_t skip = LIST ? 0u : s_skip[i];
         const int pos0 = c0 + i * TILE;
         if (masked(i, c0)) {
             asm volatile("");
-            const uint32_t nan = s_nan[i];
-            const int left = limit - pos0, h4 = 4 * opaque(hi);
+            const uint32_t nan = LIST ? 0u : s_nan[i];
+            const int left = LIST ? n_valid - i * TILE : limit - pos0, h4 = 4 * opaque(hi);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int j = 8 * (r >> 2) + h4 + (r & 3);
@@ -761,7 +812,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         p_half(e, 0, px);
         p_half(e, 1, px);
     };
-    // (656-byte rows, with_exp: the next tile but one, raw at draw, goes to V's own buffer, piece by piece)
+    // (with_exp: the next tile but one, raw at draw, goes piece by piece to V's own buffer (656-byte rows) or to
+    // buffer dpar (400-byte rows; -1: there is none))
     auto pv = [&](lds_ptr vt, lds_cptr px, First& f, const f32x16& sn, float* en, auto with_exp, lds_cptr draw, int dpar) {
         const int ln = FP8 ? opaque(lane) : lane;
         u32x4 v_cur = {};
@@ -783,6 +835,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 else if (!FP8 && u == 0) v_nxt = v_block(vt, ln, 1, 0);
                 u32x2 codes;
                 if constexpr (FP8 && decltype(with_exp)::value) codes = deq_load(draw, 4 * u + m);
+                Codes c4;
+                if constexpr (FP4 && decltype(with_exp)::value)
+                    if (dpar >= 0) c4 = fp4_load(draw, 4 * u + m);
 #pragma unroll
                 for (int h = 0; h < NWAVE; ++h) {
                     mfma_o<FP8>(o[4 * m + h], v_cur, f.p[h]);
@@ -794,6 +849,8 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     en[r0 + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0 + 1], c_s, -m_ref));
                 }
                 if constexpr (FP8 && decltype(with_exp)::value) deq_store(vt, 4 * u + m, codes, ds);
+                if constexpr (FP4 && decltype(with_exp)::value)
+                    if (dpar >= 0) fp4_store(slot_of(dpar), 4 * u + m, c4);
                 v_cur = v_nxt;
             }
         }
@@ -819,7 +876,55 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             const int c0 = k0 + c * SPAN;
             resolve(c0);
             if (ntiles == 0) continue;
-            if constexpr (!FP8) {
+            if constexpr (FP4) {
+                // Iteration i: scores of tile i + 1, PV of tile i with the exponentials of tile i + 1 and the
+                // conversion of tile i + 2, and tile i + 3 on its way.  A wave reads no other's raw rows, so that
+                // its own wait is enough; the barrier shows what all have converted, and every wave's P.
+                auto next_landed = [&](bool more) {
+                    if (more) landed(std::integral_constant<int, RAW4_LPW>{}); else landed(std::integral_constant<int, 0>{});
+                };
+                issue(load_rows(0), 0, 0);
+                if (ntiles > 1) issue(load_rows(1), 1, 1);
+                next_landed(ntiles > 1);
+                fp4_convert(raw4_of(0), slot_of(0));
+                if (masked(0, c0)) scan(0, 0);
+                tile_barrier();
+                if (ntiles > 2) issue(load_rows(2), 2, 0);
+                f32x16 s0 = qk(slot_of(0), none);
+                mask(s0, 0, c0);
+                p_first(s0, PX);
+                if (ntiles > 1) {
+                    next_landed(ntiles > 2);
+                    fp4_convert(raw4_of(1), slot_of(1));
+                }
+                Rows next = load_rows(min(3, ntiles - 1));
+                int cur = 0;
+                for (int i = 0; i + 1 < ntiles; ++i) {
+                    const int nxt = cur == 2 ? 0 : cur + 1, far = nxt == 2 ? 0 : nxt + 1;
+                    if (masked(i + 1, c0)) scan(i + 1, nxt);
+                    tile_barrier();
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i + 3 < ntiles) issue(next, cur, (i + 1) & 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    First f;
+                    f32x16 sn = qk(slot_of(nxt), [&](int k) { read_first(f, k, slot_of(cur), PX + (i & 1) * P_BYTES); });
+                    if (i + 4 < ntiles) next = load_rows(i + 4);
+                    mask(sn, i + 1, c0);
+                    next_landed(i + 3 < ntiles);
+                    float en[16];
+                    pv(slot_of(cur), PX + (i & 1) * P_BYTES, f, sn, en, std::true_type{}, raw4_of(i & 1), i + 2 < ntiles ? far : -1);
+                    const lds_ptr px = PX + ((i + 1) & 1) * P_BYTES;
+                    p_half(en, 0, px);
+                    p_half(en, 1, px);
+                    cur = nxt;
+                }
+                tile_barrier();
+                float en[16];
+                First f;
+#pragma unroll
+                for (int k = 0; k < 5; ++k) read_first(f, k, slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES);
+                pv(slot_of(cur), PX + ((ntiles - 1) & 1) * P_BYTES, f, f32x16{}, en, std::false_type{}, T0, 0);
+            } else if constexpr (!FP8) {
             issue(load_rows(0), 0);
             if (ntiles > 1) issue(load_rows(1), 1);
             Rows next = load_rows(min(2, ntiles - 1));
@@ -953,6 +1058,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     tile_barrier();
                     s = qk8(raw_of(0), 0);
                 } else {
+                    if constexpr (FP4) fp4_convert(raw4_of(0), slot_of(0));
                     if (masked(i, c0)) scan(i, 0);
                     tile_barrier();
                     s = qk(slot_of(0), none);
@@ -998,7 +1104,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         constexpr int OUT_STRIDE = D_VO * 2 + 16;
         static_assert(32 * OUT_STRIDE <= TILE_BYTES, "the stage fits a tile buffer");
         const int st_w = opaque(r_ * OUT_STRIDE + 2 * d0);
-        const bool o16 = ((o_st | o_sh) & 7) == 0 && ((uintptr_t)out & 15) == 0;
+        const bool o16 = ((o_st | o_sh | (LIST ? a_->o_sb : 0)) & 7) == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll
         for (int h = 0; h < NWAVE; ++h) {
             const lds_ptr stg = slot_of(h & 1);
@@ -1022,7 +1128,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (r0 + k >= blk.rows) break;
-                __bf16* const dst = out + t * o_st + hh * o_sh + 8 * ln;
+                __bf16* const dst = out + (LIST ? token_at(t, a_->s_q, a_->o_sb, o_st) : (int64_t)t * o_st) + hh * o_sh + 8 * ln;
                 if (o16) {
                     *reinterpret_cast<u32x4*>(dst) = v[k];
                 } else {
@@ -1757,7 +1863,7 @@ float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int 
 Plan plan_of(const dsa_mla_chunk_args* a) {
     Plan best{};
     float least = INFINITY;
-    for (int n = a->kv_format == DSA_KV_MXFP4 ? 1 : 0; n < 2; ++n) {
+    for (int n = 0; n < 2; ++n) {
         const int32_t m = n ? NARROW : BLOCK;
         const int64_t blocks = dsa_seq::block_start(a->T, a->B, a->H, m, dsa_seq::common(a->H, m));
         for (const int c : COUNTS) {
@@ -1835,9 +1941,10 @@ int dsa_list::launch(const Call& c, bool tiled, hipStream_t stream) {
     p.B = c.B, p.s_q = c.s_q, p.T = c.B * c.s_q, p.H = c.H, p.topk = c.topk;
     p.causal = c.causal, p.causal_offset = c.causal_offset, p.scale_log2 = c.scale_log2;
     p.ns = c.ns, p.per_split = c.per_split;
-    const int32_t m = NARROW;
+    const int32_t m = tiled ? BLOCK : NARROW;
     const dim3 grid((unsigned)((int64_t)p.T * ((c.H + m - 1) / m)), (unsigned)c.ns);
-    hipLaunchKernelGGL(dsa_mla_fp4_narrow_kernel<true>, grid, dim3(NTHR), 0, stream, p);
+    if (tiled) hipLaunchKernelGGL((dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4, true>), grid, dim3(NTHR), 0, stream, p);
+    else hipLaunchKernelGGL(dsa_mla_fp4_narrow_kernel<true>, grid, dim3(NTHR), 0, stream, p);
     return hipGetLastError() == hipSuccess ? DSA_OK : DSA_ERR_HIP;
 }
 
@@ -1896,7 +2003,7 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
                       plan.deal ? 1u : (unsigned)p.ns);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
     const bool fp8 = a->kv_format == DSA_KV_FP8_656;
-    if (a->kv_format == DSA_KV_MXFP4) launch(dsa_mla_fp4_narrow_kernel<false>);
+    if (a->kv_format == DSA_KV_MXFP4) launch(narrow ? dsa_mla_fp4_narrow_kernel<false> : dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4>);
     else if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
     else if (fp8) launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
     else launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);

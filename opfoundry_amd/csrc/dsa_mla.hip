@@ -4041,7 +4041,7 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
 Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
     Choice best{PAIR, requested > 0 ? requested : 1};
     double least = -1.0;
-    for (Kern k : {PAIR}) {
+    for (Kern k : {WIDE, PAIR}) {
         const int64_t wgs = tokens * groups_of(k, H);
         const int counts[] = {1, one_round_splits(wgs, by_len), one_round_splits(wgs, by_len, k == PAIR ? 2 * CUS : CUS)};
         for (int ns : counts) {
