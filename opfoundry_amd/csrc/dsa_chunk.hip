@@ -250,7 +250,7 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int32_t m, int32
     // Blocks of one sequence follow one another and read the same rows: four at a time on one XCD
     // (workgroups go to the eight in turn).
     uint32_t x = blockIdx.x;
-    if (x < (gridDim.x & ~31u) && (p.dealt || m == NARROW)) x = (x & ~31u) | (x & 7) << 2 | ((x >> 3) & 3);
+    if (x < (gridDim.x & ~31u) && (p.dealt || m != BLOCK)) x = (x & ~31u) | (x & 7) << 2 | ((x >> 3) & 3);
     // (the last block first: later tokens attend more, and the long ones must not come last)
     if (!p.dealt) return {find_block(p, (int64_t)gridDim.x - 1 - x, m), (int32_t)blockIdx.y, p.per_split};
     const int lane = threadIdx.x & 63, i = min(lane, p.B - 1);
@@ -1819,10 +1819,12 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 // the two sides of it, us: one token of 128 heads over 1501 rows, 128-row blocks 25.2, 32-row 17.7;
 // 256 of 16 heads over 4096 302 and 217; 200 of 128 heads over 1000 78 and 120; 512 tokens of
 // 16 heads over the same 4096 rows 90 (4 splits) and 120.
-constexpr Kernel KERNELS[3][2] = {       // [bf16, 656-byte, 400-byte rows][narrow]
-    {{6.3f, 1.83f, 0.0f}, {6.4f, 1.15f, 1.81f}},
-    {{10.6f, 2.47f, 0.0f}, {8.3f, 1.48f, 2.07f}},
-    {{6.3f, 1.83f, 0.0f}, {6.4f, 1.0f, 1.3f}},
+constexpr int KINDS = 3;
+constexpr int32_t KIND_ROWS[KINDS] = {BLOCK, NARROW, 16};          // rows of a workgroup
+constexpr Kernel KERNELS[3][KINDS] = {       // [bf16, 656-byte, 400-byte rows]; pair: two share a CU
+    {{6.3f, 1.83f, 0.0f}, {6.4f, 1.15f, 1.81f}, {}},
+    {{10.6f, 2.47f, 0.0f}, {8.3f, 1.48f, 2.07f}, {}},
+    {{8.0f, 2.15f, 0.0f}, {8.0f, 0.75f, 0.0f}, {8.0f, 0.58f, 0.84f}},
 };
 int kind_of(int fmt) { return fmt == DSA_KV_BF16 ? 0 : fmt == DSA_KV_FP8_656 ? 1 : 2; }
 constexpr int ROW_BYTES[] = {DSA_MLA_BF16_ROW_BYTES, DSA_MLA_FP8_ROW_BYTES, DSA_MLA_FP4_ROW_BYTES};
@@ -1839,21 +1841,20 @@ constexpr int64_t FEW_ROWS = 1024;
 constexpr int FOUR_FROM = 5;
 
 struct Plan {
-    bool narrow;
+    int kind;
     int ns;              // at most
     int32_t per;         // positions of a split
     bool deal;           // the device chooses the split's positions
 };
 
-float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int ns) {
-    const Kernel& k = KERNELS[kind_of(a->kv_format)][narrow];
+float expected_us(const dsa_mla_chunk_args* a, const Kernel& k, int64_t blocks, int ns) {
     const int64_t tiles = (a->max_kv_len + (int64_t)TILE - 1) / TILE, each = (tiles + ns - 1) / ns;
     const float groups = (float)blocks * ns;
     auto in_rounds = [](float us, float rounds) {
         return us * (rounds <= 1.0f ? 1.0f : rounds <= 3.0f ? std::ceil(rounds) : rounds + 0.5f);
     };
-    float us = narrow && groups > CUS ? in_rounds(k.start + each * k.pair, groups / (2 * CUS))
-                                      : in_rounds(k.start + each * k.tile, groups / CUS);
+    float us = k.pair > 0.0f && groups > CUS ? in_rounds(k.start + each * k.pair, groups / (2 * CUS))
+                                            : in_rounds(k.start + each * k.tile, groups / CUS);
     const float row = ROW_BYTES[kind_of(a->kv_format)];
     us = std::max(us, FIRST_US + (float)a->B * a->max_kv_len * row / BYTES_US);
     if (ns > 1) us += JOIN_US + (float)ns * a->T * a->H * (2 * 4 * (D_VO + 1)) / PART_BYTES_US;
@@ -1863,16 +1864,19 @@ float expected_us(const dsa_mla_chunk_args* a, bool narrow, int64_t blocks, int 
 Plan plan_of(const dsa_mla_chunk_args* a) {
     Plan best{};
     float least = INFINITY;
-    for (int n = 0; n < 2; ++n) {
-        const int32_t m = n ? NARROW : BLOCK;
+    for (int n = 0; n < KINDS; ++n) {
+        const Kernel& k = KERNELS[kind_of(a->kv_format)][n];
+        if (k.tile == 0.0f) continue;
+        const int32_t m = KIND_ROWS[n];
         const int64_t blocks = dsa_seq::block_start(a->T, a->B, a->H, m, dsa_seq::common(a->H, m));
+        if (blocks > MAX_GROUPS) continue;
         for (const int c : COUNTS) {
             const int ns = a->num_splits ? a->num_splits : c;
             // (a split of fewer positions than a tile is none; 64 splits of a grid's y extent)
             if (ns > 1 && !a->num_splits && (int64_t)a->max_kv_len < (int64_t)ns * TILE) break;
             if (ns > 1 && (int64_t)a->T * a->H > MAX_SPLIT_ROWS) break;
-            const float us = expected_us(a, n != 0, blocks, ns);
-            if (us < least) least = us, best.narrow = n != 0, best.ns = ns;
+            const float us = expected_us(a, k, blocks, ns);
+            if (us < least) least = us, best.kind = n, best.ns = ns;
             if (a->num_splits) break;
         }
     }
@@ -1926,7 +1930,7 @@ int validate(const dsa_mla_chunk_args* a) {
 
 }  // namespace
 
-int dsa_list::launch(const Call& c, bool tiled, hipStream_t stream) {
+int dsa_list::launch(const Call& c, int heads, hipStream_t stream) {
     ChunkParams p{};
     p.q = (const __bf16*)c.q;
     p.q_sb = c.q_sb, p.q_st = c.q_st, p.q_sh = c.q_sh;
@@ -1941,10 +1945,11 @@ int dsa_list::launch(const Call& c, bool tiled, hipStream_t stream) {
     p.B = c.B, p.s_q = c.s_q, p.T = c.B * c.s_q, p.H = c.H, p.topk = c.topk;
     p.causal = c.causal, p.causal_offset = c.causal_offset, p.scale_log2 = c.scale_log2;
     p.ns = c.ns, p.per_split = c.per_split;
-    const int32_t m = tiled ? BLOCK : NARROW;
-    const dim3 grid((unsigned)((int64_t)p.T * ((c.H + m - 1) / m)), (unsigned)c.ns);
-    if (tiled) hipLaunchKernelGGL((dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4, true>), grid, dim3(NTHR), 0, stream, p);
-    else hipLaunchKernelGGL(dsa_mla_fp4_narrow_kernel<true>, grid, dim3(NTHR), 0, stream, p);
+    const dim3 grid((unsigned)((int64_t)p.T * ((c.H + heads - 1) / heads)), (unsigned)c.ns);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(NTHR), 0, stream, p); };
+    if (heads == BLOCK) launch(dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4, true>);
+    else if (heads == 32) launch(dsa_mla_fp4_few_kernel<2, true>);
+    else launch(dsa_mla_fp4_few_kernel<1, true>);
     return hipGetLastError() == hipSuccess ? DSA_OK : DSA_ERR_HIP;
 }
 
@@ -1990,20 +1995,21 @@ int dsa_mla_chunk(const dsa_mla_chunk_args* a, void* ws, size_t ws_bytes, void* 
     p.part_o = (float*)ws;
     p.part_lse = p.part_o + (size_t)p.ns * a->T * a->H * D_VO;
     p.dealt = plan.deal ? (int32_t*)(p.part_lse + (size_t)p.ns * a->T * a->H) : nullptr;
-    p.kernel = KERNELS[kind_of(a->kv_format)][plan.narrow];
+    p.kernel = KERNELS[kind_of(a->kv_format)][plan.kind];
     p.T = a->T, p.B = a->B, p.H = a->H, p.causal = a->causal, p.max_len = a->max_kv_len;
     p.scale_log2 = a->sm_scale * LOG2E;
-    const bool narrow = plan.narrow;
+    const bool narrow = KIND_ROWS[plan.kind] == NARROW;
     const bool runs = !a->block_table || a->block_size % TILE == 0;
-    const int32_t m = narrow ? NARROW : BLOCK;
+    const int32_t m = KIND_ROWS[plan.kind];
     p.common = dsa_seq::common(a->H, m);
     const int64_t most = dsa_seq::block_start(a->T, a->B, a->H, m, p.common);
-    const int64_t places = plan.narrow ? 2 * CUS : CUS;
+    const int64_t places = p.kernel.pair > 0.0f ? 2 * CUS : CUS;
     const dim3 blocks((unsigned)(plan.deal ? std::min(most * p.ns, most <= places / 4 ? places : 3 * places + most) : most),
                       plan.deal ? 1u : (unsigned)p.ns);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, blocks, dim3(NTHR), 0, (hipStream_t)stream, p); };
     const bool fp8 = a->kv_format == DSA_KV_FP8_656;
-    if (a->kv_format == DSA_KV_MXFP4) launch(narrow ? dsa_mla_fp4_narrow_kernel<false> : dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4>);
+    if (a->kv_format == DSA_KV_MXFP4)
+        launch(m == BLOCK ? dsa_mla_chunk_tile_kernel<DSA_KV_MXFP4> : narrow ? dsa_mla_fp4_few_kernel<2, false> : dsa_mla_fp4_few_kernel<1, false>);
     else if (!narrow) launch(fp8 ? dsa_mla_chunk_tile_kernel<DSA_KV_FP8_656> : dsa_mla_chunk_tile_kernel<DSA_KV_BF16>);
     else if (fp8) launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_FP8_656, false>);
     else launch(runs ? dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, true> : dsa_mla_chunk_narrow_kernel<DSA_KV_BF16, false>);

@@ -1,32 +1,49 @@
-// dsa_chunk_fp4.h - the narrow kernel of DSA_KV_MXFP4 rows: dense attention of a
+// dsa_chunk_fp4.h - the kernels for few rows on DSA_KV_MXFP4 rows: dense attention of a
 // chunk's tokens (include/dsa_chunk.h) and attention over lists of positions
 // (dsa_mla_decode, dsa_mla_prefill).  Part of dsa_chunk.hip.
 
 // ---------------------------------------------------------------------------
-// 32 rows (heads of tokens) a workgroup, two workgroups a CU, tiles of 32 positions.
-//   K      wave w: 16 positions (half w % 2) in its registers straight from the cache, two tiles
-//          ahead: a row's codes are 256 bytes, so a lane's 7 loads hold its quarter of a row
-//   QK^T   wave w: those 16 positions x 16 rows (half w / 2), 16x16x32, the codes converted between
-//          the matrix instructions and written to LDS from there, half of the dims by each of the two
-//          waves that hold them: the tile is V of the next step, and K is never read from LDS
-//   P, PV  as in dsa_mla_chunk_narrow_kernel; V and P in two buffers, so that a tile takes one barrier
+// 16 QB rows (heads of tokens) a workgroup, tiles of 64 positions.
+//   K      wave w: positions 16 w .. +15 of the tile in its registers, straight from the cache, two
+//          tiles ahead: a row's codes are 256 bytes, so a lane's 7 loads hold a quarter of a row
+//   QK^T   wave w: those 16 positions x all rows, 16x16x32.  The codes are converted between the matrix
+//          instructions, once, and written to LDS from there: the tile is V, and K is never read from LDS
+//   P      exp2 against a fixed reference, bf16, exchanged through LDS
+//   PV     wave w: O^T[dims 128 w .. +127 x all rows]
+// QB = 1: 16 rows, two workgroups a CU, one V buffer, two barriers a tile; PV in 16x16x32.
+// QB = 2: 32 rows, one workgroup a CU (Q alone takes 144 registers), two V buffers, one barrier a tile.
 // ---------------------------------------------------------------------------
+constexpr int FTILE = 64;                    // positions of a tile
+// V in LDS: rows of 1 KB, piece c of row r at c ^ fsw(r).  A write takes eight rows' pieces of one number at a time,
+// which meet no bank of 32 twice (the low three bits tell the rows apart); half a transposed read two pieces of each of
+// eight rows, or four of each of four, no bank of 64 (the upper three, or two).
+__device__ __forceinline__ int fsw(int r) { return 9 * (r & 1) + 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1); }
+template <int QB>
+struct FewLay {
+    static constexpr int ROWS = 16 * QB;
+    static constexpr int VT = FTILE * NSTRIDE, PT = FTILE * ROWS * 2;
+    static constexpr int NB = QB == 1 ? 1 : 2;                            // V and P buffers
+    static constexpr int PLACES = QB == 1 ? 2 * CUS : CUS;
+};
 
-template <bool LIST>
-__global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(2, 2)))
-dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
-    constexpr int VT = TILE * NSTRIDE, PT = 2 * 2 * NARROW * 16;
-    // two tiles of V, then two of P: [tile % 2][u][hi][row] x 8 positions
-    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[2 * VT + 2 * PT];
+template <int QB, bool LIST>
+__global__ void __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(QB == 1 ? 2 : 1, QB == 1 ? 2 : 1)))
+dsa_mla_fp4_few_kernel(const ChunkParams p) {
+    using L = FewLay<QB>;
+    constexpr int VT = L::VT, PT = L::PT, NB = L::NB, ROWS = L::ROWS;
+    // NB tiles of V, then NB of P
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[NB * (VT + PT)];
     __shared__ __attribute__((aligned(16))) int32_t s_rows[SPAN];
-    __shared__ uint32_t s_skip[SPAN / TILE];                               // bit j: position j of the tile has no row
-    __shared__ float s_top[2][NARROW];
+    __shared__ uint32_t s_skip[SPAN / TILE];                               // bit j: position j of 32 has no row
+    __shared__ float s_top[NWAVE][ROWS];
     __shared__ int32_t s_misc[4];            // [0] a row that may be read, [1] again, [2] O may have passed fp32, [3] it has
-    const lds_ptr T0 = (lds_ptr)s_tile, PX = T0 + 2 * VT;
+    const lds_ptr T0 = (lds_ptr)s_tile, PX = T0 + NB * VT;
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Work work = LIST ? list_work(p, NARROW) : find_work(p, NARROW, 2 * CUS);
+    Work work;
+    if constexpr (LIST) work = list_work(p, ROWS);
+    else work = find_work(p, ROWS, L::PLACES);
     const Block& blk = work.blk;
     const int split = work.split, per = work.per;
     if (blk.rows == 0) return;
@@ -38,20 +55,21 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
     const int k1 = too_long ? k0 : (int)min(LIST ? (int64_t)lim_hi : min((int64_t)lim_hi, p.pages.limit), (int64_t)k0 + per);
     if (!LIST && p.ns > 1 && k1 <= k0) return;      // (the join knows; that of lists reads every split)
 
-    // scores: this lane's row of the 16 of its wave, its positions 16 half + 4 q .. +3 of a tile, and the dims
-    // 128 j + 32 q .. +31 (j < 4) and 512 + 32 j + 8 q .. +7 (j < 2) of a product's operands
-    const int half = wave & 1, rh = wave >> 1, q = lane >> 4;
-    const int my = 16 * rh + (lane & 15);
-    const int row = blk.r0 + min(my, blk.rows - 1);
-    const int tok = blk.first + row / p.H;
-    const int limit = LIST ? 0 : limit_in(p, blk, tok);
-    u32x4 qf[KS / 2];
-    {
+    // scores: this lane's row of each block of 16, its positions 16 wave + 4 q .. +3 of a tile, and the dims
+    // 128 q .. +127 and 512 + 32 j + 8 q .. +7 (j < 2) of a product's operands
+    const int q = lane >> 4;
+    int limit[QB];
+    u32x4 qf[QB][KS / 2];
+#pragma unroll
+    for (int h = 0; h < QB; ++h) {
+        const int row = blk.r0 + min(16 * h + (lane & 15), blk.rows - 1);
+        const int tok = blk.first + row / p.H;
+        limit[h] = LIST ? 0 : limit_in(p, blk, tok);
         const __bf16* qp = p.q + (LIST ? token_at(tok, p.s_q, p.q_sb, p.q_st) : (int64_t)tok * p.q_st) + (int64_t)(row % p.H) * p.q_sh;
 #pragma unroll
         for (int ks = 0; ks < KS / 2; ++ks) {
-            const int d = ks < 16 ? 128 * (ks >> 2) + 32 * q + 8 * (ks & 3) : 32 * ks + 8 * q;
-            qf[ks] = *reinterpret_cast<const u32x4*>(qp + d);
+            const int d = ks < 16 ? 128 * q + 8 * ks : 32 * ks + 8 * q;
+            qf[h][ks] = *reinterpret_cast<const u32x4*>(qp + d);
         }
     }
 
@@ -60,7 +78,7 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
     auto resolve = [&](int c0) {
         if constexpr (LIST) {
             n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc);
-            ntiles = (n_valid + TILE - 1) / TILE;
+            ntiles = (n_valid + FTILE - 1) / FTILE;
         } else {
             const int tid = 64 * wave + fresh_lane();
             const int at = c0 + 8 * tid;
@@ -105,29 +123,27 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
             for (int e = 0; e < 8; e += 4)
                 *reinterpret_cast<int4*>(&s_rows[8 * tid + e]) = int4{id[e], id[e + 1], id[e + 2], id[e + 3]};
             reinterpret_cast<unsigned char*>(s_skip)[tid] = (unsigned char)skip;
-            ntiles = safe < 0 ? 0 : (min(k1 - c0, SPAN) + TILE - 1) / TILE;
+            ntiles = safe < 0 ? 0 : (min(k1 - c0, SPAN) + FTILE - 1) / FTILE;
             __syncthreads();
         }
     };
 
-    // This lane's part of a tile: row c16 of its wave's 16
+    // This lane's quarter of row lane % 16 of its wave's 16
     struct Raw {
-        u32x4 c[4];            // codes of dims 128 j + 32 q .. +31: block 4 j + q of its row
-        u32x4 s;               // the row's scales; byte q of dword j is that block's
-        u32x4 r[2];            // RoPE
+        u32x4 v[6];            // codes of dims 128 q + 32 j .. +31 (j < 4), RoPE values 32 (j - 4) + 8 q .. +7
+        unsigned s;            // the codes' four scales
     };
     auto fetch = [&](Raw& x, int i) {
-        const int ln = opaque(lane);
-        const uint32_t id = (uint32_t)s_rows[i * TILE + 16 * half + (ln & 15)];
+        const int ln = opaque(lane), lq = ln >> 4;
+        const uint32_t id = (uint32_t)s_rows[i * FTILE + 16 * wave + (ln & 15)];
         const unsigned char* const at = p.kv + (uint64_t)id * (uint32_t)p.row_bytes;
-        const unsigned char* const mine = at + 16 * (ln >> 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.c[j] = *reinterpret_cast<const u32x4*>(mine + 64 * j);
-        x.s = *reinterpret_cast<const u32x4*>(at + FP4_SCALE_OFF);
+        for (int j = 0; j < 4; ++j) x.v[j] = *reinterpret_cast<const u32x4*>(at + 64 * lq + 16 * j);
+        x.s = *reinterpret_cast<const unsigned*>(at + FP4_SCALE_OFF + 4 * lq);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) x.r[j] = *reinterpret_cast<const u32x4*>(mine + FP4_ROPE_OFF + 64 * j);
+        for (int j = 4; j < 6; ++j) x.v[j] = *reinterpret_cast<const u32x4*>(at + FP4_ROPE_OFF + 64 * (j - 4) + 16 * lq);
     };
-    auto scale_of = [&](const Raw& x, int j) -> unsigned { return (x.s[j] >> (8 * (opaque(lane) >> 4))) & 0xFFu; };
+    auto scale_of = [&](const Raw& x, int j) -> unsigned { return (x.s >> (8 * j)) & 0xFFu; };
     // (as in the other kernels: NoPE values that are not finite must not reach rows that do not attend them.  Only
     // scale bytes from 253 on give any.)  Bit r: those of this wave's position r, which are cleared.
     auto scan = [&](Raw& x) -> uint32_t {
@@ -139,119 +155,169 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const u32x4 v = fp4_to_bf16(x.c[j][s], scale_of(x, j));
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 v = fp4_to_bf16(x.v[j][i], scale_of(x, j));
 #pragma unroll
                 for (int w = 0; w < 4; ++w) odd |= (v[w] & 0x7F800000u) == 0x7F800000u || (v[w] & 0x7F80u) == 0x7F80u;
             }
         const uint64_t who = __builtin_amdgcn_ballot_w64(odd);
         const uint32_t two = (uint32_t)who | (uint32_t)(who >> 32), rows = (two | two >> 16) & 0xFFFFu;
         if ((rows >> (lane & 15)) & 1) {
-            x.s = u32x4{0, 0, 0, 0};
+            x.s = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x.c[j] = u32x4{0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) x.v[j] = u32x4{0, 0, 0, 0};
         }
         return rows;
     };
 
     const float c_s = p.scale_log2;
-    f32x16 o[4];
-    float m_ref = 0.0f, l_lane = 0.0f;
-    bool any = false;
+    float m_ref[QB] = {}, l_lane[QB] = {};
+    bool any[QB] = {};
 
-    // S^T[4 positions of this lane x its row]; the converted codes go to V's tile at vt
-    auto qk = [&](const Raw& x, lds_ptr vt) -> f32x4 {
-        const int ln = opaque(lane), lr = 16 * half + (ln & 15);
-        const lds_ptr vr = vt + lr * NSTRIDE;
-        const int piece = 16 * ((4 * (ln >> 4)) ^ nsw(lr));
-        f32x4 a = {}, b = {};
+    // S^T[4 positions of this lane x its rows]; the converted codes go to V's tile at vt
+    auto qk = [&](const Raw& x, lds_ptr vt, f32x4 (&s)[QB]) {
+        const int ln = QB == 1 ? lane : opaque(lane), lr = 16 * wave + (ln & 15);
+        const lds_ptr vr = vt + lr * NSTRIDE + 256 * (ln >> 4);
+        const int sw = 16 * fsw(lr);
+        f32x4 a[2] = {};                       // two chains: the blocks of rows, or the even and odd k-steps
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             __builtin_amdgcn_sched_barrier(0);
             const unsigned e = scale_of(x, j);
-            u32x4 k[4];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                k[s] = fp4_to_bf16(x.c[j][s], e);
-                if (s & 1) b = mfma16(k[s], qf[4 * j + s], b);
-                else a = mfma16(k[s], qf[4 * j + s], a);
-            }
-            if (rh == (j >> 1)) {
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 k = fp4_to_bf16(x.v[j][i], e);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) lds_st<u32x4>(vr + 256 * j + (piece ^ (16 * s)), k[s]);
+                for (int h = 0; h < QB; ++h) {
+                    f32x4& c = a[QB == 2 ? h : i & 1];
+                    c = mfma16(k, qf[h][4 * j + i], c);
+                }
+                lds_st<u32x4>(vr + (sw ^ (16 * (4 * j + i))), k);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        a = mfma16(x.r[0], qf[16], a);
-        b = mfma16(x.r[1], qf[17], b);
-        return a + b;
-    };
-    auto masked = [&](int i, int c0) -> bool {
-        if constexpr (LIST) return (i + 1) * TILE > n_valid;
-        else return c0 + (i + 1) * TILE > lim_lo || __builtin_amdgcn_readfirstlane(s_skip[i]) != 0;
-    };
-    auto mask = [&](f32x4& s, uint32_t nan, int i, int c0) {
-        const uint32_t skip = LIST ? 0u : s_skip[i];
-        const int left = LIST ? n_valid - i * TILE : limit - (c0 + i * TILE), q4 = opaque(lane) >> 4 << 2;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int at = q4 + r, j = 16 * half + at;
-            const bool on = j < left && !((skip >> j) & 1);
-            any = any || on;
-            const float v = (nan >> at) & 1 ? __builtin_nanf("") : s[r];
-            s[r] = on ? v : -INFINITY;
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < QB; ++h) {
+                f32x4& c = a[QB == 2 ? h : i];
+                c = mfma16(x.v[4 + i], qf[h][16 + i], c);
+            }
+        if constexpr (QB == 2) s[0] = a[0], s[1] = a[1];
+        else s[0] = a[0] + a[1];
+    };
+    // does every row of the block attend all of this wave's positions of tile i?
+    auto skips = [&](int i) -> uint32_t {
+        return LIST ? 0u : (__builtin_amdgcn_readfirstlane(s_skip[2 * i + (wave >> 1)]) >> (16 * (wave & 1))) & 0xFFFFu;
     };
     // scores of tile i (its codes to vt), masked
-    auto scores = [&](Raw& x, int i, int c0, lds_ptr vt) -> f32x4 {
-        const bool m = masked(i, c0);
+    auto scores = [&](Raw& x, int i, int c0, lds_ptr vt, f32x4 (&s)[QB]) {
+        const uint32_t skip = skips(i);
+        const int at = i * FTILE + 16 * wave;
+        const bool m = at + 16 > (LIST ? n_valid : lim_lo - c0) || skip != 0;
         uint32_t nan = 0;
         if (!LIST && m) nan = scan(x);
-        f32x4 s = qk(x, vt);
-        if (m) mask(s, nan, i, c0);
-        else any = true;
-        return s;
-    };
-    // the largest of a row's scores in both halves of the tile
-    auto top_of = [&](const f32x4& s) -> float {
-        float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        if (q == 0) s_top[half][my] = m;
-        __syncthreads();
-        m = fmaxf(s_top[0][my], s_top[1][my]);
-        __syncthreads();
-        return m;
-    };
-    auto p_out = [&](const f32x4& s, lds_ptr px) {
-        f32x4 e;
+        qk(x, vt, s);
+        if (m) {
+            const int q4 = opaque(lane) >> 4 << 2;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c_s, -m_ref));
-        l_lane += (e[0] + e[1]) + (e[2] + e[3]);
-        // (the order of a lane's eight positions in the product: 4 hi .. +3, then 8 + 4 hi .. +3)
-        lds_st<u32x2>(px + ((2 * half + (q & 1)) * NARROW + my) * 16 + 8 * (q >> 1),
-                      __builtin_bit_cast(u32x2, __builtin_convertvector(e, bf16x4)));
+            for (int h = 0; h < QB; ++h) {
+                const int left = (LIST ? n_valid : limit[h] - c0) - at;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = q4 + r;
+                    const bool on = j < left && !((skip >> j) & 1);
+                    any[h] = any[h] || on;
+                    const float v = (nan >> j) & 1 ? __builtin_nanf("") : s[h][r];
+                    s[h][r] = on ? v : -INFINITY;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < QB; ++h) any[h] = true;
+        }
     };
+    // over the lanes that share a row, then over the waves
+    auto lanes = [&](float v, auto f) {
+        v = f(v, __shfl_xor(v, 16, 64));
+        return f(v, __shfl_xor(v, 32, 64));
+    };
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
+    auto put = [&](int h, float v) {
+        if (opaque(lane) < 16) s_top[wave][16 * h + opaque(lane)] = v;
+    };
+    auto got = [&](int w, int h) { return s_top[w][16 * h + (opaque(lane) & 15)]; };
+    // the largest of a row's scores in the tile
+    auto top_of = [&](const f32x4 (&s)[QB], float (&top)[QB]) {
+#pragma unroll
+        for (int h = 0; h < QB; ++h) put(h, lanes(fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3])), larger));
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < QB; ++h) top[h] = fmaxf(fmaxf(got(0, h), got(1, h)), fmaxf(got(2, h), got(3, h)));
+        __syncthreads();
+    };
+    // P of wave w's positions: of QB = 2 the half k = w of a 32x32x16 step pair, lane (hi, row) 8 positions:
+    // 4 hi .. +3, then 8 + 4 hi .. +3; of QB = 1 half w & 1 of 16x16x32 step w / 2, lane (q, row) 8 positions: 4 q .. +3
+    // of either wave
+    auto p_out = [&](const f32x4 (&s)[QB], lds_ptr px) {
+        const int ln = opaque(lane), lq = ln >> 4;
+#pragma unroll
+        for (int h = 0; h < QB; ++h) {
+            f32x4 e;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][r], c_s, -m_ref[h]));
+            l_lane[h] += (e[0] + e[1]) + (e[2] + e[3]);
+            const lds_ptr to = QB == 1 ? px + 1024 * (wave >> 1) + 8 * (wave & 1) + 16 * ln
+                                       : px + ((2 * wave + (lq & 1)) * ROWS + 16 * h + (ln & 15)) * 16 + 8 * (lq >> 1);
+            lds_st<u32x2>(to, __builtin_bit_cast(u32x2, __builtin_convertvector(e, bf16x4)));
+        }
+    };
+    // V^T by transposed reads: a group of 16 lanes reads four rows' 16 dims, and a lane then has one dim of four
+    // positions
+    f32x16 o[QB == 2 ? 4 : 1];                 // QB = 2: dims 128 wave + 32 m .. +31
+    f32x4 o16[QB == 1 ? 8 : 1];                // QB = 1: dims 128 wave + 16 m .. +15
+    // (QB = 1: the LDS addresses are kept in registers through the loop, as far as there are any left)
     auto pv = [&](lds_cptr vt, lds_cptr px) {
-        const int ln = opaque(lane), lhi = ln >> 5;
+        const int ln = QB == 1 && LIST ? lane : opaque(lane);
         const int g16 = ln >> 4, i16 = ln & 15, rr = i16 >> 2, pp = i16 & 3;
-        const int vx = 2 * (g16 & 1) + (pp >> 1);
-        const lds_cptr v0 = vt + (4 * lhi + rr) * NSTRIDE + 256 * wave + 8 * (pp & 1);
-        auto v_frag = [&](int i) -> u32x4 {
-            const lds_cptr at = v0 + 16 * (i >> 2) * NSTRIDE;
-            const int c = (4 * (i & 3) + vx) ^ (4 * rr + lhi);                // row 8 further on: nsw + 2
-            const s16x4 va = lds_read_tr16(at + 16 * c), vb = lds_read_tr16(at + 8 * NSTRIDE + 16 * (c ^ 2));
-            return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
-        u32x4 pb[2], v[3];
-        pb[0] = lds_ld<u32x4>(px + (lhi * NARROW + (ln & 31)) * 16);
+        constexpr int N = 16, AHEAD = 3;
+        u32x4 v[AHEAD], pb[QB == 2 ? 4 : 2];
+        if constexpr (QB == 2) {
+            const int lhi = ln >> 5, vx = 2 * (g16 & 1) + (pp >> 1);
+            const lds_cptr v0 = vt + (4 * lhi + rr) * NSTRIDE + 256 * wave + 8 * (pp & 1);
+            auto v_frag = [&](int i) -> u32x4 {
+                const lds_cptr at = v0 + 16 * (i >> 2) * NSTRIDE;
+                const int c = (4 * (i & 3) + vx) ^ fsw(4 * lhi + rr);         // (row 8 further on: the same)
+                const s16x4 va = lds_read_tr16(at + 16 * c), vb = lds_read_tr16(at + 8 * NSTRIDE + 16 * c);
+                return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
 #pragma unroll
-        for (int i = 0; i < 3; ++i) v[i] = v_frag(i);
-        pb[1] = lds_ld<u32x4>(px + ((2 + lhi) * NARROW + (ln & 31)) * 16);
+            for (int u = 0; u < 4; ++u) pb[u] = lds_ld<u32x4>(px + ((2 * u + lhi) * ROWS + (ln & 31)) * 16);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            o[i & 3] = mfma_bf16(v[i % 3], pb[i >> 2], o[i & 3]);
-            if (i + 3 < 8) v[i % 3] = v_frag(i + 3);
+            for (int i = 0; i < AHEAD; ++i) v[i] = v_frag(i);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                o[i & 3] = mfma_bf16(v[i % AHEAD], pb[i >> 2], o[i & 3]);
+                if (i + AHEAD < N) v[i % AHEAD] = v_frag(i + AHEAD);
+            }
+        } else {
+            const lds_cptr v0 = vt + (4 * g16 + rr) * NSTRIDE + 256 * wave + 8 * (pp & 1);
+            auto v_frag = [&](int i) -> u32x4 {
+                const lds_cptr at = v0 + 32 * (i >> 3) * NSTRIDE + 16 * ((2 * (i & 7) + (pp >> 1)) ^ fsw(4 * g16 + rr));
+                const s16x4 va = lds_read_tr16(at), vb = lds_read_tr16(at + 16 * NSTRIDE);      // (the same swizzle)
+                return __builtin_bit_cast(u32x4, __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pb[u] = lds_ld<u32x4>(px + 1024 * u + 16 * ln);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) v[i] = v_frag(i);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                o16[i & 7] = mfma16(v[i % AHEAD], pb[i >> 3], o16[i & 7]);
+                if (i + AHEAD < N) v[i % AHEAD] = v_frag(i + AHEAD);
+            }
         }
     };
 
@@ -260,125 +326,180 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
     bool first = true, again = false;
     // scores and probabilities of tile i, then its registers take tile i + 2
     auto take = [&](Raw& x, int i, int c0) {
-        const f32x4 s = scores(x, i, c0, T0 + (i & 1) * VT);
-        if (i + 2 < ntiles) fetch(x, i + 2);
+        // (one V buffer: every wave is done with the tile before)
+        if constexpr (NB == 1) tile_barrier();
+        f32x4 s[QB];
+        scores(x, i, c0, T0 + (NB == 1 ? 0 : (i & 1) * VT), s);
+        // (past the last tile: that one again.  Behind a branch, the wait for the tile before would have to
+        // take in these loads too.)
+        fetch(x, min(i + 2, ntiles - 1));
         if (first) {
-            const float top = top_of(s) * c_s;
-            m_ref = top == -INFINITY ? 0.0f : top;
-            m_ref -= (float)lift_of<false>(k1 - k0, false);
+            float top[QB];
+            top_of(s, top);
+#pragma unroll
+            for (int h = 0; h < QB; ++h) {
+                m_ref[h] = top[h] == -INFINITY ? 0.0f : top[h] * c_s;
+                m_ref[h] -= (float)lift_of<false>(k1 - k0, false);
+            }
             first = false;
         }
-        p_out(s, PX + (i & 1) * PT);
-        // (every wave's V and P of tile i are there, and every wave is done with tile i - 1)
+        p_out(s, PX + (NB == 1 ? 0 : (i & 1) * PT));
+        // (every wave's V and P of tile i are there; two buffers: and every wave is done with tile i - 1)
         tile_barrier();
     };
     while (true) {
+        if constexpr (QB == 2) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) o[m] = f32x16{};
-        l_lane = 0.0f;
+            for (int m = 0; m < 4; ++m) o[m] = f32x16{};
+        } else {
+#pragma unroll
+            for (int m = 0; m < 8; ++m) o16[m] = f32x4{};
+        }
+#pragma unroll
+        for (int h = 0; h < QB; ++h) l_lane[h] = 0.0f;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = start_of(c);
             resolve(c0);
             if (ntiles == 0) continue;
-            Raw x0, x1{};
+            Raw x0, x1;
             fetch(x0, 0);
-            if (ntiles > 1) fetch(x1, 1);
+            fetch(x1, min(1, ntiles - 1));
             take(x0, 0, c0);
-            for (int i = 0; i < ntiles; i += 2) {
+            // (a loop without a branch inside: where paths meet, the waits take the fewest loads in flight)
+            int i = 0;
+            for (; i + 2 < ntiles; i += 2) {
                 pv(T0, PX);
-                if (i + 1 < ntiles) {
-                    take(x1, i + 1, c0);
-                    pv(T0 + VT, PX + PT);
-                }
-                if (i + 2 < ntiles) take(x0, i + 2, c0);
+                take(x1, i + 1, c0);
+                pv(T0 + (NB - 1) * VT, PX + (NB - 1) * PT);
+                take(x0, i + 2, c0);
+            }
+            pv(T0, PX);
+            if (i + 1 < ntiles) {
+                take(x1, i + 1, c0);
+                pv(T0 + (NB - 1) * VT, PX + (NB - 1) * PT);
             }
         }
-        // row sums over the lanes and halves that share a row
-        float l = l_lane;
-        l += __shfl_xor(l, 16, 64), l += __shfl_xor(l, 32, 64);
-        const uint64_t anys = __builtin_amdgcn_ballot_w64(any);
-        any = ((anys >> (lane & 15)) & 0x0001000100010001ull) != 0;
+        // row sums over the lanes and waves that share a row (-1: no position, below every sum; a NaN stays one)
+        const int lift = lift_of<false>(k1 - k0, false);
         __syncthreads();
         if (threadIdx.x == 0) s_misc[1] = 0, s_misc[2] = 0, s_misc[3] = 0;
-        if (q == 0) s_top[half][my] = any ? l : -1.0f;
+#pragma unroll
+        for (int h = 0; h < QB; ++h) {
+            const float l = lanes(l_lane[h], [](float a, float b) { return a + b; });
+            const uint64_t anys = __builtin_amdgcn_ballot_w64(any[h]);
+            put(h, (anys >> (opaque(lane) & 15)) & 0x0001000100010001ull ? l : -1.0f);
+        }
         __syncthreads();
-        // (a half with no position: -1, below every sum; a NaN stays one)
-        const float l0 = s_top[0][my], l1 = s_top[1][my];
-        any = !(l0 == -1.0f && l1 == -1.0f);
-        l = (l0 == -1.0f ? 0.0f : l0) + (l1 == -1.0f ? 0.0f : l1);
-        const int lift = lift_of<false>(k1 - k0, false);
-        const bool held = l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
-        if (!again && any && !held) s_misc[1] = 1;
-        if (any && l >= 0.5f) s_misc[2] = 1;
-        l_lane = l;
+#pragma unroll
+        for (int h = 0; h < QB; ++h) {
+            float l = 0.0f;
+            bool on = false;
+#pragma unroll
+            for (int w = 0; w < NWAVE; ++w) {
+                const float v = got(w, h);
+                on = on || v != -1.0f;
+                l += v == -1.0f ? 0.0f : v;
+            }
+            any[h] = on;
+            l_lane[h] = l;
+            const bool held = l > __builtin_ldexpf(1.0f, lift - 40) && l < __builtin_ldexpf(1.0f, lift + 40);
+            if (!again && on && !held) s_misc[1] = 1;
+            if (on && l >= 0.5f) s_misc[2] = 1;
+        }
         __syncthreads();
         bool served = again || __builtin_amdgcn_readfirstlane(s_misc[1]) == 0;
         if (!again && __builtin_expect(served && __builtin_amdgcn_readfirstlane(s_misc[2]) != 0, false)) {
             float z = 0.0f;                    // (as in the tiled kernel)
+            if constexpr (QB == 2) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[m][r], 0.0f, z);
+                    for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[m][r], 0.0f, z);
+            } else {
+#pragma unroll
+                for (int m = 0; m < 8; ++m)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o16[m][r], 0.0f, z);
+            }
             if (z != 0.0f) s_misc[3] = 1;
             __syncthreads();
             served = __builtin_amdgcn_readfirstlane(s_misc[3]) == 0;
         }
         if (served) break;
         again = true;
-        float top = -INFINITY;
+        float top[QB];
+#pragma unroll
+        for (int h = 0; h < QB; ++h) top[h] = -INFINITY;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = start_of(c);
             resolve(c0);
             for (int i = 0; i < ntiles; ++i) {
                 Raw x;
                 fetch(x, i);
-                top = fmaxf(top, top_of(scores(x, i, c0, T0)));
+                f32x4 s[QB];
+                scores(x, i, c0, T0, s);
+                float t[QB];
+                top_of(s, t);
+#pragma unroll
+                for (int h = 0; h < QB; ++h) top[h] = fmaxf(top[h], t[h]);
             }
         }
-        m_ref = top == -INFINITY ? 0.0f : top * c_s;
-        m_ref -= (float)lift_of<false>(k1 - k0, true);
+#pragma unroll
+        for (int h = 0; h < QB; ++h) {
+            m_ref[h] = top[h] == -INFINITY ? 0.0f : top[h] * c_s;
+            m_ref[h] -= (float)lift_of<false>(k1 - k0, true);
+        }
     }
 
     // ---- O / l, LSE: rows' values from the scoring lanes to the lanes that hold O ----
-    const int lift = lift_of<false>(k1 - k0, again);
-    const float lse = too_long ? __builtin_nanf("")
-                               : (m_ref + (float)lift + __builtin_amdgcn_logf(__builtin_ldexpf(l_lane, -lift))) * LN2;
-    __syncthreads();
     // (lane numbers anew: none of what follows is kept through the tile loop)
-    const int ln = fresh_lane(), mine = 16 * rh + (ln & 15);
-    if (ln < 16 && half == 0) {
-        s_top[0][mine] = too_long ? __builtin_nanf("") : (any ? 1.0f / l_lane : 0.0f);
-        const int64_t at = (int64_t)blk.first * p.H + blk.r0 + mine;
-        if (mine >= blk.rows) {
-        } else if (p.ns > 1) {
-            p.part_lse[(int64_t)split * p.T * p.H + at] = any || too_long ? lse : -FLT_MAX;
-        } else if (p.lse) {
-            p.lse[at] = any || too_long ? lse : INFINITY;
+    const int lift = lift_of<false>(k1 - k0, again);
+    const int ln = fresh_lane();
+    __syncthreads();
+    if (wave == 0 && ln < 16) {
+#pragma unroll
+        for (int h = 0; h < QB; ++h) {
+            const int r = 16 * h + ln;
+            const float lse = too_long ? __builtin_nanf("")
+                                       : (m_ref[h] + (float)lift + __builtin_amdgcn_logf(__builtin_ldexpf(l_lane[h], -lift))) * LN2;
+            s_top[0][r] = too_long ? __builtin_nanf("") : (any[h] ? 1.0f / l_lane[h] : 0.0f);
+            const int64_t at = (int64_t)blk.first * p.H + blk.r0 + r;
+            if (r >= blk.rows) {
+            } else if (p.ns > 1) {
+                p.part_lse[(int64_t)split * p.T * p.H + at] = any[h] || too_long ? lse : -FLT_MAX;
+            } else if (p.lse) {
+                p.lse[at] = any[h] || too_long ? lse : INFINITY;
+            }
         }
     }
     __syncthreads();
-    const int hi = ln >> 5, r32 = ln & 31;
-    const float inv = s_top[0][r32];
+    // O's values by quads of dims: quad k of this lane is dims 128 wave + dim_of(k) .. +3 of row orow
+    constexpr int QUADS = QB == 2 ? 16 : 8;
+    const int orow = QB == 2 ? ln & 31 : ln & 15;
+    auto dim_of = [&](int k) { return QB == 2 ? 8 * k + 4 * (ln >> 5) : 16 * k + 4 * (ln >> 4); };
+    const float inv = s_top[0][orow];
+    auto quad = [&](int k) -> f32x4 {
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (QB == 2 ? o[QB == 2 ? k >> 2 : 0][4 * (k & 3) + i] : o16[QB == 1 ? k : 0][i]) * inv;
+        return v;
+    };
     if (p.ns == 1) {
         constexpr int OUT_STRIDE = D_VO * 2 + 16;
-        static_assert(32 * OUT_STRIDE <= 2 * VT, "the stage fits the tile buffers");
+        static_assert(ROWS * OUT_STRIDE <= NB * VT, "the stage fits the tile buffers");
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 v = {o[m][4 * g] * inv, o[m][4 * g + 1] * inv, o[m][4 * g + 2] * inv, o[m][4 * g + 3] * inv};
-                lds_st<u32x2>(T0 + r32 * OUT_STRIDE + 2 * (128 * wave + 32 * m + 8 * g + 4 * hi),
-                              __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4)));
-            }
+        for (int k = 0; k < QUADS; ++k)
+            lds_st<u32x2>(T0 + orow * OUT_STRIDE + 2 * (128 * wave + dim_of(k)),
+                          __builtin_bit_cast(u32x2, __builtin_convertvector(quad(k), bf16x4)));
         __syncthreads();
-        const bool o16 = ((p.o_sb | p.o_st | p.o_sh) & 7) == 0 && ((uintptr_t)p.out & 15) == 0;
-        for (int k = 0; k < 8; ++k) {
-            const int r = 8 * wave + k;
+        const bool wide = ((p.o_sb | p.o_st | p.o_sh) & 7) == 0 && ((uintptr_t)p.out & 15) == 0;
+        for (int k = 0; k < ROWS / NWAVE; ++k) {
+            const int r = ROWS / NWAVE * wave + k;
             if (r >= blk.rows) break;
             const int t = blk.first + (blk.r0 + r) / p.H, h = (blk.r0 + r) % p.H;
             const u32x4 v = lds_ld<u32x4>(T0 + r * OUT_STRIDE + 16 * ln);
             __bf16* const dst = p.out + (LIST ? token_at(t, p.s_q, p.o_sb, p.o_st) : (int64_t)t * p.o_st) + (int64_t)h * p.o_sh + 8 * ln;
-            if (o16) {
+            if (wide) {
                 *reinterpret_cast<u32x4*>(dst) = v;
             } else {
                 reinterpret_cast<u32x2*>(dst)[0] = u32x2{v[0], v[1]};
@@ -386,19 +507,14 @@ dsa_mla_fp4_narrow_kernel(const ChunkParams p) {
             }
         }
     } else {
-        constexpr int PST = D_VO + 16;
-        static_assert(4 * 32 * PST <= 2 * VT + 2 * PT, "four waves' stages fit the tile buffers");
-        const lds_ptr stg = T0 + wave * 32 * PST;
+        constexpr int PST = D_VO + 16;                     // a wave's 128 dims of a row, and a pad
+        static_assert(NWAVE * ROWS * PST <= NB * VT, "four waves' stages fit the tile buffers");
+        const lds_ptr stg = T0 + wave * ROWS * PST;
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 v = {o[m][4 * g] * inv, o[m][4 * g + 1] * inv, o[m][4 * g + 2] * inv, o[m][4 * g + 3] * inv};
-                lds_st<f32x4>(stg + r32 * PST + 4 * (32 * m + 8 * g + 4 * hi), v);
-            }
+        for (int k = 0; k < QUADS; ++k) lds_st<f32x4>(stg + orow * PST + 4 * dim_of(k), quad(k));
         float* const dst0 = p.part_o + ((int64_t)split * p.T * p.H + (int64_t)blk.first * p.H + blk.r0) * D_VO;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < ROWS / 2; ++k) {
             const int r = 2 * k + (ln >> 5);
             const f32x4 v = lds_ld<f32x4>(stg + r * PST + 16 * (ln & 31));
             if (r < blk.rows) *reinterpret_cast<f32x4*>(dst0 + (int64_t)r * D_VO + 128 * wave + 4 * (ln & 31)) = v;

@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t token_at(int32_t t, int32_t s_q, int64_t sb, 
 }
 
 // Entries [c0, c0 + SPAN) below k1 of a token's list -> the cache rows of the valid ones, without gaps, and how
-// many; the last tile is filled with the first row.  `counts`: four words of LDS.  (Ends with a barrier; begins
+// many; the last 64 are filled up with the first row.  `counts`: four words of LDS.  (Ends with a barrier; begins
 // with one that ends the use of the span before.)
 __device__ __forceinline__ int32_t resolve_list(const ChunkParams& p, const Block& blk, int c0, int k1, int32_t* s_rows,
                                                 int32_t* counts) {
@@ -85,8 +85,8 @@ __device__ __forceinline__ int32_t resolve_list(const ChunkParams& p, const Bloc
         if (row[e] >= 0) s_rows[at++] = row[e];
     total = __builtin_amdgcn_readfirstlane(total);
     __syncthreads();
-    const int32_t end = (total + TILE - 1) / TILE * TILE;
-    if (tid < TILE && total + tid < end) s_rows[total + tid] = s_rows[0];
+    const int32_t end = (total + 63) / 64 * 64;
+    if (tid < 64 && total + tid < end) s_rows[total + tid] = s_rows[0];
     __syncthreads();
     return total;
 }

@@ -35,8 +35,8 @@ struct Call {
     int32_t ns, per_split;         // split s takes entries [s * per_split, (s + 1) * per_split)
 };
 
-// `tiled`: 128 heads a workgroup, one a CU; else 32, two a CU.  0 or DSA_ERR_HIP.
-__attribute__((visibility("hidden"))) int launch(const Call& c, bool tiled, hipStream_t stream);
+// `heads` of a workgroup: 128 or 32 (one a CU), or 16 (two a CU).  0 or DSA_ERR_HIP.
+__attribute__((visibility("hidden"))) int launch(const Call& c, int heads, hipStream_t stream);
 
 }  // namespace dsa_list
 

@@ -3976,12 +3976,13 @@ constexpr KernTime KERN_TIME[][4] = {
     // DSA_KV_MXFP8_V4 (no NARROW kernel)
     {{13.8f, 2.23f, 0, 0, 2.7f, 0.40f, 0}, {},
      {10.4f, 2.14f, 11.9f, 2.65f, 1.6f, 0.36f, 0}, {10.8f, 2.41f, 11.8f, 3.06f, 2.0f, 0.32f, 0}},
-    // DSA_KV_MXFP4 (128 heads a workgroup, or 32 and two workgroups per CU)
-    {{13.5f, 1.83f, 0, 0, 3.2f, 0.38f, 0}, {}, {8.3f, 1.0f, 9.0f, 1.3f, 2.6f, 0.39f, 0}, {}},
+    // DSA_KV_MXFP4: 128, 32 and 16 heads a workgroup (choose_fp4)
+    {{9.0f, 2.1f, 0, 0, 3.2f, 0.38f, 0.2f}, {8.0f, 0.75f, 0, 0, 2.6f, 0.45f, 0.2f}, {8.0f, 0.58f, 8.0f, 0.84f, 2.6f, 0.45f, 0.2f}, {}},
 };
+int fp4_heads(Kern k);
 double kern_time(int fmt, Kern k, int64_t tokens, int32_t H, int64_t list, int ns) {
     const KernTime& c = KERN_TIME[fmt][k];
-    const int64_t wgs = tokens * groups_of(k, H) * ns, tiles = ((list + ns - 1) / ns + TILE - 1) / TILE;
+    const int64_t wgs = tokens * (fmt == DSA_KV_MXFP4 ? (H + fp4_heads(k) - 1) / fp4_heads(k) : groups_of(k, H)) * ns, tiles = ((list + ns - 1) / ns + TILE - 1) / TILE;
     int64_t once = (wgs + CUS - 1) / CUS, twice = 0;    // rounds of one and of two workgroups per CU
     if (k == PAIR || k == PAIR64) {
         const int64_t rest = wgs % (2 * CUS);
@@ -3989,8 +3990,10 @@ double kern_time(int fmt, Kern k, int64_t tokens, int32_t H, int64_t list, int n
         twice = wgs / (2 * CUS) + (rest > CUS ? 1 : 0);
     }
     const double work = once * (c.start + (double)tiles * c.tile) + twice * (c.start2 + (double)tiles * c.tile2);
-    const double row = fmt == DSA_KV_BF16 ? BF16_ROW : 2 * D_VO;
-    const double bytes = (double)tokens * list * row * 1e-6 * c.bytes;
+    const double row = fmt == DSA_KV_BF16 ? BF16_ROW : fmt == DSA_KV_MXFP4 ? DSA_MLA_FP4_ROW_BYTES : 2 * D_VO;
+    // (MXFP4 rows are so short that Q and O count beside them)
+    const double q_o = fmt == DSA_KV_MXFP4 ? (double)H * 2 * (D_QK + D_VO) : 0.0;
+    const double bytes = (double)tokens * (list * row + q_o) * 1e-6 * c.bytes;
     double t = std::sqrt(std::sqrt(work * work * work * work + bytes * bytes * bytes * bytes));
     if (ns > 1) t += c.split + c.part * 1e-6 * ns * tokens * H * (D_VO + 1) * sizeof(float);
     return t;
@@ -4037,12 +4040,15 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
     }
     return best;
 }
-// MXFP4 rows
+// MXFP4 rows: the kernels over lists (dsa_list.h), WIDE of 128 heads, NARROW of 32 and PAIR of 16, the last two
+// workgroups to a CU.
+int fp4_heads(Kern k) { return k == WIDE ? HEADS : k == NARROW ? 32 : 16; }
 Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
-    Choice best{PAIR, requested > 0 ? requested : 1};
+    Choice best{WIDE, requested > 0 ? requested : 1};
     double least = -1.0;
-    for (Kern k : {WIDE, PAIR}) {
-        const int64_t wgs = tokens * groups_of(k, H);
+    for (Kern k : {WIDE, NARROW, PAIR}) {
+        const int64_t wgs = tokens * ((H + fp4_heads(k) - 1) / fp4_heads(k));
+        if (wgs >= ((int64_t)1 << 32) / NTHR) continue;
         const int counts[] = {1, one_round_splits(wgs, by_len), one_round_splits(wgs, by_len, k == PAIR ? 2 * CUS : CUS)};
         for (int ns : counts) {
             if (requested > 0) ns = requested;
@@ -4081,9 +4087,9 @@ int noalloc_splits(const dsa_mla_decode_args* a) {
 
 // formats of the top-k and prefill forms
 bool list_format(int fmt) { return fmt == DSA_KV_BF16 || fmt == DSA_KV_FP8_656 || fmt == DSA_KV_MXFP4; }
-// MXFP4 rows: a grid holds below 2^32 threads, of workgroups of 32 heads
+// MXFP4 rows: a grid holds below 2^32 threads
 bool fp4_call_ok(int fmt, int64_t tokens, int32_t H) {
-    return fmt != DSA_KV_MXFP4 || tokens * narrow_groups(H) < ((int64_t)1 << 32) / NTHR;
+    return fmt != DSA_KV_MXFP4 || tokens * head_groups(H) < ((int64_t)1 << 32) / NTHR;
 }
 
 int validate_decode(const dsa_mla_decode_args* a, DecodePlan* plan) {
@@ -4132,7 +4138,7 @@ int launch_fp4(const FwdParams& fp, int ns, hipStream_t st, Kern kern) {
     c.B = fp.B, c.s_q = fp.s_q, c.H = fp.H, c.topk = fp.topk;
     c.causal = fp.causal, c.causal_offset = fp.causal_offset, c.scale_log2 = fp.scale_log2;
     c.ns = ns, c.per_split = fp.chunk;
-    return dsa_list::launch(c, kern == WIDE, st);
+    return dsa_list::launch(c, fp4_heads(kern), st);
 }
 
 int launch_fwd(const FwdParams& fp, int fmt, int B, int s_q, int ns, hipStream_t st, Kern kern = WIDE) {
