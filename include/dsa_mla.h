@@ -33,7 +33,9 @@
  *   which bf16 holds exactly: the kernels compute these rows as bf16 rows of
  *   those values.  dsa_mla_decode, dsa_mla_decode_noalloc, dsa_mla_prefill and
  *   the chunk operators (dsa_chunk.h) take them; a NaN or infinity among an
- *   attended row's values reaches the tokens that attend it.
+ *   attended row's values reaches the tokens that attend it.  Their calls need a
+ *   positive, finite sm_scale (else DSA_ERR_UNSUPPORTED) and tokens x ceil(H / 32)
+ *   below 2^24 (else DSA_ERR_BAD_SHAPE).
  *
  * Index semantics (top-k form).  indices[b][t][k] is a logical position j in
  * sequence b.  It is valid iff 0 <= j < seq_lens[b] and, when causal != 0,
@@ -131,7 +133,7 @@ enum {
  * q       : bf16 [B, s_q, H, 576] addressed by q_stride_{b,t,h} (last dim dense)
  * kv_cache: [kv_total_rows, row] in kv_format; rows are block_size-row pages,
  *           kv_stride_row elements apart (bf16 elements for DSA_KV_BF16 rows,
- *           bytes for DSA_KV_FP8_656 rows; 0 = dense rows of 576 / 656).  A
+ *           bytes for 656- and 400-byte rows; 0 = dense rows).  A
  *           row stride is at least one row, a multiple of 16 bytes and below
  *           4 GiB (else DSA_ERR_BAD_STRIDE).
  * out     : bf16 [B, s_q, H, 512] addressed by o_stride_{b,t,h}
@@ -243,7 +245,7 @@ int dsa_mla_combine(const float* partial_o, const float* partial_lse, int32_t nu
  *            (defs.h:129, "the row stride of the latent KV tensor",
  *            opus_attn/dsa_v32/README.md:99): bf16 elements for DSA_KV_BF16
  *            rows (the reference harness passes 576), bytes for
- *            DSA_KV_FP8_656 rows; 0 = dense rows.  A row stride is at least
+ *            656- and 400-byte rows; 0 = dense rows.  A row stride is at least
  *            one row, a multiple of 16 bytes and below 4 GiB.
  * kv_indptr: int32 [B + 1]; kv_indices: int32 rows.  Query token t of batch b
  *            attends kv_indices[kv_indptr[b] + p] for

@@ -283,7 +283,7 @@ def packer(cls):
 
 
 pack_norm_rope, pack_append, pack_chunk = packer(QkNormRopeArgs), packer(KvAppendArgs), packer(ChunkArgs)
-pack_read = packer(KvReadArgs)
+pack_read, pack_decode, pack_prefill = packer(KvReadArgs), packer(DecodeArgs), packer(PrefillArgs)
 
 
 class DsaError(RuntimeError):
@@ -323,9 +323,10 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     bind_torch_hip_runtime()
     lib = ctypes.CDLL(p)
     sz = ctypes.POINTER(ctypes.c_size_t)
-    lib.dsa_mla_decode_workspace_size.argtypes = [ctypes.POINTER(DecodeArgs), sz]
+    # (argument blocks of _vp: a ctypes struct's address, or packed bytes)
+    lib.dsa_mla_decode_workspace_size.argtypes = [_vp, sz]
     lib.dsa_mla_decode_num_splits.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(_i32)]
-    lib.dsa_mla_decode.argtypes = [ctypes.POINTER(DecodeArgs), _vp, ctypes.c_size_t, _vp]
+    lib.dsa_mla_decode.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_decode_noalloc.argtypes = [ctypes.POINTER(DecodeArgs), _vp]
     lib.dsa_mla_decode_csr_workspace_size.argtypes = [ctypes.POINTER(CsrArgs), sz]
     lib.dsa_mla_decode_csr.argtypes = [ctypes.POINTER(CsrArgs), _vp, ctypes.c_size_t, _vp]
@@ -334,15 +335,14 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.dsa_mla_decode_mxfp8_workspace_size.argtypes = [ctypes.POINTER(MxArgs), sz]
     lib.dsa_mla_decode_mxfp8.argtypes = [ctypes.POINTER(MxArgs), _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_combine.argtypes = [_vp, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _vp]
-    lib.dsa_mla_prefill_workspace_size.argtypes = [ctypes.POINTER(PrefillArgs), sz]
-    lib.dsa_mla_prefill.argtypes = [ctypes.POINTER(PrefillArgs), _vp, ctypes.c_size_t, _vp]
+    lib.dsa_mla_prefill_workspace_size.argtypes = [_vp, sz]
+    lib.dsa_mla_prefill.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_prefill_v4_workspace_size.argtypes = [ctypes.POINTER(PrefillV4Args), sz]
     lib.dsa_mla_prefill_v4.argtypes = [ctypes.POINTER(PrefillV4Args), _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_prefill_v4_fp8_workspace_size.argtypes = [ctypes.POINTER(PrefillV4Fp8Args), sz]
     lib.dsa_mla_prefill_v4_fp8.argtypes = [ctypes.POINTER(PrefillV4Fp8Args), _vp, ctypes.c_size_t, _vp]
     lib.dsa_kv_quantize_fp8.argtypes = [_vp, _i64, _i64, _vp, _i64, _vp, _vp]
     lib.dsa_topk_indices.argtypes = [_vp, _i64, _vp, _i32, _i32, _i32, _vp, _i64, _vp]
-    # (argument blocks as a ctypes struct's address or as packed bytes)
     lib.dsa_qk_norm_rope.argtypes = [_vp, _vp]
     lib.dsa_kv_append.argtypes = [_vp, _vp]
     lib.dsa_kv_read.argtypes = [_vp, _vp]

@@ -4087,9 +4087,9 @@ int noalloc_splits(const dsa_mla_decode_args* a) {
 
 // formats of the top-k and prefill forms
 bool list_format(int fmt) { return fmt == DSA_KV_BF16 || fmt == DSA_KV_FP8_656 || fmt == DSA_KV_MXFP4; }
-// MXFP4 rows: a grid holds below 2^32 threads
+// MXFP4 rows: a grid holds below 2^32 threads, of workgroups of 32 heads
 bool fp4_call_ok(int fmt, int64_t tokens, int32_t H) {
-    return fmt != DSA_KV_MXFP4 || tokens * head_groups(H) < ((int64_t)1 << 32) / NTHR;
+    return fmt != DSA_KV_MXFP4 || tokens * narrow_groups(H) < ((int64_t)1 << 32) / NTHR;
 }
 
 int validate_decode(const dsa_mla_decode_args* a, DecodePlan* plan) {

@@ -18,29 +18,37 @@ from . import abi
 from .abi import DecodeArgs, PrefillArgs, check, load_library
 
 
+# The current device and its current stream (torch.cuda.current_stream() takes 7 us a call).  Absent from a torch
+# without devices, where every call ends before it needs them.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
 def _stream(stream) -> Optional[int]:
     if stream is None:
-        stream = torch.cuda.current_stream()
+        return _raw_stream(_current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+_ROW_FORMATS = {(torch.bfloat16, abi.D_QK): abi.KV_BF16, (torch.uint8, abi.FP8_ROW_BYTES): abi.KV_FP8_656,
+                (torch.uint8, abi.FP4_ROW_BYTES): abi.KV_MXFP4}
 
 
 def kv_format_of(kv: torch.Tensor) -> Tuple[int, int, int]:
     """(kv_format, total_rows, row_stride) of a cache tensor: bf16 [..., 576], uint8
     [..., 656] or uint8 [..., 400] (MXFP4) with a dense last dim.  Rows may be padded (a view of wider rows): row_stride
     is the element distance between rows, 0 when they are dense."""
-    if kv.dtype == torch.bfloat16 and kv.shape[-1] == abi.D_QK:
-        fmt, width = abi.KV_BF16, abi.D_QK
-    elif kv.dtype == torch.uint8 and kv.shape[-1] == abi.FP8_ROW_BYTES:
-        fmt, width = abi.KV_FP8_656, abi.FP8_ROW_BYTES
-    elif kv.dtype == torch.uint8 and kv.shape[-1] == abi.FP4_ROW_BYTES:
-        fmt, width = abi.KV_MXFP4, abi.FP4_ROW_BYTES
-    else:
+    width = kv.shape[-1]
+    fmt = _ROW_FORMATS.get((kv.dtype, width))
+    if fmt is None:
         raise ValueError(f"kv cache must be bf16 [..., 576], uint8 [..., 656] or uint8 [..., 400], got {kv.dtype} "
                          f"{tuple(kv.shape)}")
+    if kv.is_contiguous():
+        return fmt, kv.numel() // width, 0
     if kv.stride(-1) != 1:
         raise ValueError("kv cache rows must have a dense last dim")
     rs = kv.stride(-2) if kv.dim() >= 2 else width
@@ -69,12 +77,28 @@ def _run_with_workspace(size_fn, run_fn, args, workspace, device, stream, where:
     check(run_fn(ctypes.byref(args), _ptr(workspace) if n.value else None, n.value, _stream(stream)), where)
 
 
-def make_decode_args(q, kv_cache, indices, sm_scale, out, lse, *, seq_lens, block_table=None,
-                     block_size=None, causal=False, num_splits=0, kv_batch_stride=0):
+def _sized_launch(size_fn, run_fn, packed: bytes, workspace, q, stream, where: str):
+    """_run_with_workspace for a packed argument block; `q`: a tensor on the device of the call."""
+    n = ctypes.c_size_t(0)
+    rc = size_fn(packed, ctypes.byref(n))
+    if rc:
+        check(rc, where + "_workspace_size")
+    need = n.value
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = q.new_empty((need,), dtype=torch.uint8)
+    rc = run_fn(packed, workspace.data_ptr() if need else None, need, _stream(stream))
+    if rc:
+        check(rc, where)
+
+
+def _decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal, num_splits,
+                   kv_batch_stride):
+    """The fields of dsa_mla_decode_args in order."""
     B, s_q, H, D = q.shape
-    if D != abi.D_QK or q.stride(3) != 1:
+    qs, ix, ixs, os = q.stride(), indices.shape, indices.stride(), out.stride()
+    if D != abi.D_QK or qs[3] != 1:
         raise ValueError("q must be [B, s_q, H, 576] with a dense last dim")
-    if tuple(indices.shape[:2]) != (B, s_q) or indices.stride(2) != 1:
+    if ix[0] != B or ix[1] != s_q or ixs[2] != 1:
         raise ValueError("indices must be [B, s_q, topk] with a dense last dim")
     fmt, rows, row_stride = kv_format_of(kv_cache)
     if block_table is not None:
@@ -82,32 +106,20 @@ def make_decode_args(q, kv_cache, indices, sm_scale, out, lse, *, seq_lens, bloc
             block_size = kv_cache.shape[-2] if kv_cache.dim() >= 3 else None
         if block_size is None:
             raise ValueError("block_size is required with a block table")
-        bt_stride = block_table.stride(0)
+        bt, bt_stride = block_table.data_ptr(), block_table.stride(0)
     else:
         block_size = block_size or 1
-        bt_stride = 0
-    a = DecodeArgs()
-    a.q = _ptr(q)
-    a.q_stride_b, a.q_stride_t, a.q_stride_h = q.stride(0), q.stride(1), q.stride(2)
-    a.kv_cache = _ptr(kv_cache)
-    a.kv_total_rows = rows
-    a.kv_format = fmt
-    a.block_size = int(block_size)
-    a.kv_batch_stride = int(kv_batch_stride)
-    a.kv_stride_row = row_stride
-    a.block_table = _ptr(block_table)
-    a.block_table_stride = bt_stride
-    a.seq_lens = _ptr(seq_lens)
-    a.indices = _ptr(indices)
-    a.idx_stride_b, a.idx_stride_t = indices.stride(0), indices.stride(1)
-    a.out = _ptr(out)
-    a.o_stride_b, a.o_stride_t, a.o_stride_h = out.stride(0), out.stride(1), out.stride(2)
-    a.lse = _ptr(lse)
-    a.B, a.s_q, a.H, a.topk = B, s_q, H, indices.shape[2]
-    a.num_splits = int(num_splits)
-    a.causal = 1 if causal else 0
-    a.sm_scale = float(sm_scale)
-    return a
+        bt = bt_stride = 0
+    return (q.data_ptr(), qs[0], qs[1], qs[2], kv_cache.data_ptr(), rows, fmt, int(block_size), int(kv_batch_stride),
+            row_stride, bt, bt_stride, seq_lens.data_ptr(), indices.data_ptr(), ixs[0], ixs[1], out.data_ptr(), os[0], os[1],
+            os[2], 0 if lse is None else lse.data_ptr(), B, s_q, H, ix[2], int(num_splits), 1 if causal else 0,
+            float(sm_scale))
+
+
+def make_decode_args(q, kv_cache, indices, sm_scale, out, lse, *, seq_lens, block_table=None,
+                     block_size=None, causal=False, num_splits=0, kv_batch_stride=0):
+    return DecodeArgs(*_decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal,
+                                      num_splits, kv_batch_stride))
 
 
 def decode_workspace_size(args: DecodeArgs) -> int:
@@ -132,9 +144,9 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, s
                stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Sparse MLA decode over a (paged) latent cache; returns (out bf16, lse fp32).
 
-    q [B, s_q, H, 576] bf16; kv_cache bf16 [..., 576] or uint8 [..., 656]
-    (fp8 e4m3 + per-128 scales + bf16 RoPE); indices int32 [B, s_q, topk]
-    with -1 padding; seq_lens int32 [B]; block_table int32 [B, max_blocks].
+    q [B, s_q, H, 576] bf16; kv_cache bf16 [..., 576], uint8 [..., 656]
+    (fp8 e4m3 + per-128 scales + bf16 RoPE) or uint8 [..., 400] (MXFP4: e2m1 +
+    power-of-two scales per 32 + bf16 RoPE); indices int32 [B, s_q, topk] with -1 padding; seq_lens int32 [B]; block_table int32 [B, max_blocks].
     """
     _need(q, torch.bfloat16, "q")
     _need(indices, torch.int32, "indices")
@@ -143,17 +155,13 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, s
         _need(block_table, torch.int32, "block_table")
     B, s_q, H, _ = q.shape
     if out is None:
-        out = torch.empty((B, s_q, H, abi.D_VO), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((B, s_q, H, abi.D_VO))
     if lse is None:
-        lse = torch.empty((B, s_q, H), dtype=torch.float32, device=q.device)
-    a = make_decode_args(q, kv_cache, indices, sm_scale, out, lse, seq_lens=seq_lens,
-                         block_table=block_table, block_size=block_size, causal=causal,
-                         num_splits=num_splits, kv_batch_stride=kv_batch_stride)
-    ws_bytes = decode_workspace_size(a)
-    if ws_bytes and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes):
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    check(load_library().dsa_mla_decode(ctypes.byref(a), _ptr(workspace) if ws_bytes else None,
-                                        ws_bytes, _stream(stream)), "dsa_mla_decode")
+        lse = q.new_empty((B, s_q, H), dtype=torch.float32)
+    a = abi.pack_decode(*_decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal,
+                                        num_splits, kv_batch_stride))
+    _sized_launch(load_library().dsa_mla_decode_workspace_size, load_library().dsa_mla_decode, a, workspace, q, stream,
+                  "dsa_mla_decode")
     return out, lse
 
 
@@ -329,31 +337,22 @@ def mla_combine(partial_o: torch.Tensor, partial_lse: torch.Tensor,
     return out, lse
 
 
-def make_prefill_args(q, kv, indices, sm_scale, out, lse, *, causal=False, causal_offset=0, num_splits=0):
+def _prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, num_splits):
+    """The fields of dsa_mla_prefill_args in order."""
     N, H, D = q.shape
-    if D != abi.D_QK or q.stride(2) != 1:
+    qs, ixs, os = q.stride(), indices.stride(), out.stride()
+    if D != abi.D_QK or qs[2] != 1:
         raise ValueError("q must be [N, H, 576] with a dense last dim")
-    if indices.shape[0] != N or indices.stride(1) != 1:
+    if indices.shape[0] != N or ixs[1] != 1:
         raise ValueError("indices must be [N, topk] with a dense last dim")
     fmt, rows, row_stride = kv_format_of(kv)
-    a = PrefillArgs()
-    a.q = _ptr(q)
-    a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
-    a.kv = _ptr(kv)
-    a.kv_rows = rows
-    a.kv_stride_row = row_stride
-    a.kv_format = fmt
-    a.indices = _ptr(indices)
-    a.idx_stride_n = indices.stride(0)
-    a.out = _ptr(out)
-    a.o_stride_n, a.o_stride_h = out.stride(0), out.stride(1)
-    a.lse = _ptr(lse)
-    a.N, a.H, a.topk = N, H, indices.shape[1]
-    a.causal = 1 if causal else 0
-    a.causal_offset = int(causal_offset)
-    a.sm_scale = float(sm_scale)
-    a.num_splits = int(num_splits)
-    return a
+    return (q.data_ptr(), qs[0], qs[1], kv.data_ptr(), rows, row_stride, fmt, indices.data_ptr(), ixs[0], out.data_ptr(),
+            os[0], os[1], 0 if lse is None else lse.data_ptr(), N, H, indices.shape[1], 1 if causal else 0,
+            int(causal_offset), float(sm_scale), int(num_splits))
+
+
+def make_prefill_args(q, kv, indices, sm_scale, out, lse, *, causal=False, causal_offset=0, num_splits=0):
+    return PrefillArgs(*_prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, num_splits))
 
 
 def prefill_workspace_size(args: PrefillArgs) -> int:
@@ -375,16 +374,12 @@ def mla_prefill(q: torch.Tensor, kv: torch.Tensor, indices: torch.Tensor, sm_sca
     _need(indices, torch.int32, "indices")
     N, H, _ = q.shape
     if out is None:
-        out = torch.empty((N, H, abi.D_VO), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((N, H, abi.D_VO))
     if lse is None:
-        lse = torch.empty((N, H), dtype=torch.float32, device=q.device)
-    a = make_prefill_args(q, kv, indices, sm_scale, out, lse, causal=causal,
-                          causal_offset=causal_offset, num_splits=num_splits)
-    nbytes = prefill_workspace_size(a)
-    if nbytes and (workspace is None or workspace.numel() * workspace.element_size() < nbytes):
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    check(load_library().dsa_mla_prefill(ctypes.byref(a), _ptr(workspace) if nbytes else None,
-                                         nbytes, _stream(stream)), "dsa_mla_prefill")
+        lse = q.new_empty((N, H), dtype=torch.float32)
+    a = abi.pack_prefill(*_prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, num_splits))
+    _sized_launch(load_library().dsa_mla_prefill_workspace_size, load_library().dsa_mla_prefill, a, workspace, q, stream,
+                  "dsa_mla_prefill")
     return out, lse
 
 
@@ -612,9 +607,6 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
 # cost little: one look at a tensor's type, device, shape and strides, and argument structs filled at once.
 
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
-# (absent from a torch without devices, where every call ends before it needs them)
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _bad(name: str, t, what: str):
@@ -686,18 +678,19 @@ def _pages(block_table, block_size, cache, B: int, dev: int):
     that of a cache [blocks, block_size, row]."""
     if block_table is None:
         return 0, 0, 0, 0
-    p = _addr(block_table, _I32, "block_table", dev)
-    if block_table.dim() != 2:
+    if block_table.dtype is not _I32 or block_table.get_device() != dev or dev < 0:
+        _not_this(block_table, _I32, "block_table", dev)
+    st = block_table.stride()
+    if len(st) != 2:
         _bad("block_table", block_table, f"be [{B}, blocks]")
     rows, n = block_table.shape
-    st = block_table.stride()
     if rows != B or (n > 1 and st[1] != 1):
         _bad("block_table", block_table, f"be [{B}, blocks] with a dense last dim")
     if block_size is None:
         if cache is None or cache.dim() < 3:
             raise ValueError("block_size is required with a block table")
         block_size = cache.shape[-2]
-    return p, st[0], n, int(block_size)
+    return block_table.data_ptr(), st[0], n, int(block_size)
 
 
 def _angles(cos_sin, dev: int):
@@ -880,29 +873,31 @@ _KV_NORMS = {"none": 0, "rms": 1}
 def _streams(cache, dev: int):
     """(first tensor, kv_format, values of a row, addresses of rows, scales and RoPE, rows, their strides) of a
     cache: a tensor, or the tuple of its streams."""
-    parts = cache if isinstance(cache, (tuple, list)) else (cache,)
-    first = parts[0]
-    if len(parts) == 1:
-        found = _CACHE.get((first.dtype, first.shape[-1]))
+    if isinstance(cache, (tuple, list)) and len(cache) > 1:
+        found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in cache]))
+        first = cache[0]
     else:
-        found = _CACHES.get(tuple([(t.dtype, t.shape[-1]) for t in parts]))
+        first = cache[0] if isinstance(cache, (tuple, list)) else cache
+        found = _CACHE.get((first.dtype, first.shape[-1]))
+        cache = None
     if found is None:
-        raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in parts]}")
+        raise ValueError(f"cache is of no known format: {[(t.dtype, tuple(t.shape)) for t in cache or (first,)]}")
     fmt, width, own = found
-    psc = pr = sstride = rstride = 0
-    pc = _addr(first, first.dtype, "cache", dev)
+    if first.get_device() != dev:
+        _not_this(first, first.dtype, "cache", dev)
     rows, stride = (first.numel() // own, 0) if first.is_contiguous() else _rows(first, own, "cache")
-    if len(parts) > 1:
-        last = parts[-1]
+    psc = pr = sstride = rstride = 0
+    if cache:
+        last = cache[-1]
         pr = _addr(last, _BF16, "cache", dev)
         more, rstride = _rows(last, 64, "cache")
-        if len(parts) == 3:
-            psc = _addr(parts[1], _U8, "cache", dev)
-            others, sstride = _rows(parts[1], 16, "cache")
+        if len(cache) == 3:
+            psc = _addr(cache[1], _U8, "cache", dev)
+            others, sstride = _rows(cache[1], 16, "cache")
             more = more if others == rows else -1
         if more != rows:
             raise ValueError("the cache's streams must have the same rows")
-    return first, fmt, width, pc, psc, pr, rows, stride, sstride, rstride
+    return first, fmt, width, first.data_ptr(), psc, pr, rows, stride, sstride, rstride
 
 
 def kv_append(kv: Optional[torch.Tensor], cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor,
@@ -996,10 +991,13 @@ def kv_read(cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor, rows: Optiona
     if out is None:
         if rows is None:
             raise ValueError("rows is required without out")
-        out = (_empty_like if on is None else on.empty)(first, (int(rows), width), _BF16)
-    po, T, ot = _addr2(out, width, "out", dev)
-    if rows is not None and T != rows:
-        _bad("out", out, f"have {rows} rows")
+        T, ot = int(rows), width
+        out = first.new_empty((T, width), dtype=_BF16) if on is None else on.empty(first, (T, width), _BF16)
+        po = out.data_ptr()
+    else:
+        po, T, ot = _addr2(out, width, "out", dev)
+        if rows is not None and T != rows:
+            _bad("out", out, f"have {rows} rows")
     pt, tst, blocks, bs = _pages(block_table, block_size, first, B, dev)
     a = abi.pack_read(pc, psc, pr, n, stride, sstride, rstride, fmt, T, po, ot, pi, pl, pt, tst, blocks, bs,
                       kv_batch_stride, B)
@@ -1019,6 +1017,22 @@ def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, bloc
     if q.dim() != 3:
         _bad("q", q, "be [T, H, 576]")
     T, H, _ = q.shape
+    po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev) if out is not None else (0, 0, 0)
+    ps = _dense_lse(lse, T, H, dev) if lse is not None else 0
+    return _pack_chunk(q, kv_cache, q_indptr, seq_lens, sm_scale, po, ot, oh, ps, block_table, block_size, kv_batch_stride,
+                       causal, max_kv_len, num_splits, dev, T, H)
+
+
+def _dense_lse(lse, T: int, H: int, dev: int) -> int:
+    ps = _addr(lse, _F32, "lse", dev)
+    if lse.shape != (T, H) or not lse.is_contiguous():
+        _bad("lse", lse, f"be a dense [{T}, {H}]")
+    return ps
+
+
+def _pack_chunk(q, kv_cache, q_indptr, seq_lens, sm_scale, po, ot, oh, ps, block_table, block_size, kv_batch_stride, causal,
+                max_kv_len, num_splits, dev: int, T: int, H: int) -> bytes:
+    """make_chunk_args with the outputs' addresses and strides."""
     pq, qt, qh = _addr3(q, T, H, abi.D_QK, "q", dev)
     pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     width = kv_cache.shape[-1]
@@ -1027,19 +1041,13 @@ def make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, *, bloc
         raise ValueError(f"kv cache must be bf16 [..., 576], uint8 [..., 656] or uint8 [..., 400], got {kv_cache.dtype} "
                          f"{tuple(kv_cache.shape)}")
     fmt = found[0]
-    pk = _addr(kv_cache, kv_cache.dtype, "kv_cache", dev)
+    if kv_cache.get_device() != dev:
+        _not_this(kv_cache, kv_cache.dtype, "kv_cache", dev)
     rows, stride = (kv_cache.numel() // width, 0) if kv_cache.is_contiguous() else _rows(kv_cache, width, "kv_cache")
     pt, tst, blocks, bs = _pages(block_table, block_size, kv_cache, B, dev)
     if max_kv_len is None:
         max_kv_len = blocks * bs if block_table is not None else int(kv_batch_stride) or rows
-    po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev) if out is not None else (0, 0, 0)
-    if lse is not None:
-        ps = _addr(lse, _F32, "lse", dev)
-        if lse.shape != (T, H) or not lse.is_contiguous():
-            _bad("lse", lse, f"be a dense [{T}, {H}]")
-    else:
-        ps = 0
-    return abi.pack_chunk(pq, qt, qh, pi, pl, pk, rows, stride, fmt, bs, pt, tst, kv_batch_stride, po, ot, oh, ps,
+    return abi.pack_chunk(pq, qt, qh, pi, pl, kv_cache.data_ptr(), rows, stride, fmt, bs, pt, tst, kv_batch_stride, po, ot, oh, ps,
                          blocks, T, B, H, 1 if causal else 0, max_kv_len, num_splits, sm_scale)
 
 
@@ -1064,7 +1072,7 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     """Dense attention of a chunk's tokens over the paged latent cache (dsa_mla_chunk); returns
     (out bf16 [T, H, 512], lse fp32 [T, H]).
 
-    q bf16 [T, H, 576]; kv_cache bf16 [..., 576] or uint8 [..., 656]; sequence b's tokens
+    q bf16 [T, H, 576]; kv_cache bf16 [..., 576], uint8 [..., 656] or uint8 [..., 400] (MXFP4); sequence b's tokens
     q_indptr[b] .. q_indptr[b + 1] - 1 are its last positions below seq_lens[b] (their own rows already
     in the cache) and attend positions up to their own (causal) or all.  Rows of no sequence are left as
     allocated.  max_kv_len: an upper bound of seq_lens (default: what the block table can hold; past
@@ -1077,14 +1085,25 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
     empty = _empty_like if on is None else on.empty
     T, H, _ = q.shape
+    ot, oh = H * abi.D_VO, abi.D_VO
     if out is None:
         out = empty(q, (T, H, abi.D_VO), _BF16)
+        po = out.data_ptr()
+    else:
+        po, ot, oh = _addr3(out, T, H, abi.D_VO, "out", dev)
     if lse is None:
         lse = empty(q, (T, H), _F32)
-    a = make_chunk_args(q, kv_cache, q_indptr, seq_lens, sm_scale, out, lse, block_table=block_table,
-                        block_size=block_size, kv_batch_stride=kv_batch_stride, causal=causal,
-                        max_kv_len=max_kv_len, num_splits=num_splits)
-    need = chunk_workspace_size(a)
+        ps = lse.data_ptr()
+    else:
+        ps = _dense_lse(lse, T, H, dev)
+    a = _pack_chunk(q, kv_cache, q_indptr, seq_lens, sm_scale, po, ot, oh, ps, block_table, block_size, kv_batch_stride, causal,
+                    max_kv_len, num_splits, dev, T, H)
+    n = ctypes.c_size_t(0)
+    lib = load_library()
+    rc = lib.dsa_mla_chunk_workspace_size(a, ctypes.byref(n))
+    if rc:
+        check(rc, "dsa_mla_chunk_workspace_size")
+    need = n.value
     ws = None
     if need:
         if workspace is None or workspace.numel() * workspace.element_size() < need:
@@ -1092,7 +1111,7 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
         elif not workspace.is_contiguous():
             _bad("workspace", workspace, "be dense")
         ws = _addr(workspace, workspace.dtype, "workspace", dev)
-    fn = load_library().dsa_mla_chunk
+    fn = lib.dsa_mla_chunk
     if on is None:
         rc = fn(a, ws, need, _raw_stream(dev))
         if rc:
