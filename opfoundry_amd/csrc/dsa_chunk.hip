@@ -635,17 +635,29 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     struct Codes {
         unsigned c, e;
     };
-    auto fp4_load = [&](lds_cptr rb, int k) -> Codes {
-        const int ln = opaque(lane), r = 8 * wave + k;
-        return {lds_ld<unsigned>(rb + 256 * r + 4 * ln), lds_ld<unsigned char>(rb + RAW4_SCALES + 16 * r + (ln >> 2))};
+    struct Fp4 {               // this lane's places in a raw slot and a tile buffer: row k's by constants from here
+        lds_cptr codes, scales;
+        lds_ptr to[2];         // of rows 0 .. 3 and 4 .. 7, which nope_sw() tells apart
     };
-    auto fp4_store = [&](lds_ptr tb, int k, const Codes& x) {
-        const int ln = opaque(lane), r = 8 * wave + k;
-        lds_st<u32x4>(tb + r * NOPE_STRIDE + 16 * (ln ^ nope_sw(r)), fp4_to_bf16(x.c, x.e));
+    auto fp4_at = [&](lds_cptr rb, lds_ptr tb) -> Fp4 {
+        const int ln = opaque(lane);
+        Fp4 f;
+        f.codes = rb + (2048 * wave + 4 * ln);
+        f.scales = rb + (RAW4_SCALES + 128 * wave + (ln >> 2));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f.to[i] = tb + (8 * wave * NOPE_STRIDE + 16 * (ln ^ nope_sw(8 * wave + 4 * i)));
+        return f;
+    };
+    auto fp4_load = [&](const Fp4& f, int k) -> Codes {
+        return {lds_ld<unsigned>(f.codes + 256 * k), lds_ld<unsigned char>(f.scales + 16 * k)};
+    };
+    auto fp4_store = [&](const Fp4& f, int k, const Codes& x) {
+        lds_st<u32x4>(f.to[k >> 2] + k * NOPE_STRIDE, fp4_to_bf16(x.c, x.e));
     };
     auto fp4_convert = [&](lds_cptr rb, lds_ptr tb) {
+        const Fp4 f = fp4_at(rb, tb);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) fp4_store(tb, k, fp4_load(rb, k));
+        for (int k = 0; k < 8; ++k) fp4_store(f, k, fp4_load(f, k));
     };
 
     const float c_s = p.scale_log2;
@@ -660,8 +672,12 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
 
     // PV's first operands of a tile (bf16 rows): read in the last steps of the scores before it (1024 tokens of
     // 128 heads over 8192 rows 2000 -> 1978 us; 656-byte rows, whose scores leave no idle reads: 1294 -> 1307)
+    // (400-byte rows: and the first codes to convert)
     struct First {
         u32x4 p[NWAVE], v;
+        Fp4 at;
+        Codes c;
+        u32x4 w;
     };
     // V^T block m of the wave's dims, positions 16 u .. +15 (transposed reads of rows 4 hi .. +3 and 8 further)
     auto v_block = [&](lds_cptr vt, int ln, int u, int m) -> u32x4 {
@@ -812,8 +828,9 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
         p_half(e, 0, px);
         p_half(e, 1, px);
     };
-    // (with_exp: the next tile but one, raw at draw, goes piece by piece to V's own buffer (656-byte rows) or to
-    // buffer dpar (400-byte rows; -1: there is none))
+    // (with_exp: the next tile but one goes piece by piece to V's own buffer (656-byte rows, raw at draw) or from and
+    // to the places f.at (400-byte rows; where there is none, what the slot held before goes to a buffer that nothing
+    // reads: a branch around it would leave each piece's load without work to hide behind))
     auto pv = [&](lds_ptr vt, lds_cptr px, First& f, const f32x16& sn, float* en, auto with_exp, lds_cptr draw, int dpar) {
         const int ln = FP8 ? opaque(lane) : lane;
         u32x4 v_cur = {};
@@ -831,13 +848,41 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
             for (int m = 0; m < 4; ++m) {
                 __builtin_amdgcn_sched_barrier(0);
                 u32x4 v_nxt = v_cur;
-                if (m + 1 < 4) v_nxt = v_block(vt, ln, u, m + 1);
-                else if (!FP8 && u == 0) v_nxt = v_block(vt, ln, 1, 0);
+                auto read_v = [&]() {
+                    if (m + 1 < 4) v_nxt = v_block(vt, ln, u, m + 1);
+                    else if (!FP8 && u == 0) v_nxt = v_block(vt, ln, 1, 0);
+                };
+                if constexpr (!(FP4 && decltype(with_exp)::value)) read_v();
                 u32x2 codes;
                 if constexpr (FP8 && decltype(with_exp)::value) codes = deq_load(draw, 4 * u + m);
-                Codes c4;
-                if constexpr (FP4 && decltype(with_exp)::value)
-                    if (dpar >= 0) c4 = fp4_load(draw, 4 * u + m);
+                if constexpr (FP4 && decltype(with_exp)::value) {
+                    // Behind each product a conversion and one more piece of work, which hides most of it (behind all
+                    // four it hides none); the codes are read a group ahead and written a group later.
+                    const int g = 4 * u + m;
+                    const Codes c = f.c;
+                    const float scale = __uint_as_float(c.e << 23);
+                    u32x4 w;
+                    auto step = [&](auto hc) {
+                        constexpr int h = decltype(hc)::value;
+                        mfma_o<false>(o[4 * m + h], v_cur, f.p[h]);
+                        if (u == 0 && m == 3) f.p[h] = p_block(px, ln, 1, h);
+                        __builtin_amdgcn_sched_barrier(0);
+                        w[h] = fp4_pair<h>(c.c, scale);
+                        if (h == 0) read_v();
+                        if (h == 1 && g < 7) f.c = fp4_load(f.at, g + 1);
+                        if (h == 2 && g > 0) lds_st<u32x4>(f.at.to[(g - 1) >> 2] + (g - 1) * NOPE_STRIDE, f.w);
+                        if (h & 1) en[2 * g + h / 2] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[2 * g + h / 2], c_s, -m_ref));
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    step(std::integral_constant<int, 0>{});
+                    step(std::integral_constant<int, 1>{});
+                    step(std::integral_constant<int, 2>{});
+                    step(std::integral_constant<int, 3>{});
+                    f.w = w;
+                    if (g == 7) lds_st<u32x4>(f.at.to[1] + 7 * NOPE_STRIDE, w);
+                    v_cur = v_nxt;
+                    continue;
+                }
 #pragma unroll
                 for (int h = 0; h < NWAVE; ++h) {
                     mfma_o<FP8>(o[4 * m + h], v_cur, f.p[h]);
@@ -849,8 +894,6 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     en[r0 + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sn[r0 + 1], c_s, -m_ref));
                 }
                 if constexpr (FP8 && decltype(with_exp)::value) deq_store(vt, 4 * u + m, codes, ds);
-                if constexpr (FP4 && decltype(with_exp)::value)
-                    if (dpar >= 0) fp4_store(slot_of(dpar), 4 * u + m, c4);
                 v_cur = v_nxt;
             }
         }
@@ -907,12 +950,18 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     if (i + 3 < ntiles) issue(next, cur, (i + 1) & 1);
                     __builtin_amdgcn_sched_barrier(0);
                     First f;
-                    f32x16 sn = qk(slot_of(nxt), [&](int k) { read_first(f, k, slot_of(cur), PX + (i & 1) * P_BYTES); });
+                    f32x16 sn = qk(slot_of(nxt), [&](int k) {
+                        read_first(f, k, slot_of(cur), PX + (i & 1) * P_BYTES);
+                        if (k == 4) {
+                            next_landed(i + 3 < ntiles);
+                            f.at = fp4_at(raw4_of(i & 1), slot_of(far));
+                            f.c = fp4_load(f.at, 0);
+                        }
+                    });
                     if (i + 4 < ntiles) next = load_rows(i + 4);
                     mask(sn, i + 1, c0);
-                    next_landed(i + 3 < ntiles);
                     float en[16];
-                    pv(slot_of(cur), PX + (i & 1) * P_BYTES, f, sn, en, std::true_type{}, raw4_of(i & 1), i + 2 < ntiles ? far : -1);
+                    pv(slot_of(cur), PX + (i & 1) * P_BYTES, f, sn, en, std::true_type{}, T0, 0);
                     const lds_ptr px = PX + ((i + 1) & 1) * P_BYTES;
                     p_half(en, 0, px);
                     p_half(en, 1, px);

@@ -17,6 +17,12 @@ __device__ __forceinline__ u32x4 fp4_to_bf16(unsigned c, unsigned e) {
                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
+// Two of them: values 2 SEL and 2 SEL + 1; `s` is the scale.
+template <int SEL>
+__device__ __forceinline__ unsigned fp4_pair(unsigned c, float s) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, SEL));
+}
+
 // e of the least power of two 2^e >= amax / 6 = amax / (1.5 * 2^2), at least -125, so that half of it, the
 // least value a code stands for, is a normal bf16; 0 for 0.
 __device__ __forceinline__ int fp4_exponent(float amax) {
