@@ -59,17 +59,22 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
     // 128 q .. +127 and 512 + 32 j + 8 q .. +7 (j < 2) of a product's operands
     const int q = lane >> 4;
     int limit[QB];
-    u32x4 qf[QB][KS / 2];
 #pragma unroll
-    for (int h = 0; h < QB; ++h) {
-        const int row = blk.r0 + min(16 * h + (lane & 15), blk.rows - 1);
-        const int tok = blk.first + row / p.H;
-        limit[h] = LIST ? 0 : limit_in(p, blk, tok);
-        const __bf16* qp = p.q + (LIST ? token_at(tok, p.s_q, p.q_sb, p.q_st) : (int64_t)tok * p.q_st) + (int64_t)(row % p.H) * p.q_sh;
+    for (int h = 0; h < QB; ++h)
+        limit[h] = LIST ? 0 : limit_in(p, blk, blk.first + (blk.r0 + min(16 * h + (lane & 15), blk.rows - 1)) / p.H);
+    // Q once for the workgroup, 16 bytes a lane of neighbouring ones; each lane's part comes back through LDS (in
+    // qf's order a load of 64 lanes touches 64 cache lines, and every wave would read all rows).
+    constexpr int QU = 72, QSTRIDE = 16 * QU + 16, QN = (ROWS * QU + 255) / 256;
+    static_assert(ROWS * QSTRIDE <= NB * VT, "Q fits the tile buffers");
+    u32x4 qraw[QN];
+    {
+        const int tid = 64 * wave + fresh_lane();
 #pragma unroll
-        for (int ks = 0; ks < KS / 2; ++ks) {
-            const int d = ks < 16 ? 128 * q + 8 * ks : 32 * ks + 8 * q;
-            qf[h][ks] = *reinterpret_cast<const u32x4*>(qp + d);
+        for (int n = 0; n < QN; ++n) {
+            const int u = min(tid + 256 * n, ROWS * QU - 1), row = blk.r0 + min(u / QU, blk.rows - 1);
+            const int tok = blk.first + row / p.H;
+            const __bf16* qp = p.q + (LIST ? token_at(tok, p.s_q, p.q_sb, p.q_st) : (int64_t)tok * p.q_st) + (int64_t)(row % p.H) * p.q_sh;
+            qraw[n] = *reinterpret_cast<const u32x4*>(qp + 8 * (u % QU));
         }
     }
 
@@ -128,6 +133,29 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
         }
     };
 
+    const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + SPAN - 1) / SPAN) : 0;
+    auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * SPAN); };
+    // (the first span's rows while Q is on its way)
+    bool ready = nspans > 0;
+    if (ready) resolve(start_of(0));
+    u32x4 qf[QB][KS / 2];
+    {
+        const int ln = fresh_lane();
+#pragma unroll
+        for (int n = 0; n < QN; ++n) {
+            const int u = 64 * wave + ln + 256 * n;
+            if (u < ROWS * QU) lds_st<u32x4>(T0 + (u / QU) * QSTRIDE + 16 * (u % QU), qraw[n]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < QB; ++h)
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks)
+                qf[h][ks] = lds_ld<u32x4>(T0 + (16 * h + (ln & 15)) * QSTRIDE +
+                                          (ks < 16 ? 256 * (ln >> 4) + 16 * ks : 64 * ks + 16 * (ln >> 4)));
+        __syncthreads();
+    }
+
     // This lane's quarter of row lane % 16 of its wave's 16
     struct Raw {
         u32x4 v[6];            // codes of dims 128 q + 32 j .. +31 (j < 4), RoPE values 32 (j - 4) + 8 q .. +7
@@ -176,7 +204,7 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
 
     // S^T[4 positions of this lane x its rows]; the converted codes go to V's tile at vt
     auto qk = [&](const Raw& x, lds_ptr vt, f32x4 (&s)[QB]) {
-        const int ln = QB == 1 ? lane : opaque(lane), lr = 16 * wave + (ln & 15);
+        const int ln = opaque(lane), lr = 16 * wave + (ln & 15);
         const lds_ptr vr = vt + lr * NSTRIDE + 256 * (ln >> 4);
         const int sw = 16 * fsw(lr);
         f32x4 a[2] = {};                       // two chains: the blocks of rows, or the even and odd k-steps
@@ -321,8 +349,6 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
         }
     };
 
-    const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + SPAN - 1) / SPAN) : 0;
-    auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * SPAN); };
     bool first = true, again = false;
     // scores and probabilities of tile i, then its registers take tile i + 2
     auto take = [&](Raw& x, int i, int c0) {
@@ -359,7 +385,8 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
         for (int h = 0; h < QB; ++h) l_lane[h] = 0.0f;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = start_of(c);
-            resolve(c0);
+            if (!ready) resolve(c0);
+            ready = false;
             if (ntiles == 0) continue;
             Raw x0, x1;
             fetch(x0, 0);
