@@ -590,3 +590,115 @@ def test_refuses_tensors_of_another_kind(dev):
     with pytest.raises(abi.DsaError) as e:
         dsa.mla_decode_csr(bf16(g, 1, 16, 576), kv, i32([0, 4], dev), i32([0, 1, 2, 3], dev), SM_SCALE, max_kv_len=4)
     assert e.value.code == -4
+
+
+# ------------------------------------------------------------------ the ends of the ranges
+
+def test_calls_of_nothing(dev):
+    """No tokens, no entries, no new rows: the outputs of tokens that attend nothing, and nothing else."""
+    g = gen(41, dev)
+    kv, ip, sl = _fp4.rows(g, 128), i32([0, 2], dev), i32([70], dev)
+    assert dsa.kv_read(kv, i32([0, 0], dev), sl, 0).shape == (0, 576)
+    o, l = dsa.mla_chunk(bf16(g, 0, 16, 576), kv, i32([0, 0], dev), sl, SM_SCALE)
+    assert o.shape == (0, 16, 512) and l.shape == (0, 16)
+    for H in (16, 40, 128):
+        q = bf16(g, 3, H, 576)
+        for topk, ns in ((0, 0), (0, 3), (5, 0), (300, 0), (300, 4)):
+            none = torch.full((3, topk), -1, dtype=torch.int32, device=dev)
+            for o, l in (dsa.mla_decode(q[:, None], kv, none[:, None], SM_SCALE, seq_lens=i32([128] * 3, dev), num_splits=ns),
+                         dsa.mla_prefill(q, kv, none, SM_SCALE, causal=True, causal_offset=100, num_splits=ns)):
+                torch.cuda.synchronize()
+                assert bool((o == 0).all()) and bool((l == math.inf).all())
+        o, l = dsa.mla_prefill(q[:0], kv, torch.zeros((0, 5), dtype=torch.int32, device=dev), SM_SCALE)
+        assert o.shape == (0, H, 512) and l.shape == (0, H)
+        o, l = dsa.mla_chunk(q[:2], kv, ip, i32([0], dev), SM_SCALE)           # a sequence without positions
+        torch.cuda.synchronize()
+        assert bool((o == 0).all()) and bool((l == math.inf).all())
+    # no new rows: the cache stays as it was
+    before = kv.clone()
+    dsa.kv_append(bf16(g, 4, 576), kv, i32([0, 0], dev), sl, style=None)
+    torch.cuda.synchronize()
+    assert torch.equal(kv, before)
+
+
+@pytest.mark.parametrize("H", [16, 40, 128])
+def test_one_position_many_times(dev, H):
+    """n times the same entry: its values, and a sum of n."""
+    g = gen(42, dev)
+    kv, q = _fp4.rows(g, 64), bf16(g, 2, H, 576)
+    lists = [[17] * 2500, [3] * 64 + [63]]
+    idx = torch.full((2, 2500), -1, dtype=torch.int32, device=dev)
+    for t, x in enumerate(lists):
+        idx[t, :len(x)] = i32(x, dev)
+    at, ref = _fp4.attend_lists64(q, _fp4.as_bf16(kv), lists, H)
+    for ns in (0, 1, 5):
+        o, l = dsa.mla_prefill(q, kv, idx, SM_SCALE, num_splits=ns)
+        torch.cuda.synchronize()
+        _fp4.check(at, o, l, ref)
+
+
+@pytest.mark.parametrize("T,H,n", [(300, 32, 100), (260, 64, 70), (3, 48, 130), (520, 20, 33)])
+def test_lists_of_few_heads(dev, T, H, n):
+    g = gen(43, dev)
+    kv, q = _fp4.rows(g, 900), bf16(g, T, H, 576)
+    idx = torch.randint(0, 900, (T, n), generator=g, device=dev).to(torch.int32)
+    at, ref = _fp4.attend_lists64(q, _fp4.as_bf16(kv), idx.tolist(), H)
+    for ns in (0, 1, 2):
+        o, l = dsa.mla_prefill(q, kv, idx, SM_SCALE, num_splits=ns)
+        torch.cuda.synchronize()
+        _fp4.check(at, o, l, ref)
+
+
+def test_append_and_read_in_a_graph(dev):
+    """A captured step writes and reads what its buffers hold at each replay, with eager calls between."""
+    g = gen(44, dev)
+    c = Chunk(g, [3, 1], [500, 64], 64, pad=2)
+    kv, cs = torch.zeros((c.rows, 400), dtype=torch.uint8, device=dev), cos_sin(600, dev)
+    x, w = bf16(g, c.T, 576), 1 + 0.1 * torch.randn(512, generator=g, device=dev)
+    step = lambda: (dsa.kv_append(x, kv, c.indptr, c.seq_lens, cs, weight=w, **c.kw),            # noqa: E731
+                    dsa.kv_read(kv, c.indptr, c.seq_lens, c.T, **c.kw))[1]
+    step()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step()
+    for seed in (1, 2, 3):
+        x.copy_(bf16(gen(seed, dev), c.T, 576))
+        c.seq_lens.copy_(i32([500 - seed, 64 - seed], dev))
+        out.fill_(9.0)
+        gr.replay()
+        torch.cuda.synchronize()
+        got, cache = out.clone(), kv.clone()
+        kv.zero_()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got[:4], want[:4]) and bool((got[4:] == 9).all())
+        at = torch.tensor([c.row(b, n - seed - k) for b, n, k in ((0, 500, 1), (0, 500, 2), (0, 500, 3), (1, 64, 1))], device=dev)
+        assert torch.equal(cache[at], kv[at]) and bool((got[:4] != 0).any())
+
+
+def test_two_graphs_with_one_workspace(dev):
+    """A program's own workspace, of the larger call, under two captured calls in turn."""
+    g = gen(45, dev)
+    c = Chunk(g, [2, 9], [900, 1300], 64)
+    ls = Lists(g, [1300, 1200], 1, 700, 64, True)
+    kv, kv2 = cache_of(g, c), _fp4.rows(g, ls.rows)
+    q, q2 = bf16(g, c.T, 16, 576), bf16(g, 2, 1, 128, 576)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=dev)
+    calls = (lambda **k: dsa.mla_chunk(q, kv, c.indptr, c.seq_lens, SM_SCALE, num_splits=4, **c.kw, **k),
+             lambda **k: dsa.mla_decode(q2, kv2, ls.indices, SM_SCALE, seq_lens=ls.seq_lens, causal=True, num_splits=3, **ls.kw, **k))
+    want = [f() for f in calls]
+    graphs = []
+    for f in calls:
+        f(workspace=ws)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = f(workspace=ws)
+        graphs.append((gr, res))
+    for _ in range(3):
+        ws.fill_(0xFF)
+        for (gr, res), w in zip(graphs, want):
+            res[0].zero_()
+            gr.replay()
+            calls[0](workspace=ws)
+            torch.cuda.synchronize()
+            assert torch.equal(res[0], w[0]) and torch.equal(res[1], w[1])
