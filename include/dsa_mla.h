@@ -53,7 +53,8 @@
  * DSA_ERR_BAD_SHAPE).  A query token runs in ceil(H / 128) workgroups of 128
  * heads, or in workgroups of 32 or 64 heads: at H <= 64 where those are
  * expected to take less time, and, of 32, for bf16 and 656-B fp8 rows when
- * 128-head workgroups would be too few to occupy the GPU.  The last group
+ * 128-head workgroups would be too few to occupy the GPU (400-B rows: of 128, 32
+ * or 16 heads, whichever is expected to take the least).  The last group
  * computes its heads past H on a copy of head H-1 and stores nothing for them,
  * so outputs, LSEs and partials are written for heads 0..H-1 only.  The kernel
  * choice changes dsa_mla_decode_num_splits and the workspace sizes, which
@@ -64,7 +65,7 @@
  * bounds; one call repeats its bits.
  *
  * Numerics.  Scores s = (q . k) * sm_scale in fp32; softmax probabilities are
- * rounded to the P.V product's 16-bit type before it (bf16 for bf16 and MXFP8
+ * rounded to the P.V product's 16-bit type before it (bf16 for bf16, MXFP8 and MXFP4
  * rows, as the reference does at host.cc:451; fp16 for DSA_KV_FP8_656 rows,
  * whose V is fp16), accumulation is fp32, O is written as bf16 (round to
  * nearest even) and LSE = max + ln(sum exp(s - max)) as fp32 (natural log of

@@ -117,7 +117,12 @@ constexpr int RAW_LPW = (RAW_LOADS + NWAVE - 1) / NWAVE; // of wave 0 (6); the o
 static_assert(RAW_LOADS == NWAVE * (RAW_LPW - 1) + 1 && RAW_PIECES % 64 == 32, "the last load is wave 0's, half of it spare");
 constexpr int V_BYTES = TILE * NOPE_STRIDE;
 // 400-byte rows: a tile's codes (256 bytes a row) and scales (16 a row) as they come, in two slots; its values go
-// into a tile buffer, as those of bf16 rows, which its RoPE values are loaded into.
+// into a tile buffer, as those of bf16 rows, which its RoPE values are loaded into.  From there on the kernel is that of
+// bf16 rows, with 35 % of its bytes and 16 conversions a lane and tile more.  They go one behind each of PV's
+// products, whose 32 cycles hide one (8 cycles) and not a group of them; a row's codes are read one product group ahead
+// and its values written one later.  1024 tokens over 8192 rows of 128 heads: all conversions before a tile's
+// barrier 3293 us, in front of PV 2339, behind its products 2100, in a session in which bf16 rows took 2012 (1977 to 2100
+// in different ones: 1.18 to 1.26 PFLOP/s of the 1.28 to 1.36 that a product of 16384 x 16384 reaches).
 constexpr int RAW4_SCALES = TILE * 256, RAW4_BYTES = RAW4_SCALES + TILE * 16;
 constexpr int RAW4_LPW = 4;                  // loads of a wave and tile: two of codes, one each of scales and RoPE
 __device__ __forceinline__ int nope_sw(int r) { return (r >> 2) & 3; }
@@ -1868,6 +1873,12 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 // the two sides of it, us: one token of 128 heads over 1501 rows, 128-row blocks 25.2, 32-row 17.7;
 // 256 of 16 heads over 4096 302 and 217; 200 of 128 heads over 1000 78 and 120; 512 tokens of
 // 16 heads over the same 4096 rows 90 (4 splits) and 120.
+// 400-byte rows have blocks of 16 rows too, two a CU.  Calls in blocks of 128, 32 and 16 rows, us, the taken one in
+// brackets: one token of 128 heads over 1501 rows 23.5, 18.3, [17.9]; 16 sequences of 1 to 4 tokens and up to 20011
+// rows, 16 heads, 75, 52, [54]; 11 of 1 or 2 tokens and 2431 rows, 16 heads, 31, 23, [20]; 24 of 1 to 4 and 393, 32 heads,
+// 32, 20, [17]; 7 of up to 301 and 5000, 40 heads, [386], 508, 538; 2 of 86 to 233 and 2346, 128 heads, [283], 322, 355.
+// (Constants closer to the kernels alone, 2.05, 0.66, 0.55 and 0.78, took 32-row blocks for the last one, and for 8 of up to 41
+// tokens over 5705 rows, 40 heads, where they took 137 us for 104.)
 constexpr int KINDS = 3;
 constexpr int32_t KIND_ROWS[KINDS] = {BLOCK, NARROW, 16};          // rows of a workgroup
 constexpr Kernel KERNELS[3][KINDS] = {       // [bf16, 656-byte, 400-byte rows]; pair: two share a CU

@@ -3977,12 +3977,14 @@ constexpr KernTime KERN_TIME[][4] = {
     {{13.8f, 2.23f, 0, 0, 2.7f, 0.40f, 0}, {},
      {10.4f, 2.14f, 11.9f, 2.65f, 1.6f, 0.36f, 0}, {10.8f, 2.41f, 11.8f, 3.06f, 2.0f, 0.32f, 0}},
     // DSA_KV_MXFP4: 128, 32 and 16 heads a workgroup (choose_fp4)
-    {{9.0f, 2.1f, 0, 0, 3.2f, 0.38f, 0.2f}, {8.0f, 0.75f, 0, 0, 2.6f, 0.45f, 0.2f}, {8.0f, 0.58f, 8.0f, 0.84f, 2.6f, 0.45f, 0.2f}, {}},
+    {{9.0f, 2.1f, 0, 0, 3.2f, 0.38f, 0.2f}, {8.0f, 0.75f, 0, 0, 2.6f, 0.45f, 0.2f},
+     {8.0f, 0.58f, 8.0f, 0.84f, 2.6f, 0.45f, 0.2f}, {}},
 };
 int fp4_heads(Kern k);
 double kern_time(int fmt, Kern k, int64_t tokens, int32_t H, int64_t list, int ns) {
     const KernTime& c = KERN_TIME[fmt][k];
-    const int64_t wgs = tokens * (fmt == DSA_KV_MXFP4 ? (H + fp4_heads(k) - 1) / fp4_heads(k) : groups_of(k, H)) * ns, tiles = ((list + ns - 1) / ns + TILE - 1) / TILE;
+    const int64_t groups = fmt == DSA_KV_MXFP4 ? (H + fp4_heads(k) - 1) / fp4_heads(k) : groups_of(k, H);
+    const int64_t wgs = tokens * groups * ns, tiles = ((list + ns - 1) / ns + TILE - 1) / TILE;
     int64_t once = (wgs + CUS - 1) / CUS, twice = 0;    // rounds of one and of two workgroups per CU
     if (k == PAIR || k == PAIR64) {
         const int64_t rest = wgs % (2 * CUS);
@@ -4040,8 +4042,11 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
     }
     return best;
 }
-// MXFP4 rows: the kernels over lists (dsa_list.h), WIDE of 128 heads, NARROW of 32 and PAIR of 16, the last two
-// workgroups to a CU.
+// MXFP4 rows: the kernels over lists (dsa_list.h), WIDE of 128 heads, NARROW of 32 and PAIR of 16, of which two
+// workgroups share a CU: the one of least expected time (KERN_TIME).  Each of the three on calls of 2048 entries, us,
+// the taken one in brackets: 1531 tokens of 16 heads 702, 314, [172]; 512 of 32 heads 261, [128], 149; 256 of 64
+// 137, [115], 127; 256 of 128 heads [152], 230, 246; 2 of 128 heads 28.7, 21.3, [19.2]; 300 of 40 heads, 1024
+// entries, 125, 93, [68].
 int fp4_heads(Kern k) { return k == WIDE ? HEADS : k == NARROW ? 32 : 16; }
 Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
     Choice best{WIDE, requested > 0 ? requested : 1};

@@ -282,7 +282,9 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_qk_norm_rope_kernel(const dsa_
 // bounds, then for its page and its position's angles; its values, requested
 // first, are there by then.  That chain is what a call takes: one token 2.9 us, 128
 // 3.7, 4099 tokens of V4 fp8 rows 5.5 (7.7 MB), 9238 of 656-byte rows and index
-// keys 11.8 (24 MB; 11548 waves, of which 7168 fit the chip at a time).
+// keys 11.8 (24 MB; 11548 waves, of which 7168 fit the chip at a time), of 400-byte
+// rows and index keys 8.8 in a graph, one call after another (with two latent rows
+// a wave 8.7, and 5.0 for 3.9 at 1000 tokens; with four 9.9 and 7.0).
 // ---------------------------------------------------------------------------
 struct AppendParams {
     dsa_kv_append_args a;
@@ -455,7 +457,13 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_kv_append_kernel(const AppendP
 
 // ---------------------------------------------------------------------------
 // Rows read back: a wave takes READ_ROWS tokens.  Their cache rows are looked up a
-// lane each, then every load of all of them goes out before the first is used.
+// lane each, then every load of all of them goes out before the first is used; a
+// row's codes are one load of 256 bytes, the last 64 values of the eight rows one
+// load of a lane each.  A value is one conversion and, of e4m3 codes, one fp32
+// product, rounded once.  Bound by memory where there are rows enough: 100,000 rows
+// of 400 bytes 25 us (41 MB read and 116 MB written, 6.2 TB/s; a 1 GiB copy 5.1),
+// 21,000 of 656 bytes 10.8 (38 MB).  One row takes 2.8 (a launch and a chain of loads:
+// sequence, page, row), 333 take 4.9.
 // ---------------------------------------------------------------------------
 constexpr int READ_ROWS = 8;
 struct ReadParams {
