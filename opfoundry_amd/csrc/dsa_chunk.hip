@@ -928,6 +928,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 // Iteration i: scores of tile i + 1, PV of tile i with the exponentials of tile i + 1 and the
                 // conversion of tile i + 2, and tile i + 3 on its way.  A wave reads no other's raw rows, so that
                 // its own wait is enough; the barrier shows what all have converted, and every wave's P.
+                // (A list's tiles are not scanned: every row in them is one that the token attends.)
                 auto next_landed = [&](bool more) {
                     if (more) landed(std::integral_constant<int, RAW4_LPW>{}); else landed(std::integral_constant<int, 0>{});
                 };
@@ -935,7 +936,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 if (ntiles > 1) issue(load_rows(1), 1, 1);
                 next_landed(ntiles > 1);
                 fp4_convert(raw4_of(0), slot_of(0));
-                if (masked(0, c0)) scan(0, 0);
+                if (!LIST && masked(0, c0)) scan(0, 0);
                 tile_barrier();
                 if (ntiles > 2) issue(load_rows(2), 2, 0);
                 f32x16 s0 = qk(slot_of(0), none);
@@ -949,7 +950,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                 int cur = 0;
                 for (int i = 0; i + 1 < ntiles; ++i) {
                     const int nxt = cur == 2 ? 0 : cur + 1, far = nxt == 2 ? 0 : nxt + 1;
-                    if (masked(i + 1, c0)) scan(i + 1, nxt);
+                    if (!LIST && masked(i + 1, c0)) scan(i + 1, nxt);
                     tile_barrier();
                     __builtin_amdgcn_sched_barrier(0);
                     if (i + 3 < ntiles) issue(next, cur, (i + 1) & 1);
@@ -1113,7 +1114,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
                     s = qk8(raw_of(0), 0);
                 } else {
                     if constexpr (FP4) fp4_convert(raw4_of(0), slot_of(0));
-                    if (masked(i, c0)) scan(i, 0);
+                    if (!LIST && masked(i, c0)) scan(i, 0);
                     tile_barrier();
                     s = qk(slot_of(0), none);
                 }

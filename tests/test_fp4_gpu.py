@@ -702,3 +702,32 @@ def test_two_graphs_with_one_workspace(dev):
             calls[0](workspace=ws)
             torch.cuda.synchronize()
             assert torch.equal(res[0], w[0]) and torch.equal(res[1], w[1])
+
+
+@pytest.mark.parametrize("T,H", [(256, 128), (300, 40), (2, 128)])
+@pytest.mark.parametrize("scale", [255, 254])
+def test_rows_that_are_not_finite_at_a_lists_end(dev, T, H, scale):
+    """In a list's last tile, which is filled up, as anywhere else: the tokens that name such a row are NaN."""
+    g = gen(46, dev)
+    kv, q = _fp4.rows(g, 300), bf16(g, T, H, 576)
+    kv[200, 259], kv[200, 48:64] = scale, 0x77          # of dims 96 .. 127: NaN, or 6 x 2^127
+    kv[201, 272:274] = torch.tensor([0x80, 0x7F], dtype=torch.uint8, device=dev)
+    idx = torch.stack([torch.randperm(200, generator=g, device=dev)[:70] for _ in range(T)]).to(torch.int32)
+    lists = idx.tolist()
+    if T > 2:
+        lists[2] = lists[2][:69]
+    at, ref = _fp4.attend_lists64(q, _fp4.as_bf16(kv), lists, H)
+    idx[0, 66], idx[1, 3] = 200, 200
+    for x in ref[:2]:
+        x[0], x[1] = float("nan"), float("nan")
+    if T > 2:
+        idx[2, 69], idx[T - 1, 0] = 201, 200
+        for x in ref[:2]:
+            x[T - 1] = float("nan")
+            # (an infinite RoPE value, which V does not have: a score of +inf, whose weight is exp(inf - inf), or of
+            # -inf, whose weight is 0)
+            x[2, q[2, :, 512] > 0] = float("nan")
+    for ns in (1, 2):
+        o, l = dsa.mla_prefill(q, kv, idx, SM_SCALE, num_splits=ns)
+        torch.cuda.synchronize()
+        _fp4.check(at, o, l, ref)
