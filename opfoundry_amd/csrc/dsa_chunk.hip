@@ -416,7 +416,7 @@ dsa_mla_chunk_tile_kernel(const ChunkParams p) {
     int ntiles = 0, n_valid = 0;
     auto resolve = [&](int c0) {
         if constexpr (LIST) {
-            n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc);
+            n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc, [] {});
             ntiles = (n_valid + TILE - 1) / TILE;
             return;
         }

@@ -70,31 +70,45 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
     // scores: this lane's row of each block of 16, its positions 16 wave + 4 q .. +3 of a tile, and the dims
     // 128 q .. +127 and 512 + 32 j + 8 q .. +7 (j < 2) of a product's operands
     const int q = lane >> 4;
+    // Row k of the block: its token after the block's first one's, and its head.  (Of a list all rows are one token's;
+    // elsewhere a division where a token has fewer heads than the block rows.)
+    struct HeadOf {
+        int tok, head;
+    };
+    const int tok0 = LIST ? 0 : blk.r0 / p.H, head0 = blk.r0 - tok0 * p.H;
+    auto head_of = [&](int k) -> HeadOf {
+        if constexpr (LIST) return {0, blk.r0 + k};
+        int t = 0, h = head0 + k;
+        if (p.H >= ROWS) t = h >= p.H ? 1 : 0;
+        else t = h / p.H;
+        return {tok0 + t, h - t * p.H};
+    };
     int limit[QB];
 #pragma unroll
     for (int h = 0; h < QB; ++h)
-        limit[h] = LIST ? 0 : limit_in(p, blk, blk.first + (blk.r0 + min(16 * h + (lane & 15), blk.rows - 1)) / p.H);
+        limit[h] = LIST ? 0 : limit_in(p, blk, blk.first + head_of(min(16 * h + (lane & 15), blk.rows - 1)).tok);
+    const int64_t q0 = LIST ? token_at(blk.first, p.s_q, p.q_sb, p.q_st) : (int64_t)blk.first * p.q_st;
     // Q once for the workgroup, 16 bytes a lane of neighbouring ones; each lane's part comes back through LDS (in
     // qf's order a load of 64 lanes touches 64 cache lines, and every wave would read all rows).
     constexpr int QU = 72, QSTRIDE = 16 * QU + 16, QN = (ROWS * QU + 255) / 256;
     static_assert(ROWS * QSTRIDE <= NB * VT, "Q fits the tile buffers");
     u32x4 qraw[QN];
-    {
+    auto load_q = [&] {
         const int tid = 64 * wave + fresh_lane();
 #pragma unroll
         for (int n = 0; n < QN; ++n) {
-            const int u = min(tid + 256 * n, ROWS * QU - 1), row = blk.r0 + min(u / QU, blk.rows - 1);
-            const int tok = blk.first + row / p.H;
-            const __bf16* qp = p.q + (LIST ? token_at(tok, p.s_q, p.q_sb, p.q_st) : (int64_t)tok * p.q_st) + (int64_t)(row % p.H) * p.q_sh;
+            const int u = min(tid + 256 * n, ROWS * QU - 1);
+            const HeadOf r = head_of(min(u / QU, blk.rows - 1));
+            const __bf16* qp = p.q + q0 + (int64_t)r.tok * p.q_st + (int64_t)r.head * p.q_sh;
             qraw[n] = *reinterpret_cast<const u32x4*>(qp + 8 * (u % QU));
         }
-    }
+    };
 
     // ---- positions [c0, c0 + SPAN) below k1 -> cache rows (positions without one: some row that is there) ----
     int ntiles = 0, n_valid = 0;
-    auto resolve = [&](int c0) {
+    auto resolve = [&](int c0, auto beside) {
         if constexpr (LIST) {
-            n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc);
+            n_valid = resolve_list(p, blk, c0, k1, s_rows, s_misc, beside);
             ntiles = (n_valid + FTILE - 1) / FTILE;
         } else {
             const int tid = 64 * wave + fresh_lane();
@@ -111,12 +125,14 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) id[e] = table[blk_i[e]];
+                beside();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int64_t r = (int64_t)id[e] * p.pages.block_size + (min(at + e, k1 - 1) - blk_i[e] * p.pages.block_size);
                     id[e] = r >= 0 && r < p.rows ? (int32_t)r : -1;
                 }
             } else {
+                beside();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int64_t r = blk.b * p.pages.batch_stride + min(at + e, k1 - 1);
@@ -147,9 +163,10 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
 
     const int nspans = k1 > k0 ? (int)(((int64_t)k1 - k0 + SPAN - 1) / SPAN) : 0;
     auto start_of = [&](int c) { return (int)(k0 + (int64_t)c * SPAN); };
-    // (the first span's rows while Q is on its way)
+    // (Q beside the first span's rows)
     bool ready = nspans > 0;
-    if (ready) resolve(start_of(0));
+    if (ready) resolve(start_of(0), load_q);
+    else load_q();
     u32x4 qf[QB][KS / 2];
     {
         const int ln = fresh_lane();
@@ -397,7 +414,7 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
         for (int h = 0; h < QB; ++h) l_lane[h] = 0.0f;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = start_of(c);
-            if (!ready) resolve(c0);
+            if (!ready) resolve(c0, [] {});
             ready = false;
             if (ntiles == 0) continue;
             Raw x0, x1;
@@ -471,7 +488,7 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
         for (int h = 0; h < QB; ++h) top[h] = -INFINITY;
         for (int c = 0; c < nspans; ++c) {
             const int c0 = start_of(c);
-            resolve(c0);
+            resolve(c0, [] {});
             for (int i = 0; i < ntiles; ++i) {
                 Raw x;
                 fetch(x, i);
@@ -532,12 +549,13 @@ dsa_mla_fp4_few_kernel(const ChunkParams p) {
                           __builtin_bit_cast(u32x2, __builtin_convertvector(quad(k), bf16x4)));
         __syncthreads();
         const bool wide = ((p.o_sb | p.o_st | p.o_sh) & 7) == 0 && ((uintptr_t)p.out & 15) == 0;
+        const int64_t o0 = LIST ? token_at(blk.first, p.s_q, p.o_sb, p.o_st) : (int64_t)blk.first * p.o_st;
         for (int k = 0; k < ROWS / NWAVE; ++k) {
             const int r = ROWS / NWAVE * wave + k;
             if (r >= blk.rows) break;
-            const int t = blk.first + (blk.r0 + r) / p.H, h = (blk.r0 + r) % p.H;
+            const HeadOf at = head_of(r);
             const u32x4 v = lds_ld<u32x4>(T0 + r * OUT_STRIDE + 16 * ln);
-            __bf16* const dst = p.out + (LIST ? token_at(t, p.s_q, p.o_sb, p.o_st) : (int64_t)t * p.o_st) + (int64_t)h * p.o_sh + 8 * ln;
+            __bf16* const dst = p.out + o0 + (int64_t)at.tok * p.o_st + (int64_t)at.head * p.o_sh + 8 * ln;
             if (wide) {
                 *reinterpret_cast<u32x4*>(dst) = v;
             } else {

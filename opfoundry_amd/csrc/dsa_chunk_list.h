@@ -36,10 +36,12 @@ __device__ __forceinline__ int64_t token_at(int32_t t, int32_t s_q, int64_t sb, 
 }
 
 // Entries [c0, c0 + SPAN) below k1 of a token's list -> the cache rows of the valid ones, without gaps, and how
-// many; the last 64 are filled up with the first row.  `counts`: four words of LDS.  (Ends with a barrier; begins
+// many; the last 64 are filled up with the first row.  `counts`: four words of LDS; `beside`: done while
+// the entries are on their way.  (Ends with a barrier; begins
 // with one that ends the use of the span before.)
+template <class Beside>
 __device__ __forceinline__ int32_t resolve_list(const ChunkParams& p, const Block& blk, int c0, int k1, int32_t* s_rows,
-                                                int32_t* counts) {
+                                                int32_t* counts, Beside beside) {
     const int lane = fresh_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = 64 * wave + lane;
     const int32_t tt = blk.first - blk.b * p.s_q;
     const int32_t* const idx = p.indices + blk.b * p.idx_sb + tt * p.idx_st;
@@ -49,6 +51,7 @@ __device__ __forceinline__ int32_t resolve_list(const ChunkParams& p, const Bloc
         const int k = c0 + 8 * tid + e;
         j[e] = k < k1 ? idx[k] : -1;
     }
+    beside();
     const int64_t len = p.lens ? (int64_t)p.lens[blk.b] : p.list_len;
     int64_t jmax = len;
     if (p.causal == 1) jmax = min(len, len - p.s_q + tt + 1);
