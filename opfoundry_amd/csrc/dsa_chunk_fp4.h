@@ -12,18 +12,20 @@
 //   PV     wave w: O^T[dims 128 w .. +127 x all rows]
 // QB = 1: 16 rows, two workgroups a CU, one V buffer, two barriers a tile; PV in 16x16x32.
 // QB = 2: 32 rows, one workgroup a CU (Q alone takes 144 registers), two V buffers, one barrier a tile.
-// What bounds them: not memory (rows are 400 bytes: 512 tokens x 2048 of 32 heads from HBM 128 us, 3.3 TB/s; a third
-// of 1536 tokens over 3000 rows, from the caches, 105) nor the matrix units (1531 tokens x 2048 of 16 heads: 172 us, 0.63 PFLOP/s; matrix units busy
-// 24 % of the cycles, vector instructions 36, LDS 39), but the chain of a wave's tile - codes, conversion, scores,
-// exp2, LDS, barrier, product - with one or two waves on a SIMD to run beside it.  Without one part of it (wrong
-// results) that case, at 185 us, took: without PV 151, without V's writes 141, without both 120, without the
-// conversion 163, without the scores' products 164.  A pair of tiles takes 1.6 to 1.9 us, a QB = 2 tile 1.3 to 1.5.
-// Kept on the way (303 us at first, 128-row blocks with most rows empty 702): loads without a branch around
-// them, so that a wait counts only older ones, two tiles ahead; fsw(), after whose first form bank conflicts
-// were 26.7 M cycles and are 1.7 M; Q loaded once for a workgroup (185 -> 172, with the lane numbers formed anew in qk(),
-// which leaves 222 registers of 256).  Not kept: rows loaded along their bytes and turned through LDS (98 M L1
-// accesses become 39 M, but LDS has the wait then: 185 -> 200); QB = 2 with half the next tile's conversions behind PV's
-// products and half behind the scores' (lists 318 -> 313, dense 50.3 -> 50.9: the chain is as long).
+// What bounds them: not memory (rows are 400 bytes: 512 tokens x 2048 of 32 heads from HBM 128 us, 3.3 TB/s; a
+// third of 1536 tokens over 3000 rows, from the caches, 105) nor the matrix units (1531 tokens x 2048 of 16 heads:
+// 169 us, 0.65 PFLOP/s; matrix units busy 24 % of the cycles, vector instructions 35, LDS 40), but the chain of a
+// wave's tile - codes, conversion, scores, exp2, LDS, barrier, product - with one or two waves on a SIMD to run
+// beside it.  Without one part of it (wrong results) that case, at 185 us, took: without PV 151, without V's writes
+// 141, without both 120, without the conversion 163, without the scores' products 164.  A pair of tiles takes 1.6
+// to 1.9 us, a QB = 2 tile 1.3 to 1.5. Kept on the way (303 us at first, 128-row blocks with most rows empty 702):
+// loads without a branch around them, so that a wait counts only older ones, two tiles ahead; fsw(), after whose
+// first form bank conflicts were 26.7 M cycles and are 1.7 M; Q loaded once for a workgroup (185 -> 172, with the
+// lane numbers formed anew in qk(), which leaves 222 registers of 256), beside the first rows' look-up and without
+// divisions (172 -> 169; 64 entries each for 1536 tokens 31 -> 28).  Not kept: rows loaded along their bytes and
+// turned through LDS (98 M L1 accesses become 39 M, but LDS has the wait then: 185 -> 200); QB = 2 with half the
+// next tile's conversions behind PV's products and half behind the scores' (lists 318 -> 313, dense 50.3 -> 50.9:
+// the chain is as long).
 // ---------------------------------------------------------------------------
 constexpr int FTILE = 64;                    // positions of a tile
 // V in LDS: rows of 1 KB, piece c of row r at c ^ fsw(r).  A write takes eight rows' pieces of one number at a time,
