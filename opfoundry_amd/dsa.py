@@ -28,10 +28,51 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _stream(stream) -> Optional[int]:
-    if stream is None:
-        return _raw_stream(_current_device())
-    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+class _Stream:
+    """The stream of a call on device `dev` and what it allocates.  Memory used on a stream that is not the
+    device's current one is marked so for the allocator, which then does not hand it out while the call runs."""
+
+    __slots__ = ("dev", "handle", "other")
+
+    def __init__(self, dev: int, stream):
+        self.dev = dev
+        current = _raw_stream(dev)
+        self.other = None
+        if stream is None:
+            self.handle = current
+        else:
+            self.handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            if self.handle != current:
+                self.other = (stream if isinstance(stream, torch.cuda.Stream)
+                              else torch.cuda.ExternalStream(self.handle, device=dev))
+
+    def take(self, t: torch.Tensor) -> torch.Tensor:
+        """`t`, made for this call on the current stream."""
+        if self.other is not None:
+            # (the current stream's earlier work may still use that memory)
+            self.other.wait_stream(torch.cuda.current_stream(self.dev))
+            t.record_stream(self.other)
+        return t
+
+    def empty_like(self, like: torch.Tensor) -> torch.Tensor:
+        return torch.empty_like(like) if self.other is None else self.empty(like, like.shape, like.dtype)
+
+    def empty(self, like: torch.Tensor, shape, dtype) -> torch.Tensor:
+        return self.take(like.new_empty(shape, dtype=dtype))
+
+    def call(self, fn, where: str, *args) -> None:
+        if _current_device() == self.dev:
+            rc = fn(*args, self.handle)
+        else:
+            with torch.cuda.device(self.dev):
+                rc = fn(*args, self.handle)
+        if rc:
+            check(rc, where)
+
+
+def _stream_of(dev: int, stream) -> Optional[_Stream]:
+    """None for a call on the current stream of the current device, which needs neither."""
+    return None if stream is None and _current_device() == dev else _Stream(dev, stream)
 
 
 _ROW_FORMATS = {(torch.bfloat16, abi.D_QK): abi.KV_BF16, (torch.uint8, abi.FP8_ROW_BYTES): abi.KV_FP8_656,
@@ -60,35 +101,51 @@ def kv_format_of(kv: torch.Tensor) -> Tuple[int, int, int]:
     return fmt, kv.numel() // width, (0 if rs == width else rs)
 
 
-def _need(t: torch.Tensor, dtype, name: str):
+def _need(t: torch.Tensor, dtype, name: str, dev: Optional[int] = None):
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name} must be on device {dev}, got {t.device}")
 
 
-def _run_with_workspace(size_fn, run_fn, args, workspace, device, stream, where: str):
+def _same_device(dev: int, **tensors):
+    """Tensors of a call whose other checks are elsewhere."""
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} must be on device {dev}, got {t.device}")
+
+
+def _workspace(workspace, need: int, like: torch.Tensor, on: Optional[_Stream]):
+    """The caller's workspace, or a new one where it has none or too small a one.  (A call keeps the tensor until
+    its launch: memory given back before could be marked as free for the stream too early.)"""
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        return like.new_empty((need,), dtype=torch.uint8) if on is None else on.empty(like, (need,), torch.uint8)
+    _same_device(like.get_device(), workspace=workspace)
+    if not workspace.is_contiguous():
+        _bad("workspace", workspace, "be dense")
+    return workspace
+
+
+def _run_with_workspace(size_fn, run_fn, args, workspace, like, on: Optional[_Stream], where: str):
     """Size the call's workspace (size_fn), allocate one if the caller's is missing or too small,
-    and launch (run_fn(args, ws_ptr, ws_bytes, stream))."""
+    and launch (run_fn(args, ws_ptr, ws_bytes, stream)).  args: a packed argument block or a struct's address; like:
+    a tensor on the call's device."""
     n = ctypes.c_size_t(0)
-    check(size_fn(ctypes.byref(args), ctypes.byref(n)), where + "_workspace_size")
-    if n.value and (workspace is None or workspace.numel() * workspace.element_size() < n.value):
-        workspace = torch.empty(n.value, dtype=torch.uint8, device=device)
-    check(run_fn(ctypes.byref(args), _ptr(workspace) if n.value else None, n.value, _stream(stream)), where)
-
-
-def _sized_launch(size_fn, run_fn, packed: bytes, workspace, q, stream, where: str):
-    """_run_with_workspace for a packed argument block; `q`: a tensor on the device of the call."""
-    n = ctypes.c_size_t(0)
-    rc = size_fn(packed, ctypes.byref(n))
+    rc = size_fn(args, ctypes.byref(n))
     if rc:
         check(rc, where + "_workspace_size")
-    need = n.value
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = q.new_empty((need,), dtype=torch.uint8)
-    rc = run_fn(packed, workspace.data_ptr() if need else None, need, _stream(stream))
-    if rc:
-        check(rc, where)
+    need, ws = n.value, None
+    if need:
+        workspace = _workspace(workspace, need, like, on)
+        ws = workspace.data_ptr()
+    if on is None:
+        rc = run_fn(args, ws, need, _raw_stream(like.get_device()))
+        if rc:
+            check(rc, where)
+    else:
+        on.call(run_fn, where, args, ws, need)
 
 
 def _decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal, num_splits,
@@ -149,19 +206,22 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, s
     power-of-two scales per 32 + bf16 RoPE); indices int32 [B, s_q, topk] with -1 padding; seq_lens int32 [B]; block_table int32 [B, max_blocks].
     """
     _need(q, torch.bfloat16, "q")
-    _need(indices, torch.int32, "indices")
-    _need(seq_lens, torch.int32, "seq_lens")
+    dev = q.get_device()
+    _need(indices, torch.int32, "indices", dev)
+    _need(seq_lens, torch.int32, "seq_lens", dev)
     if block_table is not None:
-        _need(block_table, torch.int32, "block_table")
+        _need(block_table, torch.int32, "block_table", dev)
+    _same_device(dev, kv_cache=kv_cache, out=out, lse=lse)
+    on = _stream_of(dev, stream)
     B, s_q, H, _ = q.shape
     if out is None:
-        out = q.new_empty((B, s_q, H, abi.D_VO))
+        out = q.new_empty((B, s_q, H, abi.D_VO)) if on is None else on.empty(q, (B, s_q, H, abi.D_VO), q.dtype)
     if lse is None:
-        lse = q.new_empty((B, s_q, H), dtype=torch.float32)
+        lse = q.new_empty((B, s_q, H), dtype=torch.float32) if on is None else on.empty(q, (B, s_q, H), torch.float32)
     a = abi.pack_decode(*_decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal,
                                         num_splits, kv_batch_stride))
-    _sized_launch(load_library().dsa_mla_decode_workspace_size, load_library().dsa_mla_decode, a, workspace, q, stream,
-                  "dsa_mla_decode")
+    lib = load_library()
+    _run_with_workspace(lib.dsa_mla_decode_workspace_size, lib.dsa_mla_decode, a, workspace, q, on, "dsa_mla_decode")
     return out, lse
 
 
@@ -203,23 +263,21 @@ def mla_decode_csr(q: torch.Tensor, kv: torch.Tensor, kv_indptr: torch.Tensor,
     """Sparse MLA decode in the reference's CSR form (kv_indptr / kv_indices, page size 1,
     count-based MTP causality); returns (out bf16 [B*s_q, H, 512], lse fp32 [B*s_q, H])."""
     _need(q, torch.bfloat16, "q")
-    _need(kv_indptr, torch.int32, "kv_indptr")
-    _need(kv_indices, torch.int32, "kv_indices")
+    dev = q.get_device()
+    _need(kv_indptr, torch.int32, "kv_indptr", dev)
+    _need(kv_indices, torch.int32, "kv_indices", dev)
+    _same_device(dev, kv=kv, out=out, lse=lse)
+    on = _Stream(dev, stream)
     total_q, H, _ = q.shape
     if out is None:
-        out = torch.empty((total_q, H, abi.D_VO), dtype=torch.bfloat16, device=q.device)
+        out = on.empty(q, (total_q, H, abi.D_VO), torch.bfloat16)
     if lse is None:
-        lse = torch.empty((total_q, H), dtype=torch.float32, device=q.device)
+        lse = on.empty(q, (total_q, H), torch.float32)
     a = make_decode_csr_args(q, kv, kv_indptr, kv_indices, sm_scale, out, lse, s_q=s_q,
                              max_kv_len=max_kv_len, num_splits=num_splits)
     lib = load_library()
-    n = ctypes.c_size_t(0)
-    check(lib.dsa_mla_decode_csr_workspace_size(ctypes.byref(a), ctypes.byref(n)),
-          "dsa_mla_decode_csr_workspace_size")
-    if n.value and (workspace is None or workspace.numel() * workspace.element_size() < n.value):
-        workspace = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-    check(lib.dsa_mla_decode_csr(ctypes.byref(a), _ptr(workspace) if n.value else None, n.value,
-                                 _stream(stream)), "dsa_mla_decode_csr")
+    _run_with_workspace(lib.dsa_mla_decode_csr_workspace_size, lib.dsa_mla_decode_csr, ctypes.byref(a), workspace, q, on,
+                        "dsa_mla_decode_csr")
     return out, lse
 
 
@@ -238,11 +296,10 @@ def csr_plan(kv_indptr: torch.Tensor, B: int, s_q: int, H: int, max_kv_len: int,
     n = ctypes.c_size_t(0)
     check(lib.dsa_mla_decode_csr_workspace_size(ctypes.byref(a), ctypes.byref(n)),
           "dsa_mla_decode_csr_workspace_size")
-    if workspace is None or workspace.numel() * workspace.element_size() < n.value:
-        workspace = torch.empty(max(n.value, 16), dtype=torch.uint8, device=kv_indptr.device)
-    check(lib.dsa_mla_csr_plan(_ptr(kv_indptr), B, s_q, H, max_kv_len, _ptr(workspace),
-                               workspace.numel() * workspace.element_size(), _stream(stream)),
-          "dsa_mla_csr_plan")
+    on = _Stream(kv_indptr.get_device(), stream)
+    workspace = _workspace(workspace, max(n.value, 16), kv_indptr, on)
+    on.call(lib.dsa_mla_csr_plan, "dsa_mla_csr_plan", _ptr(kv_indptr), B, s_q, H, max_kv_len, _ptr(workspace),
+            workspace.numel() * workspace.element_size())
     return workspace
 
 
@@ -291,28 +348,26 @@ def mla_decode_mxfp8(q_nope: torch.Tensor, q_scale: torch.Tensor, q_rope: torch.
                      stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Sparse MLA decode on MXFP8 split streams (the reference's -dtype fp8 format), CSR
     form; returns (out bf16 [B*s_q, H, 512], lse fp32 [B*s_q, H])."""
+    dev = q_nope.get_device()
     for t, n in ((q_nope, "q_nope"), (q_scale, "q_scale"), (kv_nope, "kv_nope"), (kv_scale, "kv_scale")):
-        _need(t, torch.uint8, n)
-    _need(q_rope, torch.bfloat16, "q_rope")
-    _need(kv_rope, torch.bfloat16, "kv_rope")
-    _need(kv_indptr, torch.int32, "kv_indptr")
-    _need(kv_indices, torch.int32, "kv_indices")
+        _need(t, torch.uint8, n, dev)
+    _need(q_rope, torch.bfloat16, "q_rope", dev)
+    _need(kv_rope, torch.bfloat16, "kv_rope", dev)
+    _need(kv_indptr, torch.int32, "kv_indptr", dev)
+    _need(kv_indices, torch.int32, "kv_indices", dev)
+    _same_device(dev, out=out, lse=lse)
+    on = _Stream(dev, stream)
     T, H, _ = q_nope.shape
     if out is None:
-        out = torch.empty((T, H, abi.D_VO), dtype=torch.bfloat16, device=q_nope.device)
+        out = on.empty(q_nope, (T, H, abi.D_VO), torch.bfloat16)
     if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q_nope.device)
+        lse = on.empty(q_nope, (T, H), torch.float32)
     a = make_decode_mxfp8_args(q_nope, q_scale, q_rope, kv_nope, kv_scale, kv_rope, kv_indptr,
                                kv_indices, sm_scale, out, lse, s_q=s_q, max_kv_len=max_kv_len,
                                num_splits=num_splits)
     lib = load_library()
-    n = ctypes.c_size_t(0)
-    check(lib.dsa_mla_decode_mxfp8_workspace_size(ctypes.byref(a), ctypes.byref(n)),
-          "dsa_mla_decode_mxfp8_workspace_size")
-    if n.value and (workspace is None or workspace.numel() * workspace.element_size() < n.value):
-        workspace = torch.empty(n.value, dtype=torch.uint8, device=q_nope.device)
-    check(lib.dsa_mla_decode_mxfp8(ctypes.byref(a), _ptr(workspace) if n.value else None, n.value,
-                                   _stream(stream)), "dsa_mla_decode_mxfp8")
+    _run_with_workspace(lib.dsa_mla_decode_mxfp8_workspace_size, lib.dsa_mla_decode_mxfp8, ctypes.byref(a), workspace,
+                        q_nope, on, "dsa_mla_decode_mxfp8")
     return out, lse
 
 
@@ -321,19 +376,21 @@ def mla_combine(partial_o: torch.Tensor, partial_lse: torch.Tensor,
                 stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Merge split partials fp32 [S, rows, H, 512] + [S, rows, H] -> bf16 [rows, H, 512], lse."""
     _need(partial_o, torch.float32, "partial_o")
-    _need(partial_lse, torch.float32, "partial_lse")
+    dev = partial_o.get_device()
+    _need(partial_lse, torch.float32, "partial_lse", dev)
+    _same_device(dev, out=out, lse=lse)
     S, rows, H, D = partial_o.shape
     if D != abi.D_VO or tuple(partial_lse.shape) != (S, rows, H):
         raise ValueError("partial_o must be [S, rows, H, 512] and partial_lse [S, rows, H]")
     if not (partial_o.is_contiguous() and partial_lse.is_contiguous()):
         raise ValueError("partials must be contiguous")
+    on = _Stream(dev, stream)
     if out is None:
-        out = torch.empty((rows, H, D), dtype=torch.bfloat16, device=partial_o.device)
+        out = on.empty(partial_o, (rows, H, D), torch.bfloat16)
     if lse is None:
-        lse = torch.empty((rows, H), dtype=torch.float32, device=partial_o.device)
-    check(load_library().dsa_mla_combine(_ptr(partial_o), _ptr(partial_lse), S, rows, H, _ptr(out),
-                                         out.stride(0), out.stride(1), _ptr(lse), _stream(stream)),
-          "dsa_mla_combine")
+        lse = on.empty(partial_o, (rows, H), torch.float32)
+    on.call(load_library().dsa_mla_combine, "dsa_mla_combine", _ptr(partial_o), _ptr(partial_lse), S, rows, H, _ptr(out),
+            out.stride(0), out.stride(1), _ptr(lse))
     return out, lse
 
 
@@ -371,15 +428,18 @@ def mla_prefill(q: torch.Tensor, kv: torch.Tensor, indices: torch.Tensor, sm_sca
     num_splits: split-K over each query's list (0 = automatic, more than one only for few
     queries)."""
     _need(q, torch.bfloat16, "q")
-    _need(indices, torch.int32, "indices")
+    dev = q.get_device()
+    _need(indices, torch.int32, "indices", dev)
+    _same_device(dev, kv=kv, out=out, lse=lse)
+    on = _stream_of(dev, stream)
     N, H, _ = q.shape
     if out is None:
-        out = q.new_empty((N, H, abi.D_VO))
+        out = q.new_empty((N, H, abi.D_VO)) if on is None else on.empty(q, (N, H, abi.D_VO), q.dtype)
     if lse is None:
-        lse = q.new_empty((N, H), dtype=torch.float32)
+        lse = q.new_empty((N, H), dtype=torch.float32) if on is None else on.empty(q, (N, H), torch.float32)
     a = abi.pack_prefill(*_prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, num_splits))
-    _sized_launch(load_library().dsa_mla_prefill_workspace_size, load_library().dsa_mla_prefill, a, workspace, q, stream,
-                  "dsa_mla_prefill")
+    lib = load_library()
+    _run_with_workspace(lib.dsa_mla_prefill_workspace_size, lib.dsa_mla_prefill, a, workspace, q, on, "dsa_mla_prefill")
     return out, lse
 
 
@@ -397,24 +457,27 @@ def mla_prefill_v4(q: torch.Tensor, unified_kv: torch.Tensor, kv: torch.Tensor,
     num_splits: split-K over each query's list (0 = automatic, more than one only for few
     queries); the split partials live in `workspace` (allocated here when missing)."""
     _need(q, torch.bfloat16, "q")
+    dev = q.get_device()
     for t, n in ((unified_kv, "unified_kv"), (kv, "kv")):
-        _need(t, torch.bfloat16, n)
+        _need(t, torch.bfloat16, n, dev)
         if t.shape[-1] != abi.D_V4 or t.stride(-1) != 1:
             raise ValueError(f"{n} must be [rows, 512] bf16 with a dense last dim")
     for t, n in ((kv_indptr_prefix, "kv_indptr_prefix"), (kv_indices_prefix, "kv_indices_prefix"),
                  (kv_indptr_extend, "kv_indptr_extend"), (kv_indices_extend, "kv_indices_extend")):
-        _need(t, torch.int32, n)
+        _need(t, torch.int32, n, dev)
     if attn_sink is not None:
-        _need(attn_sink, torch.float32, "attn_sink")
+        _need(attn_sink, torch.float32, "attn_sink", dev)
+    _same_device(dev, out=out, lse=lse)
+    on = _Stream(dev, stream)
     N, H, D = q.shape
     if D != abi.D_V4 or q.stride(2) != 1:
         raise ValueError("q must be [N, H, 512] with a dense last dim")
     if out is None:
-        out = torch.empty_like(q)
+        out = on.take(torch.empty_like(q))
     if out.stride() != q.stride():
         raise ValueError("out must have q's strides (the reference shares stride_qo_n / stride_qo_h)")
     if lse is None:
-        lse = torch.empty((N, H), dtype=torch.float32, device=q.device)
+        lse = on.empty(q, (N, H), torch.float32)
     if max_rows is None:
         max_rows = int(((kv_indptr_prefix[1:] - kv_indptr_prefix[:-1]) +
                         (kv_indptr_extend[1:] - kv_indptr_extend[:-1])).max()) if N else 0
@@ -433,8 +496,8 @@ def mla_prefill_v4(q: torch.Tensor, unified_kv: torch.Tensor, kv: torch.Tensor,
     a.softmax_scale = float(softmax_scale)
     a.num_splits = int(num_splits)
     lib = load_library()
-    _run_with_workspace(lib.dsa_mla_prefill_v4_workspace_size, lib.dsa_mla_prefill_v4, a, workspace,
-                        q.device, stream, "dsa_mla_prefill_v4")
+    _run_with_workspace(lib.dsa_mla_prefill_v4_workspace_size, lib.dsa_mla_prefill_v4, ctypes.byref(a), workspace,
+                        q, on, "dsa_mla_prefill_v4")
     return out, lse
 
 
@@ -444,16 +507,19 @@ def quantize_kv_fp8(src: torch.Tensor, dst: Optional[torch.Tensor] = None,
     _need(src, torch.bfloat16, "src")
     if src.shape[-1] != abi.D_QK or src.stride(-1) != 1:
         raise ValueError("src must be [n, 576] bf16 with a dense last dim")
+    dev = src.get_device()
+    on = _Stream(dev, stream)
     src2 = src.reshape(-1, abi.D_QK)
+    if src2.data_ptr() != src.data_ptr():
+        on.take(src2)                            # (a copy, of rows that no one stride reaches)
     n = src2.shape[0]
     if dst is None:
-        dst = torch.empty((n, abi.FP8_ROW_BYTES), dtype=torch.uint8, device=src.device)
-    _need(dst, torch.uint8, "dst")
+        dst = on.empty(src, (n, abi.FP8_ROW_BYTES), torch.uint8)
+    _need(dst, torch.uint8, "dst", dev)
     if dst_rows is not None:
-        _need(dst_rows, torch.int64, "dst_rows")
-    check(load_library().dsa_kv_quantize_fp8(_ptr(src2), src2.stride(0), n, _ptr(dst),
-                                             dst.numel() // abi.FP8_ROW_BYTES, _ptr(dst_rows),
-                                             _stream(stream)), "dsa_kv_quantize_fp8")
+        _need(dst_rows, torch.int64, "dst_rows", dev)
+    on.call(load_library().dsa_kv_quantize_fp8, "dsa_kv_quantize_fp8", _ptr(src2), src2.stride(0), n, _ptr(dst),
+            dst.numel() // abi.FP8_ROW_BYTES, _ptr(dst_rows))
     return dst
 
 
@@ -465,6 +531,7 @@ def topk_indices(scores: torch.Tensor, topk: int, lengths: Optional[torch.Tensor
     first lengths[t] positions.  NaN ranks above +inf, -0 equals +0, and ties at the threshold
     go to the lower positions (dsa_topk_indices in include/dsa_topk.h)."""
     _need(scores, torch.float32, "scores")
+    dev = scores.get_device()
     if scores.dim() != 2 or scores.stride(1) != 1:
         raise ValueError("scores must be [T, n] fp32 with a dense last dim")
     T, n = scores.shape
@@ -476,16 +543,17 @@ def topk_indices(scores: torch.Tensor, topk: int, lengths: Optional[torch.Tensor
         raise ValueError("scores rows must have a stride that is a multiple of 4 and be readable "
                          "up to n rounded up to a multiple of 4")
     if lengths is not None:
-        _need(lengths, torch.int32, "lengths")
+        _need(lengths, torch.int32, "lengths", dev)
         if lengths.numel() != T or not lengths.is_contiguous():
             raise ValueError("lengths must be a contiguous int32 [T]")
+    on = _Stream(dev, stream)
     if out is None:
-        out = torch.empty((T, topk), dtype=torch.int32, device=scores.device)
-    _need(out, torch.int32, "out")
+        out = on.empty(scores, (T, topk), torch.int32)
+    _need(out, torch.int32, "out", dev)
     if out.dim() != 2 or out.shape[0] != T or out.shape[1] < topk or out.stride(1) != 1:
         raise ValueError("out must be int32 [T, >= topk] with a dense last dim")
-    check(load_library().dsa_topk_indices(_ptr(scores), stride, _ptr(lengths), T, n, int(topk),
-                                          _ptr(out), out.stride(0), _stream(stream)), "dsa_topk_indices")
+    on.call(load_library().dsa_topk_indices, "dsa_topk_indices", _ptr(scores), stride, _ptr(lengths), T, n, int(topk),
+            _ptr(out), out.stride(0))
     return out
 
 
@@ -502,19 +570,22 @@ def mla_prefill_v4_fp8(q_nope: torch.Tensor, q_rope: torch.Tensor, unified_kv_no
     Q head is a 512-byte NoPE stream row (448 e4m3 codes, 14 E8M0 scales, pad; uint8) plus 64 bf16
     RoPE values; q_* [N, H, 512 | 64], pools [rows, 512 | 64].  Returns (out bf16 [N, H, 512],
     lse fp32 [N, H])."""
+    dev = q_nope.get_device()
     for t, n in ((q_nope, "q_nope"), (unified_kv_nope, "unified_kv_nope"), (kv_nope, "kv_nope")):
-        _need(t, torch.uint8, n)
+        _need(t, torch.uint8, n, dev)
         if t.shape[-1] != 512 or t.stride(-1) != 1:
             raise ValueError(f"{n} must have 512-byte rows with a dense last dim")
     for t, n in ((q_rope, "q_rope"), (unified_kv_rope, "unified_kv_rope"), (kv_rope, "kv_rope")):
-        _need(t, torch.bfloat16, n)
+        _need(t, torch.bfloat16, n, dev)
         if t.shape[-1] != 64 or t.stride(-1) != 1:
             raise ValueError(f"{n} must have 64 bf16 values per row with a dense last dim")
     for t, n in ((kv_indptr_prefix, "kv_indptr_prefix"), (kv_indices_prefix, "kv_indices_prefix"),
                  (kv_indptr_extend, "kv_indptr_extend"), (kv_indices_extend, "kv_indices_extend")):
-        _need(t, torch.int32, n)
+        _need(t, torch.int32, n, dev)
     if attn_sink is not None:
-        _need(attn_sink, torch.float32, "attn_sink")
+        _need(attn_sink, torch.float32, "attn_sink", dev)
+    _same_device(dev, out=out, lse=lse)
+    on = _Stream(dev, stream)
     N, H, _ = q_nope.shape
     if tuple(q_rope.shape[:2]) != (N, H):
         raise ValueError("q_nope and q_rope must cover the same [N, H]")
@@ -523,9 +594,9 @@ def mla_prefill_v4_fp8(q_nope: torch.Tensor, q_rope: torch.Tensor, unified_kv_no
     if unified_kv_nope.stride(0) != kv_nope.stride(0) or unified_kv_rope.stride(0) != kv_rope.stride(0):
         raise ValueError("both pools must share the row strides (stride_kv_nope_page / _rope_page)")
     if out is None:
-        out = torch.empty((N, H, abi.D_V4), dtype=torch.bfloat16, device=q_nope.device)
+        out = on.empty(q_nope, (N, H, abi.D_V4), torch.bfloat16)
     if lse is None:
-        lse = torch.empty((N, H), dtype=torch.float32, device=q_nope.device)
+        lse = on.empty(q_nope, (N, H), torch.float32)
     if max_rows is None:
         max_rows = int(((kv_indptr_prefix[1:] - kv_indptr_prefix[:-1]) +
                         (kv_indptr_extend[1:] - kv_indptr_extend[:-1])).max()) if N else 0
@@ -546,8 +617,8 @@ def mla_prefill_v4_fp8(q_nope: torch.Tensor, q_rope: torch.Tensor, unified_kv_no
     a.softmax_scale = float(softmax_scale)
     a.num_splits = int(num_splits)
     lib = load_library()
-    _run_with_workspace(lib.dsa_mla_prefill_v4_fp8_workspace_size, lib.dsa_mla_prefill_v4_fp8, a, workspace,
-                        q_nope.device, stream, "dsa_mla_prefill_v4_fp8")
+    _run_with_workspace(lib.dsa_mla_prefill_v4_fp8_workspace_size, lib.dsa_mla_prefill_v4_fp8, ctypes.byref(a), workspace,
+                        q_nope, on, "dsa_mla_prefill_v4_fp8")
     return out, lse
 
 
@@ -561,9 +632,12 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
     (-inf where k_j's row lies outside the cache); other entries are left as allocated (NaN
     here)."""
     _need(q, torch.bfloat16, "q")
-    _need(weights, torch.float32, "weights")
-    _need(k_cache, torch.bfloat16, "k_cache")
-    _need(seq_lens, torch.int32, "seq_lens")
+    dev = q.get_device()
+    _need(weights, torch.float32, "weights", dev)
+    _need(k_cache, torch.bfloat16, "k_cache", dev)
+    _need(seq_lens, torch.int32, "seq_lens", dev)
+    _same_device(dev, scores=scores)
+    on = _Stream(dev, stream)
     B, s_q, H_I, D = q.shape
     if D != 128 or q.stride(3) != 1:
         raise ValueError("q must be [B, s_q, H_I, 128] with a dense last dim")
@@ -575,7 +649,8 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
     if n_cols is None:
         n_cols = int(seq_lens.max().item()) if B else 0
     if scores is None:
-        scores = torch.full((B, s_q, max(n_cols, 1)), float("nan"), dtype=torch.float32, device=q.device)
+        # (filled before take(): the call's stream waits for it)
+        scores = on.take(q.new_full((B, s_q, max(n_cols, 1)), float("nan"), dtype=torch.float32))
     a = abi.IndexerArgs()
     a.q = _ptr(q)
     a.q_stride_b, a.q_stride_t, a.q_stride_h = q.stride(0), q.stride(1), q.stride(2)
@@ -584,7 +659,7 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
     a.k_total_rows = kc.shape[0]
     a.k_stride_row = kc.stride(0)
     if block_table is not None:
-        _need(block_table, torch.int32, "block_table")
+        _need(block_table, torch.int32, "block_table", dev)
         if block_size is None:
             block_size = k_cache.shape[-2] if k_cache.dim() >= 3 else None
         if block_size is None:
@@ -597,7 +672,7 @@ def indexer_scores(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor
     a.scores = _ptr(scores)
     a.score_stride = scores.stride(1) if scores.dim() == 3 else scores.stride(0)
     a.B, a.s_q, a.H_I, a.n_cols, a.causal = B, s_q, H_I, n_cols, 1 if causal else 0
-    check(load_library().dsa_indexer_scores(ctypes.byref(a), _stream(stream)), "dsa_indexer_scores")
+    on.call(load_library().dsa_indexer_scores, "dsa_indexer_scores", ctypes.byref(a))
     return scores
 
 
@@ -730,45 +805,6 @@ def _empty_like(like: torch.Tensor, shape, dtype) -> torch.Tensor:
     return like.new_empty(shape, dtype=dtype)
 
 
-class _Stream:
-    """The stream of a call on device `dev` and what it allocates.  Memory used on a stream that is not the
-    device's current one is marked so for the allocator, which then does not hand it out while the call runs."""
-
-    __slots__ = ("dev", "handle", "other")
-
-    def __init__(self, dev: int, stream):
-        self.dev = dev
-        current = _raw_stream(dev)
-        self.other = None
-        if stream is None:
-            self.handle = current
-        else:
-            self.handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-            if self.handle != current:
-                self.other = (stream if isinstance(stream, torch.cuda.Stream)
-                              else torch.cuda.ExternalStream(self.handle, device=dev))
-
-    def empty_like(self, like: torch.Tensor) -> torch.Tensor:
-        return torch.empty_like(like) if self.other is None else self.empty(like, like.shape, like.dtype)
-
-    def empty(self, like: torch.Tensor, shape, dtype) -> torch.Tensor:
-        t = like.new_empty(shape, dtype=dtype)
-        if self.other is not None:
-            # (the current stream's earlier work may still use that memory)
-            self.other.wait_stream(torch.cuda.current_stream(self.dev))
-            t.record_stream(self.other)
-        return t
-
-    def call(self, fn, where: str, *args) -> None:
-        if _current_device() == self.dev:
-            rc = fn(*args, self.handle)
-        else:
-            with torch.cuda.device(self.dev):
-                rc = fn(*args, self.handle)
-        if rc:
-            check(rc, where)
-
-
 def _launch(fn, where: str, dev: int, stream, *args) -> None:
     """One call that allocates nothing on a stream."""
     if stream is None and _current_device() == dev:
@@ -842,7 +878,7 @@ def qk_norm_rope(q: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,
         pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     elif rope:
         raise ValueError("a rotation needs positions, or q_indptr and seq_lens")
-    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
+    on = _stream_of(dev, stream)
     qs, q_out = _normed_rows(q, q_norm, q_weight, q_bias, q_out, T, D, norm_dim, "q", dev, on)
     if k is not None:
         if k.dim() != 3:
@@ -987,7 +1023,7 @@ def kv_read(cache, q_indptr: torch.Tensor, seq_lens: torch.Tensor, rows: Optiona
         raise ValueError("q_indptr must be a device tensor")
     pi, pl, B = _sequences(q_indptr, seq_lens, dev)
     first, fmt, width, pc, psc, pr, n, stride, sstride, rstride = _streams(cache, dev)
-    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
+    on = _stream_of(dev, stream)
     if out is None:
         if rows is None:
             raise ValueError("rows is required without out")
@@ -1082,7 +1118,7 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     if dev < 0 or q.dim() != 3:
         _bad("q", q, "be a device tensor [T, H, 576]")
     # (None: the current stream of the current device, the usual call)
-    on = None if stream is None and _current_device() == dev else _Stream(dev, stream)
+    on = _stream_of(dev, stream)
     empty = _empty_like if on is None else on.empty
     T, H, _ = q.shape
     ot, oh = H * abi.D_VO, abi.D_VO
@@ -1106,11 +1142,8 @@ def mla_chunk(q: torch.Tensor, kv_cache: torch.Tensor, q_indptr: torch.Tensor, s
     need = n.value
     ws = None
     if need:
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = empty(q, (need,), _U8)
-        elif not workspace.is_contiguous():
-            _bad("workspace", workspace, "be dense")
-        ws = _addr(workspace, workspace.dtype, "workspace", dev)
+        workspace = _workspace(workspace, need, q, on)
+        ws = workspace.data_ptr()
     fn = lib.dsa_mla_chunk
     if on is None:
         rc = fn(a, ws, need, _raw_stream(dev))
