@@ -7,6 +7,7 @@ loader raises, so a GPU run can never silently compute elsewhere.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import struct
 
@@ -267,19 +268,48 @@ class ChunkArgs(ctypes.Structure):
     ]
 
 
+def _fitting(name: str, code: str, v):
+    """`v` as its field holds it: a null pointer for None, and the nearest 32-bit integer, which the library refuses
+    itself where the field's own range ends earlier (a ctypes field would wrap it into that range)."""
+    if code == "f":
+        return float(v)
+    if v is None and code == "P":
+        return 0
+    try:
+        v = operator.index(v)
+    except TypeError:
+        raise TypeError(f"{name} must be a whole number, got {v!r}") from None
+    if code == "i":
+        return min(max(v, -2 ** 31), 2 ** 31 - 1)
+    if not (0 if code == "P" else -2 ** 63) <= v < (2 ** 64 if code == "P" else 2 ** 63):
+        raise ValueError(f"{name} is out of range: {v}")
+    return v
+
+
 def packer(cls):
     """A function of a struct's fields in order (nested structs' fields in their place; None: a null
     pointer) that gives its bytes: filling a ctypes struct of 38 fields takes three times as long."""
     codes = {_vp: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}
 
     def flat(c):
-        return "".join(codes[t] if t in codes else flat(t) for _, t in c._fields_)
+        return [f for n, t in c._fields_ for f in ([(n, codes[t])] if t in codes else flat(t))]
 
+    fields = flat(cls)
     # (0q: the padding at a struct's end)
-    s = struct.Struct("@" + flat(cls) + "0q")
+    s = struct.Struct("@" + "".join(code for _, code in fields) + "0q")
     if s.size != ctypes.sizeof(cls):
         raise RuntimeError(f"{cls.__name__}: {s.size} packed bytes, {ctypes.sizeof(cls)} in C")
-    return s.pack
+    whole = s.pack
+
+    def pack(*values) -> bytes:
+        try:
+            return whole(*values)
+        except struct.error:
+            if len(values) != len(fields):
+                raise
+            return whole(*[_fitting(n, code, v) for (n, code), v in zip(fields, values)])
+
+    return pack
 
 
 pack_norm_rope, pack_append, pack_chunk = packer(QkNormRopeArgs), packer(KvAppendArgs), packer(ChunkArgs)

@@ -168,15 +168,15 @@ def _decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_tab
         block_size = block_size or 1
         bt = bt_stride = 0
     return (q.data_ptr(), qs[0], qs[1], qs[2], kv_cache.data_ptr(), rows, fmt, int(block_size), int(kv_batch_stride),
-            row_stride, bt, bt_stride, seq_lens.data_ptr(), indices.data_ptr(), ixs[0], ixs[1], out.data_ptr(), os[0], os[1],
+            row_stride, bt, bt_stride, _ptr(seq_lens) or 0, indices.data_ptr(), ixs[0], ixs[1], out.data_ptr(), os[0], os[1],
             os[2], 0 if lse is None else lse.data_ptr(), B, s_q, H, ix[2], int(num_splits), 1 if causal else 0,
             float(sm_scale))
 
 
 def make_decode_args(q, kv_cache, indices, sm_scale, out, lse, *, seq_lens, block_table=None,
                      block_size=None, causal=False, num_splits=0, kv_batch_stride=0):
-    return DecodeArgs(*_decode_fields(q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal,
-                                      num_splits, kv_batch_stride))
+    return DecodeArgs.from_buffer_copy(abi.pack_decode(*_decode_fields(
+        q, kv_cache, indices, sm_scale, out, lse, seq_lens, block_table, block_size, causal, num_splits, kv_batch_stride)))
 
 
 def decode_workspace_size(args: DecodeArgs) -> int:
@@ -409,7 +409,8 @@ def _prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, n
 
 
 def make_prefill_args(q, kv, indices, sm_scale, out, lse, *, causal=False, causal_offset=0, num_splits=0):
-    return PrefillArgs(*_prefill_fields(q, kv, indices, sm_scale, out, lse, causal, causal_offset, num_splits))
+    return PrefillArgs.from_buffer_copy(abi.pack_prefill(*_prefill_fields(q, kv, indices, sm_scale, out, lse, causal,
+                                                                          causal_offset, num_splits)))
 
 
 def prefill_workspace_size(args: PrefillArgs) -> int:
