@@ -212,6 +212,9 @@ int dsa_mla_decode(const dsa_mla_decode_args* args, void* workspace, size_t work
  * fewest splits that give each of 256 CUs a workgroup,
  *   max(1, min(ceil(256 / (B s_q g)), ceil(topk / 128), DSA_MLA_MAX_SPLITS)),
  *   g = 1 up to 64 heads, ceil(H / 32) beyond,
+ * and on 400-byte rows, in workgroups of any size, with the most splits whose
+ * partials fit, below the automatic count (a single one always does),
+ *   max(1, floor((DSA_MLA_NOALLOC_SCRATCH_BYTES - 256) / (B s_q H 513 * 4))),
  * if those partials fit.  Calls that overlap on one GPU share its scratch and
  * race: serialise them (one stream, or events).  Results equal
  * dsa_mla_decode's on the same arguments, in the exception with that

@@ -4080,16 +4080,6 @@ DecodePlan decode_plan(const dsa_mla_decode_args* a) {
                                  decode_by_len(a->topk));
     return DecodePlan{c.ns, a->topk == 0 ? 0 : (a->topk + c.ns - 1) / c.ns, c.kern};
 }
-// The split count of a no-allocation call whose automatic partials do not fit the
-// scratch (two 32- or 64-head workgroups to a CU): the fewest splits, of at least
-// DECODE_MIN entries, that give every CU a workgroup, with all of a token's heads
-// in one up to 64 heads, 32 in each beyond.
-int noalloc_splits(const dsa_mla_decode_args* a) {
-    const int64_t wgs = (int64_t)a->B * a->s_q * (a->H <= 64 ? 1 : narrow_groups(a->H));
-    const int64_t by_len = std::max<int64_t>(1, decode_by_len(a->topk));
-    return (int)std::min<int64_t>(std::min<int64_t>((CUS + wgs - 1) / wgs, by_len), DSA_MLA_MAX_SPLITS);
-}
-
 // formats of the top-k and prefill forms
 bool list_format(int fmt) { return fmt == DSA_KV_BF16 || fmt == DSA_KV_FP8_656 || fmt == DSA_KV_MXFP4; }
 // MXFP4 rows: a grid holds below 2^32 threads, of workgroups of 32 heads
@@ -4123,10 +4113,29 @@ int validate_decode(const dsa_mla_decode_args* a, DecodePlan* plan) {
     return DSA_OK;
 }
 
+constexpr size_t WS_SPARE = 256;
+// Partials of one split.
+int64_t decode_part_bytes(const dsa_mla_decode_args* a) {
+    return (int64_t)a->B * a->s_q * a->H * (D_VO + 1) * (int64_t)sizeof(float);
+}
 size_t decode_ws_bytes(const dsa_mla_decode_args* a, int ns) {
-    if (ns <= 1 || a->B == 0) return 0;
-    const size_t rows = (size_t)a->B * a->s_q * a->H;
-    return (size_t)ns * rows * (D_VO + 1) * sizeof(float) + 256;
+    return ns <= 1 || a->B == 0 ? 0 : (size_t)ns * decode_part_bytes(a) + WS_SPARE;
+}
+
+// The split count of a no-allocation call whose automatic partials (`automatic`
+// splits) do not fit the scratch.  Two 32- or 64-head workgroups to a CU: the fewest
+// splits, of at least DECODE_MIN entries, that give every CU a workgroup, with all of
+// a token's heads in one up to 64 heads, 32 in each beyond.  MXFP4 rows, whose
+// workgroups have 16, 32 or 128 heads as the time model likes: the most that fit,
+// unsplit where two do not.
+int noalloc_splits(const dsa_mla_decode_args* a, int automatic) {
+    if (a->kv_format == DSA_KV_MXFP4) {
+        const int64_t fit = ((int64_t)DSA_MLA_NOALLOC_SCRATCH_BYTES - (int64_t)WS_SPARE) / decode_part_bytes(a);
+        return (int)std::max<int64_t>(1, std::min<int64_t>(automatic, fit));
+    }
+    const int64_t wgs = (int64_t)a->B * a->s_q * (a->H <= 64 ? 1 : narrow_groups(a->H));
+    const int64_t by_len = std::max<int64_t>(1, decode_by_len(a->topk));
+    return (int)std::min<int64_t>(std::min<int64_t>((CUS + wgs - 1) / wgs, by_len), DSA_MLA_MAX_SPLITS);
 }
 
 // MXFP4 rows: the kernels over lists of dsa_chunk.hip
@@ -4491,9 +4500,9 @@ int dsa_mla_decode_noalloc(const dsa_mla_decode_args* a, void* stream) {
     if (rc) return rc;
     if (a->B == 0) return DSA_OK;
     size_t need = decode_ws_bytes(a, plan.ns);
-    if (need > DSA_MLA_NOALLOC_SCRATCH_BYTES && !a->num_splits && plan.kern != WIDE) {
+    if (need > DSA_MLA_NOALLOC_SCRATCH_BYTES && !a->num_splits && (plan.kern != WIDE || a->kv_format == DSA_KV_MXFP4)) {
         dsa_mla_decode_args fewer = *a;
-        fewer.num_splits = noalloc_splits(a);
+        fewer.num_splits = noalloc_splits(a, plan.ns);
         plan = decode_plan(&fewer);
         need = decode_ws_bytes(a, plan.ns);
     }
