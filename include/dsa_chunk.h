@@ -280,9 +280,11 @@ typedef struct {
     float sm_scale;
 } dsa_mla_chunk_args;
 
-/* Workspace bytes dsa_mla_chunk needs (0 when it runs unsplit), and its split count. */
+/* Workspace bytes dsa_mla_chunk needs (0 when it runs unsplit), its split count, and
+ * the rows (heads of tokens; 16, 32 or 128) of a workgroup of the kernel that it runs. */
 int dsa_mla_chunk_workspace_size(const dsa_mla_chunk_args* args, size_t* bytes);
 int dsa_mla_chunk_num_splits(const dsa_mla_chunk_args* args, int32_t* num_splits);
+int dsa_mla_chunk_group_rows(const dsa_mla_chunk_args* args, int32_t* rows);
 int dsa_mla_chunk(const dsa_mla_chunk_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

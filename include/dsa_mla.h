@@ -189,6 +189,12 @@ int dsa_mla_decode_workspace_size(const dsa_mla_decode_args* args, size_t* bytes
 int dsa_mla_decode_num_splits(const dsa_mla_decode_args* args, int32_t* num_splits);
 
 /*
+ * Heads of a workgroup of the kernel that dsa_mla_decode runs for these arguments
+ * (16, 32, 64 or 128; see Heads above).  Pure host function.
+ */
+int dsa_mla_decode_group_heads(const dsa_mla_decode_args* args, int32_t* heads);
+
+/*
  * Launch the decode pipeline on `stream`: the fused gather / QK / softmax /
  * PV kernel, followed by the split combine when more than one split is used.
  * Replaces mla_decode_launch_pipeline, opus_attn/dsa_v32/common/host.cc:114-138
@@ -415,6 +421,8 @@ typedef struct {
 
 /* Workspace bytes dsa_mla_prefill needs (0 when it runs unsplit). */
 int dsa_mla_prefill_workspace_size(const dsa_mla_prefill_args* args, size_t* bytes);
+/* As dsa_mla_decode_group_heads, of dsa_mla_prefill. */
+int dsa_mla_prefill_group_heads(const dsa_mla_prefill_args* args, int32_t* heads);
 int dsa_mla_prefill(const dsa_mla_prefill_args* args, void* workspace, size_t workspace_bytes,
                     void* stream);
 

@@ -71,6 +71,9 @@ EXPORTED_SYMBOLS = (
     "dsa_kv_read",
     "dsa_mla_chunk_workspace_size",
     "dsa_mla_chunk_num_splits",
+    "dsa_mla_chunk_group_rows",
+    "dsa_mla_decode_group_heads",
+    "dsa_mla_prefill_group_heads",
     "dsa_mla_chunk",
 )
 
@@ -378,6 +381,9 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.dsa_kv_read.argtypes = [_vp, _vp]
     lib.dsa_mla_chunk_workspace_size.argtypes = [_vp, sz]
     lib.dsa_mla_chunk_num_splits.argtypes = [_vp, ctypes.POINTER(_i32)]
+    lib.dsa_mla_chunk_group_rows.argtypes = [_vp, ctypes.POINTER(_i32)]
+    lib.dsa_mla_decode_group_heads.argtypes = [_vp, ctypes.POINTER(_i32)]
+    lib.dsa_mla_prefill_group_heads.argtypes = [_vp, ctypes.POINTER(_i32)]
     lib.dsa_mla_chunk.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.dsa_mla_strerror.argtypes = [ctypes.c_int]
     lib.dsa_mla_strerror.restype = ctypes.c_char_p

@@ -2024,6 +2024,14 @@ int dsa_mla_chunk_num_splits(const dsa_mla_chunk_args* a, int32_t* num_splits) {
     return DSA_OK;
 }
 
+int dsa_mla_chunk_group_rows(const dsa_mla_chunk_args* a, int32_t* rows) {
+    if (!rows) return DSA_ERR_NULL_POINTER;
+    const int rc = validate(a);
+    if (rc) return rc;
+    *rows = KIND_ROWS[plan_of(a).kind];
+    return DSA_OK;
+}
+
 int dsa_mla_chunk_workspace_size(const dsa_mla_chunk_args* a, size_t* bytes) {
     if (!bytes) return DSA_ERR_NULL_POINTER;
     const int rc = validate(a);

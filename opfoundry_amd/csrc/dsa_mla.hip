@@ -4048,6 +4048,9 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
 // 137, [115], 127; 256 of 128 heads [152], 230, 246; 2 of 128 heads 28.7, 21.3, [19.2]; 300 of 40 heads, 1024
 // entries, 125, 93, [68].
 int fp4_heads(Kern k) { return k == WIDE ? HEADS : k == NARROW ? 32 : 16; }
+int group_heads(int fmt, Kern k) {
+    return fmt == DSA_KV_MXFP4 ? fp4_heads(k) : k == WIDE ? HEADS : k == PAIR64 ? 64 : NARROW_HEADS;
+}
 Choice choose_fp4(int64_t tokens, int32_t H, int64_t list, int requested, int64_t by_len) {
     Choice best{WIDE, requested > 0 ? requested : 1};
     double least = -1.0;
@@ -4475,6 +4478,15 @@ int dsa_mla_decode_num_splits(const dsa_mla_decode_args* a, int32_t* num_splits)
     return DSA_OK;
 }
 
+int dsa_mla_decode_group_heads(const dsa_mla_decode_args* a, int32_t* heads) {
+    if (!heads) return DSA_ERR_NULL_POINTER;
+    DecodePlan plan;
+    const int rc = validate_decode(a, &plan);
+    if (rc) return rc;
+    *heads = group_heads(a->kv_format, plan.kern);
+    return DSA_OK;
+}
+
 int dsa_mla_decode_workspace_size(const dsa_mla_decode_args* a, size_t* bytes) {
     if (!bytes) return DSA_ERR_NULL_POINTER;
     DecodePlan plan;
@@ -4689,6 +4701,15 @@ int dsa_mla_prefill_workspace_size(const dsa_mla_prefill_args* a, size_t* bytes)
     const int rc = validate_prefill(a, &ns);
     if (rc) return rc;
     *bytes = prefill_ws_bytes(ns, a->N, a->H);
+    return DSA_OK;
+}
+
+int dsa_mla_prefill_group_heads(const dsa_mla_prefill_args* a, int32_t* heads) {
+    if (!heads) return DSA_ERR_NULL_POINTER;
+    int ns;
+    const int rc = validate_prefill(a, &ns);
+    if (rc) return rc;
+    *heads = group_heads(a->kv_format, prefill_plan(a->kv_format, a->N, a->H, a->num_splits, a->topk).kern);
     return DSA_OK;
 }
 

@@ -193,6 +193,13 @@ def decode_num_splits(args: DecodeArgs) -> int:
     return n.value
 
 
+def decode_group_heads(args: DecodeArgs) -> int:
+    """Heads of a workgroup of the kernel that the call runs."""
+    n = ctypes.c_int32(0)
+    check(load_library().dsa_mla_decode_group_heads(ctypes.byref(args), ctypes.byref(n)), "dsa_mla_decode_group_heads")
+    return n.value
+
+
 def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, sm_scale: float,
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, *,
                seq_lens: torch.Tensor, block_table: Optional[torch.Tensor] = None,
@@ -417,6 +424,13 @@ def prefill_workspace_size(args: PrefillArgs) -> int:
     n = ctypes.c_size_t(0)
     check(load_library().dsa_mla_prefill_workspace_size(ctypes.byref(args), ctypes.byref(n)),
           "dsa_mla_prefill_workspace_size")
+    return n.value
+
+
+def prefill_group_heads(args: PrefillArgs) -> int:
+    """Heads of a workgroup of the kernel that the call runs."""
+    n = ctypes.c_int32(0)
+    check(load_library().dsa_mla_prefill_group_heads(ctypes.byref(args), ctypes.byref(n)), "dsa_mla_prefill_group_heads")
     return n.value
 
 
@@ -1091,6 +1105,13 @@ def _pack_chunk(q, kv_cache, q_indptr, seq_lens, sm_scale, po, ot, oh, ps, block
 def chunk_num_splits(args) -> int:
     n = ctypes.c_int32(0)
     check(load_library().dsa_mla_chunk_num_splits(args, ctypes.byref(n)), "dsa_mla_chunk_num_splits")
+    return n.value
+
+
+def chunk_group_rows(args) -> int:
+    """Rows (heads of tokens) of a workgroup of the kernel that the call runs."""
+    n = ctypes.c_int32(0)
+    check(load_library().dsa_mla_chunk_group_rows(args, ctypes.byref(n)), "dsa_mla_chunk_group_rows")
     return n.value
 
 
