@@ -187,8 +187,11 @@ int dsa_kv_append(const dsa_kv_append_args* args, void* stream);
  * the order of the pages does not matter).  A position without a row reads as
  * zeros.  Rows of out that belong to no sequence are left as they were.
  * cache    : the streams of kv_format as in dsa_kv_append; every value is the
- *            code's times its scale, in fp32 and rounded once to bf16 (exact for
- *            MXFP8, V4 fp8 and MXFP4 rows), NaN for a NaN code and for E8M0 255
+ *            code's times its scale, in fp32 and rounded once to bf16, NaN for a NaN
+ *            code and for E8M0 255.  Of MXFP8, V4 fp8 and MXFP4 rows it is exact
+ *            where bf16 holds it: infinity past bf16's largest value (the largest
+ *            e4m3 codes under scale bytes from 247 on, e2m1 codes from 253 on), a
+ *            multiple of 2^-133 where it is smaller (e4m3 codes under bytes 0 to 2)
  * out      : bf16 [T, 576], of DSA_KV_BF16_D512 and DSA_KV_MXFP8_V4 [T, 512], rows
  *            out_stride_t elements apart.  Rows that overlap one another, or
  *            memory of the cache, are refused (DSA_ERR_BAD_STRIDE).

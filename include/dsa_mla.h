@@ -30,12 +30,14 @@
  *                              for NaN
  *                    [272,400) 64 x bf16 RoPE                    =  400 B
  *   Dequantised value of NoPE dim d = e2m1(code_d) * 2^(scale[d / 32] - 127),
- *   which bf16 holds exactly: the kernels compute these rows as bf16 rows of
- *   those values.  dsa_mla_decode, dsa_mla_decode_noalloc, dsa_mla_prefill and
+ *   which bf16 holds exactly but where it reaches 2^128 (codes 4 and 6 under byte
+ *   253, from 2 on under 254), which is infinity there: the kernels compute these
+ *   rows as bf16 rows of those values.  dsa_mla_decode, dsa_mla_decode_noalloc, dsa_mla_prefill and
  *   the chunk operators (dsa_chunk.h) take them; a NaN or infinity among an
  *   attended row's values reaches the tokens that attend it.  Their calls need a
- *   positive, finite sm_scale (else DSA_ERR_UNSUPPORTED) and tokens x ceil(H / 32)
- *   below 2^24 (else DSA_ERR_BAD_SHAPE).
+ *   positive, finite sm_scale (else DSA_ERR_UNSUPPORTED: the kernels take a row's
+ *   largest q . k for its largest score) and tokens x ceil(H / 32) below 2^24 (else
+ *   DSA_ERR_BAD_SHAPE).
  *
  * Index semantics (top-k form).  indices[b][t][k] is a logical position j in
  * sequence b.  It is valid iff 0 <= j < seq_lens[b] and, when causal != 0,

@@ -1876,7 +1876,7 @@ __global__ void __launch_bounds__(NTHR) dsa_mla_chunk_combine_kernel(const Chunk
 // 16 heads over the same 4096 rows 90 (4 splits) and 120.
 // 400-byte rows have blocks of 16 rows too, two a CU.  Calls in blocks of 128, 32 and 16 rows, us, the taken one in
 // brackets: one token of 128 heads over 1501 rows 23.5, 18.3, [17.9]; 16 sequences of 1 to 4 tokens and up to 20011
-// rows, 16 heads, 75, 52, [54]; 11 of 1 or 2 tokens and 2431 rows, 16 heads, 31, 23, [20]; 24 of 1 to 4 and 393, 32 heads,
+// rows, 16 heads, 75, 52, [54] (2 us from the fastest); 11 of 1 or 2 tokens and 2431 rows, 16 heads, 31, 23, [20]; 24 of 1 to 4 and 393, 32 heads,
 // 32, 20, [17]; 7 of up to 301 and 5000, 40 heads, [386], 508, 538; 2 of 86 to 233 and 2346, 128 heads, [283], 322, 355.
 // (Constants closer to the kernels alone, 2.05, 0.66, 0.55 and 0.78, took 32-row blocks for the last one, and for 8 of up to 41
 // tokens over 5705 rows, 40 heads, where they took 137 us for 104.)

@@ -21,7 +21,7 @@
 // to 1.9 us, a QB = 2 tile 1.3 to 1.5. Kept on the way (303 us at first, 128-row blocks with most rows empty 702):
 // loads without a branch around them, so that a wait counts only older ones, two tiles ahead; fsw(), after whose
 // first form bank conflicts were 26.7 M cycles and are 1.7 M; Q loaded once for a workgroup (185 -> 172, with the
-// lane numbers formed anew in qk(), which leaves 222 registers of 256), beside the first rows' look-up and without
+// lane numbers formed anew in qk(): 222 registers of 256 over lists, 218 dense), beside the first rows' look-up and without
 // divisions (172 -> 169; 64 entries each for 1536 tokens 31 -> 28).  Not kept: rows loaded along their bytes and
 // turned through LDS (98 M L1 accesses become 39 M, but LDS has the wait then: 185 -> 200); QB = 2 with half the
 // next tile's conversions behind PV's products and half behind the scores' (lists 318 -> 313, dense 50.3 -> 50.9:

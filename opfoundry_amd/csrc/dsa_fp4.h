@@ -6,8 +6,9 @@ constexpr int FP4_ROW = DSA_MLA_FP4_ROW_BYTES;       // 256 code bytes, 16 scale
 constexpr int FP4_SCALE_OFF = 256, FP4_ROPE_OFF = 272;
 
 // 8 e2m1 codes (a dword, the first value in the low half of the low byte) times 2^(e - 127) -> 8 bf16.
-// Exact: a code has two significant bits, the scale is a power of two and bf16 has fp32's exponents (and its
-// values below the normal range, which byte 0 reaches).  The instruction takes the scale's exponent field,
+// Exact below 2^128: a code has two significant bits, the scale is a power of two and bf16 has fp32's exponents (and
+// its values below the normal range, which byte 0 reaches).  From 2^128 on (codes 4 and 6 under byte 253, from 2 on
+// under 254) it is infinity.  The instruction takes the scale's exponent field,
 // and gives NaN where that is 255, whatever the code.  All 256 x 16 pairs were compared.
 __device__ __forceinline__ u32x4 fp4_to_bf16(unsigned c, unsigned e) {
     const float s = __uint_as_float(e << 23);

@@ -3960,6 +3960,11 @@ int one_round_splits(int64_t wgs, int64_t by_len, int round = CUS) {
 // query tokens of 8 to 64 heads, lists of 200 to 16384 entries; mean error 2 to 3 %,
 // 95 % below 9 %), then moved by up to 8 % each to where the choices cost least.
 // 656-B and V4 fp8 rows are not bound by the rows' bytes.
+// MXFP4's line is not such a fit: constants by hand that order the three kernels of the
+// calls at choose_fp4 as they were measured, and no prediction of a time.  Its byte term
+// counts every token's list as read from memory, which a prompt's rows, read by many
+// tokens, are not (1531 tokens of 16 heads x 2048 over as many rows: 277 us by the
+// line, 169 measured); it is the same for the three kernels.
 struct KernTime { float start, tile, start2, tile2, split, part, bytes; };
 constexpr KernTime KERN_TIME[][4] = {
     // DSA_KV_BF16: WIDE, NARROW, PAIR, PAIR64
@@ -4046,7 +4051,8 @@ Choice choose_kern(int fmt, int64_t tokens, int32_t H, int64_t list, int request
 // workgroups share a CU: the one of least expected time (KERN_TIME).  Each of the three on calls of 2048 entries, us,
 // the taken one in brackets: 1531 tokens of 16 heads 702, 314, [172]; 512 of 32 heads 261, [128], 149; 256 of 64
 // 137, [115], 127; 256 of 128 heads [152], 230, 246; 2 of 128 heads 28.7, 21.3, [19.2]; 300 of 40 heads, 1024
-// entries, 125, 93, [68].
+// entries, 125, 93, [68].  There is no kernel between 32 and 128 heads: 33 to 64 heads take twice the time of their
+// flops at a large product's rate (256 tokens of 64 heads 109 us, 54), 128 tokens of 128 heads, in two splits, 93 for 54.
 int fp4_heads(Kern k) { return k == WIDE ? HEADS : k == NARROW ? 32 : 16; }
 int group_heads(int fmt, Kern k) {
     return fmt == DSA_KV_MXFP4 ? fp4_heads(k) : k == WIDE ? HEADS : k == PAIR64 ? 64 : NARROW_HEADS;

@@ -462,8 +462,12 @@ __global__ void __launch_bounds__(64 * WAVES) dsa_kv_append_kernel(const AppendP
 // load of a lane each.  A value is one conversion and, of e4m3 codes, one fp32
 // product, rounded once.  Bound by memory where there are rows enough: 100,000 rows
 // of 400 bytes 25 us (41 MB read and 116 MB written, 6.2 TB/s; a 1 GiB copy 5.1),
-// 21,000 of 656 bytes 10.8 (38 MB).  One row takes 2.8 (a launch and a chain of loads:
-// sequence, page, row), 333 take 4.9.
+// 21,000 of 656 bytes 10.6 (38 MB).  One row takes 2.6 (a launch and a chain of loads:
+// sequence, page, row), 333 take 4.9.  Below some 50,000 rows eight a wave leave too few
+// waves to reach the memory's rate: 9,238 rows of 400 bytes, about one wave a SIMD, 6.3 to
+// 7.6 us for 14 MB.  Calls in a graph, one after another, of 9,238 and 100,000 rows, us:
+// 400 bytes 6.3 and 25, 656 bytes 7.5 and 30, bf16 7.6 and 47, bf16 of 512 values 7.1 and
+// 44, MXFP8 6.8 and 29, V4 fp8 7.5 and 27.
 // ---------------------------------------------------------------------------
 constexpr int READ_ROWS = 8;
 struct ReadParams {
